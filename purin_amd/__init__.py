@@ -32,6 +32,14 @@ _EXPORTS = {
     "LocalQuadratic": ("local_quadratic", "LocalQuadratic"),
     "QPStructure": ("diagonal_qp", "QPStructure"),
     "QPData": ("diagonal_qp", "QPData"),
+    "Routing": ("routing", "Routing"),
+    "route": ("routing", "route"),
+    "route_experts": ("routing", "route_experts"),
+    "dispatch": ("routing", "dispatch"),
+    "combine": ("routing", "combine"),
+    "expert_product": ("routing", "expert_product"),
+    "gradient_norm": ("gradients", "gradient_norm"),
+    "clip_gradients": ("gradients", "clip_gradients"),
 }
 __all__ = list(_EXPORTS)
 

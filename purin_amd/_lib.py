@@ -1,4 +1,5 @@
-"""ctypes binding of ``libpurin_cp.so`` (the C ABI in ``include/purin_cp.h``).
+"""ctypes binding of ``libpurin_cp.so`` (the C ABI in ``include/purin_cp.h`` and
+``include/purin_train.h``).
 
 The library is required: importing this module raises if it has not been
 built (``python -m purin_amd.build`` or ``__graft_entry__.build()``).  There is
@@ -14,6 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libpurin_cp.so")
 
 F32, F64 = 0, 1
+BF16, F16 = 2, 3  # purin_train_dtype, which begins with F32 and F64
+MAX_EXPERTS = 1024  # PURIN_TRAIN_MAX_EXPERTS
 NOALLOC_SCRATCH_BYTES = 128 << 20  # PURIN_CP_NOALLOC_SCRATCH_BYTES
 OK, ERR_ARG, ERR_HIP, ERR_UNSUPPORTED, ERR_NOMEM = 0, 1, 2, 3, 4
 # purin_cp_entry (purin_cp_workspace_bytes)
@@ -48,6 +51,23 @@ SYMBOLS = (
     "purin_cp_dense_adjoint",
     "purin_cp_last_error",
     "purin_cp_build_info",
+)
+
+# every symbol include/purin_train.h declares (checked by tests/test_train_abi.py)
+TRAIN_SYMBOLS = (
+    "purin_train_route_workspace_bytes",
+    "purin_train_route",
+    "purin_train_sort",
+    "purin_train_route_vjp",
+    "purin_train_dispatch",
+    "purin_train_combine",
+    "purin_train_combine_vjp",
+    "purin_train_expert_product_workspace_bytes",
+    "purin_train_expert_product",
+    "purin_train_expert_weights_vjp_workspace_bytes",
+    "purin_train_expert_weights_vjp",
+    "purin_train_clip_workspace_bytes",
+    "purin_train_clip",
 )
 
 
@@ -124,6 +144,18 @@ class AdjointOptions(C.Structure):
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_int64),
         ("arnoldi_iterations", C.POINTER(C.c_int32)),
+    ]
+
+
+class TrainTensor(C.Structure):
+    """purin_train_tensor: one gradient of a list."""
+
+    _fields_ = [
+        ("in_", C.c_void_p),
+        ("out", C.c_void_p),
+        ("count", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
     ]
 
 
@@ -214,8 +246,31 @@ def load(path: str = LIB_PATH):
     lib.purin_cp_last_error.restype = C.c_char_p
     lib.purin_cp_build_info.argtypes = []
     lib.purin_cp_build_info.restype = C.c_char_p
+    _declare_train(lib)
     _lib = lib
     return lib
+
+
+def _declare_train(lib):
+    vp, i64, i32, dbl = C.c_void_p, C.c_int64, C.c_int32, C.c_double
+    lib.purin_train_route_workspace_bytes.argtypes = [i64, i64, i64]
+    lib.purin_train_route.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp]
+    lib.purin_train_sort.argtypes = [vp, i32, i64, i64, i64, vp, vp, i64, vp, vp, vp, vp]
+    lib.purin_train_route_vjp.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
+    lib.purin_train_dispatch.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, vp, vp, vp]
+    lib.purin_train_combine.argtypes = [vp, i32, i32, i64, i64, i64, vp, i64, vp, vp, vp]
+    lib.purin_train_combine_vjp.argtypes = [vp, i32, i32, i64, i64, i64, i64, vp, i64, vp, i64, vp,
+                                            vp, vp, vp, vp]
+    lib.purin_train_expert_product_workspace_bytes.argtypes = [i32, i64, i64, i64, i64]
+    lib.purin_train_expert_product.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, vp, i64, i64,
+                                               i64, vp, vp, i64, vp, i64]
+    lib.purin_train_expert_weights_vjp_workspace_bytes.argtypes = [i32, i64, i64, i64, i64]
+    lib.purin_train_expert_weights_vjp.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, vp, i64,
+                                                   vp, vp, i64, vp]
+    lib.purin_train_clip_workspace_bytes.argtypes = [i64]
+    lib.purin_train_clip.argtypes = [vp, i64, C.POINTER(TrainTensor), dbl, vp, i64, i32, vp]
+    for name in TRAIN_SYMBOLS:
+        getattr(lib, name).restype = i64 if name.endswith("_bytes") else C.c_int
 
 
 def check(code):

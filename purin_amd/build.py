@@ -1,8 +1,8 @@
 """Build ``libpurin_cp.so`` (HIP, gfx950) in-tree with hipcc.
 
-The library is the product: the C ABI of ``include/purin_cp.h``.  It is built
-here, into ``purin_amd/``, so that the built ``.so`` travels with the source
-tree to the GPU machine.  ``libpurin_probe.so`` (``include/purin_probe.h``)
+The library is the product: the C ABI of ``include/purin_cp.h`` and
+``include/purin_train.h``.  It is built here, into ``purin_amd/``, so that the
+built ``.so`` travels with the source tree to the GPU machine.  ``libpurin_probe.so`` (``include/purin_probe.h``)
 holds the ceiling probes that ``bench.py`` times beside the resident kernel.
 
 Each source compiles to its own object (in parallel, under ``_build/``), and
@@ -22,7 +22,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(os.path.dirname(HERE), "_build")
 LIB = os.path.join(HERE, "libpurin_cp.so")
-SOURCES = ["plan.hip", "forward.hip", "adjoint.hip", "gmres.hip", "solo.hip"]
+SOURCES = ["plan.hip", "forward.hip", "adjoint.hip", "gmres.hip", "solo.hip", "route.hip",
+           "expert.hip", "clip.hip"]
 RESIDENT_SOURCE = "resident_launch.hip"
 RESIDENT_VARIANTS = [(f64, slr) for f64 in (1, 0) for slr in (1, 2, 3, 4)]
 PROBE_LIB = os.path.join(HERE, "libpurin_probe.so")

@@ -1,0 +1,315 @@
+// The experts' products on rows sorted by expert, and the gradient of their weights
+// (include/purin_train.h: expert_product, expert_weights_vjp).
+//
+//   out(p) = a(p) W[e]                     for the rows p of expert e
+//   g_W[e] = sum over those p of a(p)^T g(p)
+//
+// Products of tiles on the matrix units; a tile belongs to one expert.  The first kernels'
+// tiles are found from the offsets on the device, so the host never waits for the counts: the
+// launch holds the most tiles that any split of the rows can need, and what is left over ends
+// at once.
+
+#include <algorithm>
+
+#include "train.hpp"
+
+namespace purin {
+namespace train {
+
+typedef bf16 B8 __attribute__((ext_vector_type(8)));
+typedef f16 H8 __attribute__((ext_vector_type(8)));
+typedef float F4 __attribute__((ext_vector_type(4)));
+typedef double D4 __attribute__((ext_vector_type(4)));
+
+// One 16x16 tile of sums per wavefront.  A lane holds kPer values along the contraction, of
+// row (or column) lane % 16 from kPer * (lane / 16) on; Steps of 4 * kPer make one kDepth.
+// sum[r] is row(lane, r) and column lane % 16.
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+  using Acc = F4;
+  static constexpr int kPer = 8, kDepth = 32;
+  static __device__ __forceinline__ Acc step(const bf16* a, const bf16* b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const B8*)a, *(const B8*)b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int lane, int r) { return 4 * (lane >> 4) + r; }
+};
+template <>
+struct Mma<f16> {
+  using Acc = F4;
+  static constexpr int kPer = 8, kDepth = 32;
+  static __device__ __forceinline__ Acc step(const f16* a, const f16* b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const H8*)a, *(const H8*)b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int lane, int r) { return 4 * (lane >> 4) + r; }
+};
+template <>
+struct Mma<float> {
+  using Acc = F4;
+  static constexpr int kPer = 1, kDepth = 16;
+  static __device__ __forceinline__ Acc step(const float* a, const float* b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(*a, *b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int lane, int r) { return 4 * (lane >> 4) + r; }
+};
+template <>
+struct Mma<double> {
+  using Acc = D4;
+  static constexpr int kPer = 1, kDepth = 16;
+  static __device__ __forceinline__ Acc step(const double* a, const double* b, Acc c) {
+    return __builtin_amdgcn_mfma_f64_16x16x4f64(*a, *b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int lane, int r) { return 4 * r + (lane >> 4); }
+};
+
+// The rows of expert e: [from, to), inside [0, rows] whatever the offsets hold.
+__device__ __forceinline__ void segment(const int32_t* offsets, int e, int64_t rows, int64_t& from,
+                                        int64_t& to) {
+  from = e ? min((int64_t)max(offsets[e], 0), rows) : 0;
+  to = min((int64_t)max(offsets[e + 1], 0), rows);
+  to = max(to, from);
+}
+
+// The expert and the first row of tile number ``tile`` where every expert's rows are cut into
+// tiles of ``height``; beyond the experts' tiles come those of the rows behind the last expert
+// (expert -1: zeros).  False where the tile is past them all.  Every wavefront finds it by
+// itself, 64 experts at a time.
+__device__ __forceinline__ bool find_tile(const int32_t* offsets, int experts, int64_t rows,
+                                          int height, int64_t tile, int& expert, int64_t& from,
+                                          int64_t& to) {
+  const int lane = threadIdx.x & 63;
+  for (int e0 = 0; e0 < experts; e0 += 64) {
+    const int e = e0 + lane;
+    int64_t a = 0, z = 0;
+    if (e < experts) segment(offsets, e, rows, a, z);
+    int32_t n = (int32_t)((z - a + height - 1) / height);
+    int32_t sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int32_t up = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += up;
+    }
+    const uint64_t here = __ballot(tile < sum);
+    if (here) {
+      const int at = __ffsll((unsigned long long)here) - 1;
+      const int32_t first = __shfl(sum - n, at, 64);
+      expert = e0 + at;
+      segment(offsets, expert, rows, from, to);
+      from += (tile - first) * height;
+      return true;
+    }
+    tile -= __shfl(sum, 63, 64);
+  }
+  int64_t unused;
+  segment(offsets, experts - 1, rows, unused, from);
+  expert = -1;
+  to = rows;
+  from += tile * height;
+  return from < to;
+}
+
+constexpr int kTile = 128;  // rows and columns of a workgroup's tile, 64 by 64 a wavefront
+
+// One operand of a tile: element (i, k) at p + i * si + k * sk, with si or sk 1.
+template <typename T>
+struct Operand {
+  const T* p;
+  int64_t si, sk;
+};
+
+template <typename T>
+constexpr int lds_pitch() {
+  // contraction-contiguous rows; the padding spreads a column's reads over the banks
+  return Mma<T>::kDepth + (Mma<T>::kPer > 1 ? Mma<T>::kPer : 1);
+}
+
+// kTile x kDepth of an operand into LDS, zeros where i >= n or k >= depth.
+template <typename T>
+__device__ __forceinline__ void stage(const Operand<T>& o, int n, int depth, T* lds) {
+  constexpr int D = Mma<T>::kDepth, P = lds_pitch<T>();
+  const bool along = o.sk == 1;
+#pragma unroll 4
+  for (int r = threadIdx.x; r < kTile * D; r += 256) {
+    const int k = along ? r % D : r / kTile;
+    const int i = along ? r / D : r % kTile;
+    lds[i * P + k] = i < n && k < depth ? o.p[i * o.si + k * o.sk] : (T)0;
+  }
+}
+
+// c (m x n of a kTile x kTile tile, row pitch ldc) = sum over k of a(i, k) b(j, k).
+template <typename T>
+__device__ __forceinline__ void tile_product(Operand<T> a, Operand<T> b, int m, int n, int64_t depth,
+                                             T* c, int64_t ldc) {
+  using M = Mma<T>;
+  constexpr int D = M::kDepth, P = lds_pitch<T>();
+  __shared__ __align__(16) T as[kTile * P];
+  __shared__ __align__(16) T bs[kTile * P];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
+  typename M::Acc acc[4][4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = typename M::Acc{0, 0, 0, 0};
+  for (int64_t k = 0; k < depth; k += D) {
+    const int d = (int)min<int64_t>(D, depth - k);
+    __syncthreads();
+    stage(a, m, d, as);
+    stage(b, n, d, bs);
+    a.p += D * a.sk;
+    b.p += D * b.sk;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < D; s += 4 * M::kPer) {
+      const int at = s + M::kPer * (lane >> 4);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          acc[x][y] = M::step(as + (wi + 16 * x + (lane & 15)) * P + at,
+                              bs + (wj + 16 * y + (lane & 15)) * P + at, acc[x][y]);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = wi + 16 * x + M::row(lane, r), j = wj + 16 * y + (lane & 15);
+        if (i < m && j < n) c[i * ldc + j] = (T)acc[x][y][r];
+      }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_product(const T* __restrict__ a, int64_t lda,
+                                                 const T* __restrict__ w, int64_t we, int64_t wi,
+                                                 int64_t wo, int64_t rows, int64_t inner,
+                                                 int64_t outer, int experts,
+                                                 const int32_t* __restrict__ offsets,
+                                                 T* __restrict__ out, int64_t ldo) {
+  int e;
+  int64_t from, to;
+  if (!find_tile(offsets, experts, rows, kTile, blockIdx.x, e, from, to)) return;
+  const int64_t col = (int64_t)blockIdx.y * kTile;
+  const int m = (int)min<int64_t>(kTile, to - from), n = (int)min<int64_t>(kTile, outer - col);
+  if (e < 0) {
+    for (int r = threadIdx.x; r < m * kTile; r += 256) {
+      const int i = r / kTile, j = r % kTile;
+      if (j < n) out[(from + i) * ldo + col + j] = (T)0;
+    }
+    return;
+  }
+  tile_product<T>({a + from * lda, lda, 1}, {w + e * we + col * wo, wo, wi}, m, n, inner,
+                  out + from * ldo + col, ldo);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_weights_vjp(const T* __restrict__ a, int64_t lda,
+                                                     const T* __restrict__ g, int64_t ldg,
+                                                     int64_t rows, int64_t inner, int64_t outer,
+                                                     const int32_t* __restrict__ offsets,
+                                                     T* __restrict__ gw) {
+  const int e = (int)blockIdx.z;
+  int64_t from, to;
+  segment(offsets, e, rows, from, to);
+  const int64_t i = (int64_t)blockIdx.x * kTile, j = (int64_t)blockIdx.y * kTile;
+  tile_product<T>({a + from * lda + i, 1, lda}, {g + from * ldg + j, 1, ldg},
+                  (int)min<int64_t>(kTile, inner - i), (int)min<int64_t>(kTile, outer - j),
+                  to - from, gw + e * inner * outer + i * outer + j, outer);
+}
+
+static int check_product(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
+                         int64_t experts) {
+  if (!known_dtype(dtype)) return refuse("unknown dtype");
+  if (rows < 0 || inner < 0 || outer < 0 || experts < 1)
+    return refuse("sizes must not be negative, experts must be positive");
+  if (experts > PURIN_TRAIN_MAX_EXPERTS)
+    return set_error(PURIN_CP_ERR_UNSUPPORTED, "more than 1024 experts");
+  if (rows >= (int64_t(1) << 31))
+    return set_error(PURIN_CP_ERR_UNSUPPORTED, "rows must stay below 2^31");
+  // a launch's second dimension counts tiles
+  if (inner > (int64_t(1) << 22) || outer > (int64_t(1) << 22))
+    return set_error(PURIN_CP_ERR_UNSUPPORTED, "inner and outer must not exceed 2^22");
+  return PURIN_CP_OK;
+}
+
+}  // namespace train
+}  // namespace purin
+
+using namespace purin;
+using namespace purin::train;
+
+extern "C" {
+
+int64_t purin_train_expert_product_workspace_bytes(int32_t dtype, int64_t rows, int64_t inner,
+                                                   int64_t outer, int64_t experts) {
+  int64_t need = -1;
+  (void)guarded([&] {
+    if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
+    need = 0;
+    return (int)PURIN_CP_OK;
+  });
+  return need;
+}
+
+int purin_train_expert_product(void* stream, int32_t dtype, int64_t rows, int64_t inner,
+                               int64_t outer, int64_t experts, const void* a, int64_t lda,
+                               const void* weight, int64_t we, int64_t wi, int64_t wo,
+                               const int32_t* offsets, void* workspace, int64_t workspace_bytes,
+                               void* out, int64_t ldo) {
+  return guarded([&] {
+    if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
+    if (!rows || !outer) return (int)PURIN_CP_OK;
+    if (!offsets || !out || (inner && (!a || !weight))) return refuse("NULL array");
+    if ((rows > 1 && lda < inner) || (rows > 1 && ldo < outer))
+      return refuse("a row pitch is below the row's length");
+    if (wi != 1 && wo != 1 && inner > 1 && outer > 1)
+      return refuse("the weight needs a unit stride along inner or outer");
+    if (we < 0 || wi < 0 || wo < 0) return refuse("the weight's strides must not be negative");
+    return by_dtype(dtype, [&](auto v) {
+      using T = decltype(v);
+      const dim3 grid((unsigned)((rows + kTile - 1) / kTile + experts),
+                      (unsigned)((outer + kTile - 1) / kTile));
+      k_product<T><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
+          (const T*)a, lda, (const T*)weight, we, wi, wo, rows, inner, outer, (int)experts,
+          offsets, (T*)out, ldo);
+      return launched("k_product");
+    });
+  });
+}
+
+int64_t purin_train_expert_weights_vjp_workspace_bytes(int32_t dtype, int64_t rows, int64_t inner,
+                                                       int64_t outer, int64_t experts) {
+  int64_t need = -1;
+  (void)guarded([&] {
+    if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
+    need = 0;
+    return (int)PURIN_CP_OK;
+  });
+  return need;
+}
+
+int purin_train_expert_weights_vjp(void* stream, int32_t dtype, int64_t rows, int64_t inner,
+                                   int64_t outer, int64_t experts, const void* a, int64_t lda,
+                                   const void* g, int64_t ldg, const int32_t* offsets,
+                                   void* workspace, int64_t workspace_bytes, void* g_weight) {
+  return guarded([&] {
+    if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
+    if (!inner || !outer) return (int)PURIN_CP_OK;
+    if (!offsets || !g_weight || (rows && (!a || !g))) return refuse("NULL array");
+    if (rows > 1 && (lda < inner || ldg < outer))
+      return refuse("a row pitch is below the row's length");
+    return by_dtype(dtype, [&](auto v) {
+      using T = decltype(v);
+      const dim3 grid((unsigned)((inner + kTile - 1) / kTile),
+                      (unsigned)((outer + kTile - 1) / kTile), (unsigned)experts);
+      k_weights_vjp<T><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
+          (const T*)a, lda, (const T*)g, ldg, rows, inner, outer, offsets, (T*)g_weight);
+      return launched("k_weights_vjp");
+    });
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,622 @@
+// Tokens to experts and back (include/purin_train.h: route, sort, dispatch, combine and
+// their gradients).
+//
+// With e(t, j) and w(t, j) a token's chosen experts and weights, place(t, j) the pair's row
+// among the pairs sorted stably by expert:
+//   rows[place(t, j)] = x(t)                     g_x(t) = sum_j g_rows[place(t, j)]
+//   out(t) = sum_j w(t, j) rows[place(t, j)]     g_rows[place(t, j)] = w(t, j) g_out(t)
+//                                                g_w(t, j) = <g_out(t), rows[place(t, j)]>
+// The order is made by counting: every chunk of pairs counts its experts, then every chunk
+// places its pairs behind the earlier experts' and the earlier chunks'.  Ranks inside a
+// wavefront come from ballots on the expert's bits, so the order is the pairs' own.
+
+#include <algorithm>
+
+#include "train.hpp"
+
+namespace purin {
+namespace train {
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int64_t kSortChunk = 2048;  // pairs of a workgroup, at least
+constexpr int64_t kSortGroups = 256;  // workgroups, at most
+
+struct SortShape {
+  int64_t chunk, groups;
+};
+static SortShape sort_shape(int64_t pairs) {
+  int64_t chunk = std::max<int64_t>(kSortChunk, (pairs + kSortGroups - 1) / kSortGroups);
+  chunk = (chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
+  return {chunk, std::max<int64_t>(1, (pairs + chunk - 1) / chunk)};
+}
+
+// ---------------------------------------------------------------------------
+// choosing a token's experts
+// ---------------------------------------------------------------------------
+
+// A positive number's bits ascend with it, NaN above infinity; 0 for what is not chosen.
+__device__ __forceinline__ uint32_t weight_key(float v) {
+  return v != v ? 0x7fc00000u : v > 0.0f ? __builtin_bit_cast(uint32_t, v) : 0u;
+}
+__device__ __forceinline__ uint64_t weight_key(double v) {
+  return v != v ? 0x7ff8000000000000ull : v > 0.0 ? __builtin_bit_cast(uint64_t, v) : 0ull;
+}
+template <typename T>
+struct Key {
+  using K = uint32_t;
+  static __device__ __forceinline__ K of(T v) { return weight_key((float)v); }
+  static __device__ __forceinline__ T value(K k) { return (T)__builtin_bit_cast(float, k); }
+};
+template <>
+struct Key<double> {
+  using K = uint64_t;
+  static __device__ __forceinline__ K of(double v) { return weight_key(v); }
+  static __device__ __forceinline__ double value(K k) { return __builtin_bit_cast(double, k); }
+};
+
+// G lanes to a token, V weights to a lane (expert i * G + lane): slots times, the lanes'
+// best by (weight, lowest expert), then the group's.
+template <typename T, int G, int V>
+__device__ __forceinline__ void choose(const T* row, int experts, int slots, int lane,
+                                       int32_t* ids, T* chosen) {
+  using K = typename Key<T>::K;
+  K key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = i * G + lane;
+    key[i] = e < experts ? Key<T>::of(row[e]) : K(0);
+  }
+  int32_t my_id = -1;
+  K my_key = 0;
+  for (int j = 0; j < slots; ++j) {
+    K best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    int e = at * G + lane;
+#pragma unroll
+    for (int m = 1; m < G; m <<= 1) {
+      const K other = __shfl_xor(best, m, 64);
+      const int oe = __shfl_xor(e, m, 64);
+      if (other > best || (other == best && oe < e)) {
+        best = other;
+        e = oe;
+      }
+    }
+    const int owner = e / G;  // the winner's register, in lane e % G
+    if (best != 0 && e % G == lane) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i == owner) key[i] = 0;
+    }
+    if (j % G == lane) {
+      my_id = best != 0 ? e : -1;
+      my_key = best;
+    }
+    if (j % G == G - 1 || j == slots - 1) {  // G slots are written together
+      const int base = j - j % G;
+      if (base + lane < slots) {
+        ids[base + lane] = my_id;
+        chosen[base + lane] = my_key ? Key<T>::value(my_key) : (T)0;
+      }
+    }
+  }
+}
+
+template <typename T, int G, int V>
+__global__ __launch_bounds__(256) void k_choose(const T* __restrict__ weights, int64_t ld,
+                                                int64_t tokens, int experts, int slots,
+                                                int32_t* __restrict__ ids,
+                                                T* __restrict__ chosen) {
+  const int lane = threadIdx.x % G;
+  const int64_t step = (int64_t)gridDim.x * (256 / G);
+  for (int64_t t = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; t < tokens; t += step)
+    choose<T, G, V>(weights + t * ld, experts, slots, lane, ids + t * slots, chosen + t * slots);
+}
+
+template <typename T, int G, int V>
+static int launch_choose(hipStream_t st, const T* w, int64_t ld, int64_t tokens, int experts,
+                         int slots, int32_t* ids, T* chosen) {
+  k_choose<T, G, V><<<grid_of(tokens, 256 / G), dim3(256), 0, st>>>(
+      w, ld, tokens, experts, slots, ids, chosen);
+  return launched("k_choose");
+}
+
+template <typename T>
+static int choose_experts(hipStream_t st, const T* w, int64_t ld, int64_t tokens, int experts,
+                          int slots, int32_t* ids, T* chosen) {
+  // the fewest lanes that hold a token's weights in at most 16 registers: fewer lanes, fewer
+  // exchanges
+  if (experts <= 32) return launch_choose<T, 16, 2>(st, w, ld, tokens, experts, slots, ids, chosen);
+  if (experts <= 64) return launch_choose<T, 16, 4>(st, w, ld, tokens, experts, slots, ids, chosen);
+  if (experts <= 128) return launch_choose<T, 16, 8>(st, w, ld, tokens, experts, slots, ids, chosen);
+  if (experts <= 256) return launch_choose<T, 16, 16>(st, w, ld, tokens, experts, slots, ids, chosen);
+  return launch_choose<T, 64, 16>(st, w, ld, tokens, experts, slots, ids, chosen);
+}
+
+// g_weights(t, e) = the sum of g_chosen(t, j) over the slots with ids(t, j) = e (one at most).
+template <typename T>
+__global__ __launch_bounds__(256) void k_choose_vjp(const int32_t* __restrict__ ids,
+                                                    const T* __restrict__ g_chosen,
+                                                    int64_t tokens, int experts, int slots,
+                                                    T* __restrict__ g_weights) {
+  const int64_t n = tokens * experts, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const int64_t t = i / experts;
+    const int e = (int)(i - t * experts);
+    T g = (T)0;
+    for (int j = 0; j < slots; ++j)
+      if (ids[t * slots + j] == e) g = g_chosen[t * slots + j];
+    g_weights[i] = g;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// sorting pairs by expert
+// ---------------------------------------------------------------------------
+
+// Experts given by the caller, with -1 for what names none.
+template <typename I>
+__global__ __launch_bounds__(256) void k_ids(const I* __restrict__ given, int64_t pairs,
+                                             int experts, int32_t* __restrict__ ids) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= pairs) return;
+  const I e = given[i];
+  ids[i] = e >= 0 && e < experts ? (int32_t)e : -1;
+}
+
+// counts[g][e]: the pairs of chunk g that go to expert e.
+__global__ __launch_bounds__(kSortThreads) void k_sort_count(const int32_t* __restrict__ ids,
+                                                             int64_t pairs, int experts,
+                                                             int64_t chunk,
+                                                             int32_t* __restrict__ counts) {
+  __shared__ int32_t hist[PURIN_TRAIN_MAX_EXPERTS];
+  for (int e = threadIdx.x; e < experts; e += kSortThreads) hist[e] = 0;
+  __syncthreads();
+  const int64_t from = (int64_t)blockIdx.x * chunk, to = min(pairs, from + chunk);
+  for (int64_t i = from + threadIdx.x; i < to; i += kSortThreads) {
+    const int32_t e = ids[i];
+    if (e >= 0) atomicAdd(&hist[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kSortThreads)
+    counts[(int64_t)blockIdx.x * experts + e] = hist[e];
+}
+
+// Places the pairs of one chunk: expert e's rows begin at the sum of all smaller experts'
+// counts; the chunk's first pair of e follows the earlier chunks' pairs of e, a wavefront's
+// first the earlier wavefronts'.  LDS: per-wavefront running places [kSortWaves][experts].
+__global__ __launch_bounds__(kSortThreads) void k_sort_place(
+    const int32_t* __restrict__ ids, int64_t pairs, int experts, int bits, int64_t chunk,
+    const int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
+    int32_t* __restrict__ place, int32_t* __restrict__ source) {
+  extern __shared__ int32_t run[];
+  __shared__ int32_t total[PURIN_TRAIN_MAX_EXPERTS];
+  __shared__ int32_t before[PURIN_TRAIN_MAX_EXPERTS];
+  __shared__ int32_t wave_sum[kSortWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int groups = (int)gridDim.x, group = (int)blockIdx.x;
+  for (int e = tid; e < experts; e += kSortThreads) total[e] = before[e] = 0;
+  for (int i = tid; i < kSortWaves * experts; i += kSortThreads) run[i] = 0;
+  __syncthreads();
+  const int64_t from = (int64_t)group * chunk, to = min(pairs, from + chunk);
+  const int64_t part = chunk / kSortWaves;  // a multiple of 64
+  const int64_t wfrom = from + wave * part, wto = min(to, wfrom + part);
+  int32_t* mine = run + wave * experts;
+  for (int64_t i = wfrom + lane; i < wto; i += 64) {
+    const int32_t e = ids[i];
+    if (e >= 0) atomicAdd(&mine[e], 1);
+  }
+  if (groups > 1) {
+    const int n = groups * experts;
+    for (int i = tid; i < n; i += kSortThreads) {
+      const int32_t c = counts[i];
+      const int g = i / experts, e = i - g * experts;
+      if (c) {
+        atomicAdd(&total[e], c);
+        if (g < group) atomicAdd(&before[e], c);
+      }
+    }
+  }
+  __syncthreads();
+  if (groups == 1) {
+    for (int e = tid; e < experts; e += kSortThreads) {
+      int32_t s = 0;
+      for (int w = 0; w < kSortWaves; ++w) s += run[w * experts + e];
+      total[e] = s;
+    }
+    __syncthreads();
+  }
+  // exclusive sums of the totals over the experts (at most one expert to a thread)
+  int32_t mine_total = tid < experts ? total[tid] : 0;
+  int32_t sum = mine_total;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t up = __shfl_up(sum, d, 64);
+    if (lane >= d) sum += up;
+  }
+  if (lane == 63) wave_sum[wave] = sum;
+  __syncthreads();
+  int32_t base = 0, all = 0;
+  for (int w = 0; w < kSortWaves; ++w) {
+    const int32_t s = wave_sum[w];
+    if (w < wave) base += s;
+    all += s;
+  }
+  if (tid < experts) {
+    const int32_t first = base + sum - mine_total;
+    if (group == 0) {
+      offsets[tid] = first;
+      if (tid == experts - 1) offsets[experts] = all;
+    }
+    int32_t next = first + before[tid];
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int32_t c = run[w * experts + tid];
+      run[w * experts + tid] = next;
+      next += c;
+    }
+  }
+  __syncthreads();
+  volatile int32_t* next = mine;  // this wavefront's alone
+  for (int64_t i0 = wfrom; i0 < wto; i0 += 64) {
+    const int64_t i = i0 + lane;
+    const int32_t e = i < wto ? ids[i] : -1;
+    const uint32_t key = e >= 0 ? (uint32_t)e : (uint32_t)experts;
+    uint64_t same = ~0ull;
+    for (int b = 0; b < bits; ++b) {
+      const bool on = (key >> b) & 1u;
+      const uint64_t votes = __ballot(on);
+      same &= on ? votes : ~votes;
+    }
+    int32_t p = -1;
+    const int rank = __popcll(same & ((1ull << lane) - 1ull));
+    if (e >= 0) p = next[e] + rank;
+    __builtin_amdgcn_wave_barrier();
+    if (e >= 0 && rank == 0) next[e] = p + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    if (i < wto) {
+      place[i] = p;
+      if (e >= 0) source[p] = (int32_t)i;
+    }
+  }
+  // the rows that no pair has
+  for (int64_t i = max<int64_t>(from, all) + tid; i < to; i += kSortThreads) source[i] = -1;
+}
+
+static int sort_pairs(hipStream_t st, int64_t pairs, int experts, const int32_t* ids, void* ws,
+                      int32_t* offsets, int32_t* place, int32_t* source) {
+  const SortShape s = sort_shape(pairs);
+  int bits = 1;
+  while ((1 << bits) <= experts) ++bits;  // the key ``experts`` stands for none
+  if (s.groups > 1) {
+    k_sort_count<<<dim3((unsigned)s.groups), dim3(kSortThreads), 0, st>>>(
+        ids, pairs, experts, s.chunk, (int32_t*)ws);
+    if (int rc = launched("k_sort_count")) return rc;
+  }
+  const size_t lds = (size_t)kSortWaves * experts * sizeof(int32_t);
+  if (lds > 32 * 1024)
+    if (int rc = raise_lds_cap((const void*)k_sort_place, lds)) return rc;
+  k_sort_place<<<dim3((unsigned)s.groups), dim3(kSortThreads), lds, st>>>(
+      ids, pairs, experts, bits, s.chunk, (const int32_t*)ws, offsets, place, source);
+  return launched("k_sort_place");
+}
+
+// ---------------------------------------------------------------------------
+// moving rows
+// ---------------------------------------------------------------------------
+
+// Threads of a workgroup: cx along a row's 16-byte vectors, 256 / cx tokens.
+static int row_threads(int64_t width, int vec) {
+  const int64_t n = (width + vec - 1) / vec;
+  int cx = 8;
+  while (cx < 256 && cx < n) cx *= 2;
+  return cx;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_dispatch(const T* __restrict__ x, int64_t ldx,
+                                                  int64_t tokens, int slots, int64_t width,
+                                                  int cx, int64_t pairs,
+                                                  const int32_t* __restrict__ total,
+                                                  const int32_t* __restrict__ place,
+                                                  T* __restrict__ rows) {
+  const int tx = threadIdx.x % cx;
+  const int64_t last = max(*total, 0), step = (int64_t)gridDim.x * (256 / cx);
+  for (int64_t t = (int64_t)blockIdx.x * (256 / cx) + threadIdx.x / cx; t < tokens; t += step) {
+    const int32_t* at = place + t * slots;
+    for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
+      const Pack<T> v = load_upto(x + t * ldx + c, width - c);
+      for (int j = 0; j < slots; ++j) {
+        const int64_t p = at[j];
+        if (p >= 0 && p < pairs) store_upto(rows + p * width + c, v, width - c);
+      }
+      // the rows that no pair has, shared out over the tokens
+      for (int64_t p = last + t; p < pairs; p += tokens)
+        store_upto(rows + p * width + c, zeros16<T>(), width - c);
+    }
+  }
+}
+
+template <typename T, bool WEIGHTED>
+__global__ __launch_bounds__(256) void k_combine(const T* __restrict__ rows, int64_t ldr,
+                                                 int64_t tokens, int slots, int64_t width, int cx,
+                                                 int64_t pairs, const int32_t* __restrict__ place,
+                                                 const void* __restrict__ weights, int32_t wdtype,
+                                                 T* __restrict__ out) {
+  using A = typename Elem<T>::Acc;
+  constexpr int B = 4;  // rows in flight
+  const int tx = threadIdx.x % cx;
+  const int64_t step = (int64_t)gridDim.x * (256 / cx);
+  for (int64_t t = (int64_t)blockIdx.x * (256 / cx) + threadIdx.x / cx; t < tokens; t += step)
+  for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
+    A sum[kVec<T>];
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) sum[i] = A(0);
+    for (int j0 = 0; j0 < slots; j0 += B) {
+      Pack<T> v[B];
+      A w[B];
+      bool in[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const int64_t p = j0 + b < slots ? place[t * slots + j0 + b] : -1;
+        in[b] = p >= 0 && p < pairs;
+        w[b] = A(1);
+        if (in[b]) {
+          v[b] = load_upto(rows + p * ldr + c, width - c);
+          if constexpr (WEIGHTED) w[b] = load_weight<A>(weights, wdtype, t * slots + j0 + b);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (in[b]) {
+#pragma unroll
+          for (int i = 0; i < kVec<T>; ++i) {
+            if constexpr (WEIGHTED) sum[i] += w[b] * (A)v[b].v[i];
+            else sum[i] += (A)v[b].v[i];
+          }
+        }
+    }
+    Pack<T> r;
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)sum[i];
+    store_upto(out + t * width + c, r, width - c);
+  }
+}
+
+// g lanes (a power of two up to 64) to a token.
+template <typename T>
+__global__ __launch_bounds__(256) void k_combine_vjp(
+    const T* __restrict__ g_out, int64_t ldg, const T* __restrict__ rows, int64_t ldr,
+    int64_t tokens, int slots, int64_t width, int g, int64_t pairs,
+    const int32_t* __restrict__ total, const int32_t* __restrict__ place,
+    const void* __restrict__ weights, int32_t wdtype, T* __restrict__ g_rows,
+    void* __restrict__ g_weights) {
+  using A = typename Elem<T>::Acc;
+  constexpr int B = 4;  // slots at once
+  const int tx = threadIdx.x % g;
+  const int64_t last = max(*total, 0), step = (int64_t)gridDim.x * (256 / g);
+  // a token's lanes stay together, so the exchanges below are whole
+  for (int64_t t = (int64_t)blockIdx.x * (256 / g) + threadIdx.x / g; t < tokens; t += step) {
+    for (int j0 = 0; j0 < slots; j0 += B) {
+      A w[B], dot[B];
+      int64_t at[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const int64_t p = j0 + b < slots ? place[t * slots + j0 + b] : -1;
+        at[b] = p < pairs ? p : -1;
+        dot[b] = w[b] = A(0);
+        if (at[b] >= 0) w[b] = load_weight<A>(weights, wdtype, t * slots + j0 + b);
+      }
+      for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)g * kVec<T>) {
+        const int64_t n = width - c;
+        const Pack<T> go = load_upto(g_out + t * ldg + c, n);
+        Pack<T> y[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+          if (g_weights && at[b] >= 0) y[b] = load_upto(rows + at[b] * ldr + c, n);
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          if (at[b] < 0) continue;
+          if (g_weights) {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) dot[b] += (A)go.v[i] * (A)y[b].v[i];
+          }
+          if (g_rows) {
+            Pack<T> r;
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)(w[b] * (A)go.v[i]);
+            store_upto(g_rows + at[b] * width + c, r, n);
+          }
+        }
+      }
+      if (g_weights) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          for (int m = g >> 1; m > 0; m >>= 1) dot[b] += __shfl_xor(dot[b], m, 64);
+          if (tx == 0 && j0 + b < slots)
+            store_weight<A>(g_weights, wdtype, t * slots + j0 + b, dot[b]);
+        }
+      }
+    }
+    if (g_rows)
+      for (int64_t p = last + t; p < pairs; p += tokens)
+        for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)g * kVec<T>)
+          store_upto(g_rows + p * width + c, zeros16<T>(), width - c);
+  }
+}
+
+static int check_pairs(int64_t tokens, int64_t experts, int64_t slots) {
+  if (tokens < 0 || experts < 1 || slots < 1)
+    return refuse("tokens must not be negative, experts and slots must be positive");
+  if (experts > PURIN_TRAIN_MAX_EXPERTS)
+    return set_error(PURIN_CP_ERR_UNSUPPORTED, "more than 1024 experts");
+  if (tokens >= (int64_t(1) << 31) || tokens * slots >= (int64_t(1) << 31))
+    return set_error(PURIN_CP_ERR_UNSUPPORTED, "tokens * slots must stay below 2^31");
+  return PURIN_CP_OK;
+}
+
+}  // namespace train
+}  // namespace purin
+
+using namespace purin;
+using namespace purin::train;
+
+extern "C" {
+
+int64_t purin_train_route_workspace_bytes(int64_t tokens, int64_t experts, int64_t slots) {
+  int64_t need = -1;
+  (void)guarded([&] {
+    if (int rc = check_pairs(tokens, experts, slots)) return rc;
+    const SortShape s = sort_shape(tokens * slots);
+    need = s.groups > 1 ? s.groups * experts * (int64_t)sizeof(int32_t) : 0;
+    return (int)PURIN_CP_OK;
+  });
+  return need;
+}
+
+int purin_train_route(void* stream, int32_t dtype, int64_t tokens, int64_t experts, int64_t slots,
+                      const void* weights, int64_t ld, void* workspace, int64_t workspace_bytes,
+                      int32_t* ids, void* chosen, int32_t* offsets, int32_t* place,
+                      int32_t* source) {
+  return guarded([&] {
+    if (int rc = check_pairs(tokens, experts, slots)) return rc;
+    if (!known_dtype(dtype)) return refuse("unknown dtype");
+    if (slots > experts) return refuse("slots must not exceed experts");
+    if (!offsets || (tokens && (!weights || !ids || !chosen || !place || !source)))
+      return refuse("NULL array");
+    if (ld < experts && tokens > 1) return refuse("the weights' row pitch is below experts");
+    if (int rc = check_workspace(workspace, workspace_bytes,
+                                 purin_train_route_workspace_bytes(tokens, experts, slots)))
+      return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (tokens) {
+      const int rc = by_dtype(dtype, [&](auto x) {
+        using T = decltype(x);
+        return choose_experts<T>(st, (const T*)weights, ld, tokens, (int)experts, (int)slots, ids,
+                                 (T*)chosen);
+      });
+      if (rc) return rc;
+    }
+    return sort_pairs(st, tokens * slots, (int)experts, ids, workspace, offsets, place, source);
+  });
+}
+
+int purin_train_sort(void* stream, int32_t wide, int64_t tokens, int64_t experts, int64_t slots,
+                     const void* given, void* workspace, int64_t workspace_bytes, int32_t* ids,
+                     int32_t* offsets, int32_t* place, int32_t* source) {
+  return guarded([&] {
+    if (int rc = check_pairs(tokens, experts, slots)) return rc;
+    const int64_t pairs = tokens * slots;
+    if (!offsets || (pairs && (!given || !ids || !place || !source))) return refuse("NULL array");
+    if (int rc = check_workspace(workspace, workspace_bytes,
+                                 purin_train_route_workspace_bytes(tokens, experts, slots)))
+      return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (pairs) {
+      const dim3 grid((unsigned)((pairs + 255) / 256));
+      if (wide)
+        k_ids<int64_t><<<grid, dim3(256), 0, st>>>((const int64_t*)given, pairs, (int)experts, ids);
+      else
+        k_ids<int32_t><<<grid, dim3(256), 0, st>>>((const int32_t*)given, pairs, (int)experts, ids);
+      if (int rc = launched("k_ids")) return rc;
+    }
+    return sort_pairs(st, pairs, (int)experts, ids, workspace, offsets, place, source);
+  });
+}
+
+int purin_train_route_vjp(void* stream, int32_t dtype, int64_t tokens, int64_t experts,
+                          int64_t slots, const int32_t* ids, const void* g_chosen,
+                          void* g_weights) {
+  return guarded([&] {
+    if (int rc = check_pairs(tokens, experts, slots)) return rc;
+    if (!known_dtype(dtype)) return refuse("unknown dtype");
+    if (!tokens) return (int)PURIN_CP_OK;
+    if (!ids || !g_chosen || !g_weights) return refuse("NULL array");
+    return by_dtype(dtype, [&](auto x) {
+      using T = decltype(x);
+      const int64_t n = tokens * experts;
+      k_choose_vjp<T><<<grid_of(n, 256), dim3(256), 0, (hipStream_t)stream>>>(
+          ids, (const T*)g_chosen, tokens, (int)experts, (int)slots, (T*)g_weights);
+      return launched("k_choose_vjp");
+    });
+  });
+}
+
+int purin_train_dispatch(void* stream, int32_t dtype, int64_t tokens, int64_t experts,
+                         int64_t slots, int64_t width, const void* x, int64_t ldx,
+                         const int32_t* offsets, const int32_t* place, void* rows) {
+  return guarded([&] {
+    if (int rc = check_pairs(tokens, experts, slots)) return rc;
+    if (!known_dtype(dtype)) return refuse("unknown dtype");
+    if (width < 0) return refuse("width must not be negative");
+    if (!tokens || !width) return (int)PURIN_CP_OK;
+    if (!x || !offsets || !place || !rows) return refuse("NULL array");
+    if (ldx < width && tokens > 1) return refuse("a row pitch is below the width");
+    return by_dtype(dtype, [&](auto v) {
+      using T = decltype(v);
+      const int cx = row_threads(width, kVec<T>);
+      k_dispatch<T><<<grid_of(tokens, 256 / cx), dim3(256), 0, (hipStream_t)stream>>>((const T*)x, ldx, tokens, (int)slots, width, cx,
+                                             tokens * slots, offsets + experts, place, (T*)rows);
+      return launched("k_dispatch");
+    });
+  });
+}
+
+int purin_train_combine(void* stream, int32_t dtype, int32_t wdtype, int64_t tokens,
+                        int64_t slots, int64_t width, const void* rows, int64_t ldr,
+                        const int32_t* place, const void* weights, void* out) {
+  return guarded([&] {
+    if (int rc = check_pairs(tokens, 1, slots)) return rc;
+    if (!known_dtype(dtype) || (weights && !known_dtype(wdtype))) return refuse("unknown dtype");
+    if (width < 0) return refuse("width must not be negative");
+    if (!tokens || !width) return (int)PURIN_CP_OK;
+    if (!rows || !place || !out) return refuse("NULL array");
+    if (ldr < width && tokens * slots > 1) return refuse("a row pitch is below the width");
+    return by_dtype(dtype, [&](auto v) {
+      using T = decltype(v);
+      const int cx = row_threads(width, kVec<T>);
+      const dim3 grid = grid_of(tokens, 256 / cx);
+      if (weights)
+        k_combine<T, true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
+            (const T*)rows, ldr, tokens, (int)slots, width, cx, tokens * slots, place, weights,
+            wdtype, (T*)out);
+      else
+        k_combine<T, false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
+            (const T*)rows, ldr, tokens, (int)slots, width, cx, tokens * slots, place, nullptr, 0,
+            (T*)out);
+      return launched("k_combine");
+    });
+  });
+}
+
+int purin_train_combine_vjp(void* stream, int32_t dtype, int32_t wdtype, int64_t tokens,
+                            int64_t experts, int64_t slots, int64_t width, const void* g_out,
+                            int64_t ldg, const void* rows, int64_t ldr, const int32_t* offsets,
+                            const int32_t* place, const void* weights, void* g_rows,
+                            void* g_weights) {
+  return guarded([&] {
+    if (int rc = check_pairs(tokens, experts, slots)) return rc;
+    if (!known_dtype(dtype) || !known_dtype(wdtype)) return refuse("unknown dtype");
+    if (width < 0) return refuse("width must not be negative");
+    if (!tokens || (!g_rows && !g_weights)) return (int)PURIN_CP_OK;
+    if (!offsets || !place || !weights || (width && (!g_out || (g_weights && !rows))))
+      return refuse("NULL array");
+    if ((ldg < width && tokens > 1) || (g_weights && ldr < width && tokens * slots > 1))
+      return refuse("a row pitch is below the width");
+    return by_dtype(dtype, [&](auto v) {
+      using T = decltype(v);
+      const int g = std::min(64, row_threads(width, kVec<T>));
+      k_combine_vjp<T><<<grid_of(tokens, 256 / g), dim3(256), 0, (hipStream_t)stream>>>(
+          (const T*)g_out, ldg, (const T*)rows, ldr, tokens, (int)slots, width, g, tokens * slots,
+          offsets + experts, place, weights, wdtype, (T*)g_rows, g_weights);
+      return launched("k_combine_vjp");
+    });
+  });
+}
+
+}  // extern "C"
