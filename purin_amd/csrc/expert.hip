@@ -11,13 +11,12 @@
 
 #include <algorithm>
 
+#include "expert16.hpp"
 #include "train.hpp"
 
 namespace purin {
 namespace train {
 
-typedef bf16 B8 __attribute__((ext_vector_type(8)));
-typedef f16 H8 __attribute__((ext_vector_type(8)));
 typedef float F4 __attribute__((ext_vector_type(4)));
 typedef double D4 __attribute__((ext_vector_type(4)));
 
@@ -220,6 +219,119 @@ __global__ __launch_bounds__(256) void k_weights_vjp(const T* __restrict__ a, in
                   to - from, gw + e * inner * outer + i * outer + j, outer);
 }
 
+// 16-bit types: BM x BN tiles in 1-D order, XCD by XCD (workgroups are dealt to the 8 XCDs in
+// turn, so number i is on XCD i % 8): an XCD's workgroups take neighbouring tiles, kGroup rows
+// of tiles at a time, and find each other's operands in its L2.
+constexpr int kGroup = 4;
+__device__ __forceinline__ void tile_order(int64_t tiles_m, int64_t tiles_n, int64_t& tm,
+                                           int64_t& tn) {
+  const int64_t n = tiles_m * tiles_n, per = (n + 7) / 8, id = blockIdx.x;
+  int64_t at = (id & 7) * per + (id >> 3);
+  const int64_t whole = n - (per - 1) * 8;  // XCDs that have per tiles, the others one fewer
+  if ((id & 7) > whole) at -= (id & 7) - whole;
+  const int64_t group = at / (kGroup * tiles_n), first = group * kGroup;
+  const int64_t high = min<int64_t>(kGroup, tiles_m - first), in = at - first * tiles_n;
+  tm = first + in % high;
+  tn = in / high;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool ALONG_B, bool DIRECT>
+__global__ __launch_bounds__(WM* WN * 64) void k_product16(
+    const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
+    int64_t rows, int64_t inner, int64_t outer, int experts, int64_t tiles_m, int64_t tiles_n,
+    const int32_t* __restrict__ offsets, T* __restrict__ out, int64_t ldo) {
+  extern __shared__ __align__(16) unsigned char lds16[];
+  int64_t tm, tn;
+  tile_order(tiles_m, tiles_n, tm, tn);
+  int e;
+  int64_t from, to;
+  if (!find_tile(offsets, experts, rows, BM, tm, e, from, to)) return;
+  e = __builtin_amdgcn_readfirstlane(e);
+  const int64_t col = tn * BN;
+  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
+  const int n = (int)min<int64_t>(BN, outer - col);
+  if (e < 0) {
+    for (int r = threadIdx.x; r < m * (BN / 8); r += WM * WN * 64) {
+      const int i = r / (BN / 8), j = r % (BN / 8) * 8;
+      if (j < n) store_upto(out + (from + i) * ldo + col + j, zeros16<T>(), n - j);
+    }
+    return;
+  }
+  tile16<T, BM, BN, WM, WN, true, ALONG_B, DIRECT>(
+      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner,
+      (T*)lds16, out + from * ldo + col, ldo);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(WM* WN * 64) void k_weights_vjp16(
+    const T* __restrict__ a, int64_t lda, const T* __restrict__ g, int64_t ldg, int64_t rows,
+    int64_t inner, int64_t outer, int64_t tiles_m, int64_t tiles_n,
+    const int32_t* __restrict__ offsets, T* __restrict__ gw) {
+  extern __shared__ __align__(16) unsigned char lds16[];
+  int64_t tm, tn;
+  tile_order(tiles_m, tiles_n, tm, tn);
+  const int e = (int)blockIdx.y;
+  int64_t from, to;
+  segment(offsets, e, rows, from, to);
+  const int64_t i = tm * BM, j = tn * BN;
+  tile16<T, BM, BN, WM, WN, false, false, DIRECT>(
+      {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i)},
+      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, to - from, (T*)lds16,
+      gw + e * inner * outer + i * outer + j, outer);
+}
+
+template <typename K, typename... A>
+static int launch16(const char* name, K kernel, dim3 grid, int threads, int lds, hipStream_t st,
+                    A... args) {
+  if (int rc = raise_lds_cap((const void*)kernel, (size_t)lds)) return rc;
+  kernel<<<grid, dim3((unsigned)threads), (size_t)lds, st>>>(args...);
+  return launched(name);
+}
+
+// Whether 16-byte pieces of rows ``ld`` elements apart lie at 16-byte addresses, all of a row's
+// length, and the rows of one stage (at most 256) are within 31 bits of its first.
+static bool direct_ok(const void* p, int64_t ld, int64_t length) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && length % 8 == 0 &&
+         ld < (int64_t(1) << 21);
+}
+
+template <typename T>
+static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
+                     const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,
+                     const int32_t* offsets, T* out, int64_t ldo) {
+  constexpr int BM = 256, BN = 256;
+  const bool along = wi == 1 && (wo != 1 || inner > 1);
+  const int64_t ldw = along ? wo : wi;
+  const bool direct = direct_ok(a, lda, inner) && direct_ok(w, ldw, along ? inner : outer) &&
+                      we % 8 == 0;
+  const int64_t tm = (rows + BM - 1) / BM + experts, tn = (outer + BN - 1) / BN;
+  auto go = [&](auto kernel) {
+    return launch16("k_product16", kernel, dim3((unsigned)(tm * tn)), 512,
+                    2 * (BM + BN) * kDepth16 * 2, st, a, lda, w, we, ldw, rows, inner, outer,
+                    (int)experts, tm, tn, offsets, out, ldo);
+  };
+  if (along) return direct ? go(k_product16<T, BM, BN, 2, 4, true, true>)
+                           : go(k_product16<T, BM, BN, 2, 4, true, false>);
+  return direct ? go(k_product16<T, BM, BN, 2, 4, false, true>)
+                : go(k_product16<T, BM, BN, 2, 4, false, false>);
+}
+
+template <typename T>
+static int weights_vjp16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
+                         int64_t experts, const T* a, int64_t lda, const T* g, int64_t ldg,
+                         const int32_t* offsets, T* gw) {
+  constexpr int BM = 256, BN = 256;
+  const bool direct = direct_ok(a, lda, inner) && direct_ok(g, ldg, outer);
+  const int64_t tm = (inner + BM - 1) / BM, tn = (outer + BN - 1) / BN;
+  auto go = [&](auto kernel) {
+    return launch16("k_weights_vjp16", kernel, dim3((unsigned)(tm * tn), (unsigned)experts), 512,
+                    2 * (BM + BN) * kDepth16 * 2, st, a, lda, g, ldg, rows, inner, outer, tm, tn,
+                    offsets, gw);
+  };
+  return direct ? go(k_weights_vjp16<T, BM, BN, 2, 4, true>)
+                : go(k_weights_vjp16<T, BM, BN, 2, 4, false>);
+}
+
 static int check_product(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
                          int64_t experts) {
   if (!known_dtype(dtype)) return refuse("unknown dtype");
@@ -270,6 +382,9 @@ int purin_train_expert_product(void* stream, int32_t dtype, int64_t rows, int64_
     if (we < 0 || wi < 0 || wo < 0) return refuse("the weight's strides must not be negative");
     return by_dtype(dtype, [&](auto v) {
       using T = decltype(v);
+      if constexpr (sizeof(T) == 2)
+        return product16<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
+                            (const T*)weight, we, wi, wo, offsets, (T*)out, ldo);
       const dim3 grid((unsigned)((rows + kTile - 1) / kTile + experts),
                       (unsigned)((outer + kTile - 1) / kTile));
       k_product<T><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
@@ -303,6 +418,9 @@ int purin_train_expert_weights_vjp(void* stream, int32_t dtype, int64_t rows, in
       return refuse("a row pitch is below the row's length");
     return by_dtype(dtype, [&](auto v) {
       using T = decltype(v);
+      if constexpr (sizeof(T) == 2)
+        return weights_vjp16<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
+                                (const T*)g, ldg, offsets, (T*)g_weight);
       const dim3 grid((unsigned)((inner + kTile - 1) / kTile),
                       (unsigned)((outer + kTile - 1) / kTile), (unsigned)experts);
       k_weights_vjp<T><<<grid, dim3(256), 0, (hipStream_t)stream>>>(

@@ -1,0 +1,269 @@
+// Tiles of the experts' products in 16-bit types on the matrix units: c = sum over k of
+// a(i, k) b(j, k), sums in 32 bits, for a workgroup's BM x BN tile.
+//
+// The operands pass through LDS kDepth16 of the contraction at a time, two stages, the next one
+// loading while the present one is multiplied.  A stage of an operand whose contraction is
+// contiguous in memory is [i][k]; one whose rows are contiguous is [k][i], and is transposed by
+// the LDS reads themselves (ds_read_b64_tr_b16: 16 lanes read a 4 x 16 block and get its
+// columns).  Both are stored in 16-byte pieces whose places are exchanged by an XOR, so that the
+// lanes of one read fall on different banks:
+//   [i][k]   piece k / 8 of row i at (k / 8) ^ (i % 8): 8 rows' reads of one piece cover all banks
+//   [k][i]   pair i / 16 of row k at (i / 16) ^ s(k), s(k) = 2 (k % 4) + (k / 8) % 2: the 8
+//            blocks of 32 bytes that half a wavefront reads at once fall on 8 places
+// With 16-byte rows at 16-byte addresses the stages are loaded straight into LDS (buffer loads
+// whose addresses outside the operand read zeros); others pass through registers.
+#pragma once
+
+#include "train.hpp"
+
+namespace purin {
+namespace train {
+
+typedef bf16 B8 __attribute__((ext_vector_type(8)));
+typedef f16 H8 __attribute__((ext_vector_type(8)));
+typedef short S4 __attribute__((ext_vector_type(4)));
+typedef short S8 __attribute__((ext_vector_type(8)));
+typedef float F16x __attribute__((ext_vector_type(16)));
+
+constexpr int kDepth16 = 64;
+
+__device__ __forceinline__ F16x mma32(bf16, S8 a, S8 b, F16x c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(B8, a),
+                                                 __builtin_bit_cast(B8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ F16x mma32(f16, S8 a, S8 b, F16x c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(H8, a),
+                                                __builtin_bit_cast(H8, b), c, 0, 0, 0);
+}
+
+typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+
+// A pointer that is the same in all lanes, in scalar registers.
+template <typename T>
+__device__ __forceinline__ const T* uniform(const T* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+  return reinterpret_cast<const T*>(((uint64_t)hi << 32) | lo);
+}
+// A buffer descriptor of 2 GiB from p on: reads beyond give zeros.
+template <typename T>
+__device__ __forceinline__ U4 buffer_at(const T* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  return U4{(uint32_t)u, (uint32_t)(u >> 32) & 0xffffu, 0x7ffffff0u, 0x00020000u};
+}
+template <typename T>
+__device__ __forceinline__ uint32_t lds_address(const T* lds) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) T*)lds;
+}
+// 16 bytes a lane from the buffer to ``to`` + 16 * lane in LDS.  Written out, without an output
+// register: the compiler would have every later LDS read wait for it, also one of the other
+// stage.  The loop waits for its stage itself.  (M0 holds the place; nothing else in these
+// kernels uses it.)
+__device__ __forceinline__ void load_to_lds(U4 r, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)to)), "v"(at), "s"(r)
+               : "memory");
+}
+
+// An operand of a tile: element (i, k) at p + i * ld + k where its contraction is contiguous
+// (ALONG), at p + k * ld + i where its rows are; n rows are there.
+template <typename T>
+struct Side {
+  const T* p;
+  int64_t ld;
+  int n;
+};
+
+template <typename T, int N, bool ALONG, int THREADS, bool DIRECT>
+struct Stage {
+  static constexpr int kPieces = N * kDepth16 / 8;  // 16 bytes each
+  static constexpr int kMine = kPieces / THREADS;
+  static constexpr int kElems = N * kDepth16;
+  static_assert(kPieces % THREADS == 0, "whole pieces per thread");
+
+  // piece number m of this thread: its row (i or k) and its 8 elements' first (k or i)
+  static __device__ __forceinline__ void piece(int m, int& row, int& first) {
+    const int at = m * THREADS + (int)threadIdx.x;
+    if constexpr (ALONG) {
+      row = at >> 3;
+      first = ((at & 7) ^ (row & 7)) * 8;
+    } else {
+      constexpr int per = N / 8;
+      row = at / per;
+      const int c = at % per, s = 2 * (row & 3) + ((row >> 3) & 1);
+      first = ((((c >> 1) ^ s) << 1) | (c & 1)) * 8;
+    }
+  }
+
+  // byte offsets of this thread's pieces from the stage's first element; ~0 outside the rows
+  static __device__ __forceinline__ void offsets(const Side<T>& o, uint32_t (&off)[kMine]) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      int row, first;
+      piece(m, row, first);
+      const bool in = (ALONG ? row : first) < o.n;
+      off[m] = in ? (uint32_t)(row * (int)o.ld + first) * 2u : 0x80000000u;
+    }
+  }
+
+  // straight into LDS; ``left``: what is left of the contraction
+  static __device__ __forceinline__ void load_lds(const T* p, const uint32_t (&off)[kMine],
+                                                  int64_t left, T* lds) {
+    const U4 r = buffer_at(p);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      uint32_t at = off[m];
+      if (left < kDepth16) {
+        int row, first;
+        piece(m, row, first);
+        if ((ALONG ? first : row) >= left) at = 0x80000000u;
+      }
+      load_to_lds(r, at, lds_address(lds) + (uint32_t)(m * THREADS + wave * 64) * 16u);
+    }
+  }
+
+  // through registers: any alignment, rows and a contraction of any length
+  static __device__ __forceinline__ void load_regs(const Side<T>& o, const T* p, int64_t left,
+                                                   Pack<T> (&v)[kMine]) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      int row, first;
+      piece(m, row, first);
+      const int64_t rows = ALONG ? o.n : left, cols = ALONG ? left : o.n;
+      const T* q = p + row * o.ld + first;
+      if (row >= rows || first >= cols) v[m] = zeros16<T>();
+      else v[m] = load_upto(q, cols - first);
+    }
+  }
+  static __device__ __forceinline__ void store_lds(const Pack<T> (&v)[kMine], T* lds) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m)
+      *reinterpret_cast<S8*>(lds + (m * THREADS + (int)threadIdx.x) * 8) =
+          __builtin_bit_cast(S8, v[m]);
+  }
+};
+
+// The matrix units' operand of rows i0 + lane % 32 and contraction 16 * s + 8 * (lane / 32) + 0..7.
+template <typename T, int N, bool ALONG>
+__device__ __forceinline__ S8 fragment(const T* lds, int i0, int s) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (ALONG) {
+    const int i = i0 + (lane & 31);
+    return *reinterpret_cast<const S8*>(lds + i * kDepth16 + (((2 * s + (lane >> 5)) ^ (lane & 7)) << 3));
+  } else {
+    const int k = 16 * s + 8 * (lane >> 5) + ((lane & 15) >> 2);
+    const int swap = 2 * ((lane & 15) >> 2) + (lane >> 5);
+    const int pair = ((i0 >> 4) + ((lane >> 4) & 1)) ^ swap;
+    const T* at = lds + k * N + pair * 16 + (lane & 3) * 4;
+    using L = __attribute__((address_space(3))) S4;
+    const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)at);
+    const S4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(at + 4 * N));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// A workgroup of WM * WN wavefronts; ``lds`` holds 2 * (BM + BN) * kDepth16 elements.
+template <typename T, int BM, int BN, int WM, int WN, bool ALONG_A, bool ALONG_B, bool DIRECT>
+__device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, T* lds, T* c,
+                                       int64_t ldc) {
+  constexpr int THREADS = WM * WN * 64, X = BM / WM / 32, Y = BN / WN / 32;
+  using SA = Stage<T, BM, ALONG_A, THREADS, DIRECT>;
+  using SB = Stage<T, BN, ALONG_B, THREADS, DIRECT>;
+  constexpr int kStage = SA::kElems + SB::kElems;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
+  F16x acc[X][Y];
+#pragma unroll
+  for (int x = 0; x < X; ++x)
+#pragma unroll
+    for (int y = 0; y < Y; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+  uint32_t off_a[SA::kMine], off_b[SB::kMine];
+  Pack<T> va[SA::kMine], vb[SB::kMine];
+  if constexpr (DIRECT) {
+    SA::offsets(a, off_a);
+    SB::offsets(b, off_b);
+  }
+  const T *pa = uniform(a.p), *pb = uniform(b.p);
+  int64_t left = depth;
+  auto load = [&](T* to) {
+    if constexpr (DIRECT) {
+      SA::load_lds(pa, off_a, left, to);
+      SB::load_lds(pb, off_b, left, to + SA::kElems);
+    } else {
+      SA::load_regs(a, pa, left, va);
+      SB::load_regs(b, pb, left, vb);
+    }
+    pa += ALONG_A ? kDepth16 : kDepth16 * a.ld;
+    pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
+    left -= kDepth16;
+  };
+  auto put = [&](T* to) {
+    if constexpr (!DIRECT) {
+      SA::store_lds(va, to);
+      SB::store_lds(vb, to + SA::kElems);
+    }
+  };
+  if (depth > 0) {
+    load(lds);
+    put(lds);
+  }
+  int64_t steps = (depth + kDepth16 - 1) / kDepth16;
+  T *now = lds, *next = lds + kStage;
+  for (int64_t t = 0; t < steps; ++t) {
+    if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this stage is in LDS
+    __syncthreads();
+    if (t + 1 < steps) load(next);
+    const T *la = now, *lb = now + SA::kElems;
+#pragma unroll
+    for (int s = 0; s < kDepth16 / 16; ++s) {
+      S8 fa[X], fb[Y];
+#pragma unroll
+      for (int x = 0; x < X; ++x) fa[x] = fragment<T, BM, ALONG_A>(la, wi + 32 * x, s);
+#pragma unroll
+      for (int y = 0; y < Y; ++y) fb[y] = fragment<T, BN, ALONG_B>(lb, wj + 32 * y, s);
+#pragma unroll
+      for (int x = 0; x < X; ++x)
+#pragma unroll
+        for (int y = 0; y < Y; ++y) acc[x][y] = mma32(T{}, fb[y], fa[x], acc[x][y]);
+    }
+    if (t + 1 < steps) put(next);
+    T* swap = now;
+    now = next;
+    next = swap;
+  }
+  // b's rows run along the sums' registers: 4 neighbours of c's row to a lane
+#pragma unroll
+  for (int x = 0; x < X; ++x) {
+    const int i = wi + 32 * x + (lane & 31);
+#pragma unroll
+    for (int y = 0; y < Y; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int j = wj + 32 * y + 2 * r + 4 * (lane >> 5);
+        if (i >= a.n || j >= b.n) continue;
+        T v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = (T)acc[x][y][r + q];
+        T* to = c + i * ldc + j;
+        typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        if (j + 4 <= b.n) {
+          V4 w;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[q] = v[q];
+          *reinterpret_cast<V4*>(to) = w;
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (j + q < b.n) to[q] = v[q];
+        }
+      }
+  }
+}
+
+}  // namespace train
+}  // namespace purin
