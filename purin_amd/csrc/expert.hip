@@ -262,6 +262,34 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product16(
       (T*)lds16, out + from * ldo + col, ldo);
 }
 
+// Experts with few rows: every column tile of one expert's weights is read once, by a workgroup
+// that has all of the expert's rows (32 at a time).
+template <typename T, int BN, bool ALONG_B, bool DIRECT>
+__global__ __launch_bounds__(256) void k_product_thin(
+    const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
+    int64_t rows, int64_t inner, int64_t outer, int experts, int64_t tiles_n,
+    const int32_t* __restrict__ offsets, T* __restrict__ out, int64_t ldo) {
+  extern __shared__ __align__(16) unsigned char lds16[];
+  const int64_t tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
+  int e;
+  int64_t from, to;
+  if (!find_tile(offsets, experts, rows, 32, tm, e, from, to)) return;
+  e = __builtin_amdgcn_readfirstlane(e);
+  const int64_t col = tn * BN;
+  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(32, to - from));
+  const int n = (int)min<int64_t>(BN, outer - col);
+  if (e < 0) {
+    for (int r = threadIdx.x; r < m * (BN / 8); r += 256) {
+      const int i = r / (BN / 8), j = r % (BN / 8) * 8;
+      if (j < n) store_upto(out + (from + i) * ldo + col + j, zeros16<T>(), n - j);
+    }
+    return;
+  }
+  thin16<T, BN, ALONG_B, DIRECT>(
+      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner, lds16,
+      out + from * ldo + col, ldo);
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool DIRECT>
 __global__ __launch_bounds__(WM* WN * 64) void k_weights_vjp16(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ g, int64_t ldg, int64_t rows,
@@ -295,6 +323,12 @@ static bool direct_ok(const void* p, int64_t ld, int64_t length) {
          ld < (int64_t(1) << 21);
 }
 
+// The most tiles of ``height`` rows that any split of the rows over the experts needs, the rows
+// behind the last expert among them.
+static int64_t most_tiles(int64_t rows, int64_t experts, int64_t height) {
+  return (rows + std::min(rows, experts + 1) * (height - 1)) / height;
+}
+
 template <typename T>
 static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
                      const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,
@@ -304,7 +338,20 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
   const int64_t ldw = along ? wo : wi;
   const bool direct = direct_ok(a, lda, inner) && direct_ok(w, ldw, along ? inner : outer) &&
                       we % 8 == 0;
-  const int64_t tm = (rows + BM - 1) / BM + experts, tn = (outer + BN - 1) / BN;
+  if (rows <= 32 * experts) {
+    constexpr int TN = 64;
+    const int64_t tn = (outer + TN - 1) / TN;
+    auto thin = [&](auto kernel) {
+      return launch16("k_product_thin", kernel, dim3((unsigned)(most_tiles(rows, experts, 32) * tn)),
+                      256, thin_lds<TN>(), st, a, lda, w, we, ldw, rows, inner, outer,
+                      (int)experts, tn, offsets, out, ldo);
+    };
+    if (along) return direct ? thin(k_product_thin<T, TN, true, true>)
+                             : thin(k_product_thin<T, TN, true, false>);
+    return direct ? thin(k_product_thin<T, TN, false, true>)
+                  : thin(k_product_thin<T, TN, false, false>);
+  }
+  const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + BN - 1) / BN;
   auto go = [&](auto kernel) {
     return launch16("k_product16", kernel, dim3((unsigned)(tm * tn)), 512,
                     2 * (BM + BN) * kDepth16 * 2, st, a, lda, w, we, ldw, rows, inner, outer,

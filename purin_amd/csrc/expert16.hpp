@@ -8,8 +8,9 @@
 // columns).  Both are stored in 16-byte pieces whose places are exchanged by an XOR, so that the
 // lanes of one read fall on different banks:
 //   [i][k]   piece k / 8 of row i at (k / 8) ^ (i % 8): 8 rows' reads of one piece cover all banks
-//   [k][i]   pair i / 16 of row k at (i / 16) ^ s(k), s(k) = 2 (k % 4) + (k / 8) % 2: the 8
-//            blocks of 32 bytes that half a wavefront reads at once fall on 8 places
+//   [k][i]   pair i / 16 of row k at (i / 16) ^ s(k), s(k) = 2 (k % 4) + (k / 8) % 2 (2 ((k / 2) % 2)
+//            in rows of 64, two of which cover the banks): the 8 blocks of 32 bytes that half a
+//            wavefront reads at once fall on 8 places
 // With 16-byte rows at 16-byte addresses the stages are loaded straight into LDS (buffer loads
 // whose addresses outside the operand read zeros); others pass through registers.
 #pragma once
@@ -76,6 +77,12 @@ struct Side {
   int n;
 };
 
+template <int N>
+__device__ __forceinline__ int pair_swap(int k) {
+  if constexpr (N == 64) return 2 * ((k >> 1) & 1);
+  else return 2 * (k & 3) + ((k >> 3) & 1);
+}
+
 template <typename T, int N, bool ALONG, int THREADS, bool DIRECT>
 struct Stage {
   static constexpr int kPieces = N * kDepth16 / 8;  // 16 bytes each
@@ -92,8 +99,8 @@ struct Stage {
     } else {
       constexpr int per = N / 8;
       row = at / per;
-      const int c = at % per, s = 2 * (row & 3) + ((row >> 3) & 1);
-      first = ((((c >> 1) ^ s) << 1) | (c & 1)) * 8;
+      const int c = at % per;
+      first = ((((c >> 1) ^ pair_swap<N>(row)) << 1) | (c & 1)) * 8;
     }
   }
 
@@ -154,9 +161,9 @@ __device__ __forceinline__ S8 fragment(const T* lds, int i0, int s) {
     const int i = i0 + (lane & 31);
     return *reinterpret_cast<const S8*>(lds + i * kDepth16 + (((2 * s + (lane >> 5)) ^ (lane & 7)) << 3));
   } else {
-    const int k = 16 * s + 8 * (lane >> 5) + ((lane & 15) >> 2);
-    const int swap = 2 * ((lane & 15) >> 2) + (lane >> 5);
-    const int pair = ((i0 >> 4) + ((lane >> 4) & 1)) ^ swap;
+    const int k4 = 8 * (lane >> 5) + ((lane & 15) >> 2);  // the places repeat after 16
+    const int k = 16 * s + k4;
+    const int pair = ((i0 >> 4) + ((lane >> 4) & 1)) ^ pair_swap<N>(k4);
     const T* at = lds + k * N + pair * 16 + (lane & 3) * 4;
     using L = __attribute__((address_space(3))) S4;
     const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)at);
@@ -262,6 +269,109 @@ __device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, T* l
             if (j + q < b.n) to[q] = v[q];
         }
       }
+  }
+}
+
+// Few rows: at most 32, by BN, where reading b is the work.  kThin stages, all but one of them
+// on their way at any time; the 4 wavefronts share a stage's contraction (16 each) and add up
+// their sums at the end, in LDS, in their order.  ``lds`` holds thin_lds<BN>() bytes.
+constexpr int kThin = 4;
+template <int BN>
+constexpr int thin_lds() {
+  constexpr int stages = kThin * (32 + BN) * kDepth16 * 2, sums = 4 * 32 * (BN + 4) * 4;
+  return stages > sums ? stages : sums;
+}
+
+template <typename T, int BN, bool ALONG_B, bool DIRECT>
+__device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsigned char* lds,
+                                       T* c, int64_t ldc) {
+  constexpr int THREADS = 256, Y = BN / 32, P = BN + 4;
+  using SA = Stage<T, 32, true, THREADS, DIRECT>;
+  using SB = Stage<T, BN, ALONG_B, THREADS, DIRECT>;
+  constexpr int kStage = SA::kElems + SB::kElems;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T* stages = reinterpret_cast<T*>(lds);
+  F16x acc[Y];
+#pragma unroll
+  for (int y = 0; y < Y; ++y)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[y][r] = 0.0f;
+  uint32_t off_a[SA::kMine], off_b[SB::kMine];
+  Pack<T> va[SA::kMine], vb[SB::kMine];
+  const T *pa = uniform(a.p), *pb = uniform(b.p);
+  int64_t left = depth;
+  const int64_t steps = (depth + kDepth16 - 1) / kDepth16;
+  // DIRECT: a stage past the end reads nothing (its addresses are outside), and counts
+  auto load = [&](T* to) {
+    if constexpr (DIRECT) {
+      SA::load_lds(pa, off_a, left, to);
+      SB::load_lds(pb, off_b, left, to + SA::kElems);
+    } else {
+      SA::load_regs(a, pa, left, va);
+      SB::load_regs(b, pb, left, vb);
+    }
+    pa += kDepth16;
+    pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
+    left -= kDepth16;
+  };
+  auto put = [&](T* to) {
+    SA::store_lds(va, to);
+    SB::store_lds(vb, to + SA::kElems);
+  };
+  if constexpr (DIRECT) {
+    SA::offsets(a, off_a);
+    SB::offsets(b, off_b);
+#pragma unroll
+    for (int s = 0; s < kThin - 1; ++s) load(stages + s * kStage);
+  } else if (steps > 0) {
+    load(stages);
+    put(stages);
+  }
+  int now = 0;
+  for (int64_t t = 0; t < steps; ++t) {
+    int next = now + (DIRECT ? kThin - 1 : 1);
+    if (next >= kThin) next -= kThin;
+    if constexpr (DIRECT) {
+      // the loads of the kThin - 2 later stages may be on their way still
+      constexpr int later = (kThin - 2) * (SA::kMine + SB::kMine);
+      static_assert(later < 64, "the counter's range");
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (later & 15) | ((later >> 4) << 14));
+    }
+    __syncthreads();
+    if (DIRECT || t + 1 < steps) load(stages + next * kStage);
+    const T *la = stages + now * kStage, *lb = la + SA::kElems;
+    const S8 fa = fragment<T, 32, true>(la, 0, wave);
+    S8 fb[Y];
+#pragma unroll
+    for (int y = 0; y < Y; ++y) fb[y] = fragment<T, BN, ALONG_B>(lb, 32 * y, wave);
+#pragma unroll
+    for (int y = 0; y < Y; ++y) acc[y] = mma32(T{}, fb[y], fa, acc[y]);
+    if constexpr (!DIRECT)
+      if (t + 1 < steps) put(stages + next * kStage);
+    now = now + 1 == kThin ? 0 : now + 1;
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // the stages past the end
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int y = 0; y < Y; ++y)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      sums[(wave * 32 + (lane & 31)) * P + 32 * y + 2 * (r & ~3) + 4 * (lane >> 5) + (r & 3)] =
+          acc[y][r];
+  __syncthreads();
+  for (int at = threadIdx.x; at < 32 * BN / 8; at += THREADS) {
+    const int i = at / (BN / 8), j = at % (BN / 8) * 8;
+    if (i >= a.n || j >= b.n) continue;
+    Pack<T> v;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      float s = sums[i * P + j + q];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) s += sums[(w * 32 + i) * P + j + q];
+      v.v[q] = (T)s;
+    }
+    store_upto(c + i * ldc + j, v, b.n - j);
   }
 }
 
