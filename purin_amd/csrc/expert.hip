@@ -10,57 +10,14 @@
 // at once.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "expert16.hpp"
+#include "expert32.hpp"
 #include "train.hpp"
 
 namespace purin {
 namespace train {
-
-typedef float F4 __attribute__((ext_vector_type(4)));
-typedef double D4 __attribute__((ext_vector_type(4)));
-
-// One 16x16 tile of sums per wavefront.  A lane holds kPer values along the contraction, of
-// row (or column) lane % 16 from kPer * (lane / 16) on; Steps of 4 * kPer make one kDepth.
-// sum[r] is row(lane, r) and column lane % 16.
-template <typename T>
-struct Mma;
-template <>
-struct Mma<bf16> {
-  using Acc = F4;
-  static constexpr int kPer = 8, kDepth = 32;
-  static __device__ __forceinline__ Acc step(const bf16* a, const bf16* b, Acc c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const B8*)a, *(const B8*)b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ int row(int lane, int r) { return 4 * (lane >> 4) + r; }
-};
-template <>
-struct Mma<f16> {
-  using Acc = F4;
-  static constexpr int kPer = 8, kDepth = 32;
-  static __device__ __forceinline__ Acc step(const f16* a, const f16* b, Acc c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const H8*)a, *(const H8*)b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ int row(int lane, int r) { return 4 * (lane >> 4) + r; }
-};
-template <>
-struct Mma<float> {
-  using Acc = F4;
-  static constexpr int kPer = 1, kDepth = 16;
-  static __device__ __forceinline__ Acc step(const float* a, const float* b, Acc c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(*a, *b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ int row(int lane, int r) { return 4 * (lane >> 4) + r; }
-};
-template <>
-struct Mma<double> {
-  using Acc = D4;
-  static constexpr int kPer = 1, kDepth = 16;
-  static __device__ __forceinline__ Acc step(const double* a, const double* b, Acc c) {
-    return __builtin_amdgcn_mfma_f64_16x16x4f64(*a, *b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ int row(int lane, int r) { return 4 * r + (lane >> 4); }
-};
 
 // The rows of expert e: [from, to), inside [0, rows] whatever the offsets hold.
 __device__ __forceinline__ void segment(const int32_t* offsets, int e, int64_t rows, int64_t& from,
@@ -108,118 +65,17 @@ __device__ __forceinline__ bool find_tile(const int32_t* offsets, int experts, i
   return from < to;
 }
 
-constexpr int kTile = 128;  // rows and columns of a workgroup's tile, 64 by 64 a wavefront
-
-// One operand of a tile: element (i, k) at p + i * si + k * sk, with si or sk 1.
+// Zeros for the rows behind the last expert's.
 template <typename T>
-struct Operand {
-  const T* p;
-  int64_t si, sk;
-};
-
-template <typename T>
-constexpr int lds_pitch() {
-  // contraction-contiguous rows; the padding spreads a column's reads over the banks
-  return Mma<T>::kDepth + (Mma<T>::kPer > 1 ? Mma<T>::kPer : 1);
-}
-
-// kTile x kDepth of an operand into LDS, zeros where i >= n or k >= depth.
-template <typename T>
-__device__ __forceinline__ void stage(const Operand<T>& o, int n, int depth, T* lds) {
-  constexpr int D = Mma<T>::kDepth, P = lds_pitch<T>();
-  const bool along = o.sk == 1;
-#pragma unroll 4
-  for (int r = threadIdx.x; r < kTile * D; r += 256) {
-    const int k = along ? r % D : r / kTile;
-    const int i = along ? r / D : r % kTile;
-    lds[i * P + k] = i < n && k < depth ? o.p[i * o.si + k * o.sk] : (T)0;
+__device__ __forceinline__ void zero_tile(T* c, int64_t ldc, int m, int n) {
+  const int per = (n + kVec<T> - 1) / kVec<T>;
+  for (int r = threadIdx.x; r < m * per; r += blockDim.x) {
+    const int i = r / per, j = r % per * kVec<T>;
+    store_upto(c + i * ldc + j, zeros16<T>(), n - j);
   }
 }
 
-// c (m x n of a kTile x kTile tile, row pitch ldc) = sum over k of a(i, k) b(j, k).
-template <typename T>
-__device__ __forceinline__ void tile_product(Operand<T> a, Operand<T> b, int m, int n, int64_t depth,
-                                             T* c, int64_t ldc) {
-  using M = Mma<T>;
-  constexpr int D = M::kDepth, P = lds_pitch<T>();
-  __shared__ __align__(16) T as[kTile * P];
-  __shared__ __align__(16) T bs[kTile * P];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
-  typename M::Acc acc[4][4];
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int y = 0; y < 4; ++y) acc[x][y] = typename M::Acc{0, 0, 0, 0};
-  for (int64_t k = 0; k < depth; k += D) {
-    const int d = (int)min<int64_t>(D, depth - k);
-    __syncthreads();
-    stage(a, m, d, as);
-    stage(b, n, d, bs);
-    a.p += D * a.sk;
-    b.p += D * b.sk;
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < D; s += 4 * M::kPer) {
-      const int at = s + M::kPer * (lane >> 4);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-          acc[x][y] = M::step(as + (wi + 16 * x + (lane & 15)) * P + at,
-                              bs + (wj + 16 * y + (lane & 15)) * P + at, acc[x][y]);
-    }
-  }
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int y = 0; y < 4; ++y)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = wi + 16 * x + M::row(lane, r), j = wj + 16 * y + (lane & 15);
-        if (i < m && j < n) c[i * ldc + j] = (T)acc[x][y][r];
-      }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_product(const T* __restrict__ a, int64_t lda,
-                                                 const T* __restrict__ w, int64_t we, int64_t wi,
-                                                 int64_t wo, int64_t rows, int64_t inner,
-                                                 int64_t outer, int experts,
-                                                 const int32_t* __restrict__ offsets,
-                                                 T* __restrict__ out, int64_t ldo) {
-  int e;
-  int64_t from, to;
-  if (!find_tile(offsets, experts, rows, kTile, blockIdx.x, e, from, to)) return;
-  const int64_t col = (int64_t)blockIdx.y * kTile;
-  const int m = (int)min<int64_t>(kTile, to - from), n = (int)min<int64_t>(kTile, outer - col);
-  if (e < 0) {
-    for (int r = threadIdx.x; r < m * kTile; r += 256) {
-      const int i = r / kTile, j = r % kTile;
-      if (j < n) out[(from + i) * ldo + col + j] = (T)0;
-    }
-    return;
-  }
-  tile_product<T>({a + from * lda, lda, 1}, {w + e * we + col * wo, wo, wi}, m, n, inner,
-                  out + from * ldo + col, ldo);
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_weights_vjp(const T* __restrict__ a, int64_t lda,
-                                                     const T* __restrict__ g, int64_t ldg,
-                                                     int64_t rows, int64_t inner, int64_t outer,
-                                                     const int32_t* __restrict__ offsets,
-                                                     T* __restrict__ gw) {
-  const int e = (int)blockIdx.z;
-  int64_t from, to;
-  segment(offsets, e, rows, from, to);
-  const int64_t i = (int64_t)blockIdx.x * kTile, j = (int64_t)blockIdx.y * kTile;
-  tile_product<T>({a + from * lda + i, 1, lda}, {g + from * ldg + j, 1, ldg},
-                  (int)min<int64_t>(kTile, inner - i), (int)min<int64_t>(kTile, outer - j),
-                  to - from, gw + e * inner * outer + i * outer + j, outer);
-}
-
-// 16-bit types: BM x BN tiles in 1-D order, XCD by XCD (workgroups are dealt to the 8 XCDs in
+// Tiles in 1-D order, XCD by XCD (workgroups are dealt to the 8 XCDs in
 // turn, so number i is on XCD i % 8): an XCD's workgroups take neighbouring tiles, kGroup rows
 // of tiles at a time, and find each other's operands in its L2.
 constexpr int kGroup = 4;
@@ -251,10 +107,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product16(
   const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
   const int n = (int)min<int64_t>(BN, outer - col);
   if (e < 0) {
-    for (int r = threadIdx.x; r < m * (BN / 8); r += WM * WN * 64) {
-      const int i = r / (BN / 8), j = r % (BN / 8) * 8;
-      if (j < n) store_upto(out + (from + i) * ldo + col + j, zeros16<T>(), n - j);
-    }
+    zero_tile(out + from * ldo + col, ldo, m, n);
     return;
   }
   tile16<T, BM, BN, WM, WN, true, ALONG_B, DIRECT>(
@@ -279,10 +132,7 @@ __global__ __launch_bounds__(256) void k_product_thin(
   const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(32, to - from));
   const int n = (int)min<int64_t>(BN, outer - col);
   if (e < 0) {
-    for (int r = threadIdx.x; r < m * (BN / 8); r += 256) {
-      const int i = r / (BN / 8), j = r % (BN / 8) * 8;
-      if (j < n) store_upto(out + (from + i) * ldo + col + j, zeros16<T>(), n - j);
-    }
+    zero_tile(out + from * ldo + col, ldo, m, n);
     return;
   }
   thin16<T, BN, ALONG_B, DIRECT>(
@@ -305,6 +155,49 @@ __global__ __launch_bounds__(WM* WN * 64) void k_weights_vjp16(
   tile16<T, BM, BN, WM, WN, false, false, DIRECT>(
       {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i)},
       {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, to - from, (T*)lds16,
+      gw + e * inner * outer + i * outer + j, outer);
+}
+
+// 32- and 64-bit types.
+template <typename T, int BM, int BN, int WM, int WN, bool ALONG_B>
+__global__ __launch_bounds__(256, 2) void k_product32(
+    const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
+    int64_t rows, int64_t inner, int64_t outer, int experts, int64_t tiles_m, int64_t tiles_n,
+    const int32_t* __restrict__ offsets, T* __restrict__ out, int64_t ldo) {
+  __shared__ __align__(16) unsigned char lds[lds32<T, BM, BN, true, ALONG_B>()];
+  int64_t tm, tn;
+  tile_order(tiles_m, tiles_n, tm, tn);
+  int e;
+  int64_t from, to;
+  if (!find_tile(offsets, experts, rows, BM, tm, e, from, to)) return;
+  e = __builtin_amdgcn_readfirstlane(e);
+  const int64_t col = tn * BN;
+  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
+  const int n = (int)min<int64_t>(BN, outer - col);
+  if (e < 0) {
+    zero_tile(out + from * ldo + col, ldo, m, n);
+    return;
+  }
+  tile32<T, BM, BN, WM, WN, true, ALONG_B>(
+      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner, (T*)lds,
+      out + from * ldo + col, ldo);
+}
+
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256, 2) void k_weights_vjp32(
+    const T* __restrict__ a, int64_t lda, const T* __restrict__ g, int64_t ldg, int64_t rows,
+    int64_t inner, int64_t outer, int64_t tiles_m, int64_t tiles_n,
+    const int32_t* __restrict__ offsets, T* __restrict__ gw) {
+  __shared__ __align__(16) unsigned char lds[lds32<T, BM, BN, false, false>()];
+  int64_t tm, tn;
+  tile_order(tiles_m, tiles_n, tm, tn);
+  const int e = (int)blockIdx.y;
+  int64_t from, to;
+  segment(offsets, e, rows, from, to);
+  const int64_t i = tm * BM, j = tn * BN;
+  tile32<T, BM, BN, 2, 2, false, false>(
+      {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i)},
+      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, to - from, (T*)lds,
       gw + e * inner * outer + i * outer + j, outer);
 }
 
@@ -379,6 +272,54 @@ static int weights_vjp16(hipStream_t st, int64_t rows, int64_t inner, int64_t ou
                 : go(k_weights_vjp16<T, BM, BN, 2, 4, false>);
 }
 
+template <typename T>
+static int product32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
+                     const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,
+                     const int32_t* offsets, T* out, int64_t ldo) {
+  const bool along = wi == 1 && (wo != 1 || inner > 1);
+  const int64_t ldw = along ? wo : wi;
+  auto go = [&](int BM, int BN, auto kernel) {
+    const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + BN - 1) / BN;
+    kernel<<<dim3((unsigned)(tm * tn)), dim3(256), 0, st>>>(a, lda, w, we, ldw, rows, inner, outer,
+                                                           (int)experts, tm, tn, offsets, out, ldo);
+    return launched("k_product32");
+  };
+  auto shape = [&](auto bm, auto bn, auto wm, auto wn) {
+    constexpr int BM = bm, BN = bn, WM = wm, WN = wn;
+    return along ? go(BM, BN, k_product32<T, BM, BN, WM, WN, true>)
+                 : go(BM, BN, k_product32<T, BM, BN, WM, WN, false>);
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 1> i1;
+  constexpr integral_constant<int, 2> i2;
+  constexpr integral_constant<int, 4> i4;
+  constexpr integral_constant<int, 32> i32;
+  constexpr integral_constant<int, 64> i64;
+  constexpr integral_constant<int, 128> i128;
+  if (rows <= 32 * experts) return shape(i32, i64, i1, i4);
+  // large tiles where they fill the 256 CUs twice
+  if constexpr (sizeof(T) == 4)
+    if (most_tiles(rows, experts, 128) * ((outer + 127) / 128) >= 512)
+      return shape(i128, i128, i2, i2);
+  return shape(i64, i64, i2, i2);
+}
+
+template <typename T>
+static int weights_vjp32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
+                         int64_t experts, const T* a, int64_t lda, const T* g, int64_t ldg,
+                         const int32_t* offsets, T* gw) {
+  auto go = [&](int BM, int BN, auto kernel) {
+    const int64_t tm = (inner + BM - 1) / BM, tn = (outer + BN - 1) / BN;
+    kernel<<<dim3((unsigned)(tm * tn), (unsigned)experts), dim3(256), 0, st>>>(
+        a, lda, g, ldg, rows, inner, outer, tm, tn, offsets, gw);
+    return launched("k_weights_vjp32");
+  };
+  if constexpr (sizeof(T) == 4)
+    if (((inner + 127) / 128) * ((outer + 127) / 128) * experts >= 512)
+      return go(128, 128, k_weights_vjp32<T, 128, 128>);
+  return go(64, 64, k_weights_vjp32<T, 64, 64>);
+}
+
 static int check_product(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
                          int64_t experts) {
   if (!known_dtype(dtype)) return refuse("unknown dtype");
@@ -432,12 +373,9 @@ int purin_train_expert_product(void* stream, int32_t dtype, int64_t rows, int64_
       if constexpr (sizeof(T) == 2)
         return product16<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
                             (const T*)weight, we, wi, wo, offsets, (T*)out, ldo);
-      const dim3 grid((unsigned)((rows + kTile - 1) / kTile + experts),
-                      (unsigned)((outer + kTile - 1) / kTile));
-      k_product<T><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
-          (const T*)a, lda, (const T*)weight, we, wi, wo, rows, inner, outer, (int)experts,
-          offsets, (T*)out, ldo);
-      return launched("k_product");
+      else
+        return product32<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
+                            (const T*)weight, we, wi, wo, offsets, (T*)out, ldo);
     });
   });
 }
@@ -468,11 +406,9 @@ int purin_train_expert_weights_vjp(void* stream, int32_t dtype, int64_t rows, in
       if constexpr (sizeof(T) == 2)
         return weights_vjp16<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
                                 (const T*)g, ldg, offsets, (T*)g_weight);
-      const dim3 grid((unsigned)((inner + kTile - 1) / kTile),
-                      (unsigned)((outer + kTile - 1) / kTile), (unsigned)experts);
-      k_weights_vjp<T><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
-          (const T*)a, lda, (const T*)g, ldg, rows, inner, outer, offsets, (T*)g_weight);
-      return launched("k_weights_vjp");
+      else
+        return weights_vjp32<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
+                                (const T*)g, ldg, offsets, (T*)g_weight);
     });
   });
 }
