@@ -9,6 +9,9 @@ Each source compiles to its own object (in parallel, under ``_build/``), and
 the objects link into the shared library; every call recompiles.
 ``resident_launch.hip`` compiles once per (element type, row-slot count) pair
 (``RESIDENT_VARIANTS``), so the resident kernel's variants build in parallel.
+
+``_front.so`` (``front.cpp``) is the torch front end of ``include/purin_train.h``: host code
+alone, compiled against torch's headers and linked to the library beside it.
 """
 
 from __future__ import annotations
@@ -16,7 +19,9 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib.util import find_spec
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -26,6 +31,8 @@ SOURCES = ["plan.hip", "forward.hip", "adjoint.hip", "gmres.hip", "solo.hip", "r
            "expert.hip", "clip.hip"]
 RESIDENT_SOURCE = "resident_launch.hip"
 RESIDENT_VARIANTS = [(f64, slr) for f64 in (1, 0) for slr in (1, 2, 3, 4)]
+FRONT = os.path.join(HERE, "_front.so")
+FRONT_SOURCE = "front.cpp"
 PROBE_LIB = os.path.join(HERE, "libpurin_probe.so")
 PROBE_SOURCES = ["probe.hip"]
 ARCH = os.environ.get("PURIN_OFFLOAD_ARCH", "gfx950")
@@ -82,6 +89,35 @@ def _link(objs, out, verbose):
     os.replace(tmp, out)
 
 
+def _torch_dir():
+    return find_spec("torch").submodule_search_locations[0]
+
+
+def _compile_front(verbose):
+    """Object of the torch front end (g++; the torch package's own C++ ABI, the new one)."""
+    os.makedirs(OBJ, exist_ok=True)
+    obj = os.path.join(OBJ, FRONT_SOURCE + ".o")
+    inc = os.path.join(_torch_dir(), "include")
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
+          "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_front",
+          "-D_GLIBCXX_USE_CXX11_ABI=1", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+          "-isystem", os.path.join(rocm, "include"),
+          "-isystem", sysconfig.get_paths()["include"],
+          "-c", os.path.join(CSRC, FRONT_SOURCE), "-o", obj + ".tmp"], FRONT_SOURCE, verbose)
+    os.replace(obj + ".tmp", obj)
+    return obj
+
+
+def _link_front(obj, verbose):
+    lib = os.path.join(_torch_dir(), "lib")
+    tmp = FRONT + ".tmp"
+    _run(["g++", "-shared", obj, "-L" + HERE, "-l:" + os.path.basename(LIB), "-L" + lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+          "-ltorch_python", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + lib, "-o", tmp], os.path.basename(FRONT), verbose)
+    os.replace(tmp, FRONT)
+
+
 def build(verbose: bool = False) -> str:
     lib_jobs = _jobs()
     probe_jobs = [(s, [], "") for s in sources(PROBE_SOURCES)]
@@ -89,8 +125,10 @@ def build(verbose: bool = False) -> str:
     jobs = lib_jobs[len(SOURCES):] + lib_jobs[:len(SOURCES)][::-1] + probe_jobs
     workers = max(1, min(len(jobs), int(os.environ.get("MAX_JOBS", "8"))))
     with ThreadPoolExecutor(workers) as pool:
+        front = pool.submit(_compile_front, verbose)
         objs = dict(zip([id(j) for j in jobs], pool.map(lambda j: _compile(j, verbose), jobs)))
     _link([objs[id(j)] for j in lib_jobs], LIB, verbose)
+    _link_front(front.result(), verbose)
     _link([objs[id(j)] for j in probe_jobs], PROBE_LIB, verbose)
     return LIB
 

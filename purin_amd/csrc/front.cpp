@@ -1,0 +1,512 @@
+// The torch front end of include/purin_train.h: argument checks, outputs from torch's allocator,
+// the current stream, and the gradients as autograd nodes in C++.  A small call's time is the
+// host's: the same front end over ctypes and Python autograd functions took 213 us for a training
+// step of route, dispatch and combine whose kernels run for 20.
+//
+// No kernel is here; libpurin_cp.so, which this links to, holds them and knows nothing of torch.
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <optional>
+#include <sstream>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "../../include/purin_cp.h"
+#include "../../include/purin_train.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+// An error code and message of the library; Python sees purin_amd._lib.PurinError.
+struct LibraryError : std::exception {
+  int code;
+  std::string message;
+  explicit LibraryError(int c) : code(c), message(purin_cp_last_error()) {}
+  const char* what() const noexcept override { return message.c_str(); }
+};
+
+void check(int code) {
+  if (code != PURIN_CP_OK) throw LibraryError(code);
+}
+int64_t bytes(int64_t need) {
+  if (need < 0) throw LibraryError(PURIN_CP_ERR_ARG);
+  return need;
+}
+
+template <typename... A>
+[[noreturn]] void refuse(const A&... parts) {
+  std::ostringstream s;
+  (s << ... << parts);
+  throw py::value_error(s.str());
+}
+
+int32_t code_of(const Tensor& t, const char* name) {
+  if (!t.is_cuda()) refuse(name, " must be a tensor on the GPU");
+  switch (t.scalar_type()) {
+    case at::kFloat: return PURIN_TRAIN_F32;
+    case at::kDouble: return PURIN_TRAIN_F64;
+    case at::kBFloat16: return PURIN_TRAIN_BF16;
+    case at::kHalf: return PURIN_TRAIN_F16;
+    default: refuse(name, " must be float32, float64, bfloat16 or float16; got ", t.scalar_type());
+  }
+}
+
+void same_device(const Tensor& a, const Tensor& b, const char* name) {
+  if (a.device() != b.device()) refuse(name, " must be on ", a.device(), "; got ", b.device());
+}
+
+// A matrix with adjacent elements in a row and rows that do not overlap.
+Tensor matrix(const Tensor& t) {
+  if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1)))
+    return t.contiguous();
+  return t;
+}
+
+// The device made current, and its current stream, for one entry point.
+struct Call {
+  c10::DeviceGuard guard;
+  void* stream;
+  explicit Call(const Tensor& t)
+      : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+};
+
+// A call's scratch: the caller's, or new memory, which the allocator gives to nothing else
+// before the stream's kernels are done with it.
+struct Workspace {
+  Tensor held;
+  void* at = nullptr;
+  int64_t size = 0;
+  Workspace(const std::optional<Tensor>& given, int64_t need, const Tensor& like) {
+    if (given) {
+      if (!given->is_cuda()) refuse("workspace must be a device tensor");
+      held = *given;
+    } else if (bytes(need)) {
+      held = at::empty({need}, like.options().dtype(at::kByte).requires_grad(false));
+    } else {
+      return;
+    }
+    at = held.data_ptr();
+    size = (int64_t)held.nbytes();
+  }
+};
+
+bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
+// Gradients of gradients are not there: with a graph wanted of the backward pass, what it
+// returns raises in its own.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list some;
+  for (Tensor& g : grads)
+    if (g.defined()) some.push_back(g.detach().requires_grad_());
+  if (some.empty()) return grads;
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "this operator is differentiable once", (int64_t)some.size());
+  some = (*node)(std::move(some));
+  size_t k = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = some[k++];
+  return grads;
+}
+
+// -- routing ------------------------------------------------------------------------------
+
+struct Index {
+  Tensor ids, offsets, place, source;
+};
+
+Index new_index(int64_t tokens, int64_t count, int64_t slots, const Tensor& like) {
+  const int64_t pairs = tokens * slots;
+  const auto o = like.options().dtype(at::kInt).requires_grad(false);
+  return {at::empty({tokens, slots}, o), at::empty({count + 1}, o), at::empty({tokens, slots}, o),
+          at::empty({pairs}, o)};
+}
+
+int32_t* ints(const Tensor& t) { return (int32_t*)t.data_ptr(); }
+
+Tensor run_route(const Tensor& weights, int64_t slots, const std::optional<Tensor>& workspace,
+                 Index* index) {
+  const Tensor w = matrix(weights);
+  const int64_t tokens = w.size(0), count = w.size(1);
+  const Call call(w);
+  const Workspace ws(workspace, purin_train_route_workspace_bytes(tokens, count, slots), w);
+  *index = new_index(tokens, count, slots, w);
+  Tensor chosen = at::empty({tokens, slots}, w.options().requires_grad(false));
+  check(purin_train_route(call.stream, code_of(w, "weights"), tokens, count, slots, w.data_ptr(),
+                          w.stride(0), ws.at, ws.size, ints(index->ids), chosen.data_ptr(),
+                          ints(index->offsets), ints(index->place), ints(index->source)));
+  return chosen;
+}
+
+struct RouteFn : torch::autograd::Function<RouteFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weights, int64_t slots,
+                        const std::optional<Tensor>& workspace, Index* index) {
+    Tensor chosen = run_route(weights, slots, workspace, index);
+    ctx->save_for_backward({index->ids});
+    ctx->saved_data["count"] = weights.size(1);
+    return chosen;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor ids = ctx->get_saved_variables()[0], g = grads[0].contiguous();
+    const int64_t count = ctx->saved_data["count"].toInt();
+    const Call call(g);
+    Tensor out = at::empty({ids.size(0), count}, g.options().requires_grad(false));
+    check(purin_train_route_vjp(call.stream, code_of(g, "gradient"), ids.size(0), count,
+                                ids.size(1), ints(ids), g.data_ptr(), out.data_ptr()));
+    return once({out, Tensor(), Tensor(), Tensor()});
+  }
+};
+
+using Routed = std::tuple<int64_t, int64_t, int64_t, Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+Routed route(const Tensor& weights, int64_t slots, const std::optional<Tensor>& workspace) {
+  code_of(weights, "weights");
+  if (weights.dim() != 2) refuse("weights must have two dimensions; got shape ", weights.sizes());
+  const int64_t count = weights.size(1);
+  if (slots < 1) refuse("slots must be a positive integer; got ", slots);
+  if (count < 1 || slots > count) refuse("slots must not exceed the ", count, " experts; got ", slots);
+  Index index;
+  Tensor chosen = wants_grad(weights) ? RouteFn::apply(weights, slots, workspace, &index)
+                                      : run_route(weights, slots, workspace, &index);
+  return {weights.size(0), count, slots, index.ids, chosen, index.offsets, index.place, index.source};
+}
+
+Routed route_experts(const Tensor& experts, int64_t count, const std::optional<Tensor>& weights,
+                     const std::optional<Tensor>& workspace) {
+  if (!experts.is_cuda()) refuse("experts must be a tensor on the GPU");
+  if ((experts.scalar_type() != at::kInt && experts.scalar_type() != at::kLong) ||
+      experts.dim() != 2)
+    refuse("experts must be an int32 or int64 tensor (tokens, slots); got ", experts.scalar_type(),
+           " ", experts.sizes());
+  const int64_t tokens = experts.size(0), slots = experts.size(1);
+  if (slots < 1) refuse("experts must have a slot");
+  if (count < 1) refuse("count must be a positive integer; got ", count);
+  if (weights) {
+    code_of(*weights, "weights");
+    same_device(experts, *weights, "weights");
+    if (weights->sizes() != experts.sizes())
+      refuse("weights must have shape ", experts.sizes(), "; got ", weights->sizes());
+  }
+  const Tensor given = experts.contiguous();
+  const Call call(given);
+  const Workspace ws(workspace, purin_train_route_workspace_bytes(tokens, count, slots), given);
+  const Index x = new_index(tokens, count, slots, given);
+  check(purin_train_sort(call.stream, given.scalar_type() == at::kLong, tokens, count, slots,
+                         given.data_ptr(), ws.at, ws.size, ints(x.ids), ints(x.offsets),
+                         ints(x.place), ints(x.source)));
+  return {tokens, count, slots, x.ids, weights ? *weights : Tensor(), x.offsets, x.place, x.source};
+}
+
+// -- rows ---------------------------------------------------------------------------------
+
+Tensor run_combine(const Tensor& given, const Tensor& place, const Tensor* weights) {
+  const Tensor rows = matrix(given);
+  const Call call(rows);
+  Tensor out = at::empty({place.size(0), rows.size(1)}, rows.options().requires_grad(false));
+  check(purin_train_combine(call.stream, code_of(rows, "rows"),
+                            weights ? code_of(*weights, "weights") : 0, place.size(0),
+                            place.size(1), rows.size(1), rows.data_ptr(), rows.stride(0),
+                            ints(place), weights ? weights->data_ptr() : nullptr, out.data_ptr()));
+  return out;
+}
+
+Tensor run_dispatch(const Tensor& given, const Tensor& place, const Tensor& offsets) {
+  const Tensor x = matrix(given);
+  const Call call(x);
+  Tensor rows = at::empty({place.numel(), x.size(1)}, x.options().requires_grad(false));
+  check(purin_train_dispatch(call.stream, code_of(x, "x"), place.size(0), offsets.numel() - 1,
+                             place.size(1), x.size(1), x.data_ptr(), x.stride(0), ints(offsets),
+                             ints(place), rows.data_ptr()));
+  return rows;
+}
+
+struct DispatchFn : torch::autograd::Function<DispatchFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& place,
+                        const Tensor& offsets) {
+    ctx->save_for_backward({place});
+    return run_dispatch(x, place, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return once({run_combine(grads[0], ctx->get_saved_variables()[0], nullptr), Tensor(), Tensor()});
+  }
+};
+
+Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets) {
+  code_of(x, "x");
+  same_device(place, x, "x");
+  if (x.dim() != 2 || x.size(0) != place.size(0))
+    refuse("x must have shape (", place.size(0), ", width); got ", x.sizes());
+  return wants_grad(x) ? DispatchFn::apply(x, place, offsets) : run_dispatch(x, place, offsets);
+}
+
+struct CombineFn : torch::autograd::Function<CombineFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights,
+                        const Tensor& place, const Tensor& offsets) {
+    ctx->save_for_backward({rows, weights, place, offsets});
+    const Tensor w = weights.contiguous();
+    return run_combine(rows, place, &w);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor rows = matrix(saved[0]), w = saved[1].contiguous(), g = matrix(grads[0]);
+    const Tensor &place = saved[2], &offsets = saved[3];
+    const Call call(g);
+    Tensor g_rows, g_weights;
+    if (ctx->needs_input_grad(0))
+      g_rows = at::empty(rows.sizes(), rows.options().requires_grad(false));
+    if (ctx->needs_input_grad(1))
+      g_weights = at::empty(w.sizes(), w.options().requires_grad(false));
+    check(purin_train_combine_vjp(
+        call.stream, code_of(g, "gradient"), code_of(w, "weights"), place.size(0),
+        offsets.numel() - 1, place.size(1), g.size(1), g.data_ptr(), g.stride(0), rows.data_ptr(),
+        rows.stride(0), ints(offsets), ints(place), w.data_ptr(),
+        g_rows.defined() ? g_rows.data_ptr() : nullptr,
+        g_weights.defined() ? g_weights.data_ptr() : nullptr));
+    return once({g_rows, g_weights, Tensor(), Tensor()});
+  }
+};
+
+Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place,
+               const Tensor& offsets) {
+  code_of(rows, "rows");
+  same_device(place, rows, "rows");
+  if (rows.dim() != 2 || rows.size(0) != place.numel())
+    refuse("rows must have shape (", place.numel(), ", width); got ", rows.sizes());
+  code_of(weights, "weights");
+  same_device(rows, weights, "weights");
+  if (weights.sizes() != place.sizes())
+    refuse("weights must have shape ", place.sizes(), "; got ", weights.sizes());
+  if (wants_grad(rows) || wants_grad(weights)) return CombineFn::apply(rows, weights, place, offsets);
+  const Tensor w = weights.contiguous();
+  return run_combine(rows, place, &w);
+}
+
+// -- the experts' products ------------------------------------------------------------------
+
+// A weight with a unit stride along inner or outer and no overlap inside a matrix; a broadcast
+// over the experts stays one.
+Tensor weight_strides(const Tensor& w) {
+  const int64_t inner = w.size(1), outer = w.size(2), si = w.stride(1), so = w.stride(2);
+  if ((so == 1 || outer <= 1) && (si >= outer || inner <= 1)) return w;
+  if ((si == 1 || inner <= 1) && (so >= inner || outer <= 1)) return w;
+  return w.contiguous();
+}
+
+Tensor run_product(const Tensor& rows, const Tensor& w, const Tensor& offsets) {
+  const Tensor a = matrix(rows);
+  const int32_t code = code_of(a, "rows");
+  const int64_t p = a.size(0), inner = a.size(1), outer = w.size(2), experts = w.size(0);
+  const Call call(a);
+  const Workspace ws(
+      std::nullopt, purin_train_expert_product_workspace_bytes(code, p, inner, outer, experts), a);
+  Tensor out = at::empty({p, outer}, a.options().requires_grad(false));
+  check(purin_train_expert_product(call.stream, code, p, inner, outer, experts, a.data_ptr(),
+                                   a.stride(0), w.data_ptr(), w.stride(0), w.stride(1), w.stride(2),
+                                   ints(offsets), ws.at, ws.size, out.data_ptr(), outer));
+  return out;
+}
+
+Tensor run_weights_vjp(const Tensor& a, const Tensor& g, const Tensor& offsets, int64_t experts) {
+  const int32_t code = code_of(a, "rows");
+  const int64_t p = a.size(0), inner = a.size(1), outer = g.size(1);
+  const Call call(a);
+  const Workspace ws(
+      std::nullopt, purin_train_expert_weights_vjp_workspace_bytes(code, p, inner, outer, experts),
+      a);
+  Tensor out = at::empty({experts, inner, outer}, a.options().requires_grad(false));
+  check(purin_train_expert_weights_vjp(call.stream, code, p, inner, outer, experts, a.data_ptr(),
+                                       a.stride(0), g.data_ptr(), g.stride(0), ints(offsets), ws.at,
+                                       ws.size, out.data_ptr()));
+  return out;
+}
+
+struct ProductFn : torch::autograd::Function<ProductFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weight,
+                        const Tensor& offsets) {
+    ctx->save_for_backward({rows, weight, offsets});
+    return run_product(rows, weight_strides(weight), offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor a = matrix(saved[0]), w = weight_strides(saved[1]), g = matrix(grads[0]);
+    const Tensor& offsets = saved[2];
+    Tensor g_rows, g_weight;
+    if (ctx->needs_input_grad(0)) g_rows = run_product(g, w.transpose(1, 2), offsets);
+    if (ctx->needs_input_grad(1)) {
+      if (w.stride(2) == 1 || w.size(2) <= 1)
+        g_weight = run_weights_vjp(a, g, offsets, w.size(0));
+      else  // the weight's own order: (a^T g)^T = g^T a
+        g_weight = run_weights_vjp(g, a, offsets, w.size(0)).transpose(1, 2);
+    }
+    return once({g_rows, g_weight, Tensor()});
+  }
+};
+
+Tensor expert_product(const Tensor& rows, const Tensor& weight, const Tensor& offsets) {
+  code_of(rows, "rows");
+  code_of(weight, "weight");
+  if (rows.scalar_type() != weight.scalar_type())
+    refuse("rows and weight must have one type; got ", rows.scalar_type(), " and ",
+           weight.scalar_type());
+  if (rows.dim() != 2 || weight.dim() != 3 || rows.size(1) != weight.size(1))
+    refuse("rows must have shape (rows, inner) and weight (experts, inner, outer); got ",
+           rows.sizes(), " and ", weight.sizes());
+  if (offsets.scalar_type() != at::kInt || offsets.dim() != 1 ||
+      offsets.size(0) != weight.size(0) + 1)
+    refuse("offsets must be a Routing or an int32 tensor of ", weight.size(0) + 1, " entries");
+  same_device(rows, weight, "weight");
+  same_device(rows, offsets, "offsets");
+  const Tensor at = offsets.contiguous();
+  return wants_grad(rows) || wants_grad(weight) ? ProductFn::apply(rows, weight, at)
+                                                : run_product(rows, weight_strides(weight), at);
+}
+
+// -- the global norm ------------------------------------------------------------------------
+
+using Tensors = std::vector<std::optional<Tensor>>;
+
+// A tensor's (stride, size) pairs from the smallest stride on, without sizes of one.
+std::vector<std::pair<int64_t, int64_t>> steps_of(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> s;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) s.emplace_back(t.stride(d), t.size(d));
+  std::sort(s.begin(), s.end());
+  return s;
+}
+// Whether the elements fill one span of memory, each once, in whatever order.
+bool dense(const Tensor& t) {
+  if (t.is_contiguous()) return true;
+  int64_t need = 1;
+  for (const auto& [stride, size] : steps_of(t)) {
+    if (stride != need) return false;
+    need *= size;
+  }
+  return true;
+}
+// Whether some element may share its place with another.
+bool overlaps_itself(const Tensor& t) {
+  int64_t need = 1;
+  for (const auto& [stride, size] : steps_of(t)) {
+    if (stride < need) return true;
+    need += stride * (size - 1);
+  }
+  return false;
+}
+
+int32_t gradient_code(const Tensor& t, const char* name, size_t i) {
+  const std::string each = std::string(name) + "[" + std::to_string(i) + "]";
+  if (t.layout() != at::kStrided) refuse(each, " must be a dense tensor");
+  return code_of(t, each.c_str());
+}
+
+struct List {
+  std::vector<purin_train_tensor> table;
+  std::vector<std::pair<Tensor, Tensor>> held;  // the copies' owners among them
+  bool wide = false;
+  void add(const Tensor& in, const Tensor& out, int32_t code) {
+    if (!held.empty() && held[0].first.device() != in.device())
+      refuse("gradients must be on one device; got ", held[0].first.device(), " and ", in.device());
+    if (out.device() != in.device()) refuse("out must be on ", in.device(), "; got ", out.device());
+    wide = wide || code == PURIN_TRAIN_F64;
+    table.push_back({in.data_ptr(), out.data_ptr(), in.numel(), code, 0});
+    held.emplace_back(in, out);
+  }
+  Tensor run(double largest, const std::optional<Tensor>& workspace) {
+    const auto dtype = wide ? at::kDouble : at::kFloat;
+    Tensor norm = at::empty({}, held.empty() ? at::TensorOptions().device(at::kCUDA).dtype(dtype)
+                                             : held[0].first.options().dtype(dtype));
+    const int64_t n = (int64_t)table.size();
+    const Call call(norm);
+    const Workspace ws(workspace, purin_train_clip_workspace_bytes(n), norm);
+    check(purin_train_clip(call.stream, n, table.data(), largest, ws.at, ws.size,
+                           wide ? PURIN_TRAIN_F64 : PURIN_TRAIN_F32, norm.data_ptr()));
+    return norm;
+  }
+};
+
+Tensor gradient_norm(const Tensors& gradients, const std::optional<Tensor>& workspace) {
+  const at::NoGradGuard no_grad;
+  List list;
+  for (size_t i = 0; i < gradients.size(); ++i) {
+    if (!gradients[i]) continue;
+    const int32_t code = gradient_code(*gradients[i], "gradients", i);
+    const Tensor g = dense(*gradients[i]) ? *gradients[i] : gradients[i]->contiguous();
+    list.add(g, g, code);
+  }
+  return list.run(-1.0, workspace);
+}
+
+Tensor clip_gradients(const Tensors& gradients, double largest, const std::optional<Tensors>& out,
+                      const std::optional<Tensor>& workspace) {
+  if (!(largest >= 0.0)) refuse("largest must not be negative; got ", largest);
+  const at::NoGradGuard no_grad;
+  const Tensors& outs = out ? *out : gradients;
+  if (outs.size() != gradients.size())
+    refuse("out must hold ", gradients.size(), " tensors; got ", outs.size());
+  List list;
+  std::vector<std::pair<Tensor, Tensor>> back;
+  for (size_t i = 0; i < gradients.size(); ++i) {
+    if (gradients[i].has_value() != outs[i].has_value())
+      refuse("out[", i, "] must be None exactly where the gradient is");
+    if (!gradients[i]) continue;
+    const Tensor &g = *gradients[i], &o = *outs[i];
+    const int32_t code = gradient_code(g, "gradients", i);
+    const bool in_place = o.is_same(g);
+    if (!in_place) {
+      gradient_code(o, "out", i);
+      if (o.sizes() != g.sizes() || o.scalar_type() != g.scalar_type())
+        refuse("out[", i, "] must have shape ", g.sizes(), " and type ", g.scalar_type(), "; got ",
+               o.sizes(), " and ", o.scalar_type());
+    }
+    if (o.is_contiguous() && (in_place || g.is_contiguous())) {
+      list.add(g, o, code);
+    } else if (overlaps_itself(o)) {
+      refuse("out[", i, "] (or the gradient in place) has elements that share memory");
+    } else if (in_place && dense(g)) {
+      list.add(g, g, code);
+    } else {  // any other order goes through a copy in order
+      const Tensor c = at::empty(o.sizes(), o.options().requires_grad(false));
+      list.add(g.contiguous(), c, code);
+      back.emplace_back(o, c);
+    }
+  }
+  const Tensor norm = list.run(largest, workspace);
+  for (auto& [o, c] : back) o.copy_(c);
+  // autograd's check for tensors that changed after they were saved
+  for (const auto& o : outs)
+    if (o && !o->is_inference()) o->unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_front, m) {
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const LibraryError& e) {
+      const py::object type = py::module_::import("purin_amd._lib").attr("PurinError");
+      PyErr_SetObject(type.ptr(), type(e.code, e.message).ptr());
+    }
+  });
+  m.def("route", &route);
+  m.def("route_experts", &route_experts);
+  m.def("dispatch", &dispatch);
+  m.def("combine", &combine);
+  m.def("expert_product", &expert_product);
+  m.def("gradient_norm", &gradient_norm);
+  m.def("clip_gradients", &clip_gradients);
+}
