@@ -139,21 +139,29 @@ static int choose_experts(hipStream_t st, const T* w, int64_t ld, int64_t tokens
   return launch_choose<T, 64, 16>(st, w, ld, tokens, experts, slots, ids, chosen);
 }
 
-// g_weights(t, e) = the sum of g_chosen(t, j) over the slots with ids(t, j) = e (one at most).
+// g_weights(t, e) = g_chosen(t, j) where ids(t, j) = e, 0 elsewhere.  cx threads to a token, its
+// experts cx apart; the token's slots are the same addresses in all of them.
 template <typename T>
 __global__ __launch_bounds__(256) void k_choose_vjp(const int32_t* __restrict__ ids,
                                                     const T* __restrict__ g_chosen,
-                                                    int64_t tokens, int experts, int slots,
+                                                    int64_t tokens, int experts, int slots, int cx,
                                                     T* __restrict__ g_weights) {
-  const int64_t n = tokens * experts, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const int64_t t = i / experts;
-    const int e = (int)(i - t * experts);
-    T g = (T)0;
-    for (int j = 0; j < slots; ++j)
-      if (ids[t * slots + j] == e) g = g_chosen[t * slots + j];
-    g_weights[i] = g;
-  }
+  const int tx = threadIdx.x % cx;
+  const int64_t step = (int64_t)gridDim.x * (256 / cx);
+  for (int64_t t = (int64_t)blockIdx.x * (256 / cx) + threadIdx.x / cx; t < tokens; t += step)
+    for (int e0 = tx; e0 < experts; e0 += 4 * cx) {
+      T g[4] = {(T)0, (T)0, (T)0, (T)0};
+      for (int j = 0; j < slots; ++j) {
+        const int32_t e = ids[t * slots + j];
+        const T v = g_chosen[t * slots + j];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (e == e0 + u * cx) g[u] = v;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (e0 + u * cx < experts) g_weights[t * experts + e0 + u * cx] = g[u];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -310,7 +318,10 @@ static int sort_pairs(hipStream_t st, int64_t pairs, int experts, const int32_t*
 // moving rows
 // ---------------------------------------------------------------------------
 
-// Threads of a workgroup: cx along a row's 16-byte vectors, 256 / cx tokens.
+// Threads of a workgroup: cx along a row's 16-byte vectors, 256 / cx tokens.  From 64 on a
+// wavefront has one token, whose places and weights are then scalar loads: as vector loads, the
+// same address in every lane, they took as long as the rows (8192 tokens of 6 slots, 2048 bf16:
+// 70 us for combine, 41 with scalar loads).
 static int row_threads(int64_t width, int vec) {
   const int64_t n = (width + vec - 1) / vec;
   int cx = 8;
@@ -318,16 +329,25 @@ static int row_threads(int64_t width, int vec) {
   return cx;
 }
 
-template <typename T>
+// This thread's number among its token's, and its token.
+template <bool WIDE>
+__device__ __forceinline__ int64_t first_token(int cx, int& tx) {
+  tx = threadIdx.x % cx;
+  int k = threadIdx.x / cx;
+  if constexpr (WIDE) k = __builtin_amdgcn_readfirstlane(k);
+  return (int64_t)blockIdx.x * (256 / cx) + k;
+}
+
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void k_dispatch(const T* __restrict__ x, int64_t ldx,
                                                   int64_t tokens, int slots, int64_t width,
                                                   int cx, int64_t pairs,
                                                   const int32_t* __restrict__ total,
                                                   const int32_t* __restrict__ place,
                                                   T* __restrict__ rows) {
-  const int tx = threadIdx.x % cx;
+  int tx;
   const int64_t last = max(*total, 0), step = (int64_t)gridDim.x * (256 / cx);
-  for (int64_t t = (int64_t)blockIdx.x * (256 / cx) + threadIdx.x / cx; t < tokens; t += step) {
+  for (int64_t t = first_token<WIDE>(cx, tx); t < tokens; t += step) {
     const int32_t* at = place + t * slots;
     for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
       const Pack<T> v = load_upto(x + t * ldx + c, width - c);
@@ -342,7 +362,16 @@ __global__ __launch_bounds__(256) void k_dispatch(const T* __restrict__ x, int64
   }
 }
 
-template <typename T, bool WEIGHTED>
+// How weights are read: none (ones), 32-bit, or by the type given at the call.
+enum { kOnes = 0, kFloats = 1, kAny = 2 };
+template <typename A, int W>
+__device__ __forceinline__ A weight_at(const void* w, int32_t dtype, int64_t i) {
+  if constexpr (W == kOnes) return A(1);
+  else if constexpr (W == kFloats) return (A) reinterpret_cast<const float*>(w)[i];
+  else return load_weight<A>(w, dtype, i);
+}
+
+template <typename T, bool WIDE, int W>
 __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ rows, int64_t ldr,
                                                  int64_t tokens, int slots, int64_t width, int cx,
                                                  int64_t pairs, const int32_t* __restrict__ place,
@@ -350,58 +379,59 @@ __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ rows, int
                                                  T* __restrict__ out) {
   using A = typename Elem<T>::Acc;
   constexpr int B = 4;  // rows in flight
-  const int tx = threadIdx.x % cx;
+  int tx;
   const int64_t step = (int64_t)gridDim.x * (256 / cx);
-  for (int64_t t = (int64_t)blockIdx.x * (256 / cx) + threadIdx.x / cx; t < tokens; t += step)
-  for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
-    A sum[kVec<T>];
+  for (int64_t t = first_token<WIDE>(cx, tx); t < tokens; t += step)
+    for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
+      A sum[kVec<T>];
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) sum[i] = A(0);
-    for (int j0 = 0; j0 < slots; j0 += B) {
-      Pack<T> v[B];
-      A w[B];
-      bool in[B];
+      for (int i = 0; i < kVec<T>; ++i) sum[i] = A(0);
+      for (int j0 = 0; j0 < slots; j0 += B) {
+        Pack<T> v[B];
+        A w[B];
+        int64_t p[B];
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        const int64_t p = j0 + b < slots ? place[t * slots + j0 + b] : -1;
-        in[b] = p >= 0 && p < pairs;
-        w[b] = A(1);
-        if (in[b]) {
-          v[b] = load_upto(rows + p * ldr + c, width - c);
-          if constexpr (WEIGHTED) w[b] = load_weight<A>(weights, wdtype, t * slots + j0 + b);
+        for (int b = 0; b < B; ++b) {
+          p[b] = j0 + b < slots ? place[t * slots + j0 + b] : -1;
+          if (p[b] >= pairs) p[b] = -1;
+          w[b] = p[b] >= 0 ? weight_at<A, W>(weights, wdtype, t * slots + j0 + b) : A(0);
         }
-      }
 #pragma unroll
-      for (int b = 0; b < B; ++b)
-        if (in[b]) {
+        for (int b = 0; b < B; ++b)
+          if (p[b] >= 0) v[b] = load_upto(rows + p[b] * ldr + c, width - c);
 #pragma unroll
-          for (int i = 0; i < kVec<T>; ++i) {
-            if constexpr (WEIGHTED) sum[i] += w[b] * (A)v[b].v[i];
-            else sum[i] += (A)v[b].v[i];
+        for (int b = 0; b < B; ++b)
+          if (p[b] >= 0) {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) {
+              if constexpr (W == kOnes) sum[i] += (A)v[b].v[i];
+              else sum[i] += w[b] * (A)v[b].v[i];
+            }
           }
-        }
-    }
-    Pack<T> r;
+      }
+      Pack<T> r;
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)sum[i];
-    store_upto(out + t * width + c, r, width - c);
-  }
+      for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)sum[i];
+      store_upto(out + t * width + c, r, width - c);
+    }
 }
 
-// g lanes (a power of two up to 64) to a token.
-template <typename T>
+// cx threads to a token (a power of two); beyond 64 their parts of a sum meet in LDS.
+template <typename T, bool WIDE, int W>
 __global__ __launch_bounds__(256) void k_combine_vjp(
     const T* __restrict__ g_out, int64_t ldg, const T* __restrict__ rows, int64_t ldr,
-    int64_t tokens, int slots, int64_t width, int g, int64_t pairs,
+    int64_t tokens, int slots, int64_t width, int cx, int64_t pairs,
     const int32_t* __restrict__ total, const int32_t* __restrict__ place,
     const void* __restrict__ weights, int32_t wdtype, T* __restrict__ g_rows,
     void* __restrict__ g_weights) {
   using A = typename Elem<T>::Acc;
   constexpr int B = 4;  // slots at once
-  const int tx = threadIdx.x % g;
-  const int64_t last = max(*total, 0), step = (int64_t)gridDim.x * (256 / g);
-  // a token's lanes stay together, so the exchanges below are whole
-  for (int64_t t = (int64_t)blockIdx.x * (256 / g) + threadIdx.x / g; t < tokens; t += step) {
+  __shared__ A part[2][4][B];
+  int tx, turn = 0;
+  const int64_t last = max(*total, 0), step = (int64_t)gridDim.x * (256 / cx);
+  // a token's threads stay together, so the exchanges below are whole; with more than a
+  // wavefront to a token the workgroup has one
+  for (int64_t t = first_token<WIDE>(cx, tx); t < tokens; t += step) {
     for (int j0 = 0; j0 < slots; j0 += B) {
       A w[B], dot[B];
       int64_t at[B];
@@ -409,43 +439,64 @@ __global__ __launch_bounds__(256) void k_combine_vjp(
       for (int b = 0; b < B; ++b) {
         const int64_t p = j0 + b < slots ? place[t * slots + j0 + b] : -1;
         at[b] = p < pairs ? p : -1;
-        dot[b] = w[b] = A(0);
-        if (at[b] >= 0) w[b] = load_weight<A>(weights, wdtype, t * slots + j0 + b);
+        dot[b] = A(0);
+        w[b] = at[b] >= 0 ? weight_at<A, W>(weights, wdtype, t * slots + j0 + b) : A(0);
       }
-      for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)g * kVec<T>) {
+      for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
         const int64_t n = width - c;
         const Pack<T> go = load_upto(g_out + t * ldg + c, n);
         Pack<T> y[B];
+        if (g_weights) {
 #pragma unroll
-        for (int b = 0; b < B; ++b)
-          if (g_weights && at[b] >= 0) y[b] = load_upto(rows + at[b] * ldr + c, n);
+          for (int b = 0; b < B; ++b)
+            if (at[b] >= 0) y[b] = load_upto(rows + at[b] * ldr + c, n);
+        }
+        if (g_rows) {
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-          if (at[b] < 0) continue;
-          if (g_weights) {
-#pragma unroll
-            for (int i = 0; i < kVec<T>; ++i) dot[b] += (A)go.v[i] * (A)y[b].v[i];
-          }
-          if (g_rows) {
+          for (int b = 0; b < B; ++b) {
+            if (at[b] < 0) continue;
             Pack<T> r;
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)(w[b] * (A)go.v[i]);
             store_upto(g_rows + at[b] * width + c, r, n);
           }
         }
+        if (g_weights) {
+#pragma unroll
+          for (int b = 0; b < B; ++b) {
+            if (at[b] < 0) continue;
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) dot[b] += (A)go.v[i] * (A)y[b].v[i];
+          }
+        }
       }
       if (g_weights) {
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-          for (int m = g >> 1; m > 0; m >>= 1) dot[b] += __shfl_xor(dot[b], m, 64);
-          if (tx == 0 && j0 + b < slots)
-            store_weight<A>(g_weights, wdtype, t * slots + j0 + b, dot[b]);
+        for (int b = 0; b < B; ++b)
+          for (int m = min(cx, 64) >> 1; m > 0; m >>= 1) dot[b] += __shfl_xor(dot[b], m, 64);
+        if (cx > 64) {
+          if (tx % 64 == 0) {
+#pragma unroll
+            for (int b = 0; b < B; ++b) part[turn][tx / 64][b] = dot[b];
+          }
+          __syncthreads();
+#pragma unroll
+          for (int b = 0; b < B; ++b) {
+            dot[b] = part[turn][0][b];
+            for (int v = 1; v < 4; ++v) dot[b] += part[turn][v][b];
+          }
+          turn ^= 1;
+        }
+        if (tx == 0) {
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+            if (j0 + b < slots) store_weight<A>(g_weights, wdtype, t * slots + j0 + b, dot[b]);
         }
       }
     }
     if (g_rows)
       for (int64_t p = last + t; p < pairs; p += tokens)
-        for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)g * kVec<T>)
+        for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>)
           store_upto(g_rows + p * width + c, zeros16<T>(), width - c);
   }
 }
@@ -539,9 +590,10 @@ int purin_train_route_vjp(void* stream, int32_t dtype, int64_t tokens, int64_t e
     if (!ids || !g_chosen || !g_weights) return refuse("NULL array");
     return by_dtype(dtype, [&](auto x) {
       using T = decltype(x);
-      const int64_t n = tokens * experts;
-      k_choose_vjp<T><<<grid_of(n, 256), dim3(256), 0, (hipStream_t)stream>>>(
-          ids, (const T*)g_chosen, tokens, (int)experts, (int)slots, (T*)g_weights);
+      int cx = 8;
+      while (cx < 64 && cx * 4 < experts) cx *= 2;
+      k_choose_vjp<T><<<grid_of(tokens, 256 / cx), dim3(256), 0, (hipStream_t)stream>>>(
+          ids, (const T*)g_chosen, tokens, (int)experts, (int)slots, cx, (T*)g_weights);
       return launched("k_choose_vjp");
     });
   });
@@ -560,8 +612,13 @@ int purin_train_dispatch(void* stream, int32_t dtype, int64_t tokens, int64_t ex
     return by_dtype(dtype, [&](auto v) {
       using T = decltype(v);
       const int cx = row_threads(width, kVec<T>);
-      k_dispatch<T><<<grid_of(tokens, 256 / cx), dim3(256), 0, (hipStream_t)stream>>>((const T*)x, ldx, tokens, (int)slots, width, cx,
-                                             tokens * slots, offsets + experts, place, (T*)rows);
+      auto go = [&](auto kernel) {
+        kernel<<<grid_of(tokens, 256 / cx), dim3(256), 0, (hipStream_t)stream>>>(
+            (const T*)x, ldx, tokens, (int)slots, width, cx, tokens * slots, offsets + experts,
+            place, (T*)rows);
+      };
+      if (cx >= 64) go(k_dispatch<T, true>);
+      else go(k_dispatch<T, false>);
       return launched("k_dispatch");
     });
   });
@@ -580,15 +637,21 @@ int purin_train_combine(void* stream, int32_t dtype, int32_t wdtype, int64_t tok
     return by_dtype(dtype, [&](auto v) {
       using T = decltype(v);
       const int cx = row_threads(width, kVec<T>);
-      const dim3 grid = grid_of(tokens, 256 / cx);
-      if (weights)
-        k_combine<T, true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
+      auto go = [&](auto kernel) {
+        kernel<<<grid_of(tokens, 256 / cx), dim3(256), 0, (hipStream_t)stream>>>(
             (const T*)rows, ldr, tokens, (int)slots, width, cx, tokens * slots, place, weights,
             wdtype, (T*)out);
-      else
-        k_combine<T, false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(
-            (const T*)rows, ldr, tokens, (int)slots, width, cx, tokens * slots, place, nullptr, 0,
-            (T*)out);
+      };
+      if (cx < 64) {
+        if (weights) go(k_combine<T, false, kAny>);
+        else go(k_combine<T, false, kOnes>);
+      } else if (!weights) {
+        go(k_combine<T, true, kOnes>);
+      } else if (wdtype == PURIN_TRAIN_F32) {
+        go(k_combine<T, true, kFloats>);
+      } else {
+        go(k_combine<T, true, kAny>);
+      }
       return launched("k_combine");
     });
   });
@@ -610,10 +673,18 @@ int purin_train_combine_vjp(void* stream, int32_t dtype, int32_t wdtype, int64_t
       return refuse("a row pitch is below the width");
     return by_dtype(dtype, [&](auto v) {
       using T = decltype(v);
-      const int g = std::min(64, row_threads(width, kVec<T>));
-      k_combine_vjp<T><<<grid_of(tokens, 256 / g), dim3(256), 0, (hipStream_t)stream>>>(
-          (const T*)g_out, ldg, (const T*)rows, ldr, tokens, (int)slots, width, g, tokens * slots,
-          offsets + experts, place, weights, wdtype, (T*)g_rows, g_weights);
+      // a wavefront to a token; a workgroup where the tokens' wavefronts would leave most of the
+      // 256 CUs' room empty
+      int cx = row_threads(width, kVec<T>);
+      if (cx > 64) cx = cx == 256 && tokens < 2048 ? 256 : 64;
+      auto go = [&](auto kernel) {
+        kernel<<<grid_of(tokens, 256 / cx), dim3(256), 0, (hipStream_t)stream>>>(
+            (const T*)g_out, ldg, (const T*)rows, ldr, tokens, (int)slots, width, cx,
+            tokens * slots, offsets + experts, place, weights, wdtype, (T*)g_rows, g_weights);
+      };
+      if (cx < 64) go(k_combine_vjp<T, false, kAny>);
+      else if (wdtype == PURIN_TRAIN_F32) go(k_combine_vjp<T, true, kFloats>);
+      else go(k_combine_vjp<T, true, kAny>);
       return launched("k_combine_vjp");
     });
   });
