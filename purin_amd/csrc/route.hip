@@ -11,6 +11,7 @@
 // wavefront come from ballots on the expert's bits, so the order is the pairs' own.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "train.hpp"
 
@@ -55,6 +56,29 @@ struct Key<double> {
   static __device__ __forceinline__ double value(K k) { return __builtin_bit_cast(double, k); }
 };
 
+// The value of the lane N further on in the 16 (around), without a trip through LDS.
+template <int N>
+__device__ __forceinline__ uint32_t around16(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xf, 0xf, true);
+}
+template <int N>
+__device__ __forceinline__ uint64_t around16(uint64_t v) {
+  return ((uint64_t)around16<N>((uint32_t)(v >> 32)) << 32) | around16<N>((uint32_t)v);
+}
+// The largest value of a group of G lanes (16 or all 64), in all of them.
+template <int G, typename K>
+__device__ __forceinline__ K group_max(K v) {
+  v = max(v, around16<8>(v));
+  v = max(v, around16<4>(v));
+  v = max(v, around16<2>(v));
+  v = max(v, around16<1>(v));
+  if constexpr (G == 64) {
+    v = max(v, (K)__shfl_xor(v, 16, 64));
+    v = max(v, (K)__shfl_xor(v, 32, 64));
+  }
+  return v;
+}
+
 // G lanes to a token, V weights to a lane (expert i * G + lane): slots times, the lanes'
 // best by (weight, lowest expert), then the group's.
 template <typename T, int G, int V>
@@ -78,16 +102,10 @@ __device__ __forceinline__ void choose(const T* row, int experts, int slots, int
         best = key[i];
         at = i;
       }
-    int e = at * G + lane;
-#pragma unroll
-    for (int m = 1; m < G; m <<= 1) {
-      const K other = __shfl_xor(best, m, 64);
-      const int oe = __shfl_xor(e, m, 64);
-      if (other > best || (other == best && oe < e)) {
-        best = other;
-        e = oe;
-      }
-    }
+    // the largest weight, then the lowest expert that has it (the largest of the complements)
+    const K top = group_max<G>(best);
+    const int e = (int)~group_max<G>(best == top ? ~(uint32_t)(at * G + lane) : 0u);
+    best = top;
     const int owner = e / G;  // the winner's register, in lane e % G
     if (best != 0 && e % G == lane) {
 #pragma unroll
@@ -119,24 +137,17 @@ __global__ __launch_bounds__(256) void k_choose(const T* __restrict__ weights, i
     choose<T, G, V>(weights + t * ld, experts, slots, lane, ids + t * slots, chosen + t * slots);
 }
 
-template <typename T, int G, int V>
-static int launch_choose(hipStream_t st, const T* w, int64_t ld, int64_t tokens, int experts,
-                         int slots, int32_t* ids, T* chosen) {
-  k_choose<T, G, V><<<grid_of(tokens, 256 / G), dim3(256), 0, st>>>(
-      w, ld, tokens, experts, slots, ids, chosen);
-  return launched("k_choose");
-}
-
-template <typename T>
-static int choose_experts(hipStream_t st, const T* w, int64_t ld, int64_t tokens, int experts,
-                          int slots, int32_t* ids, T* chosen) {
-  // the fewest lanes that hold a token's weights in at most 16 registers: fewer lanes, fewer
-  // exchanges
-  if (experts <= 32) return launch_choose<T, 16, 2>(st, w, ld, tokens, experts, slots, ids, chosen);
-  if (experts <= 64) return launch_choose<T, 16, 4>(st, w, ld, tokens, experts, slots, ids, chosen);
-  if (experts <= 128) return launch_choose<T, 16, 8>(st, w, ld, tokens, experts, slots, ids, chosen);
-  if (experts <= 256) return launch_choose<T, 16, 16>(st, w, ld, tokens, experts, slots, ids, chosen);
-  return launch_choose<T, 64, 16>(st, w, ld, tokens, experts, slots, ids, chosen);
+// Calls f with the fewest lanes that hold a token's weights in at most 16 registers each: fewer
+// lanes, fewer exchanges.
+template <typename F>
+static int by_lanes(int experts, F&& f) {
+  using std::integral_constant;
+  constexpr integral_constant<int, 16> g16;
+  if (experts <= 32) return f(g16, integral_constant<int, 2>{});
+  if (experts <= 64) return f(g16, integral_constant<int, 4>{});
+  if (experts <= 128) return f(g16, integral_constant<int, 8>{});
+  if (experts <= 256) return f(g16, g16);
+  return f(integral_constant<int, 64>{}, g16);
 }
 
 // g_weights(t, e) = g_chosen(t, j) where ids(t, j) = e, 0 elsewhere.  cx threads to a token, its
@@ -199,16 +210,14 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const int32_t* __re
 // Places the pairs of one chunk: expert e's rows begin at the sum of all smaller experts'
 // counts; the chunk's first pair of e follows the earlier chunks' pairs of e, a wavefront's
 // first the earlier wavefronts'.  LDS: per-wavefront running places [kSortWaves][experts].
-__global__ __launch_bounds__(kSortThreads) void k_sort_place(
-    const int32_t* __restrict__ ids, int64_t pairs, int experts, int bits, int64_t chunk,
-    const int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
-    int32_t* __restrict__ place, int32_t* __restrict__ source) {
-  extern __shared__ int32_t run[];
+__device__ __forceinline__ void place_chunk(const int32_t* ids, int64_t pairs, int experts,
+                                            int bits, int64_t chunk, int groups, int group,
+                                            const int32_t* counts, int32_t* run, int32_t* offsets,
+                                            int32_t* place, int32_t* source) {
   __shared__ int32_t total[PURIN_TRAIN_MAX_EXPERTS];
   __shared__ int32_t before[PURIN_TRAIN_MAX_EXPERTS];
   __shared__ int32_t wave_sum[kSortWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int groups = (int)gridDim.x, group = (int)blockIdx.x;
   for (int e = tid; e < experts; e += kSortThreads) total[e] = before[e] = 0;
   for (int i = tid; i < kSortWaves * experts; i += kSortThreads) run[i] = 0;
   __syncthreads();
@@ -296,17 +305,51 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(
   for (int64_t i = max<int64_t>(from, all) + tid; i < to; i += kSortThreads) source[i] = -1;
 }
 
+__global__ __launch_bounds__(kSortThreads) void k_sort_place(
+    const int32_t* __restrict__ ids, int64_t pairs, int experts, int bits, int64_t chunk,
+    const int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
+    int32_t* __restrict__ place, int32_t* __restrict__ source) {
+  extern __shared__ int32_t run[];
+  place_chunk(ids, pairs, experts, bits, chunk, (int)gridDim.x, (int)blockIdx.x, counts, run,
+              offsets, place, source);
+}
+
+// Both parts of a small route in one workgroup.
+template <typename T, int G, int V>
+__global__ __launch_bounds__(kSortThreads) void k_route(const T* __restrict__ weights, int64_t ld,
+                                                        int64_t tokens, int experts, int slots,
+                                                        int bits, int64_t chunk, int32_t* ids,
+                                                        T* __restrict__ chosen,
+                                                        int32_t* __restrict__ offsets,
+                                                        int32_t* __restrict__ place,
+                                                        int32_t* __restrict__ source) {
+  extern __shared__ int32_t run[];
+  const int lane = threadIdx.x % G;
+  for (int64_t t = threadIdx.x / G; t < tokens; t += kSortThreads / G)
+    choose<T, G, V>(weights + t * ld, experts, slots, lane, ids + t * slots, chosen + t * slots);
+  __syncthreads();  // the choices are written and seen
+  place_chunk(ids, tokens * slots, experts, bits, chunk, 1, 0, nullptr, run, offsets, place,
+              source);
+}
+
+// Bits of the keys 0 .. experts, the last of which stands for none.
+static int key_bits(int experts) {
+  int bits = 1;
+  while ((1 << bits) <= experts) ++bits;
+  return bits;
+}
+static size_t sort_lds(int experts) { return (size_t)kSortWaves * experts * sizeof(int32_t); }
+
 static int sort_pairs(hipStream_t st, int64_t pairs, int experts, const int32_t* ids, void* ws,
                       int32_t* offsets, int32_t* place, int32_t* source) {
   const SortShape s = sort_shape(pairs);
-  int bits = 1;
-  while ((1 << bits) <= experts) ++bits;  // the key ``experts`` stands for none
+  const int bits = key_bits(experts);
   if (s.groups > 1) {
     k_sort_count<<<dim3((unsigned)s.groups), dim3(kSortThreads), 0, st>>>(
         ids, pairs, experts, s.chunk, (int32_t*)ws);
     if (int rc = launched("k_sort_count")) return rc;
   }
-  const size_t lds = (size_t)kSortWaves * experts * sizeof(int32_t);
+  const size_t lds = sort_lds(experts);
   if (lds > 32 * 1024)
     if (int rc = raise_lds_cap((const void*)k_sort_place, lds)) return rc;
   k_sort_place<<<dim3((unsigned)s.groups), dim3(kSortThreads), lds, st>>>(
@@ -321,7 +364,7 @@ static int sort_pairs(hipStream_t st, int64_t pairs, int experts, const int32_t*
 // Threads of a workgroup: cx along a row's 16-byte vectors, 256 / cx tokens.  From 64 on a
 // wavefront has one token, whose places and weights are then scalar loads: as vector loads, the
 // same address in every lane, they took as long as the rows (8192 tokens of 6 slots, 2048 bf16:
-// 70 us for combine, 41 with scalar loads).
+// 70 us for combine, 65 with scalar loads).
 static int row_threads(int64_t width, int vec) {
   const int64_t n = (width + vec - 1) / vec;
   int cx = 8;
@@ -381,38 +424,54 @@ __global__ __launch_bounds__(256) void k_combine(const T* __restrict__ rows, int
   constexpr int B = 4;  // rows in flight
   int tx;
   const int64_t step = (int64_t)gridDim.x * (256 / cx);
+  // one 16-byte column: ``load`` reads it of a row
+  auto column = [&](int64_t t, auto&& load) {
+    Pack<T> r;
+    A sum[kVec<T>];
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) sum[i] = A(0);
+    for (int j0 = 0; j0 < slots; j0 += B) {
+      Pack<T> v[B];
+      A w[B];
+      int64_t p[B], any = -1;
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        // read without a condition, so that one wait covers them all
+        const int64_t i = t * slots + min(j0 + b, slots - 1);
+        p[b] = place[i];
+        w[b] = weight_at<A, W>(weights, wdtype, i);
+      }
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (j0 + b >= slots || p[b] >= pairs) p[b] = -1;
+        if (p[b] >= 0) any = p[b];
+      }
+      if (any < 0) continue;
+      // the loads go out together: an empty slot's reads a row that another slot reads
+#pragma unroll
+      for (int b = 0; b < B; ++b) v[b] = load(p[b] >= 0 ? p[b] : any);
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (p[b] >= 0) {
+#pragma unroll
+          for (int i = 0; i < kVec<T>; ++i) {
+            if constexpr (W == kOnes) sum[i] += (A)v[b].v[i];
+            else sum[i] += w[b] * (A)v[b].v[i];
+          }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)sum[i];
+    return r;
+  };
   for (int64_t t = first_token<WIDE>(cx, tx); t < tokens; t += step)
     for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
-      A sum[kVec<T>];
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) sum[i] = A(0);
-      for (int j0 = 0; j0 < slots; j0 += B) {
-        Pack<T> v[B];
-        A w[B];
-        int64_t p[B];
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-          p[b] = j0 + b < slots ? place[t * slots + j0 + b] : -1;
-          if (p[b] >= pairs) p[b] = -1;
-          w[b] = p[b] >= 0 ? weight_at<A, W>(weights, wdtype, t * slots + j0 + b) : A(0);
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b)
-          if (p[b] >= 0) v[b] = load_upto(rows + p[b] * ldr + c, width - c);
-#pragma unroll
-        for (int b = 0; b < B; ++b)
-          if (p[b] >= 0) {
-#pragma unroll
-            for (int i = 0; i < kVec<T>; ++i) {
-              if constexpr (W == kOnes) sum[i] += (A)v[b].v[i];
-              else sum[i] += w[b] * (A)v[b].v[i];
-            }
-          }
-      }
-      Pack<T> r;
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)sum[i];
-      store_upto(out + t * width + c, r, width - c);
+      const int n = (int)min<int64_t>(width - c, kVec<T>);
+      if (n == kVec<T>)
+        store16(out + t * width + c, column(t, [&](int64_t p) { return load16(rows + p * ldr + c); }));
+      else
+        store_some(out + t * width + c,
+                   column(t, [&](int64_t p) { return load_some(rows + p * ldr + c, n); }), n);
     }
 }
 
@@ -437,19 +496,25 @@ __global__ __launch_bounds__(256) void k_combine_vjp(
       int64_t at[B];
 #pragma unroll
       for (int b = 0; b < B; ++b) {
-        const int64_t p = j0 + b < slots ? place[t * slots + j0 + b] : -1;
-        at[b] = p < pairs ? p : -1;
+        const int64_t i = t * slots + min(j0 + b, slots - 1);  // no condition: one wait for all
+        at[b] = place[i];
+        w[b] = weight_at<A, W>(weights, wdtype, i);
         dot[b] = A(0);
-        w[b] = at[b] >= 0 ? weight_at<A, W>(weights, wdtype, t * slots + j0 + b) : A(0);
       }
-      for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
-        const int64_t n = width - c;
-        const Pack<T> go = load_upto(g_out + t * ldg + c, n);
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (j0 + b >= slots || at[b] >= pairs) at[b] = -1;
+      int64_t any = -1;
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (at[b] >= 0) any = at[b];
+      // one 16-byte column; an empty slot's load is of a row that another slot reads
+      auto column = [&](auto&& load, auto&& store, int64_t c) {
+        const Pack<T> go = load(g_out + t * ldg + c);
         Pack<T> y[B];
         if (g_weights) {
 #pragma unroll
-          for (int b = 0; b < B; ++b)
-            if (at[b] >= 0) y[b] = load_upto(rows + at[b] * ldr + c, n);
+          for (int b = 0; b < B; ++b) y[b] = load(rows + (at[b] >= 0 ? at[b] : any) * ldr + c);
         }
         if (g_rows) {
 #pragma unroll
@@ -458,7 +523,7 @@ __global__ __launch_bounds__(256) void k_combine_vjp(
             Pack<T> r;
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) r.v[i] = (T)(w[b] * (A)go.v[i]);
-            store_upto(g_rows + at[b] * width + c, r, n);
+            store(g_rows + at[b] * width + c, r);
           }
         }
         if (g_weights) {
@@ -469,7 +534,17 @@ __global__ __launch_bounds__(256) void k_combine_vjp(
             for (int i = 0; i < kVec<T>; ++i) dot[b] += (A)go.v[i] * (A)y[b].v[i];
           }
         }
-      }
+      };
+      if (any >= 0)
+        for (int64_t c = (int64_t)tx * kVec<T>; c < width; c += (int64_t)cx * kVec<T>) {
+          const int n = (int)min<int64_t>(width - c, kVec<T>);
+          if (n == kVec<T>)
+            column([](const T* p) { return load16(p); },
+                   [](T* p, const Pack<T>& v) { store16(p, v); }, c);
+          else
+            column([n](const T* p) { return load_some(p, n); },
+                   [n](T* p, const Pack<T>& v) { store_some(p, v, n); }, c);
+        }
       if (g_weights) {
 #pragma unroll
         for (int b = 0; b < B; ++b)
@@ -545,13 +620,31 @@ int purin_train_route(void* stream, int32_t dtype, int64_t tokens, int64_t exper
                                  purin_train_route_workspace_bytes(tokens, experts, slots)))
       return rc;
     hipStream_t st = (hipStream_t)stream;
+    const SortShape s = sort_shape(tokens * slots);
+    const int bits = key_bits((int)experts);
+    // one workgroup for both parts where each of its lane groups has few tokens (four at most):
+    // one launch for two (1 token of 64 experts: 5.6 us for 3 and 4 in two launches)
+    const bool small = s.groups == 1 && tokens * (experts > 256 ? 64 : 16) <= 4 * kSortThreads;
     if (tokens) {
       const int rc = by_dtype(dtype, [&](auto x) {
         using T = decltype(x);
-        return choose_experts<T>(st, (const T*)weights, ld, tokens, (int)experts, (int)slots, ids,
-                                 (T*)chosen);
+        return by_lanes((int)experts, [&](auto gg, auto vv) {
+          constexpr int G = gg, V = vv;
+          if (small) {
+            const size_t lds = sort_lds((int)experts);
+            if (lds > 32 * 1024)
+              if (int e = raise_lds_cap((const void*)k_route<T, G, V>, lds)) return e;
+            k_route<T, G, V><<<dim3(1), dim3(kSortThreads), lds, st>>>(
+                (const T*)weights, ld, tokens, (int)experts, (int)slots, bits, s.chunk, ids,
+                (T*)chosen, offsets, place, source);
+            return launched("k_route");
+          }
+          k_choose<T, G, V><<<grid_of(tokens, 256 / G), dim3(256), 0, st>>>(
+              (const T*)weights, ld, tokens, (int)experts, (int)slots, ids, (T*)chosen);
+          return launched("k_choose");
+        });
       });
-      if (rc) return rc;
+      if (rc || small) return rc;
     }
     return sort_pairs(st, tokens * slots, (int)experts, ids, workspace, offsets, place, source);
   });
