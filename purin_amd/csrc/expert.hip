@@ -91,11 +91,21 @@ __device__ __forceinline__ void tile_order(int64_t tiles_m, int64_t tiles_n, int
   tn = in / high;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool ALONG_B, bool DIRECT>
+// The part of a contraction of ``depth`` that split number ``split`` of ``splits`` has: whole
+// stages of kDepth16, the last one's end apart.
+__device__ __forceinline__ void part_of(int64_t depth, int split, int splits, int64_t& first,
+                                        int64_t& length) {
+  const int64_t steps = (depth + kDepth16 - 1) / kDepth16, per = (steps + splits - 1) / splits;
+  first = min(depth, split * per * kDepth16);
+  length = min(depth - first, per * kDepth16);
+}
+
+// Split number blockIdx.y of the contraction writes its own ``out`` (rows x outer).
+template <typename T, typename C, int BM, int BN, int WM, int WN, bool ALONG_B, bool DIRECT, int S>
 __global__ __launch_bounds__(WM* WN * 64) void k_product16(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
     int64_t rows, int64_t inner, int64_t outer, int experts, int64_t tiles_m, int64_t tiles_n,
-    const int32_t* __restrict__ offsets, T* __restrict__ out, int64_t ldo) {
+    const int32_t* __restrict__ offsets, C* __restrict__ out, int64_t ldo) {
   extern __shared__ __align__(16) unsigned char lds16[];
   int64_t tm, tn;
   tile_order(tiles_m, tiles_n, tm, tn);
@@ -106,13 +116,42 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product16(
   const int64_t col = tn * BN;
   const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
   const int n = (int)min<int64_t>(BN, outer - col);
+  C* c = out + (int64_t)blockIdx.y * rows * ldo + from * ldo + col;
   if (e < 0) {
-    zero_tile(out + from * ldo + col, ldo, m, n);
+    zero_tile(c, ldo, m, n);
     return;
   }
-  tile16<T, BM, BN, WM, WN, true, ALONG_B, DIRECT>(
-      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner,
-      (T*)lds16, out + from * ldo + col, ldo);
+  int64_t k, length;
+  part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
+  tile16<T, C, BM, BN, WM, WN, true, ALONG_B, DIRECT, S>(
+      {a + from * lda + k, lda, m},
+      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n}, length, lds16, c, ldo);
+}
+
+// out = the sum of ``splits`` parts, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, int splits,
+                                              int64_t count, T* __restrict__ out) {
+  constexpr int V = 4;
+  typedef float F __attribute__((ext_vector_type(V), aligned(4)));
+  const int64_t step = (int64_t)gridDim.x * 256 * V;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < count; i += step) {
+    if (i + V <= count) {
+      F sum = *reinterpret_cast<const F*>(parts + i);
+      for (int s = 1; s < splits; ++s) sum += *reinterpret_cast<const F*>(parts + s * count + i);
+      typedef T O __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+      O v;
+#pragma unroll
+      for (int q = 0; q < V; ++q) v[q] = (T)sum[q];
+      *reinterpret_cast<O*>(out + i) = v;
+    } else {
+      for (int64_t j = i; j < count; ++j) {
+        float sum = parts[j];
+        for (int s = 1; s < splits; ++s) sum += parts[s * count + j];
+        out[j] = (T)sum;
+      }
+    }
+  }
 }
 
 // Experts with few rows: every column tile of one expert's weights is read once, by a workgroup
@@ -140,22 +179,25 @@ __global__ __launch_bounds__(256) void k_product_thin(
       out + from * ldo + col, ldo);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool DIRECT>
+// Split number blockIdx.z of an expert's rows writes its own ``gw`` (experts x inner x outer).
+template <typename T, typename C, int BM, int BN, int WM, int WN, bool DIRECT, int S>
 __global__ __launch_bounds__(WM* WN * 64) void k_weights_vjp16(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ g, int64_t ldg, int64_t rows,
     int64_t inner, int64_t outer, int64_t tiles_m, int64_t tiles_n,
-    const int32_t* __restrict__ offsets, T* __restrict__ gw) {
+    const int32_t* __restrict__ offsets, C* __restrict__ gw) {
   extern __shared__ __align__(16) unsigned char lds16[];
   int64_t tm, tn;
   tile_order(tiles_m, tiles_n, tm, tn);
   const int e = (int)blockIdx.y;
-  int64_t from, to;
+  int64_t from, to, k, length;
   segment(offsets, e, rows, from, to);
+  part_of(to - from, (int)blockIdx.z, (int)gridDim.z, k, length);
+  from += k;
   const int64_t i = tm * BM, j = tn * BN;
-  tile16<T, BM, BN, WM, WN, false, false, DIRECT>(
+  tile16<T, C, BM, BN, WM, WN, false, false, DIRECT, S>(
       {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i)},
-      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, to - from, (T*)lds16,
-      gw + e * inner * outer + i * outer + j, outer);
+      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, length, lds16,
+      gw + ((int64_t)blockIdx.z * gridDim.y + e) * inner * outer + i * outer + j, outer);
 }
 
 // 32- and 64-bit types.
@@ -216,22 +258,65 @@ static bool direct_ok(const void* p, int64_t ld, int64_t length) {
          ld < (int64_t(1) << 21);
 }
 
+using std::integral_constant;
+constexpr integral_constant<int, 1> i1;
+constexpr integral_constant<int, 2> i2;
+constexpr integral_constant<int, 4> i4;
+constexpr integral_constant<int, 32> i32;
+constexpr integral_constant<int, 64> i64;
+constexpr integral_constant<int, 128> i128;
+constexpr integral_constant<int, 256> i256;
+
 // The most tiles of ``height`` rows that any split of the rows over the experts needs, the rows
 // behind the last expert among them.
 static int64_t most_tiles(int64_t rows, int64_t experts, int64_t height) {
   return (rows + std::min(rows, experts + 1) * (height - 1)) / height;
 }
 
+// How the 16-bit kernels cut a product of ``tiles`` 128 x 128 tiles, each ``steps`` stages long.
+//   large   256 x 256 tiles: half the LDS reads and operand traffic of 128 x 128; from 4 to a CU
+//           on (of 128 x 128: 16) its single workgroup a CU does not leave CUs idle at the end.
+//           32768 x 2048 x 4096: 600 us, 128 x 128 tiles 660; 2048 x 2048 x 2048: 57 and 35
+//   deep    up to one 128 x 128 tile a CU there is room for 4 stages, three on their way: the
+//           stages' latency is what counts then.  With more tiles, two workgroups of 2 stages
+//   splits  where even so CUs are idle and the contraction is long, parts of at least kPart
+//           stages into 32-bit sums, and a second kernel that adds them up
+struct Cut16 {
+  bool large, deep;
+  int splits;
+};
+constexpr int64_t kPart = 12;
+static Cut16 cut16(int64_t tiles, int64_t steps) {
+  if (tiles >= 16 * 256) return {true, false, 1};
+  int64_t splits = 1;
+  if (tiles <= 128) splits = std::max<int64_t>(1, std::min(256 / std::max<int64_t>(tiles, 1), steps / kPart));
+  return {false, tiles * splits <= 256, (int)splits};
+}
+static int64_t steps16(int64_t depth) { return (depth + kDepth16 - 1) / kDepth16; }
+static Cut16 cut_product16(int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
+  return cut16(most_tiles(rows, experts, 128) * ((outer + 127) / 128), steps16(inner));
+}
+static Cut16 cut_weights16(int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
+  return cut16(((inner + 127) / 128) * ((outer + 127) / 128) * experts, steps16(rows / experts));
+}
+static bool thin16(int64_t rows, int64_t experts) { return rows <= 32 * experts; }
+
+// The ``splits`` parts of ``count`` sums added up into out.
+template <typename T>
+static int join(hipStream_t st, const float* parts, int splits, int64_t count, T* out) {
+  k_join<T><<<grid_of(count, 1024), dim3(256), 0, st>>>(parts, splits, count, out);
+  return launched("k_join");
+}
+
 template <typename T>
 static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
                      const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,
-                     const int32_t* offsets, T* out, int64_t ldo) {
-  constexpr int BM = 256, BN = 256;
+                     const int32_t* offsets, void* ws, T* out, int64_t ldo) {
   const bool along = wi == 1 && (wo != 1 || inner > 1);
   const int64_t ldw = along ? wo : wi;
   const bool direct = direct_ok(a, lda, inner) && direct_ok(w, ldw, along ? inner : outer) &&
                       we % 8 == 0;
-  if (rows <= 32 * experts) {
+  if (thin16(rows, experts)) {
     constexpr int TN = 64;
     const int64_t tn = (outer + TN - 1) / TN;
     auto thin = [&](auto kernel) {
@@ -244,32 +329,53 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
     return direct ? thin(k_product_thin<T, TN, false, true>)
                   : thin(k_product_thin<T, TN, false, false>);
   }
-  const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + BN - 1) / BN;
-  auto go = [&](auto kernel) {
-    return launch16("k_product16", kernel, dim3((unsigned)(tm * tn)), 512,
-                    2 * (BM + BN) * kDepth16 * 2, st, a, lda, w, we, ldw, rows, inner, outer,
-                    (int)experts, tm, tn, offsets, out, ldo);
+  Cut16 cut = cut_product16(rows, inner, outer, experts);
+  if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
+  auto go = [&](auto c, auto bm, auto wn, auto s) {
+    using C = decltype(c);
+    constexpr int B = bm, WN = wn, S = s;
+    const int64_t tm = most_tiles(rows, experts, B), tn = (outer + B - 1) / B;
+    C* to = cut.splits > 1 ? (C*)ws : (C*)out;
+    const int64_t ldc = cut.splits > 1 ? outer : ldo;
+    auto kernel = along ? (direct ? k_product16<T, C, B, B, 2, WN, true, true, S>
+                                  : k_product16<T, C, B, B, 2, WN, true, false, S>)
+                        : (direct ? k_product16<T, C, B, B, 2, WN, false, true, S>
+                                  : k_product16<T, C, B, B, 2, WN, false, false, S>);
+    return launch16("k_product16", kernel, dim3((unsigned)(tm * tn), (unsigned)cut.splits),
+                    2 * WN * 64, tile16_lds<T, C, B, B, S>(), st, a, lda, w, we, ldw, rows, inner,
+                    outer, (int)experts, tm, tn, offsets, to, ldc);
   };
-  if (along) return direct ? go(k_product16<T, BM, BN, 2, 4, true, true>)
-                           : go(k_product16<T, BM, BN, 2, 4, true, false>);
-  return direct ? go(k_product16<T, BM, BN, 2, 4, false, true>)
-                : go(k_product16<T, BM, BN, 2, 4, false, false>);
+  if (cut.splits > 1) {
+    if (int rc = go(float{}, i128, i2, i4)) return rc;
+    return join(st, (const float*)ws, cut.splits, rows * outer, out);
+  }
+  if (cut.large) return go(T{}, i256, i4, i2);
+  return cut.deep ? go(T{}, i128, i2, i4) : go(T{}, i128, i2, i2);
 }
 
 template <typename T>
 static int weights_vjp16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
                          int64_t experts, const T* a, int64_t lda, const T* g, int64_t ldg,
-                         const int32_t* offsets, T* gw) {
-  constexpr int BM = 256, BN = 256;
+                         const int32_t* offsets, void* ws, T* gw) {
   const bool direct = direct_ok(a, lda, inner) && direct_ok(g, ldg, outer);
-  const int64_t tm = (inner + BM - 1) / BM, tn = (outer + BN - 1) / BN;
-  auto go = [&](auto kernel) {
-    return launch16("k_weights_vjp16", kernel, dim3((unsigned)(tm * tn), (unsigned)experts), 512,
-                    2 * (BM + BN) * kDepth16 * 2, st, a, lda, g, ldg, rows, inner, outer, tm, tn,
-                    offsets, gw);
+  const Cut16 cut = cut_weights16(rows, inner, outer, experts);
+  auto go = [&](auto c, auto bm, auto wn, auto s) {
+    using C = decltype(c);
+    constexpr int B = bm, WN = wn, S = s;
+    const int64_t tm = (inner + B - 1) / B, tn = (outer + B - 1) / B;
+    auto kernel = direct ? k_weights_vjp16<T, C, B, B, 2, WN, true, S>
+                         : k_weights_vjp16<T, C, B, B, 2, WN, false, S>;
+    return launch16("k_weights_vjp16", kernel,
+                    dim3((unsigned)(tm * tn), (unsigned)experts, (unsigned)cut.splits), 2 * WN * 64,
+                    tile16_lds<T, C, B, B, S>(), st, a, lda, g, ldg, rows, inner, outer, tm, tn,
+                    offsets, cut.splits > 1 ? (C*)ws : (C*)gw);
   };
-  return direct ? go(k_weights_vjp16<T, BM, BN, 2, 4, true>)
-                : go(k_weights_vjp16<T, BM, BN, 2, 4, false>);
+  if (cut.splits > 1) {
+    if (int rc = go(float{}, i128, i2, i4)) return rc;
+    return join(st, (const float*)ws, cut.splits, experts * inner * outer, gw);
+  }
+  if (cut.large) return go(T{}, i256, i4, i2);
+  return cut.deep ? go(T{}, i128, i2, i4) : go(T{}, i128, i2, i2);
 }
 
 template <typename T>
@@ -289,13 +395,6 @@ static int product32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
     return along ? go(BM, BN, k_product32<T, BM, BN, WM, WN, true>)
                  : go(BM, BN, k_product32<T, BM, BN, WM, WN, false>);
   };
-  using std::integral_constant;
-  constexpr integral_constant<int, 1> i1;
-  constexpr integral_constant<int, 2> i2;
-  constexpr integral_constant<int, 4> i4;
-  constexpr integral_constant<int, 32> i32;
-  constexpr integral_constant<int, 64> i64;
-  constexpr integral_constant<int, 128> i128;
   if (rows <= 32 * experts) return shape(i32, i64, i1, i4);
   // large tiles where they fill the 256 CUs twice
   if constexpr (sizeof(T) == 4)
@@ -349,6 +448,10 @@ int64_t purin_train_expert_product_workspace_bytes(int32_t dtype, int64_t rows, 
   (void)guarded([&] {
     if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
     need = 0;
+    if (dtype_bytes(dtype) == 2 && rows && outer && !thin16(rows, experts)) {
+      const int splits = cut_product16(rows, inner, outer, experts).splits;
+      if (splits > 1) need = splits * rows * outer * (int64_t)sizeof(float);
+    }
     return (int)PURIN_CP_OK;
   });
   return need;
@@ -368,11 +471,15 @@ int purin_train_expert_product(void* stream, int32_t dtype, int64_t rows, int64_
     if (wi != 1 && wo != 1 && inner > 1 && outer > 1)
       return refuse("the weight needs a unit stride along inner or outer");
     if (we < 0 || wi < 0 || wo < 0) return refuse("the weight's strides must not be negative");
+    if (int rc = check_workspace(workspace, workspace_bytes,
+                                 purin_train_expert_product_workspace_bytes(dtype, rows, inner,
+                                                                            outer, experts)))
+      return rc;
     return by_dtype(dtype, [&](auto v) {
       using T = decltype(v);
       if constexpr (sizeof(T) == 2)
         return product16<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
-                            (const T*)weight, we, wi, wo, offsets, (T*)out, ldo);
+                            (const T*)weight, we, wi, wo, offsets, workspace, (T*)out, ldo);
       else
         return product32<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
                             (const T*)weight, we, wi, wo, offsets, (T*)out, ldo);
@@ -386,6 +493,10 @@ int64_t purin_train_expert_weights_vjp_workspace_bytes(int32_t dtype, int64_t ro
   (void)guarded([&] {
     if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
     need = 0;
+    if (dtype_bytes(dtype) == 2 && inner && outer) {
+      const int splits = cut_weights16(rows, inner, outer, experts).splits;
+      if (splits > 1) need = splits * experts * inner * outer * (int64_t)sizeof(float);
+    }
     return (int)PURIN_CP_OK;
   });
   return need;
@@ -401,11 +512,15 @@ int purin_train_expert_weights_vjp(void* stream, int32_t dtype, int64_t rows, in
     if (!offsets || !g_weight || (rows && (!a || !g))) return refuse("NULL array");
     if (rows > 1 && (lda < inner || ldg < outer))
       return refuse("a row pitch is below the row's length");
+    if (int rc = check_workspace(workspace, workspace_bytes,
+                                 purin_train_expert_weights_vjp_workspace_bytes(
+                                     dtype, rows, inner, outer, experts)))
+      return rc;
     return by_dtype(dtype, [&](auto v) {
       using T = decltype(v);
       if constexpr (sizeof(T) == 2)
         return weights_vjp16<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
-                                (const T*)g, ldg, offsets, (T*)g_weight);
+                                (const T*)g, ldg, offsets, workspace, (T*)g_weight);
       else
         return weights_vjp32<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
                                 (const T*)g, ldg, offsets, (T*)g_weight);

@@ -172,14 +172,87 @@ __device__ __forceinline__ S8 fragment(const T* lds, int i0, int s) {
   }
 }
 
-// A workgroup of WM * WN wavefronts; ``lds`` holds 2 * (BM + BN) * kDepth16 elements.
-template <typename T, int BM, int BN, int WM, int WN, bool ALONG_A, bool ALONG_B, bool DIRECT>
-__device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, T* lds, T* c,
-                                       int64_t ldc) {
-  constexpr int THREADS = WM * WN * 64, X = BM / WM / 32, Y = BN / WN / 32;
+// Waits until at most N of this wavefront's loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "the counter's range");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// The contraction's stages in a ring of S places: S - 1 on their way while one is multiplied.
+// DIRECT: a stage past the end reads nothing (its addresses are outside) and counts all the same.
+// Through registers one stage is on its way, whatever S.
+template <typename T, int BM, int BN, int THREADS, bool ALONG_A, bool ALONG_B, bool DIRECT, int S>
+struct Ring {
   using SA = Stage<T, BM, ALONG_A, THREADS, DIRECT>;
   using SB = Stage<T, BN, ALONG_B, THREADS, DIRECT>;
-  constexpr int kStage = SA::kElems + SB::kElems;
+  static constexpr int kStage = SA::kElems + SB::kElems;
+  static constexpr int kBytes = S * kStage * 2;
+
+  template <typename F>
+  static __device__ __forceinline__ void run(const Side<T>& a, const Side<T>& b, int64_t depth,
+                                             T* lds, F&& multiply) {
+    uint32_t off_a[SA::kMine], off_b[SB::kMine];
+    Pack<T> va[SA::kMine], vb[SB::kMine];
+    const T *pa = uniform(a.p), *pb = uniform(b.p);
+    int64_t left = depth;
+    auto load = [&](T* to) {
+      if constexpr (DIRECT) {
+        SA::load_lds(pa, off_a, left, to);
+        SB::load_lds(pb, off_b, left, to + SA::kElems);
+      } else {
+        SA::load_regs(a, pa, left, va);
+        SB::load_regs(b, pb, left, vb);
+      }
+      pa += ALONG_A ? kDepth16 : kDepth16 * a.ld;
+      pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
+      left -= kDepth16;
+    };
+    auto put = [&](T* to) {
+      SA::store_lds(va, to);
+      SB::store_lds(vb, to + SA::kElems);
+    };
+    const int64_t steps = (depth + kDepth16 - 1) / kDepth16;
+    if constexpr (DIRECT) {
+      SA::offsets(a, off_a);
+      SB::offsets(b, off_b);
+#pragma unroll
+      for (int s = 0; s < S - 1; ++s) load(lds + s * kStage);
+    } else if (steps > 0) {
+      load(lds);
+      put(lds);
+    }
+    int now = 0;
+    for (int64_t t = 0; t < steps; ++t) {
+      int next = now + (DIRECT ? S - 1 : 1);
+      if (next >= S) next -= S;
+      // this stage is in LDS; the later ones may be on their way still
+      if constexpr (DIRECT) wait_loads<(S - 2) * (SA::kMine + SB::kMine)>();
+      __syncthreads();
+      if (S > 2 && DIRECT ? true : t + 1 < steps) load(lds + next * kStage);
+      multiply(lds + now * kStage, lds + now * kStage + SA::kElems);
+      if constexpr (!DIRECT)
+        if (t + 1 < steps) put(lds + next * kStage);
+      now = now + 1 == S ? 0 : now + 1;
+    }
+    if constexpr (DIRECT) wait_loads<0>();  // stages past the end
+    __syncthreads();
+  }
+};
+
+// The bytes of LDS that tile16 needs: the ring, and the tile itself on its way out.
+template <typename T, typename C, int BM, int BN, int S>
+constexpr int tile16_lds() {
+  constexpr int ring = S * (BM + BN) * kDepth16 * 2, out = BM * BN * (int)sizeof(C);
+  return ring > out ? ring : out;
+}
+
+// A workgroup of WM * WN wavefronts; sums are written as C.
+template <typename T, typename C, int BM, int BN, int WM, int WN, bool ALONG_A, bool ALONG_B,
+          bool DIRECT, int S>
+__device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, unsigned char* lds,
+                                       C* c, int64_t ldc) {
+  constexpr int THREADS = WM * WN * 64, X = BM / WM / 32, Y = BN / WN / 32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
   F16x acc[X][Y];
@@ -189,61 +262,26 @@ __device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, T* l
     for (int y = 0; y < Y; ++y)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
-  uint32_t off_a[SA::kMine], off_b[SB::kMine];
-  Pack<T> va[SA::kMine], vb[SB::kMine];
-  if constexpr (DIRECT) {
-    SA::offsets(a, off_a);
-    SB::offsets(b, off_b);
-  }
-  const T *pa = uniform(a.p), *pb = uniform(b.p);
-  int64_t left = depth;
-  auto load = [&](T* to) {
-    if constexpr (DIRECT) {
-      SA::load_lds(pa, off_a, left, to);
-      SB::load_lds(pb, off_b, left, to + SA::kElems);
-    } else {
-      SA::load_regs(a, pa, left, va);
-      SB::load_regs(b, pb, left, vb);
-    }
-    pa += ALONG_A ? kDepth16 : kDepth16 * a.ld;
-    pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
-    left -= kDepth16;
-  };
-  auto put = [&](T* to) {
-    if constexpr (!DIRECT) {
-      SA::store_lds(va, to);
-      SB::store_lds(vb, to + SA::kElems);
-    }
-  };
-  if (depth > 0) {
-    load(lds);
-    put(lds);
-  }
-  int64_t steps = (depth + kDepth16 - 1) / kDepth16;
-  T *now = lds, *next = lds + kStage;
-  for (int64_t t = 0; t < steps; ++t) {
-    if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this stage is in LDS
-    __syncthreads();
-    if (t + 1 < steps) load(next);
-    const T *la = now, *lb = now + SA::kElems;
+  Ring<T, BM, BN, THREADS, ALONG_A, ALONG_B, DIRECT, S>::run(
+      a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb) {
 #pragma unroll
-    for (int s = 0; s < kDepth16 / 16; ++s) {
-      S8 fa[X], fb[Y];
+        for (int s = 0; s < kDepth16 / 16; ++s) {
+          S8 fa[X], fb[Y];
 #pragma unroll
-      for (int x = 0; x < X; ++x) fa[x] = fragment<T, BM, ALONG_A>(la, wi + 32 * x, s);
+          for (int x = 0; x < X; ++x) fa[x] = fragment<T, BM, ALONG_A>(la, wi + 32 * x, s);
 #pragma unroll
-      for (int y = 0; y < Y; ++y) fb[y] = fragment<T, BN, ALONG_B>(lb, wj + 32 * y, s);
+          for (int y = 0; y < Y; ++y) fb[y] = fragment<T, BN, ALONG_B>(lb, wj + 32 * y, s);
 #pragma unroll
-      for (int x = 0; x < X; ++x)
+          for (int x = 0; x < X; ++x)
 #pragma unroll
-        for (int y = 0; y < Y; ++y) acc[x][y] = mma32(T{}, fb[y], fa[x], acc[x][y]);
-    }
-    if (t + 1 < steps) put(next);
-    T* swap = now;
-    now = next;
-    next = swap;
-  }
-  // b's rows run along the sums' registers: 4 neighbours of c's row to a lane
+            for (int y = 0; y < Y; ++y) acc[x][y] = mma32(T{}, fb[y], fa[x], acc[x][y]);
+        }
+      });
+  // b's rows run along the sums' registers: 4 neighbours of c's row to a lane.  The tile passes
+  // through LDS, so that whole rows leave in 16-byte pieces; a row's pieces are exchanged by its
+  // number, so that a wavefront's writes, one column of 32 rows, fall on different banks.
+  constexpr int V = kVec<C>, kPieces = BN / V;
+  C* out = reinterpret_cast<C*>(lds);
 #pragma unroll
   for (int x = 0; x < X; ++x) {
     const int i = wi + 32 * x + (lane & 31);
@@ -252,23 +290,20 @@ __device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, T* l
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int j = wj + 32 * y + 2 * r + 4 * (lane >> 5);
-        if (i >= a.n || j >= b.n) continue;
-        T v[4];
+        typedef C V4 __attribute__((ext_vector_type(4)));
+        V4 v;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = (T)acc[x][y][r + q];
-        T* to = c + i * ldc + j;
-        typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-        if (j + 4 <= b.n) {
-          V4 w;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) w[q] = v[q];
-          *reinterpret_cast<V4*>(to) = w;
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (j + q < b.n) to[q] = v[q];
-        }
+        for (int q = 0; q < 4; ++q) v[q] = (C)acc[x][y][r + q];
+        *reinterpret_cast<V4*>(out + i * BN + (((j / V) ^ (i & (kPieces - 1))) * V + j % V)) = v;
       }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int at = threadIdx.x; at < BM * kPieces; at += THREADS) {
+    const int i = at / kPieces, j = at % kPieces * V;
+    if (i >= a.n || j >= b.n) continue;
+    store_upto(c + i * ldc + j, load16(out + i * BN + ((j / V) ^ (i & (kPieces - 1))) * V),
+               b.n - j);
   }
 }
 
@@ -286,72 +321,21 @@ template <typename T, int BN, bool ALONG_B, bool DIRECT>
 __device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsigned char* lds,
                                        T* c, int64_t ldc) {
   constexpr int THREADS = 256, Y = BN / 32, P = BN + 4;
-  using SA = Stage<T, 32, true, THREADS, DIRECT>;
-  using SB = Stage<T, BN, ALONG_B, THREADS, DIRECT>;
-  constexpr int kStage = SA::kElems + SB::kElems;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T* stages = reinterpret_cast<T*>(lds);
   F16x acc[Y];
 #pragma unroll
   for (int y = 0; y < Y; ++y)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[y][r] = 0.0f;
-  uint32_t off_a[SA::kMine], off_b[SB::kMine];
-  Pack<T> va[SA::kMine], vb[SB::kMine];
-  const T *pa = uniform(a.p), *pb = uniform(b.p);
-  int64_t left = depth;
-  const int64_t steps = (depth + kDepth16 - 1) / kDepth16;
-  // DIRECT: a stage past the end reads nothing (its addresses are outside), and counts
-  auto load = [&](T* to) {
-    if constexpr (DIRECT) {
-      SA::load_lds(pa, off_a, left, to);
-      SB::load_lds(pb, off_b, left, to + SA::kElems);
-    } else {
-      SA::load_regs(a, pa, left, va);
-      SB::load_regs(b, pb, left, vb);
-    }
-    pa += kDepth16;
-    pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
-    left -= kDepth16;
-  };
-  auto put = [&](T* to) {
-    SA::store_lds(va, to);
-    SB::store_lds(vb, to + SA::kElems);
-  };
-  if constexpr (DIRECT) {
-    SA::offsets(a, off_a);
-    SB::offsets(b, off_b);
+  Ring<T, 32, BN, THREADS, true, ALONG_B, DIRECT, kThin>::run(
+      a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb) {
+        const S8 fa = fragment<T, 32, true>(la, 0, wave);
+        S8 fb[Y];
 #pragma unroll
-    for (int s = 0; s < kThin - 1; ++s) load(stages + s * kStage);
-  } else if (steps > 0) {
-    load(stages);
-    put(stages);
-  }
-  int now = 0;
-  for (int64_t t = 0; t < steps; ++t) {
-    int next = now + (DIRECT ? kThin - 1 : 1);
-    if (next >= kThin) next -= kThin;
-    if constexpr (DIRECT) {
-      // the loads of the kThin - 2 later stages may be on their way still
-      constexpr int later = (kThin - 2) * (SA::kMine + SB::kMine);
-      static_assert(later < 64, "the counter's range");
-      __builtin_amdgcn_s_waitcnt(0x0f70 | (later & 15) | ((later >> 4) << 14));
-    }
-    __syncthreads();
-    if (DIRECT || t + 1 < steps) load(stages + next * kStage);
-    const T *la = stages + now * kStage, *lb = la + SA::kElems;
-    const S8 fa = fragment<T, 32, true>(la, 0, wave);
-    S8 fb[Y];
+        for (int y = 0; y < Y; ++y) fb[y] = fragment<T, BN, ALONG_B>(lb, 32 * y, wave);
 #pragma unroll
-    for (int y = 0; y < Y; ++y) fb[y] = fragment<T, BN, ALONG_B>(lb, 32 * y, wave);
-#pragma unroll
-    for (int y = 0; y < Y; ++y) acc[y] = mma32(T{}, fb[y], fa, acc[y]);
-    if constexpr (!DIRECT)
-      if (t + 1 < steps) put(stages + next * kStage);
-    now = now + 1 == kThin ? 0 : now + 1;
-  }
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // the stages past the end
-  __syncthreads();
+        for (int y = 0; y < Y; ++y) acc[y] = mma32(T{}, fb[y], fa, acc[y]);
+      });
   float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int y = 0; y < Y; ++y)
