@@ -100,12 +100,11 @@ __device__ __forceinline__ void part_of(int64_t depth, int split, int splits, in
   length = min(depth - first, per * kDepth16);
 }
 
-// Split number blockIdx.y of the contraction writes its own ``out`` (rows x outer).
-template <typename T, typename C, int BM, int BN, int WM, int WN, bool ALONG_B, bool DIRECT, int S>
+template <typename T, int BM, int BN, int WM, int WN, bool ALONG_B, bool DIRECT, int S>
 __global__ __launch_bounds__(WM* WN * 64) void k_product16(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
     int64_t rows, int64_t inner, int64_t outer, int experts, int64_t tiles_m, int64_t tiles_n,
-    const int32_t* __restrict__ offsets, C* __restrict__ out, int64_t ldo) {
+    const int32_t* __restrict__ offsets, T* __restrict__ out, int64_t ldo) {
   extern __shared__ __align__(16) unsigned char lds16[];
   int64_t tm, tn;
   tile_order(tiles_m, tiles_n, tm, tn);
@@ -116,16 +115,14 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product16(
   const int64_t col = tn * BN;
   const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
   const int n = (int)min<int64_t>(BN, outer - col);
-  C* c = out + (int64_t)blockIdx.y * rows * ldo + from * ldo + col;
+  T* c = out + from * ldo + col;
   if (e < 0) {
     zero_tile(c, ldo, m, n);
     return;
   }
-  int64_t k, length;
-  part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
-  tile16<T, C, BM, BN, WM, WN, true, ALONG_B, DIRECT, S>(
-      {a + from * lda + k, lda, m},
-      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n}, length, lds16, c, ldo);
+  tile16<T, T, BM, BN, WM, WN, true, ALONG_B, DIRECT, S>(
+      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner, lds16, c,
+      ldo);
 }
 
 // out = the sum of ``splits`` parts, in their order.
@@ -154,13 +151,13 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, i
   }
 }
 
-// Experts with few rows: every column tile of one expert's weights is read once, by a workgroup
-// that has all of the expert's rows (32 at a time).
-template <typename T, int BN, bool ALONG_B, bool DIRECT>
+// Experts with few rows, or few tiles in all: column tiles of 64 for 32 rows at a time.  Split
+// number blockIdx.y of the contraction writes its own ``out``.
+template <typename T, typename C, int BN, bool ALONG_B, bool DIRECT>
 __global__ __launch_bounds__(256) void k_product_thin(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
     int64_t rows, int64_t inner, int64_t outer, int experts, int64_t tiles_n,
-    const int32_t* __restrict__ offsets, T* __restrict__ out, int64_t ldo) {
+    const int32_t* __restrict__ offsets, C* __restrict__ out, int64_t ldo) {
   extern __shared__ __align__(16) unsigned char lds16[];
   const int64_t tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
   int e;
@@ -170,13 +167,16 @@ __global__ __launch_bounds__(256) void k_product_thin(
   const int64_t col = tn * BN;
   const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(32, to - from));
   const int n = (int)min<int64_t>(BN, outer - col);
+  C* c = out + (int64_t)blockIdx.y * rows * ldo + from * ldo + col;
   if (e < 0) {
-    zero_tile(out + from * ldo + col, ldo, m, n);
+    zero_tile(c, ldo, m, n);
     return;
   }
-  thin16<T, BN, ALONG_B, DIRECT>(
-      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner, lds16,
-      out + from * ldo + col, ldo);
+  int64_t k, length;
+  part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
+  thin16<T, C, BN, ALONG_B, DIRECT>(
+      {a + from * lda + k, lda, m},
+      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n}, length, lds16, c, ldo);
 }
 
 // Split number blockIdx.z of an expert's rows writes its own ``gw`` (experts x inner x outer).
@@ -273,33 +273,41 @@ static int64_t most_tiles(int64_t rows, int64_t experts, int64_t height) {
   return (rows + std::min(rows, experts + 1) * (height - 1)) / height;
 }
 
-// How the 16-bit kernels cut a product of ``tiles`` 128 x 128 tiles, each ``steps`` stages long.
-//   large   256 x 256 tiles: half the LDS reads and operand traffic of 128 x 128; from 4 to a CU
-//           on (of 128 x 128: 16) its single workgroup a CU does not leave CUs idle at the end.
-//           32768 x 2048 x 4096: 600 us, 128 x 128 tiles 660; 2048 x 2048 x 2048: 57 and 35
+// How the 16-bit kernels cut a product.  ``tiles``: the 128 x 128 tiles, ``steps``: the stages of
+// the contraction.  us of 1000 rows, 8 experts, 1024 x 1024 | 3000, 60, 2048 x 512 | 2048, 2,
+// 2048 x 2048 | 32768, 16, 2048 x 4096, bf16:
+//   thin    32 x 64 tiles: the experts' weights at the rate of memory where rows are few, and
+//           eight times the workgroups where tiles are few       9.5 |  41 |   - |   -
 //   deep    up to one 128 x 128 tile a CU there is room for 4 stages, three on their way: the
-//           stages' latency is what counts then.  With more tiles, two workgroups of 2 stages
-//   splits  where even so CUs are idle and the contraction is long, parts of at least kPart
-//           stages into 32-bit sums, and a second kernel that adds them up
+//           stages' latency is what counts then                 15.5 |   - |   - |   -
+//   128     two workgroups a CU of 2 stages                        - |  32 |  34 | 660
+//   256     half the LDS reads and operand traffic of 128; from 4 tiles to a CU on its single
+//           workgroup a CU does not leave CUs idle at the end      - |   - |  57 | 600
+// Where even so CUs are idle and the contraction is long, it is split into parts of 32-bit
+// sums, which a second kernel adds up.
+enum Shape16 { kThin16, kDeep16, k128, k256 };
 struct Cut16 {
-  bool large, deep;
+  Shape16 shape;
   int splits;
 };
-constexpr int64_t kPart = 12;
-static Cut16 cut16(int64_t tiles, int64_t steps) {
-  if (tiles >= 16 * 256) return {true, false, 1};
-  int64_t splits = 1;
-  if (tiles <= 128) splits = std::max<int64_t>(1, std::min(256 / std::max<int64_t>(tiles, 1), steps / kPart));
-  return {false, tiles * splits <= 256, (int)splits};
-}
 static int64_t steps16(int64_t depth) { return (depth + kDepth16 - 1) / kDepth16; }
+// Splits of at least ``part`` stages that fill the CUs with ``groups`` workgroups each.
+static int splits16(int64_t groups, int64_t steps, int64_t part) {
+  return (int)std::max<int64_t>(1, std::min(256 / std::max<int64_t>(groups, 1), steps / part));
+}
 static Cut16 cut_product16(int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
-  return cut16(most_tiles(rows, experts, 128) * ((outer + 127) / 128), steps16(inner));
+  const int64_t tiles = most_tiles(rows, experts, 128) * ((outer + 127) / 128);
+  if (rows <= 32 * experts || tiles <= 128) {
+    const int64_t groups = most_tiles(rows, experts, 32) * ((outer + 63) / 64);
+    return {kThin16, splits16(groups, steps16(inner), 16)};
+  }
+  return {tiles <= 256 ? kDeep16 : tiles < 16 * 256 ? k128 : k256, 1};
 }
 static Cut16 cut_weights16(int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
-  return cut16(((inner + 127) / 128) * ((outer + 127) / 128) * experts, steps16(rows / experts));
+  const int64_t tiles = ((inner + 127) / 128) * ((outer + 127) / 128) * experts;
+  const int splits = splits16(tiles, steps16(rows / experts), 12);
+  return {tiles * splits <= 256 ? kDeep16 : tiles < 16 * 256 ? k128 : k256, splits};
 }
-static bool thin16(int64_t rows, int64_t experts) { return rows <= 32 * experts; }
 
 // The ``splits`` parts of ``count`` sums added up into out.
 template <typename T>
@@ -316,41 +324,38 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
   const int64_t ldw = along ? wo : wi;
   const bool direct = direct_ok(a, lda, inner) && direct_ok(w, ldw, along ? inner : outer) &&
                       we % 8 == 0;
-  if (thin16(rows, experts)) {
-    constexpr int TN = 64;
-    const int64_t tn = (outer + TN - 1) / TN;
-    auto thin = [&](auto kernel) {
-      return launch16("k_product_thin", kernel, dim3((unsigned)(most_tiles(rows, experts, 32) * tn)),
-                      256, thin_lds<TN>(), st, a, lda, w, we, ldw, rows, inner, outer,
-                      (int)experts, tn, offsets, out, ldo);
-    };
-    if (along) return direct ? thin(k_product_thin<T, TN, true, true>)
-                             : thin(k_product_thin<T, TN, true, false>);
-    return direct ? thin(k_product_thin<T, TN, false, true>)
-                  : thin(k_product_thin<T, TN, false, false>);
-  }
   Cut16 cut = cut_product16(rows, inner, outer, experts);
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
-  auto go = [&](auto c, auto bm, auto wn, auto s) {
-    using C = decltype(c);
-    constexpr int B = bm, WN = wn, S = s;
-    const int64_t tm = most_tiles(rows, experts, B), tn = (outer + B - 1) / B;
-    C* to = cut.splits > 1 ? (C*)ws : (C*)out;
-    const int64_t ldc = cut.splits > 1 ? outer : ldo;
-    auto kernel = along ? (direct ? k_product16<T, C, B, B, 2, WN, true, true, S>
-                                  : k_product16<T, C, B, B, 2, WN, true, false, S>)
-                        : (direct ? k_product16<T, C, B, B, 2, WN, false, true, S>
-                                  : k_product16<T, C, B, B, 2, WN, false, false, S>);
-    return launch16("k_product16", kernel, dim3((unsigned)(tm * tn), (unsigned)cut.splits),
-                    2 * WN * 64, tile16_lds<T, C, B, B, S>(), st, a, lda, w, we, ldw, rows, inner,
-                    outer, (int)experts, tm, tn, offsets, to, ldc);
-  };
-  if (cut.splits > 1) {
-    if (int rc = go(float{}, i128, i2, i4)) return rc;
+  if (cut.shape == kThin16) {
+    constexpr int TN = 64;
+    const int64_t tm = most_tiles(rows, experts, 32), tn = (outer + TN - 1) / TN;
+    auto thin = [&](auto c) {
+      using C = decltype(c);
+      auto kernel = along ? (direct ? k_product_thin<T, C, TN, true, true>
+                                    : k_product_thin<T, C, TN, true, false>)
+                          : (direct ? k_product_thin<T, C, TN, false, true>
+                                    : k_product_thin<T, C, TN, false, false>);
+      return launch16("k_product_thin", kernel, dim3((unsigned)(tm * tn), (unsigned)cut.splits),
+                      256, thin_lds<TN>(), st, a, lda, w, we, ldw, rows, inner, outer,
+                      (int)experts, tn, offsets, cut.splits > 1 ? (C*)ws : (C*)out, ldo);
+    };
+    if (cut.splits == 1) return thin(T{});
+    if (int rc = thin(float{})) return rc;
     return join(st, (const float*)ws, cut.splits, rows * outer, out);
   }
-  if (cut.large) return go(T{}, i256, i4, i2);
-  return cut.deep ? go(T{}, i128, i2, i4) : go(T{}, i128, i2, i2);
+  auto go = [&](auto bm, auto wn, auto s) {
+    constexpr int B = bm, WN = wn, S = s;
+    const int64_t tm = most_tiles(rows, experts, B), tn = (outer + B - 1) / B;
+    auto kernel = along ? (direct ? k_product16<T, B, B, 2, WN, true, true, S>
+                                  : k_product16<T, B, B, 2, WN, true, false, S>)
+                        : (direct ? k_product16<T, B, B, 2, WN, false, true, S>
+                                  : k_product16<T, B, B, 2, WN, false, false, S>);
+    return launch16("k_product16", kernel, dim3((unsigned)(tm * tn)), 2 * WN * 64,
+                    tile16_lds<T, T, B, B, S>(), st, a, lda, w, we, ldw, rows, inner, outer,
+                    (int)experts, tm, tn, offsets, out, ldo);
+  };
+  if (cut.shape == k256) return go(i256, i4, i2);
+  return cut.shape == kDeep16 ? go(i128, i2, i4) : go(i128, i2, i2);
 }
 
 template <typename T>
@@ -374,8 +379,8 @@ static int weights_vjp16(hipStream_t st, int64_t rows, int64_t inner, int64_t ou
     if (int rc = go(float{}, i128, i2, i4)) return rc;
     return join(st, (const float*)ws, cut.splits, experts * inner * outer, gw);
   }
-  if (cut.large) return go(T{}, i256, i4, i2);
-  return cut.deep ? go(T{}, i128, i2, i4) : go(T{}, i128, i2, i2);
+  if (cut.shape == k256) return go(T{}, i256, i4, i2);
+  return cut.shape == kDeep16 ? go(T{}, i128, i2, i4) : go(T{}, i128, i2, i2);
 }
 
 template <typename T>
@@ -448,7 +453,7 @@ int64_t purin_train_expert_product_workspace_bytes(int32_t dtype, int64_t rows, 
   (void)guarded([&] {
     if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
     need = 0;
-    if (dtype_bytes(dtype) == 2 && rows && outer && !thin16(rows, experts)) {
+    if (dtype_bytes(dtype) == 2 && rows && outer) {
       const int splits = cut_product16(rows, inner, outer, experts).splits;
       if (splits > 1) need = splits * rows * outer * (int64_t)sizeof(float);
     }

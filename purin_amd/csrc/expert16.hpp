@@ -132,17 +132,27 @@ struct Stage {
     }
   }
 
-  // through registers: any alignment, rows and a contraction of any length
+  // Through registers: any alignment, rows and a contraction of any length.  Whole stages load
+  // without a condition (rows past the last are read as the last: they reach no sum that is
+  // kept), so that no load waits for another's.
   static __device__ __forceinline__ void load_regs(const Side<T>& o, const T* p, int64_t left,
                                                    Pack<T> (&v)[kMine]) {
+    if (left >= kDepth16 && (ALONG || o.n == N)) {
+#pragma unroll
+      for (int m = 0; m < kMine; ++m) {
+        int row, first;
+        piece(m, row, first);
+        v[m] = load16(p + (ALONG ? min(row, o.n - 1) : row) * o.ld + first);
+      }
+      return;
+    }
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       int row, first;
       piece(m, row, first);
       const int64_t rows = ALONG ? o.n : left, cols = ALONG ? left : o.n;
-      const T* q = p + row * o.ld + first;
       if (row >= rows || first >= cols) v[m] = zeros16<T>();
-      else v[m] = load_upto(q, cols - first);
+      else v[m] = load_upto(p + row * o.ld + first, cols - first);
     }
   }
   static __device__ __forceinline__ void store_lds(const Pack<T> (&v)[kMine], T* lds) {
@@ -181,8 +191,9 @@ __device__ __forceinline__ void wait_loads() {
 
 // The contraction's stages in a ring of S places: S - 1 on their way while one is multiplied.
 // DIRECT: a stage past the end reads nothing (its addresses are outside) and counts all the same.
-// Through registers one stage is on its way, whatever S.
-template <typename T, int BM, int BN, int THREADS, bool ALONG_A, bool ALONG_B, bool DIRECT, int S>
+// Through registers AHEAD stages are on their way, each in registers of its own.
+template <typename T, int BM, int BN, int THREADS, bool ALONG_A, bool ALONG_B, bool DIRECT, int S,
+          int AHEAD = 1>
 struct Ring {
   using SA = Stage<T, BM, ALONG_A, THREADS, DIRECT>;
   using SB = Stage<T, BN, ALONG_B, THREADS, DIRECT>;
@@ -192,48 +203,61 @@ struct Ring {
   template <typename F>
   static __device__ __forceinline__ void run(const Side<T>& a, const Side<T>& b, int64_t depth,
                                              T* lds, F&& multiply) {
-    uint32_t off_a[SA::kMine], off_b[SB::kMine];
-    Pack<T> va[SA::kMine], vb[SB::kMine];
     const T *pa = uniform(a.p), *pb = uniform(b.p);
     int64_t left = depth;
-    auto load = [&](T* to) {
-      if constexpr (DIRECT) {
-        SA::load_lds(pa, off_a, left, to);
-        SB::load_lds(pb, off_b, left, to + SA::kElems);
-      } else {
-        SA::load_regs(a, pa, left, va);
-        SB::load_regs(b, pb, left, vb);
-      }
+    const int64_t steps = (depth + kDepth16 - 1) / kDepth16;
+    auto advance = [&]() {
       pa += ALONG_A ? kDepth16 : kDepth16 * a.ld;
       pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
       left -= kDepth16;
     };
-    auto put = [&](T* to) {
-      SA::store_lds(va, to);
-      SB::store_lds(vb, to + SA::kElems);
-    };
-    const int64_t steps = (depth + kDepth16 - 1) / kDepth16;
+    int now = 0;
     if constexpr (DIRECT) {
+      uint32_t off_a[SA::kMine], off_b[SB::kMine];
       SA::offsets(a, off_a);
       SB::offsets(b, off_b);
+      auto load = [&](T* to) {
+        SA::load_lds(pa, off_a, left, to);
+        SB::load_lds(pb, off_b, left, to + SA::kElems);
+        advance();
+      };
 #pragma unroll
       for (int s = 0; s < S - 1; ++s) load(lds + s * kStage);
-    } else if (steps > 0) {
-      load(lds);
-      put(lds);
-    }
-    int now = 0;
-    for (int64_t t = 0; t < steps; ++t) {
-      int next = now + (DIRECT ? S - 1 : 1);
-      if (next >= S) next -= S;
-      // this stage is in LDS; the later ones may be on their way still
-      if constexpr (DIRECT) wait_loads<(S - 2) * (SA::kMine + SB::kMine)>();
-      __syncthreads();
-      if (S > 2 && DIRECT ? true : t + 1 < steps) load(lds + next * kStage);
-      multiply(lds + now * kStage, lds + now * kStage + SA::kElems);
-      if constexpr (!DIRECT)
-        if (t + 1 < steps) put(lds + next * kStage);
-      now = now + 1 == S ? 0 : now + 1;
+      for (int64_t t = 0; t < steps; ++t) {
+        const int next = now == 0 ? S - 1 : now - 1;
+        // this stage is in LDS; the later ones may be on their way still
+        wait_loads<(S - 2) * (SA::kMine + SB::kMine)>();
+        __syncthreads();
+        if (S > 2 || t + 1 < steps) load(lds + next * kStage);
+        multiply(lds + now * kStage, lds + now * kStage + SA::kElems);
+        now = now + 1 == S ? 0 : now + 1;
+      }
+    } else {
+      Pack<T> va[AHEAD][SA::kMine], vb[AHEAD][SB::kMine];
+      auto load = [&](int v) {
+        SA::load_regs(a, pa, left, va[v]);
+        SB::load_regs(b, pb, left, vb[v]);
+        advance();
+      };
+      auto put = [&](int v, T* to) {
+        SA::store_lds(va[v], to);
+        SB::store_lds(vb[v], to + SA::kElems);
+      };
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) load(s);
+      put(0, lds);
+      for (int64_t t = 0; t < steps; t += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          if (t + u >= steps) break;
+          const int next = now + 1 == S ? 0 : now + 1;
+          __syncthreads();
+          if (t + u + AHEAD < steps) load(u);
+          multiply(lds + now * kStage, lds + now * kStage + SA::kElems);
+          if (t + u + 1 < steps) put((u + 1) % AHEAD, lds + next * kStage);
+          now = next;
+        }
+      }
     }
     if constexpr (DIRECT) wait_loads<0>();  // stages past the end
     __syncthreads();
@@ -317,9 +341,9 @@ constexpr int thin_lds() {
   return stages > sums ? stages : sums;
 }
 
-template <typename T, int BN, bool ALONG_B, bool DIRECT>
+template <typename T, typename C, int BN, bool ALONG_B, bool DIRECT>
 __device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsigned char* lds,
-                                       T* c, int64_t ldc) {
+                                       C* c, int64_t ldc) {
   constexpr int THREADS = 256, Y = BN / 32, P = BN + 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   F16x acc[Y];
@@ -327,7 +351,7 @@ __device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsi
   for (int y = 0; y < Y; ++y)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[y][r] = 0.0f;
-  Ring<T, 32, BN, THREADS, true, ALONG_B, DIRECT, kThin>::run(
+  Ring<T, 32, BN, THREADS, true, ALONG_B, DIRECT, kThin, kThin - 1>::run(
       a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb) {
         const S8 fa = fragment<T, 32, true>(la, 0, wave);
         S8 fb[Y];
@@ -344,16 +368,17 @@ __device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsi
       sums[(wave * 32 + (lane & 31)) * P + 32 * y + 2 * (r & ~3) + 4 * (lane >> 5) + (r & 3)] =
           acc[y][r];
   __syncthreads();
-  for (int at = threadIdx.x; at < 32 * BN / 8; at += THREADS) {
-    const int i = at / (BN / 8), j = at % (BN / 8) * 8;
+  constexpr int V = kVec<C>;
+  for (int at = threadIdx.x; at < 32 * BN / V; at += THREADS) {
+    const int i = at / (BN / V), j = at % (BN / V) * V;
     if (i >= a.n || j >= b.n) continue;
-    Pack<T> v;
+    Pack<C> v;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
+    for (int q = 0; q < V; ++q) {
       float s = sums[i * P + j + q];
 #pragma unroll
       for (int w = 1; w < 4; ++w) s += sums[(w * 32 + i) * P + j + q];
-      v.v[q] = (T)s;
+      v.v[q] = (C)s;
     }
     store_upto(c + i * ldc + j, v, b.n - j);
   }
