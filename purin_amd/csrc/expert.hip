@@ -200,7 +200,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_weights_vjp16(
       gw + ((int64_t)blockIdx.z * gridDim.y + e) * inner * outer + i * outer + j, outer);
 }
 
-// 32- and 64-bit types.
+// 32- and 64-bit types.  Split number blockIdx.y of the contraction writes its own ``out``.
 template <typename T, int BM, int BN, int WM, int WN, bool ALONG_B>
 __global__ __launch_bounds__(256, 2) void k_product32(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
@@ -216,15 +216,19 @@ __global__ __launch_bounds__(256, 2) void k_product32(
   const int64_t col = tn * BN;
   const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
   const int n = (int)min<int64_t>(BN, outer - col);
+  T* c = out + (int64_t)blockIdx.y * rows * ldo + from * ldo + col;
   if (e < 0) {
-    zero_tile(out + from * ldo + col, ldo, m, n);
+    zero_tile(c, ldo, m, n);
     return;
   }
-  tile32<T, BM, BN, WM, WN, true, ALONG_B>(
-      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner, (T*)lds,
-      out + from * ldo + col, ldo);
+  int64_t k, length;
+  part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
+  tile32<T, BM, BN, WM, WN, true, ALONG_B, BM == 128 ? 1 : 3>(
+      {a + from * lda + k, lda, m},
+      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n}, length, (T*)lds, c, ldo);
 }
 
+// Split number blockIdx.z of an expert's rows writes its own ``gw``.
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256, 2) void k_weights_vjp32(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ g, int64_t ldg, int64_t rows,
@@ -234,13 +238,15 @@ __global__ __launch_bounds__(256, 2) void k_weights_vjp32(
   int64_t tm, tn;
   tile_order(tiles_m, tiles_n, tm, tn);
   const int e = (int)blockIdx.y;
-  int64_t from, to;
+  int64_t from, to, k, length;
   segment(offsets, e, rows, from, to);
+  part_of(to - from, (int)blockIdx.z, (int)gridDim.z, k, length);
+  from += k;
   const int64_t i = tm * BM, j = tn * BN;
-  tile32<T, BM, BN, 2, 2, false, false>(
+  tile32<T, BM, BN, 2, 2, false, false, BM == 128 ? 1 : 3>(
       {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i)},
-      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, to - from, (T*)lds,
-      gw + e * inner * outer + i * outer + j, outer);
+      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, length, (T*)lds,
+      gw + ((int64_t)blockIdx.z * gridDim.y + e) * inner * outer + i * outer + j, outer);
 }
 
 template <typename K, typename... A>
@@ -383,45 +389,75 @@ static int weights_vjp16(hipStream_t st, int64_t rows, int64_t inner, int64_t ou
   return cut.shape == kDeep16 ? go(T{}, i128, i2, i4) : go(T{}, i128, i2, i2);
 }
 
+// How the 32- and 64-bit kernels cut a product: 32 x 64 tiles where rows are few, 128 x 128 (32
+// bits) where they fill the CUs twice, 64 x 64 between; 32-bit contractions are split as the
+// 16-bit ones.
+struct Cut32 {
+  int height, splits;
+};
+static Cut32 cut_product32(bool wide, int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
+  if (!wide && most_tiles(rows, experts, 128) * ((outer + 127) / 128) >= 512 && rows > 32 * experts)
+    return {128, 1};
+  const int64_t across = (outer + 63) / 64;
+  const int height = rows <= 32 * experts || most_tiles(rows, experts, 64) * across < 512 ? 32 : 64;
+  const int64_t groups = most_tiles(rows, experts, height) * across;
+  return {height, wide ? 1 : splits16(groups, steps16(inner), 8)};
+}
+static Cut32 cut_weights32(bool wide, int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
+  if (!wide && ((inner + 127) / 128) * ((outer + 127) / 128) * experts >= 512) return {128, 1};
+  const int64_t groups = ((inner + 63) / 64) * ((outer + 63) / 64) * experts;
+  return {64, wide ? 1 : splits16(groups, steps16(rows / experts), 8)};
+}
+
 template <typename T>
 static int product32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
                      const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,
-                     const int32_t* offsets, T* out, int64_t ldo) {
+                     const int32_t* offsets, void* ws, T* out, int64_t ldo) {
   const bool along = wi == 1 && (wo != 1 || inner > 1);
   const int64_t ldw = along ? wo : wi;
-  auto go = [&](int BM, int BN, auto kernel) {
-    const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + BN - 1) / BN;
-    kernel<<<dim3((unsigned)(tm * tn)), dim3(256), 0, st>>>(a, lda, w, we, ldw, rows, inner, outer,
-                                                           (int)experts, tm, tn, offsets, out, ldo);
-    return launched("k_product32");
-  };
+  Cut32 cut = cut_product32(sizeof(T) == 8, rows, inner, outer, experts);
+  if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
   auto shape = [&](auto bm, auto bn, auto wm, auto wn) {
     constexpr int BM = bm, BN = bn, WM = wm, WN = wn;
-    return along ? go(BM, BN, k_product32<T, BM, BN, WM, WN, true>)
-                 : go(BM, BN, k_product32<T, BM, BN, WM, WN, false>);
+    const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + BN - 1) / BN;
+    auto kernel = along ? k_product32<T, BM, BN, WM, WN, true> : k_product32<T, BM, BN, WM, WN, false>;
+    kernel<<<dim3((unsigned)(tm * tn), (unsigned)cut.splits), dim3(256), 0, st>>>(
+        a, lda, w, we, ldw, rows, inner, outer, (int)experts, tm, tn, offsets,
+        cut.splits > 1 ? (T*)ws : out, ldo);
+    return launched("k_product32");
   };
-  if (rows <= 32 * experts) return shape(i32, i64, i1, i4);
-  // large tiles where they fill the 256 CUs twice
+  int rc = PURIN_CP_OK;
+  if (cut.height == 32) rc = shape(i32, i64, i1, i4);
+  else if (cut.height == 64) rc = shape(i64, i64, i2, i2);
+  else if constexpr (sizeof(T) == 4) rc = shape(i128, i128, i2, i2);
   if constexpr (sizeof(T) == 4)
-    if (most_tiles(rows, experts, 128) * ((outer + 127) / 128) >= 512)
-      return shape(i128, i128, i2, i2);
-  return shape(i64, i64, i2, i2);
+    if (!rc && cut.splits > 1) return join(st, (const float*)ws, cut.splits, rows * outer, out);
+  return rc;
 }
 
 template <typename T>
 static int weights_vjp32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
                          int64_t experts, const T* a, int64_t lda, const T* g, int64_t ldg,
-                         const int32_t* offsets, T* gw) {
-  auto go = [&](int BM, int BN, auto kernel) {
-    const int64_t tm = (inner + BM - 1) / BM, tn = (outer + BN - 1) / BN;
-    kernel<<<dim3((unsigned)(tm * tn), (unsigned)experts), dim3(256), 0, st>>>(
-        a, lda, g, ldg, rows, inner, outer, tm, tn, offsets, gw);
+                         const int32_t* offsets, void* ws, T* gw) {
+  const Cut32 cut = cut_weights32(sizeof(T) == 8, rows, inner, outer, experts);
+  auto go = [&](int b, auto kernel) {
+    const int64_t tm = (inner + b - 1) / b, tn = (outer + b - 1) / b;
+    kernel<<<dim3((unsigned)(tm * tn), (unsigned)experts, (unsigned)cut.splits), dim3(256), 0, st>>>(
+        a, lda, g, ldg, rows, inner, outer, tm, tn, offsets, cut.splits > 1 ? (T*)ws : gw);
     return launched("k_weights_vjp32");
   };
+  int rc = PURIN_CP_OK;
+  if (cut.height == 64) rc = go(64, k_weights_vjp32<T, 64, 64>);
+  else if constexpr (sizeof(T) == 4) rc = go(128, k_weights_vjp32<T, 128, 128>);
   if constexpr (sizeof(T) == 4)
-    if (((inner + 127) / 128) * ((outer + 127) / 128) * experts >= 512)
-      return go(128, 128, k_weights_vjp32<T, 128, 128>);
-  return go(64, 64, k_weights_vjp32<T, 64, 64>);
+    if (!rc && cut.splits > 1)
+      return join(st, (const float*)ws, cut.splits, experts * inner * outer, gw);
+  return rc;
+}
+
+// 32-bit sums of the parts, where a product is split.
+static int64_t parts_bytes(int splits, int64_t count) {
+  return splits > 1 ? splits * count * (int64_t)sizeof(float) : 0;
 }
 
 static int check_product(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
@@ -453,10 +489,12 @@ int64_t purin_train_expert_product_workspace_bytes(int32_t dtype, int64_t rows, 
   (void)guarded([&] {
     if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
     need = 0;
-    if (dtype_bytes(dtype) == 2 && rows && outer) {
-      const int splits = cut_product16(rows, inner, outer, experts).splits;
-      if (splits > 1) need = splits * rows * outer * (int64_t)sizeof(float);
-    }
+    if (rows && outer)
+      need = parts_bytes(dtype_bytes(dtype) == 2
+                             ? cut_product16(rows, inner, outer, experts).splits
+                             : cut_product32(dtype == PURIN_TRAIN_F64, rows, inner, outer, experts)
+                                   .splits,
+                         rows * outer);
     return (int)PURIN_CP_OK;
   });
   return need;
@@ -487,7 +525,7 @@ int purin_train_expert_product(void* stream, int32_t dtype, int64_t rows, int64_
                             (const T*)weight, we, wi, wo, offsets, workspace, (T*)out, ldo);
       else
         return product32<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
-                            (const T*)weight, we, wi, wo, offsets, (T*)out, ldo);
+                            (const T*)weight, we, wi, wo, offsets, workspace, (T*)out, ldo);
     });
   });
 }
@@ -498,10 +536,12 @@ int64_t purin_train_expert_weights_vjp_workspace_bytes(int32_t dtype, int64_t ro
   (void)guarded([&] {
     if (int rc = check_product(dtype, rows, inner, outer, experts)) return rc;
     need = 0;
-    if (dtype_bytes(dtype) == 2 && inner && outer) {
-      const int splits = cut_weights16(rows, inner, outer, experts).splits;
-      if (splits > 1) need = splits * experts * inner * outer * (int64_t)sizeof(float);
-    }
+    if (inner && outer)
+      need = parts_bytes(dtype_bytes(dtype) == 2
+                             ? cut_weights16(rows, inner, outer, experts).splits
+                             : cut_weights32(dtype == PURIN_TRAIN_F64, rows, inner, outer, experts)
+                                   .splits,
+                         experts * inner * outer);
     return (int)PURIN_CP_OK;
   });
   return need;
@@ -528,7 +568,7 @@ int purin_train_expert_weights_vjp(void* stream, int32_t dtype, int64_t rows, in
                                 (const T*)g, ldg, offsets, workspace, (T*)g_weight);
       else
         return weights_vjp32<T>((hipStream_t)stream, rows, inner, outer, experts, (const T*)a, lda,
-                                (const T*)g, ldg, offsets, (T*)g_weight);
+                                (const T*)g, ldg, offsets, workspace, (T*)g_weight);
     });
   });
 }

@@ -3,7 +3,7 @@
 //
 // The matrix units take one value a lane of these types (16 x 16 x 4), at 64 operations a cycle
 // and SIMD (32 in 64 bits), so that their time covers the LDS reads with room to spare and one
-// stage of 64 bytes along the contraction on its way is enough.  Stages pass
+// stage of 128 bytes along the contraction on its way is enough.  Stages pass
 // through registers, which takes any alignment and length.  A lane reads 16 bytes along the
 // contraction at once: step t of a stage multiplies the t-th value of each lane group's 16
 // bytes, an order that both operands share.
@@ -40,7 +40,7 @@ struct Wide<double> {
 };
 
 template <typename T>
-constexpr int kDepth32 = 64 / (int)sizeof(T);
+constexpr int kDepth32 = 128 / (int)sizeof(T);
 constexpr int kBlock32 = 64;
 
 // An operand: element (i, k) at p + i * ld + k (ALONG) or p + k * ld + i; n rows are there.
@@ -54,7 +54,7 @@ struct Side32 {
 template <typename T, int N, bool ALONG, int THREADS>
 struct Stage32 {
   static constexpr int V = kVec<T>, D = kDepth32<T>;
-  // elements of a row in LDS: 80 bytes a row, whose 16-byte pieces at 8 rows fall on different
+  // elements of a row in LDS: 144 bytes a row, whose 16-byte pieces at 8 rows fall on different
   // banks; or N elements and a pad that puts the 4 lane groups' rows on different banks
   static constexpr int kPitch = ALONG ? D + V : N + (sizeof(T) == 4 ? 4 : 8);
   static constexpr int kElems = (ALONG ? N : D) * kPitch;
@@ -70,6 +70,16 @@ struct Stage32 {
   }
   static __device__ __forceinline__ void load(const Side32<T>& o, const T* p, int64_t left,
                                               Pack<T> (&v)[kMine]) {
+    // whole stages load without a condition (rows past the last are read as the last: they reach
+    // no sum that is kept), so that no load waits for another's
+    if (left >= D && (ALONG || o.n == N)) {
+#pragma unroll
+      for (int m = 0; m < kMine; ++m) {
+        int row, first;
+        if (piece(m, row, first)) v[m] = load16(p + (ALONG ? min(row, o.n - 1) : row) * o.ld + first);
+      }
+      return;
+    }
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       int row, first;
@@ -92,9 +102,9 @@ struct Stage32 {
       }
     }
   }
-  // a lane's V values of row i0 + lane % 16
-  static __device__ __forceinline__ Pack<T> fragment(const T* lds, int i0) {
-    const int lane = threadIdx.x & 63, i = i0 + (lane & 15), k = V * (lane >> 4);
+  // a lane's V values of row i0 + lane % 16 in part ``half`` of the stage
+  static __device__ __forceinline__ Pack<T> fragment(const T* lds, int i0, int half) {
+    const int lane = threadIdx.x & 63, i = i0 + (lane & 15), k = V * (lane >> 4) + half * (D / 2);
     Pack<T> f;
     if constexpr (ALONG) {
       typedef T W __attribute__((ext_vector_type(V)));
@@ -115,8 +125,8 @@ constexpr int lds32() {
          (int)sizeof(T);
 }
 
-// A workgroup of WM * WN = 4 wavefronts.
-template <typename T, int BM, int BN, int WM, int WN, bool ALONG_A, bool ALONG_B>
+// A workgroup of WM * WN = 4 wavefronts; AHEAD stages are on their way in registers.
+template <typename T, int BM, int BN, int WM, int WN, bool ALONG_A, bool ALONG_B, int AHEAD>
 __device__ __forceinline__ void tile32(Side32<T> a, Side32<T> b, int64_t depth, T* lds, T* c,
                                        int64_t ldc) {
   static_assert(WM * WN == 4, "four wavefronts");
@@ -132,54 +142,61 @@ __device__ __forceinline__ void tile32(Side32<T> a, Side32<T> b, int64_t depth, 
   for (int x = 0; x < X; ++x)
 #pragma unroll
     for (int y = 0; y < Y; ++y) acc[x][y] = all[x][y] = Acc{0, 0, 0, 0};
-  Pack<T> va[SA::kMine], vb[SB::kMine];
+  Pack<T> va[AHEAD][SA::kMine], vb[AHEAD][SB::kMine];
   const T *pa = a.p, *pb = b.p;
   int64_t left = depth;
-  auto load = [&]() {
-    SA::load(a, pa, left, va);
-    SB::load(b, pb, left, vb);
+  auto load = [&](int v) {
+    SA::load(a, pa, left, va[v]);
+    SB::load(b, pb, left, vb[v]);
     pa += ALONG_A ? D : D * a.ld;
     pb += ALONG_B ? D : D * b.ld;
     left -= D;
   };
-  auto put = [&](T* to) {
-    SA::store(va, to);
-    SB::store(vb, to + SA::kElems);
+  auto put = [&](int v, T* to) {
+    SA::store(va[v], to);
+    SB::store(vb[v], to + SA::kElems);
   };
-  if (depth > 0) {
-    load();
-    put(lds);
-  }
   const int64_t steps = (depth + D - 1) / D;
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) load(s);
+  put(0, lds);
   T *now = lds, *next = lds + kStage;
-  for (int64_t t = 0; t < steps; ++t) {
-    __syncthreads();
-    if (t + 1 < steps) load();
-    Pack<T> fa[X], fb[Y];
+  for (int64_t t0 = 0; t0 < steps; t0 += AHEAD) {
 #pragma unroll
-    for (int x = 0; x < X; ++x) fa[x] = SA::fragment(now, wi + 16 * x);
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t t = t0 + u;
+      if (t >= steps) break;
+      __syncthreads();
+      if (t + AHEAD < steps) load(u);
 #pragma unroll
-    for (int y = 0; y < Y; ++y) fb[y] = SB::fragment(now + SA::kElems, wj + 16 * y);
+      for (int half = 0; half < 2; ++half) {
+        Pack<T> fa[X], fb[Y];
 #pragma unroll
-    for (int q = 0; q < V; ++q)
+        for (int x = 0; x < X; ++x) fa[x] = SA::fragment(now, wi + 16 * x, half);
 #pragma unroll
-      for (int x = 0; x < X; ++x)
+        for (int y = 0; y < Y; ++y) fb[y] = SB::fragment(now + SA::kElems, wj + 16 * y, half);
 #pragma unroll
-        for (int y = 0; y < Y; ++y) acc[x][y] = mma4(fa[x].v[q], fb[y].v[q], acc[x][y]);
-    if constexpr (sizeof(T) == 4)
-      if (t % (kBlock32 / D) == kBlock32 / D - 1) {
+        for (int q = 0; q < V; ++q)
 #pragma unroll
-        for (int x = 0; x < X; ++x)
+          for (int x = 0; x < X; ++x)
 #pragma unroll
-          for (int y = 0; y < Y; ++y) {
-            all[x][y] += acc[x][y];
-            acc[x][y] = Acc{0, 0, 0, 0};
-          }
+            for (int y = 0; y < Y; ++y) acc[x][y] = mma4(fa[x].v[q], fb[y].v[q], acc[x][y]);
       }
-    if (t + 1 < steps) put(next);
-    T* swap = now;
-    now = next;
-    next = swap;
+      if constexpr (sizeof(T) == 4)
+        if (t % (kBlock32 / D) == kBlock32 / D - 1) {
+#pragma unroll
+          for (int x = 0; x < X; ++x)
+#pragma unroll
+            for (int y = 0; y < Y; ++y) {
+              all[x][y] += acc[x][y];
+              acc[x][y] = Acc{0, 0, 0, 0};
+            }
+        }
+      if (t + 1 < steps) put((u + 1) % AHEAD, next);
+      T* swap = now;
+      now = next;
+      next = swap;
+    }
   }
 #pragma unroll
   for (int x = 0; x < X; ++x)
