@@ -15,7 +15,7 @@
 // whose addresses outside the operand read zeros); others pass through registers.
 #pragma once
 
-#include "train.hpp"
+#include "stages.hpp"
 
 namespace purin {
 namespace train {
@@ -39,14 +39,6 @@ __device__ __forceinline__ F16x mma32(f16, S8 a, S8 b, F16x c) {
 
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
-// A pointer that is the same in all lanes, in scalar registers.
-template <typename T>
-__device__ __forceinline__ const T* uniform(const T* p) {
-  const uint64_t u = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
-  return reinterpret_cast<const T*>(((uint64_t)hi << 32) | lo);
-}
 // A buffer descriptor of 2 GiB from p on: reads beyond give zeros.
 template <typename T>
 __device__ __forceinline__ U4 buffer_at(const T* p) {
@@ -68,30 +60,19 @@ __device__ __forceinline__ void load_to_lds(U4 r, uint32_t at, uint32_t to) {
                : "memory");
 }
 
-// An operand of a tile: element (i, k) at p + i * ld + k where its contraction is contiguous
-// (ALONG), at p + k * ld + i where its rows are; n rows are there.
-template <typename T>
-struct Side {
-  const T* p;
-  int64_t ld;
-  int n;
-};
-
 template <int N>
 __device__ __forceinline__ int pair_swap(int k) {
   if constexpr (N == 64) return 2 * ((k >> 1) & 1);
   else return 2 * (k & 3) + ((k >> 3) & 1);
 }
 
-template <typename T, int N, bool ALONG, int THREADS, bool DIRECT>
-struct Stage {
+template <int N, bool ALONG, int THREADS>
+struct Layout16 {
   static constexpr int kPieces = N * kDepth16 / 8;  // 16 bytes each
   static constexpr int kMine = kPieces / THREADS;
-  static constexpr int kElems = N * kDepth16;
   static_assert(kPieces % THREADS == 0, "whole pieces per thread");
 
-  // piece number m of this thread: its row (i or k) and its 8 elements' first (k or i)
-  static __device__ __forceinline__ void piece(int m, int& row, int& first) {
+  static __device__ __forceinline__ bool piece(int m, int& row, int& first) {
     const int at = m * THREADS + (int)threadIdx.x;
     if constexpr (ALONG) {
       row = at >> 3;
@@ -102,14 +83,23 @@ struct Stage {
       const int c = at % per;
       first = ((((c >> 1) ^ pair_swap<N>(row)) << 1) | (c & 1)) * 8;
     }
+    return true;
   }
+};
+
+template <typename T, int N, bool ALONG, int THREADS>
+struct Stage : Pieces<T, N, kDepth16, ALONG, Layout16<N, ALONG, THREADS>> {
+  using Layout = Layout16<N, ALONG, THREADS>;
+  static constexpr int kMine = Layout::kMine;
+  static constexpr int kElems = N * kDepth16;
+  static constexpr bool kAlong = ALONG;
 
   // byte offsets of this thread's pieces from the stage's first element; ~0 outside the rows
   static __device__ __forceinline__ void offsets(const Side<T>& o, uint32_t (&off)[kMine]) {
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       int row, first;
-      piece(m, row, first);
+      Layout::piece(m, row, first);
       const bool in = (ALONG ? row : first) < o.n;
       off[m] = in ? (uint32_t)(row * (int)o.ld + first) * 2u : 0x80000000u;
     }
@@ -125,41 +115,27 @@ struct Stage {
       uint32_t at = off[m];
       if (left < kDepth16) {
         int row, first;
-        piece(m, row, first);
+        Layout::piece(m, row, first);
         if ((ALONG ? first : row) >= left) at = 0x80000000u;
       }
       load_to_lds(r, at, lds_address(lds) + (uint32_t)(m * THREADS + wave * 64) * 16u);
     }
   }
 
-  // Through registers: any alignment, rows and a contraction of any length.  Whole stages load
-  // without a condition (rows past the last are read as the last: they reach no sum that is
-  // kept), so that no load waits for another's.
-  static __device__ __forceinline__ void load_regs(const Side<T>& o, const T* p, int64_t left,
-                                                   Pack<T> (&v)[kMine]) {
-    if (left >= kDepth16 && (ALONG || o.n == N)) {
-#pragma unroll
-      for (int m = 0; m < kMine; ++m) {
-        int row, first;
-        piece(m, row, first);
-        v[m] = load16(p + (ALONG ? min(row, o.n - 1) : row) * o.ld + first);
-      }
-      return;
-    }
-#pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-      int row, first;
-      piece(m, row, first);
-      const int64_t rows = ALONG ? o.n : left, cols = ALONG ? left : o.n;
-      if (row >= rows || first >= cols) v[m] = zeros16<T>();
-      else v[m] = load_upto(p + row * o.ld + first, cols - first);
-    }
+  static __device__ __forceinline__ void store_piece(int m, const Pack<T>& v, T* lds) {
+    *reinterpret_cast<S8*>(lds + (m * THREADS + (int)threadIdx.x) * 8) = __builtin_bit_cast(S8, v);
   }
-  static __device__ __forceinline__ void store_lds(const Pack<T> (&v)[kMine], T* lds) {
+  static __device__ __forceinline__ void store(const Pack<T> (&v)[kMine], T* lds) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) store_piece(m, v[m], lds);
+  }
+  // the pieces that ``move`` names moved into place on their way
+  static __device__ __forceinline__ void store_settled(uint32_t move, int by,
+                                                       const Pack<T> (&v)[kMine], T* lds) {
+    if (ALONG || by == 0) return store(v, lds);
 #pragma unroll
     for (int m = 0; m < kMine; ++m)
-      *reinterpret_cast<S8*>(lds + (m * THREADS + (int)threadIdx.x) * 8) =
-          __builtin_bit_cast(S8, v[m]);
+      store_piece(m, moved(v[m], (move >> m) & 1u ? by : 0), lds);
   }
 };
 
@@ -195,32 +171,29 @@ __device__ __forceinline__ void wait_loads() {
 template <typename T, int BM, int BN, int THREADS, bool ALONG_A, bool ALONG_B, bool DIRECT, int S,
           int AHEAD = 1>
 struct Ring {
-  using SA = Stage<T, BM, ALONG_A, THREADS, DIRECT>;
-  using SB = Stage<T, BN, ALONG_B, THREADS, DIRECT>;
+  using SA = Stage<T, BM, ALONG_A, THREADS>;
+  using SB = Stage<T, BN, ALONG_B, THREADS>;
   static constexpr int kStage = SA::kElems + SB::kElems;
   static constexpr int kBytes = S * kStage * 2;
 
   template <typename F>
   static __device__ __forceinline__ void run(const Side<T>& a, const Side<T>& b, int64_t depth,
                                              T* lds, F&& multiply) {
-    const T *pa = uniform(a.p), *pb = uniform(b.p);
-    int64_t left = depth;
-    const int64_t steps = (depth + kDepth16 - 1) / kDepth16;
-    auto advance = [&]() {
-      pa += ALONG_A ? kDepth16 : kDepth16 * a.ld;
-      pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
-      left -= kDepth16;
-    };
-    int now = 0;
     if constexpr (DIRECT) {
+      const T *pa = uniform(a.p), *pb = uniform(b.p);
+      int64_t left = depth;
+      const int64_t steps = (depth + kDepth16 - 1) / kDepth16;
       uint32_t off_a[SA::kMine], off_b[SB::kMine];
       SA::offsets(a, off_a);
       SB::offsets(b, off_b);
       auto load = [&](T* to) {
         SA::load_lds(pa, off_a, left, to);
         SB::load_lds(pb, off_b, left, to + SA::kElems);
-        advance();
+        pa += ALONG_A ? kDepth16 : kDepth16 * a.ld;
+        pb += ALONG_B ? kDepth16 : kDepth16 * b.ld;
+        left -= kDepth16;
       };
+      int now = 0;
 #pragma unroll
       for (int s = 0; s < S - 1; ++s) load(lds + s * kStage);
       for (int64_t t = 0; t < steps; ++t) {
@@ -229,38 +202,14 @@ struct Ring {
         wait_loads<(S - 2) * (SA::kMine + SB::kMine)>();
         __syncthreads();
         if (S > 2 || t + 1 < steps) load(lds + next * kStage);
-        multiply(lds + now * kStage, lds + now * kStage + SA::kElems);
+        multiply(lds + now * kStage, lds + now * kStage + SA::kElems, t);
         now = now + 1 == S ? 0 : now + 1;
       }
+      wait_loads<0>();  // stages past the end
+      __syncthreads();
     } else {
-      Pack<T> va[AHEAD][SA::kMine], vb[AHEAD][SB::kMine];
-      auto load = [&](int v) {
-        SA::load_regs(a, pa, left, va[v]);
-        SB::load_regs(b, pb, left, vb[v]);
-        advance();
-      };
-      auto put = [&](int v, T* to) {
-        SA::store_lds(va[v], to);
-        SB::store_lds(vb[v], to + SA::kElems);
-      };
-#pragma unroll
-      for (int s = 0; s < AHEAD; ++s) load(s);
-      put(0, lds);
-      for (int64_t t = 0; t < steps; t += AHEAD) {
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          if (t + u >= steps) break;
-          const int next = now + 1 == S ? 0 : now + 1;
-          __syncthreads();
-          if (t + u + AHEAD < steps) load(u);
-          multiply(lds + now * kStage, lds + now * kStage + SA::kElems);
-          if (t + u + 1 < steps) put((u + 1) % AHEAD, lds + next * kStage);
-          now = next;
-        }
-      }
+      through_registers<T, kDepth16, SA, SB, S, AHEAD>(a, b, depth, lds, multiply);
     }
-    if constexpr (DIRECT) wait_loads<0>();  // stages past the end
-    __syncthreads();
   }
 };
 
@@ -287,7 +236,7 @@ __device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, unsi
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
   Ring<T, BM, BN, THREADS, ALONG_A, ALONG_B, DIRECT, S>::run(
-      a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb) {
+      a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb, int64_t) {
 #pragma unroll
         for (int s = 0; s < kDepth16 / 16; ++s) {
           S8 fa[X], fb[Y];
@@ -352,7 +301,7 @@ __device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsi
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[y][r] = 0.0f;
   Ring<T, 32, BN, THREADS, true, ALONG_B, DIRECT, kThin, kThin - 1>::run(
-      a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb) {
+      a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb, int64_t) {
         const S8 fa = fragment<T, 32, true>(la, 0, wave);
         S8 fb[Y];
 #pragma unroll

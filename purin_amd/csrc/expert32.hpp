@@ -13,7 +13,7 @@
 // and of the number of blocks, not of the whole length.
 #pragma once
 
-#include "train.hpp"
+#include "stages.hpp"
 
 namespace purin {
 namespace train {
@@ -43,21 +43,9 @@ template <typename T>
 constexpr int kDepth32 = 128 / (int)sizeof(T);
 constexpr int kBlock32 = 64;
 
-// An operand: element (i, k) at p + i * ld + k (ALONG) or p + k * ld + i; n rows are there.
-template <typename T>
-struct Side32 {
-  const T* p;
-  int64_t ld;
-  int n;
-};
-
 template <typename T, int N, bool ALONG, int THREADS>
-struct Stage32 {
+struct Layout32 {
   static constexpr int V = kVec<T>, D = kDepth32<T>;
-  // elements of a row in LDS: 144 bytes a row, whose 16-byte pieces at 8 rows fall on different
-  // banks; or N elements and a pad that puts the 4 lane groups' rows on different banks
-  static constexpr int kPitch = ALONG ? D + V : N + (sizeof(T) == 4 ? 4 : 8);
-  static constexpr int kElems = (ALONG ? N : D) * kPitch;
   static constexpr int kPieces = N * D / V;
   static constexpr int kMine = (kPieces + THREADS - 1) / THREADS;
 
@@ -68,39 +56,38 @@ struct Stage32 {
     first = at % per * V;
     return kPieces % THREADS == 0 || at < kPieces;
   }
-  static __device__ __forceinline__ void load(const Side32<T>& o, const T* p, int64_t left,
-                                              Pack<T> (&v)[kMine]) {
-    // whole stages load without a condition (rows past the last are read as the last: they reach
-    // no sum that is kept), so that no load waits for another's
-    if (left >= D && (ALONG || o.n == N)) {
+};
+
+template <typename T, int N, bool ALONG, int THREADS>
+struct Stage32 : Pieces<T, N, kDepth32<T>, ALONG, Layout32<T, N, ALONG, THREADS>> {
+  using Layout = Layout32<T, N, ALONG, THREADS>;
+  static constexpr int V = kVec<T>, D = kDepth32<T>, kMine = Layout::kMine;
+  static constexpr bool kAlong = ALONG;
+  // elements of a row in LDS: 144 bytes a row, whose 16-byte pieces at 8 rows fall on different
+  // banks; or N elements and a pad that puts the 4 lane groups' rows on different banks
+  static constexpr int kPitch = ALONG ? D + V : N + (sizeof(T) == 4 ? 4 : 8);
+  static constexpr int kElems = (ALONG ? N : D) * kPitch;
+
+  static __device__ __forceinline__ void store_piece(int m, const Pack<T>& v, T* lds) {
+    int row, first;
+    if (!Layout::piece(m, row, first)) return;
+    typedef T W __attribute__((ext_vector_type(V)));
+    W x;
 #pragma unroll
-      for (int m = 0; m < kMine; ++m) {
-        int row, first;
-        if (piece(m, row, first)) v[m] = load16(p + (ALONG ? min(row, o.n - 1) : row) * o.ld + first);
-      }
-      return;
-    }
-#pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-      int row, first;
-      const bool in = piece(m, row, first);
-      const int64_t rows = ALONG ? o.n : left, cols = ALONG ? left : o.n;
-      if (!in || row >= rows || first >= cols) v[m] = zeros16<T>();
-      else v[m] = load_upto(p + row * o.ld + first, cols - first);
-    }
+    for (int q = 0; q < V; ++q) x[q] = v.v[q];
+    *reinterpret_cast<W*>(lds + row * kPitch + first) = x;
   }
   static __device__ __forceinline__ void store(const Pack<T> (&v)[kMine], T* lds) {
 #pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-      int row, first;
-      if (piece(m, row, first)) {
-        typedef T W __attribute__((ext_vector_type(V)));
-        W x;
+    for (int m = 0; m < kMine; ++m) store_piece(m, v[m], lds);
+  }
+  // the pieces that ``move`` names moved into place on their way
+  static __device__ __forceinline__ void store_settled(uint32_t move, int by,
+                                                       const Pack<T> (&v)[kMine], T* lds) {
+    if (ALONG || by == 0) return store(v, lds);
 #pragma unroll
-        for (int q = 0; q < V; ++q) x[q] = v[m].v[q];
-        *reinterpret_cast<W*>(lds + row * kPitch + first) = x;
-      }
-    }
+    for (int m = 0; m < kMine; ++m)
+      store_piece(m, moved(v[m], (move >> m) & 1u ? by : 0), lds);
   }
   // a lane's V values of row i0 + lane % 16 in part ``half`` of the stage
   static __device__ __forceinline__ Pack<T> fragment(const T* lds, int i0, int half) {
@@ -127,14 +114,13 @@ constexpr int lds32() {
 
 // A workgroup of WM * WN = 4 wavefronts; AHEAD stages are on their way in registers.
 template <typename T, int BM, int BN, int WM, int WN, bool ALONG_A, bool ALONG_B, int AHEAD>
-__device__ __forceinline__ void tile32(Side32<T> a, Side32<T> b, int64_t depth, T* lds, T* c,
+__device__ __forceinline__ void tile32(Side<T> a, Side<T> b, int64_t depth, T* lds, T* c,
                                        int64_t ldc) {
   static_assert(WM * WN == 4, "four wavefronts");
   constexpr int X = BM / WM / 16, Y = BN / WN / 16, V = kVec<T>, D = kDepth32<T>;
   using SA = Stage32<T, BM, ALONG_A, 256>;
   using SB = Stage32<T, BN, ALONG_B, 256>;
   using Acc = typename Wide<T>::Acc;
-  constexpr int kStage = SA::kElems + SB::kElems;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
   Acc acc[X][Y], all[X][Y];
@@ -142,62 +128,33 @@ __device__ __forceinline__ void tile32(Side32<T> a, Side32<T> b, int64_t depth, 
   for (int x = 0; x < X; ++x)
 #pragma unroll
     for (int y = 0; y < Y; ++y) acc[x][y] = all[x][y] = Acc{0, 0, 0, 0};
-  Pack<T> va[AHEAD][SA::kMine], vb[AHEAD][SB::kMine];
-  const T *pa = a.p, *pb = b.p;
-  int64_t left = depth;
-  auto load = [&](int v) {
-    SA::load(a, pa, left, va[v]);
-    SB::load(b, pb, left, vb[v]);
-    pa += ALONG_A ? D : D * a.ld;
-    pb += ALONG_B ? D : D * b.ld;
-    left -= D;
-  };
-  auto put = [&](int v, T* to) {
-    SA::store(va[v], to);
-    SB::store(vb[v], to + SA::kElems);
-  };
-  const int64_t steps = (depth + D - 1) / D;
+  through_registers<T, D, SA, SB, 2, AHEAD>(
+      a, b, depth, lds, [&](const T* la, const T* lb, int64_t t) {
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s) load(s);
-  put(0, lds);
-  T *now = lds, *next = lds + kStage;
-  for (int64_t t0 = 0; t0 < steps; t0 += AHEAD) {
+        for (int half = 0; half < 2; ++half) {
+          Pack<T> fa[X], fb[Y];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int64_t t = t0 + u;
-      if (t >= steps) break;
-      __syncthreads();
-      if (t + AHEAD < steps) load(u);
+          for (int x = 0; x < X; ++x) fa[x] = SA::fragment(la, wi + 16 * x, half);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        Pack<T> fa[X], fb[Y];
+          for (int y = 0; y < Y; ++y) fb[y] = SB::fragment(lb, wj + 16 * y, half);
 #pragma unroll
-        for (int x = 0; x < X; ++x) fa[x] = SA::fragment(now, wi + 16 * x, half);
+          for (int q = 0; q < V; ++q)
 #pragma unroll
-        for (int y = 0; y < Y; ++y) fb[y] = SB::fragment(now + SA::kElems, wj + 16 * y, half);
+            for (int x = 0; x < X; ++x)
 #pragma unroll
-        for (int q = 0; q < V; ++q)
-#pragma unroll
-          for (int x = 0; x < X; ++x)
-#pragma unroll
-            for (int y = 0; y < Y; ++y) acc[x][y] = mma4(fa[x].v[q], fb[y].v[q], acc[x][y]);
-      }
-      if constexpr (sizeof(T) == 4)
-        if (t % (kBlock32 / D) == kBlock32 / D - 1) {
-#pragma unroll
-          for (int x = 0; x < X; ++x)
-#pragma unroll
-            for (int y = 0; y < Y; ++y) {
-              all[x][y] += acc[x][y];
-              acc[x][y] = Acc{0, 0, 0, 0};
-            }
+              for (int y = 0; y < Y; ++y) acc[x][y] = mma4(fa[x].v[q], fb[y].v[q], acc[x][y]);
         }
-      if (t + 1 < steps) put((u + 1) % AHEAD, next);
-      T* swap = now;
-      now = next;
-      next = swap;
-    }
-  }
+        if constexpr (sizeof(T) == 4)
+          if (t % (kBlock32 / D) == kBlock32 / D - 1) {
+#pragma unroll
+            for (int x = 0; x < X; ++x)
+#pragma unroll
+              for (int y = 0; y < Y; ++y) {
+                all[x][y] += acc[x][y];
+                acc[x][y] = Acc{0, 0, 0, 0};
+              }
+          }
+      });
 #pragma unroll
   for (int x = 0; x < X; ++x)
 #pragma unroll
