@@ -121,7 +121,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product16(
     return;
   }
   tile16<T, T, BM, BN, WM, WN, true, ALONG_B, DIRECT, S>(
-      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n}, inner, lds16, c,
+      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n, col > 0}, inner, lds16, c,
       ldo);
 }
 
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256) void k_product_thin(
   part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
   thin16<T, C, BN, ALONG_B, DIRECT>(
       {a + from * lda + k, lda, m},
-      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n}, length, lds16, c, ldo);
+      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n, col > 0}, length, lds16, c, ldo);
 }
 
 // Split number blockIdx.z of an expert's rows writes its own ``gw`` (experts x inner x outer).
@@ -195,8 +195,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_weights_vjp16(
   from += k;
   const int64_t i = tm * BM, j = tn * BN;
   tile16<T, C, BM, BN, WM, WN, false, false, DIRECT, S>(
-      {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i)},
-      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, length, lds16,
+      {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i), i > 0},
+      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j), j > 0}, length, lds16,
       gw + ((int64_t)blockIdx.z * gridDim.y + e) * inner * outer + i * outer + j, outer);
 }
 
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(256, 2) void k_product32(
   part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
   tile32<T, BM, BN, WM, WN, true, ALONG_B, BM == 128 ? 1 : 3>(
       {a + from * lda + k, lda, m},
-      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n}, length, (T*)lds, c, ldo);
+      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n, col > 0}, length, (T*)lds, c, ldo);
 }
 
 // Split number blockIdx.z of an expert's rows writes its own ``gw``.
@@ -244,8 +244,8 @@ __global__ __launch_bounds__(256, 2) void k_weights_vjp32(
   from += k;
   const int64_t i = tm * BM, j = tn * BN;
   tile32<T, BM, BN, 2, 2, false, false, BM == 128 ? 1 : 3>(
-      {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i)},
-      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j)}, length, (T*)lds,
+      {a + from * lda + i, lda, (int)min<int64_t>(BM, inner - i), i > 0},
+      {g + from * ldg + j, ldg, (int)min<int64_t>(BN, outer - j), j > 0}, length, (T*)lds,
       gw + ((int64_t)blockIdx.z * gridDim.y + e) * inner * outer + i * outer + j, outer);
 }
 

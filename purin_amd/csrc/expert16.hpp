@@ -235,7 +235,8 @@ __device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, unsi
     for (int y = 0; y < Y; ++y)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
-  Ring<T, BM, BN, THREADS, ALONG_A, ALONG_B, DIRECT, S>::run(
+  constexpr int AHEAD = BM == 128 ? 2 : 1;  // as many registers as there are
+  Ring<T, BM, BN, THREADS, ALONG_A, ALONG_B, DIRECT, S, AHEAD>::run(
       a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb, int64_t) {
 #pragma unroll
         for (int s = 0; s < kDepth16 / 16; ++s) {

@@ -22,12 +22,14 @@ __device__ __forceinline__ const T* uniform(const T* p) {
 }
 
 // An operand of a tile: element (i, k) at p + i * ld + k where its contraction is contiguous
-// (ALONG), at p + k * ld + i where its rows are; n rows are there.
+// (ALONG), at p + k * ld + i where its rows are; n rows are there.  ``before``: whether those
+// that precede them in memory are rows of the same operand.
 template <typename T>
 struct Side {
   const T* p;
   int64_t ld;
   int n;
+  bool before = false;
 };
 
 // The elements moved down by ``by`` places (below the full width), zeros behind.
@@ -58,9 +60,13 @@ struct Pieces {
   // Whether whole stages may take the way without conditions: a piece that reaches past the
   // rows has a full piece's room before the end; offsets inside a stage fit 32 bits.
   static __device__ __forceinline__ bool whole(const Side<T>& o) {
-    return (ALONG || o.n >= kVec<T>) && o.ld < (int64_t(1) << 21);
+    return (ALONG || o.before || o.n >= kVec<T>) && o.ld < (int64_t(1) << 21);
   }
-  // byte offsets from the stage's first element, and the pieces that are moved into place
+  // how far before the stage's first element the loads begin
+  static __device__ __forceinline__ int lead(const Side<T>& o) {
+    return ALONG ? 0 : max(0, kVec<T> - o.n);
+  }
+  // byte offsets from there, and the pieces that are moved into place
   static __device__ __forceinline__ uint32_t reach(const Side<T>& o, uint32_t (&off)[kMine]) {
     uint32_t move = 0;
 #pragma unroll
@@ -77,7 +83,7 @@ struct Pieces {
           move |= 1u << m;
         }
       }
-      off[m] = ((uint32_t)row * (uint32_t)o.ld + (uint32_t)first) * (uint32_t)sizeof(T);
+      off[m] = ((uint32_t)row * (uint32_t)o.ld + (uint32_t)(first + lead(o))) * (uint32_t)sizeof(T);
     }
     return move;
   }
@@ -127,9 +133,10 @@ __device__ __forceinline__ void through_registers(const Side<T>& a, const Side<T
     // without a condition here too, so that the waits count on it: past the last whole stage,
     // that one again
     int64_t at = 0;
+    const T *from_a = pa - SA::lead(a), *from_b = pb - SB::lead(b);
     auto load = [&](int v) {
-      SA::load(pa + at * step_a, off_a, va[v]);
-      SB::load(pb + at * step_b, off_b, vb[v]);
+      SA::load(from_a + at * step_a, off_a, va[v]);
+      SB::load(from_b + at * step_b, off_b, vb[v]);
       if (at + 1 < whole) ++at;
     };
     auto put = [&](int v, T* to) {
