@@ -643,3 +643,120 @@ def test_refusals():
     (g,) = torch.autograd.grad(route(w, 2).weights.square().sum(), w, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), w)
+
+
+# ---------------------------------------------------------------------------
+# the products at sizes that take every cut of the kernels
+# ---------------------------------------------------------------------------
+
+# rows, experts, inner, outer: 16-bit products of 32 x 64 tiles with and without splits, 128 x 128
+# with four and with two stages, 256 x 256; weights' gradients split, 128 x 128 of both kinds and
+# 256 x 256; 32-bit ones of 32, 64 and 128 rows, split and whole; and the same off 16-byte rows
+LARGE = [(700, 4, 2048, 256), (1203, 3, 3000, 101), (2048, 2, 512, 1024), (2049, 2, 515, 1027),
+         (4096, 3, 256, 2048), (4100, 3, 259, 2051), (16400, 4, 72, 4104), (16401, 4, 77, 4099),
+         (9000, 2, 128, 136), (20000, 3, 200, 137), (1500, 16, 2048, 2056), (1400, 17, 2051, 2050),
+         (6000, 1, 64, 64), (30000, 100, 67, 70)]
+
+
+def _counts(rows, experts, seed):
+    """Unequal shares with an expert that has none (of three or more), and rows left over."""
+    rng = np.random.default_rng(seed)
+    share = rng.uniform(0.5, 1.5, experts)
+    if experts > 2:
+        share[1] = 0.0
+    return np.floor(share / share.sum() * rows * 0.97).astype(int)
+
+
+@pytest.mark.parametrize("rows,experts,inner,outer", LARGE)
+@pytest.mark.parametrize("order", ["io", "oi"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_large_products(rows, experts, inner, outer, order, dtype):
+    torch = require_gpu()
+    from purin_amd import expert_product
+
+    print(f"large product {rows} {experts} {inner} {outer} {order} {dtype}", flush=True)
+    t = _types(torch)[dtype]
+    counts = _counts(rows, experts, rows)
+    offsets = np.concatenate(([0], np.cumsum(counts)))
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    make = lambda *shape: torch.randn(shape, generator=g, device="cuda").to(t)
+    a = make(rows, inner).requires_grad_()
+    w = make(experts, inner, outer) if order == "io" else make(experts, outer, inner).transpose(1, 2)
+    w.requires_grad_()
+    cot = make(rows, outer)
+    out = expert_product(a, w, torch.as_tensor(offsets, dtype=torch.int32).cuda())
+    g_a, g_w = torch.autograd.grad(out, (a, w), cot)
+    u, s = UNIT[dtype], SUMS[dtype]
+
+    def check(got, x, y, what):  # got against x @ y in 64 bits
+        x, y = x.double(), y.double()
+        want, terms = x @ y, x.abs() @ y.abs()
+        bound = u * want.abs() + 2 * (x.shape[1] + 2) * s * terms * (1 + u) + STEP[dtype]
+        bad = ~((got.double() - want).abs() <= bound)
+        assert not bad.any(), (what, int(bad.sum()), bad.nonzero()[:3].tolist())
+
+    a, w = a.detach(), w.detach()
+    for e in range(experts):
+        i, j = int(offsets[e]), int(offsets[e + 1])
+        if i < j:
+            check(out[i:j], a[i:j], w[e], ("out", e))
+            check(g_a[i:j], cot[i:j], w[e].T, ("rows", e))
+            check(g_w[e], a[i:j].T, cot[i:j], ("weight", e))
+        else:
+            assert (g_w[e] == 0).all()
+    last = int(offsets[-1])
+    assert last < rows and (out[last:] == 0).all() and (g_a[last:] == 0).all()
+
+
+def test_long_sums_in_32_bits():
+    """A contraction of 40,000 in f32: the error against 64 bits stays what sums in blocks leave
+    (kBlock32 = 64 in one run, 625 such runs), far below that of one running sum."""
+    torch = require_gpu()
+    from purin_amd import expert_product
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    a = torch.rand((64, 40000), generator=g, device="cuda")
+    w = torch.rand((1, 40000, 64), generator=g, device="cuda")
+    at = torch.tensor([0, 64], dtype=torch.int32, device="cuda")
+    want = a.double() @ w[0].double()
+    got = expert_product(a, w, at).double()
+    # every partial sum is positive: 64 + 625 additions, half a unit each at most
+    assert float(((got - want).abs() / want).max()) <= (64 + 625 + 4) * 2.0 ** -24
+
+
+def test_gradients_against_differences():
+    """All calls in f64 through torch's own check by differences."""
+    torch = require_gpu()
+    from purin_amd import combine, dispatch, expert_product, route
+
+    w = _weights(torch, 3, 7, 5, "f64")
+    r0 = route(w, 2)
+    x = _randn(torch, 1, (7, 6), torch.float64).requires_grad_()
+    m = _randn(torch, 2, (5, 6, 4), torch.float64).requires_grad_()
+    # weights that keep their order under the differences' steps
+    w = (w * 1.0 + torch.arange(5, device="cuda") * 1e-3 * (w > 0)).requires_grad_()
+    assert torch.equal(route(w, 2).experts >= 0, r0.experts >= 0)
+
+    def f(x, m, w):
+        r = route(w, 2)
+        return combine(expert_product(dispatch(x, r), m, r), r)
+
+    # entries at zero have no difference to both sides: only the chosen weights are checked
+    chosen = route(w.detach(), 2)
+    c = chosen.weights.clone().requires_grad_()
+
+    def h(x, m, c):
+        return combine(expert_product(dispatch(x, chosen), m, chosen), chosen, c)
+
+    assert torch.autograd.gradcheck(h, (x, m, c), eps=1e-6, atol=1e-7, rtol=0)
+    out = f(x, m, w)
+    cot = _randn(torch, 5, (7, 4), torch.float64)
+    (g,) = torch.autograd.grad(out, w, cot)
+    for t, e in [(0, int(chosen.experts[0, 0])), (3, int(chosen.experts[3, 0]))]:
+        if e < 0:
+            continue
+        d = torch.zeros_like(w)
+        d[t, e] = 1e-6
+        with torch.no_grad():
+            slope = ((f(x, m, w + d) - f(x, m, w - d)) * cot).sum() / 2e-6
+        assert abs(float(slope - g[t, e])) <= 1e-7
