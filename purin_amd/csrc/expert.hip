@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256, 2) void k_product32(
   }
   int64_t k, length;
   part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
-  tile32<T, BM, BN, WM, WN, true, ALONG_B, BM == 128 ? 1 : 3>(
+  tile32<T, BM, BN, WM, WN, true, ALONG_B, 3>(
       {a + from * lda + k, lda, m},
       {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n, col > 0}, length, (T*)lds, c, ldo);
 }
@@ -389,22 +389,23 @@ static int weights_vjp16(hipStream_t st, int64_t rows, int64_t inner, int64_t ou
   return cut.shape == kDeep16 ? go(T{}, i128, i2, i4) : go(T{}, i128, i2, i2);
 }
 
-// How the 32- and 64-bit kernels cut a product: 32 x 64 tiles where rows are few, 128 x 128 (32
-// bits) where they fill the CUs twice, 64 x 64 between.  32-bit contractions are split as the
-// 16-bit ones, but up to four workgroups a CU: what one wavefront a SIMD leaves of the matrix
-// units' time between its reads and barriers, others use (f32, 700 rows, 4 experts, 4096 x 256:
-// 43 us with one, 31 with four).
+// How the 32- and 64-bit kernels cut a product: 32 x 64 tiles where rows, or tiles, are few, else
+// 64 x 64, in 32 bits with the contraction split as in 16, but up to four workgroups a CU: what
+// one wavefront a SIMD leaves of the matrix units' time between its reads and barriers, others
+// use (f32, 700 rows, 4 experts, 4096 x 256: 43 us with one, 31 with four).  128 x 128 tiles read
+// half as much, and were 2 % faster at 32768 rows, 16 experts, 2048 x 4096 (4630 us against 4740)
+// and slower wherever fewer of them run side by side (16384, 8, 512 x 512: 113 against 101).
 struct Cut32 {
   int height, splits;
 };
 static Cut32 cut_product32(bool wide, int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
-  if (!wide && most_tiles(rows, experts, 128) * ((outer + 127) / 128) >= 512 && rows > 32 * experts)
-    return {128, 1};
   const int64_t across = (outer + 63) / 64;
   const int height = rows <= 32 * experts || most_tiles(rows, experts, 64) * across < 512 ? 32 : 64;
   const int64_t groups = most_tiles(rows, experts, height) * across;
   return {height, wide ? 1 : splits_of(1024, groups, steps16(inner), 4)};
 }
+// The weights' gradient: both operands are read across their rows, and 128 x 128 tiles are ahead
+// from twice the CUs on (8192 rows, 64 experts, 1024 x 1024: 200 us against 213).
 static Cut32 cut_weights32(bool wide, int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
   if (!wide && ((inner + 127) / 128) * ((outer + 127) / 128) * experts >= 512) return {128, 1};
   const int64_t groups = ((inner + 63) / 64) * ((outer + 63) / 64) * experts;
@@ -419,19 +420,16 @@ static int product32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
   const int64_t ldw = along ? wo : wi;
   Cut32 cut = cut_product32(sizeof(T) == 8, rows, inner, outer, experts);
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
-  auto shape = [&](auto bm, auto bn, auto wm, auto wn) {
-    constexpr int BM = bm, BN = bn, WM = wm, WN = wn;
-    const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + BN - 1) / BN;
-    auto kernel = along ? k_product32<T, BM, BN, WM, WN, true> : k_product32<T, BM, BN, WM, WN, false>;
+  auto shape = [&](auto bm, auto wm, auto wn) {
+    constexpr int BM = bm, WM = wm, WN = wn;
+    const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + 63) / 64;
+    auto kernel = along ? k_product32<T, BM, 64, WM, WN, true> : k_product32<T, BM, 64, WM, WN, false>;
     kernel<<<dim3((unsigned)(tm * tn), (unsigned)cut.splits), dim3(256), 0, st>>>(
         a, lda, w, we, ldw, rows, inner, outer, (int)experts, tm, tn, offsets,
         cut.splits > 1 ? (T*)ws : out, ldo);
     return launched("k_product32");
   };
-  int rc = PURIN_CP_OK;
-  if (cut.height == 32) rc = shape(i32, i64, i1, i4);
-  else if (cut.height == 64) rc = shape(i64, i64, i2, i2);
-  else if constexpr (sizeof(T) == 4) rc = shape(i128, i128, i2, i2);
+  const int rc = cut.height == 32 ? shape(i32, i1, i4) : shape(i64, i2, i2);
   if constexpr (sizeof(T) == 4)
     if (!rc && cut.splits > 1) return join(st, (const float*)ws, cut.splits, rows * outer, out);
   return rc;
@@ -448,13 +446,13 @@ static int weights_vjp32(hipStream_t st, int64_t rows, int64_t inner, int64_t ou
         a, lda, g, ldg, rows, inner, outer, tm, tn, offsets, cut.splits > 1 ? (T*)ws : gw);
     return launched("k_weights_vjp32");
   };
-  int rc = PURIN_CP_OK;
-  if (cut.height == 64) rc = go(64, k_weights_vjp32<T, 64, 64>);
-  else if constexpr (sizeof(T) == 4) rc = go(128, k_weights_vjp32<T, 128, 128>);
   if constexpr (sizeof(T) == 4)
-    if (!rc && cut.splits > 1)
+    if (cut.height == 128) return go(128, k_weights_vjp32<T, 128, 128>);
+  if (int rc = go(64, k_weights_vjp32<T, 64, 64>)) return rc;
+  if constexpr (sizeof(T) == 4)
+    if (cut.splits > 1)
       return join(st, (const float*)ws, cut.splits, experts * inner * outer, gw);
-  return rc;
+  return PURIN_CP_OK;
 }
 
 // 32-bit sums of the parts, where a product is split.
