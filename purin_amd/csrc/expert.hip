@@ -249,9 +249,17 @@ __global__ __launch_bounds__(256, 2) void k_weights_vjp32(
       gw + ((int64_t)blockIdx.z * gridDim.y + e) * inner * outer + i * outer + j, outer);
 }
 
+// A launch holds fewer than 2^32 threads: more tiles than that do not fit the card's memory.
+static int check_grid(int64_t tiles, int threads) {
+  if (tiles * threads < (int64_t(1) << 32)) return PURIN_CP_OK;
+  return set_error(PURIN_CP_ERR_UNSUPPORTED, "too many tiles for a launch");
+}
+
 template <typename K, typename... A>
-static int launch16(const char* name, K kernel, dim3 grid, int threads, int lds, hipStream_t st,
-                    A... args) {
+static int launch16(const char* name, K kernel, int64_t tiles, unsigned gy, unsigned gz,
+                    int threads, int lds, hipStream_t st, A... args) {
+  if (int rc = check_grid(tiles, threads)) return rc;
+  const dim3 grid((unsigned)tiles, gy, gz);
   if (int rc = raise_lds_cap((const void*)kernel, (size_t)lds)) return rc;
   kernel<<<grid, dim3((unsigned)threads), (size_t)lds, st>>>(args...);
   return launched(name);
@@ -341,8 +349,7 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
                                     : k_product_thin<T, C, TN, true, false>)
                           : (direct ? k_product_thin<T, C, TN, false, true>
                                     : k_product_thin<T, C, TN, false, false>);
-      return launch16("k_product_thin", kernel, dim3((unsigned)(tm * tn), (unsigned)cut.splits),
-                      256, thin_lds<TN>(), st, a, lda, w, we, ldw, rows, inner, outer,
+      return launch16("k_product_thin", kernel, tm * tn, (unsigned)cut.splits, 1, 256, thin_lds<TN>(), st, a, lda, w, we, ldw, rows, inner, outer,
                       (int)experts, tn, offsets, cut.splits > 1 ? (C*)ws : (C*)out, ldo);
     };
     if (cut.splits == 1) return thin(T{});
@@ -356,7 +363,7 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
                                   : k_product16<T, B, B, 2, WN, true, false, S>)
                         : (direct ? k_product16<T, B, B, 2, WN, false, true, S>
                                   : k_product16<T, B, B, 2, WN, false, false, S>);
-    return launch16("k_product16", kernel, dim3((unsigned)(tm * tn)), 2 * WN * 64,
+    return launch16("k_product16", kernel, tm * tn, 1, 1, 2 * WN * 64,
                     tile16_lds<T, T, B, B, S>(), st, a, lda, w, we, ldw, rows, inner, outer,
                     (int)experts, tm, tn, offsets, out, ldo);
   };
@@ -376,9 +383,8 @@ static int weights_vjp16(hipStream_t st, int64_t rows, int64_t inner, int64_t ou
     const int64_t tm = (inner + B - 1) / B, tn = (outer + B - 1) / B;
     auto kernel = direct ? k_weights_vjp16<T, C, B, B, 2, WN, true, S>
                          : k_weights_vjp16<T, C, B, B, 2, WN, false, S>;
-    return launch16("k_weights_vjp16", kernel,
-                    dim3((unsigned)(tm * tn), (unsigned)experts, (unsigned)cut.splits), 2 * WN * 64,
-                    tile16_lds<T, C, B, B, S>(), st, a, lda, g, ldg, rows, inner, outer, tm, tn,
+    return launch16("k_weights_vjp16", kernel, tm * tn, (unsigned)experts,
+                    (unsigned)cut.splits, 2 * WN * 64, tile16_lds<T, C, B, B, S>(), st, a, lda, g, ldg, rows, inner, outer, tm, tn,
                     offsets, cut.splits > 1 ? (C*)ws : (C*)gw);
   };
   if (cut.splits > 1) {
@@ -423,6 +429,7 @@ static int product32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
   auto shape = [&](auto bm, auto wm, auto wn) {
     constexpr int BM = bm, WM = wm, WN = wn;
     const int64_t tm = most_tiles(rows, experts, BM), tn = (outer + 63) / 64;
+    if (int e = check_grid(tm * tn, 256)) return e;
     auto kernel = along ? k_product32<T, BM, 64, WM, WN, true> : k_product32<T, BM, 64, WM, WN, false>;
     kernel<<<dim3((unsigned)(tm * tn), (unsigned)cut.splits), dim3(256), 0, st>>>(
         a, lda, w, we, ldw, rows, inner, outer, (int)experts, tm, tn, offsets,
@@ -442,6 +449,7 @@ static int weights_vjp32(hipStream_t st, int64_t rows, int64_t inner, int64_t ou
   const Cut32 cut = cut_weights32(sizeof(T) == 8, rows, inner, outer, experts);
   auto go = [&](int b, auto kernel) {
     const int64_t tm = (inner + b - 1) / b, tn = (outer + b - 1) / b;
+    if (int e = check_grid(tm * tn, 256)) return e;
     kernel<<<dim3((unsigned)(tm * tn), (unsigned)experts, (unsigned)cut.splits), dim3(256), 0, st>>>(
         a, lda, g, ldg, rows, inner, outer, tm, tn, offsets, cut.splits > 1 ? (T*)ws : gw);
     return launched("k_weights_vjp32");

@@ -68,7 +68,7 @@ def _same_index(routing, ids, offsets, place, source):
 # ---------------------------------------------------------------------------
 
 ROUTES = [(1, 1, 1), (1, 64, 8), (3, 5, 5), (37, 9, 3), (200, 33, 4), (257, 130, 6),
-          (700, 16, 16), (1500, 300, 2), (130, 1024, 40), (4100, 65, 3)]
+          (700, 16, 16), (1500, 300, 2), (130, 1024, 40), (4100, 65, 3), (50, 100, 37), (90, 300, 70)]
 
 
 @pytest.mark.parametrize("tokens,count,slots", ROUTES)
