@@ -121,8 +121,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product16(
     return;
   }
   tile16<T, T, BM, BN, WM, WN, true, ALONG_B, DIRECT, S>(
-      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n, col > 0}, inner, lds16, c,
-      ldo);
+      {a + from * lda, lda, m}, {w + e * we + (ALONG_B ? col * ldw : col), ldw, n, col > 0}, inner,
+      lds16, c, ldo);
 }
 
 // out = the sum of ``splits`` parts, in their order.
@@ -151,9 +151,9 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, i
   }
 }
 
-// Experts with few rows, or few tiles in all: column tiles of 64 for 32 rows at a time.  Split
+// Experts with few rows, or few tiles in all: column tiles of 64 for BM rows at a time.  Split
 // number blockIdx.y of the contraction writes its own ``out``.
-template <typename T, typename C, int BN, bool ALONG_B, bool DIRECT>
+template <typename T, typename C, int BM, int BN, bool ALONG_B, bool DIRECT>
 __global__ __launch_bounds__(256) void k_product_thin(
     const T* __restrict__ a, int64_t lda, const T* __restrict__ w, int64_t we, int64_t ldw,
     int64_t rows, int64_t inner, int64_t outer, int experts, int64_t tiles_n,
@@ -162,10 +162,10 @@ __global__ __launch_bounds__(256) void k_product_thin(
   const int64_t tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
   int e;
   int64_t from, to;
-  if (!find_tile(offsets, experts, rows, 32, tm, e, from, to)) return;
+  if (!find_tile(offsets, experts, rows, BM, tm, e, from, to)) return;
   e = __builtin_amdgcn_readfirstlane(e);
   const int64_t col = tn * BN;
-  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(32, to - from));
+  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
   const int n = (int)min<int64_t>(BN, outer - col);
   C* c = out + (int64_t)blockIdx.y * rows * ldo + from * ldo + col;
   if (e < 0) {
@@ -174,9 +174,10 @@ __global__ __launch_bounds__(256) void k_product_thin(
   }
   int64_t k, length;
   part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
-  thin16<T, C, BN, ALONG_B, DIRECT>(
+  thin16<T, C, BM, BN, ALONG_B, DIRECT>(
       {a + from * lda + k, lda, m},
-      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n, col > 0}, length, lds16, c, ldo);
+      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n, col > 0}, length, lds16, c,
+      ldo);
 }
 
 // Split number blockIdx.z of an expert's rows writes its own ``gw`` (experts x inner x outer).
@@ -225,7 +226,8 @@ __global__ __launch_bounds__(256, 2) void k_product32(
   part_of(inner, (int)blockIdx.y, (int)gridDim.y, k, length);
   tile32<T, BM, BN, WM, WN, true, ALONG_B, 3>(
       {a + from * lda + k, lda, m},
-      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n, col > 0}, length, (T*)lds, c, ldo);
+      {w + e * we + (ALONG_B ? col * ldw + k : col + k * ldw), ldw, n, col > 0}, length, (T*)lds, c,
+      ldo);
 }
 
 // Split number blockIdx.z of an expert's rows writes its own ``gw``.
@@ -292,6 +294,9 @@ static int64_t most_tiles(int64_t rows, int64_t experts, int64_t height) {
 // 2048 x 2048 | 32768, 16, 2048 x 4096, bf16:
 //   thin    32 x 64 tiles: the experts' weights at the rate of memory where rows are few, and
 //           eight times the workgroups where tiles are few       9.5 |  41 |   - |   -
+//           64 x 64 ones from 16 rows to an expert on, where they fill the CUs: a second tile of
+//           an expert reads its weights again (768 rows, 32 experts of unequal shares,
+//           4096 x 1536: 99 us with 32, 87 with 64; 512 rows, 64 experts, 1024 x 1024: 30, 32)
 //   deep    up to one 128 x 128 tile a CU there is room for 4 stages, three on their way: the
 //           stages' latency is what counts then                 15.5 |   - |   - |   -
 //   128     two workgroups a CU of 2 stages                        - |  32 |  34 | 660
@@ -302,7 +307,7 @@ static int64_t most_tiles(int64_t rows, int64_t experts, int64_t height) {
 enum Shape16 { kThin16, kDeep16, k128, k256 };
 struct Cut16 {
   Shape16 shape;
-  int splits;
+  int height, splits;
 };
 static int64_t steps16(int64_t depth) { return (depth + kDepth16 - 1) / kDepth16; }
 // Splits of at least ``part`` stages, ``groups`` workgroups each, up to ``room`` workgroups.
@@ -312,15 +317,20 @@ static int splits_of(int64_t room, int64_t groups, int64_t steps, int64_t part) 
 static Cut16 cut_product16(int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
   const int64_t tiles = most_tiles(rows, experts, 128) * ((outer + 127) / 128);
   if (rows <= 32 * experts || tiles <= 128) {
-    const int64_t groups = most_tiles(rows, experts, 32) * ((outer + 63) / 64);
-    return {kThin16, splits_of(256, groups, steps16(inner), 16)};
+    const int64_t across = (outer + 63) / 64;
+    const bool tall = rows > 16 * experts && most_tiles(rows, experts, 64) * across >= 256;
+    const int height = tall ? 64 : 32;
+    return {kThin16, height,
+            splits_of(256, most_tiles(rows, experts, height) * across, steps16(inner), 16)};
   }
-  return {tiles <= 256 ? kDeep16 : tiles < 16 * 256 ? k128 : k256, 1};
+  if (tiles >= 16 * 256) return {k256, 256, 1};
+  return {tiles <= 256 ? kDeep16 : k128, 128, 1};
 }
 static Cut16 cut_weights16(int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
   const int64_t tiles = ((inner + 127) / 128) * ((outer + 127) / 128) * experts;
   const int splits = splits_of(256, tiles, steps16(rows / experts), 12);
-  return {tiles * splits <= 256 ? kDeep16 : tiles < 16 * 256 ? k128 : k256, splits};
+  if (tiles >= 16 * 256) return {k256, 256, 1};
+  return {tiles * splits <= 256 ? kDeep16 : k128, 128, splits};
 }
 
 // The ``splits`` parts of ``count`` sums added up into out.
@@ -330,11 +340,16 @@ static int join(hipStream_t st, const float* parts, int splits, int64_t count, T
   return launched("k_join");
 }
 
+// Whether a weight is read along inner (a length of one has any stride); along outer otherwise.
+static bool along_inner(int64_t inner, int64_t wi, int64_t wo) {
+  return wo != 1 && (wi == 1 || inner <= 1);
+}
+
 template <typename T>
 static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
                      const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,
                      const int32_t* offsets, void* ws, T* out, int64_t ldo) {
-  const bool along = wi == 1 && (wo != 1 || inner > 1);
+  const bool along = along_inner(inner, wi, wo);
   const int64_t ldw = along ? wo : wi;
   const bool direct = direct_ok(a, lda, inner) && direct_ok(w, ldw, along ? inner : outer) &&
                       we % 8 == 0;
@@ -342,16 +357,19 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
   if (cut.shape == kThin16) {
     constexpr int TN = 64;
-    const int64_t tm = most_tiles(rows, experts, 32), tn = (outer + TN - 1) / TN;
-    auto thin = [&](auto c) {
+    const int64_t tm = most_tiles(rows, experts, cut.height), tn = (outer + TN - 1) / TN;
+    auto tall = [&](auto c, auto h) {
       using C = decltype(c);
-      auto kernel = along ? (direct ? k_product_thin<T, C, TN, true, true>
-                                    : k_product_thin<T, C, TN, true, false>)
-                          : (direct ? k_product_thin<T, C, TN, false, true>
-                                    : k_product_thin<T, C, TN, false, false>);
-      return launch16("k_product_thin", kernel, tm * tn, (unsigned)cut.splits, 1, 256, thin_lds<TN>(), st, a, lda, w, we, ldw, rows, inner, outer,
-                      (int)experts, tn, offsets, cut.splits > 1 ? (C*)ws : (C*)out, ldo);
+      constexpr int TM = h;
+      auto kernel = along ? (direct ? k_product_thin<T, C, TM, TN, true, true>
+                                    : k_product_thin<T, C, TM, TN, true, false>)
+                          : (direct ? k_product_thin<T, C, TM, TN, false, true>
+                                    : k_product_thin<T, C, TM, TN, false, false>);
+      return launch16("k_product_thin", kernel, tm * tn, (unsigned)cut.splits, 1, 256,
+                      thin_lds<TM, TN>(), st, a, lda, w, we, ldw, rows, inner, outer, (int)experts,
+                      tn, offsets, cut.splits > 1 ? (C*)ws : (C*)out, ldo);
     };
+    auto thin = [&](auto c) { return cut.height == 32 ? tall(c, i32) : tall(c, i64); };
     if (cut.splits == 1) return thin(T{});
     if (int rc = thin(float{})) return rc;
     return join(st, (const float*)ws, cut.splits, rows * outer, out);
@@ -422,7 +440,7 @@ template <typename T>
 static int product32(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
                      const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,
                      const int32_t* offsets, void* ws, T* out, int64_t ldo) {
-  const bool along = wi == 1 && (wo != 1 || inner > 1);
+  const bool along = along_inner(inner, wi, wo);
   const int64_t ldw = along ? wo : wi;
   Cut32 cut = cut_product32(sizeof(T) == 8, rows, inner, outer, experts);
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row

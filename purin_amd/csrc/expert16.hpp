@@ -281,45 +281,52 @@ __device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, unsi
   }
 }
 
-// Few rows: at most 32, by BN, where reading b is the work.  kThin stages, all but one of them
+// Few rows: at most BM, by BN, where reading b is the work.  kThin stages, all but one of them
 // on their way at any time; the 4 wavefronts share a stage's contraction (16 each) and add up
-// their sums at the end, in LDS, in their order.  ``lds`` holds thin_lds<BN>() bytes.
+// their sums at the end, in LDS, in their order.  ``lds`` holds thin_lds<BM, BN>() bytes.
 constexpr int kThin = 4;
-template <int BN>
+template <int BM, int BN>
 constexpr int thin_lds() {
-  constexpr int stages = kThin * (32 + BN) * kDepth16 * 2, sums = 4 * 32 * (BN + 4) * 4;
+  constexpr int stages = kThin * (BM + BN) * kDepth16 * 2, sums = 4 * BM * (BN + 4) * 4;
   return stages > sums ? stages : sums;
 }
 
-template <typename T, typename C, int BN, bool ALONG_B, bool DIRECT>
+template <typename T, typename C, int BM, int BN, bool ALONG_B, bool DIRECT>
 __device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsigned char* lds,
                                        C* c, int64_t ldc) {
-  constexpr int THREADS = 256, Y = BN / 32, P = BN + 4;
+  constexpr int THREADS = 256, X = BM / 32, Y = BN / 32, P = BN + 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  F16x acc[Y];
+  F16x acc[X][Y];
 #pragma unroll
-  for (int y = 0; y < Y; ++y)
+  for (int x = 0; x < X; ++x)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[y][r] = 0.0f;
-  Ring<T, 32, BN, THREADS, true, ALONG_B, DIRECT, kThin, kThin - 1>::run(
+    for (int y = 0; y < Y; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+  Ring<T, BM, BN, THREADS, true, ALONG_B, DIRECT, kThin, kThin - 1>::run(
       a, b, depth, reinterpret_cast<T*>(lds), [&](const T* la, const T* lb, int64_t) {
-        const S8 fa = fragment<T, 32, true>(la, 0, wave);
-        S8 fb[Y];
+        S8 fa[X], fb[Y];
+#pragma unroll
+        for (int x = 0; x < X; ++x) fa[x] = fragment<T, BM, true>(la, 32 * x, wave);
 #pragma unroll
         for (int y = 0; y < Y; ++y) fb[y] = fragment<T, BN, ALONG_B>(lb, 32 * y, wave);
 #pragma unroll
-        for (int y = 0; y < Y; ++y) acc[y] = mma32(T{}, fb[y], fa, acc[y]);
+        for (int x = 0; x < X; ++x)
+#pragma unroll
+          for (int y = 0; y < Y; ++y) acc[x][y] = mma32(T{}, fb[y], fa[x], acc[x][y]);
       });
   float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int y = 0; y < Y; ++y)
+  for (int x = 0; x < X; ++x)
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      sums[(wave * 32 + (lane & 31)) * P + 32 * y + 2 * (r & ~3) + 4 * (lane >> 5) + (r & 3)] =
-          acc[y][r];
+    for (int y = 0; y < Y; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        sums[(wave * BM + 32 * x + (lane & 31)) * P + 32 * y + 2 * (r & ~3) + 4 * (lane >> 5) +
+             (r & 3)] = acc[x][y][r];
   __syncthreads();
   constexpr int V = kVec<C>;
-  for (int at = threadIdx.x; at < 32 * BN / V; at += THREADS) {
+  for (int at = threadIdx.x; at < BM * BN / V; at += THREADS) {
     const int i = at / (BN / V), j = at % (BN / V) * V;
     if (i >= a.n || j >= b.n) continue;
     Pack<C> v;
@@ -327,7 +334,7 @@ __device__ __forceinline__ void thin16(Side<T> a, Side<T> b, int64_t depth, unsi
     for (int q = 0; q < V; ++q) {
       float s = sums[i * P + j + q];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) s += sums[(w * 32 + i) * P + j + q];
+      for (int w = 1; w < 4; ++w) s += sums[(w * BM + i) * P + j + q];
       v.v[q] = (C)s;
     }
     store_upto(c + i * ldc + j, v, b.n - j);

@@ -318,7 +318,9 @@ def test_product_strides_and_alignment(dtype):
     for a, z in ((0, 128), (1, 129), (3, 100)):
         rows = wide[:, a:z]
         for w in (big[:, a:z, :], big[:, a:z, 1:130], big[:, :, a:z].transpose(1, 2)[:, :, :],
-                  big[1:2, a:z, :].expand(3, z - a, 140), big[:, a:z, ::2]):
+                  big[1:2, a:z, :].expand(3, z - a, 140), big[:, a:z, ::2],
+                  big[:, a:a + 1, ::3], big[:, a:z, 5:6], big[:, a:z:2, 5:6],
+                  big[:, a:a + 1, 7:8], big.transpose(1, 2)[:, a:a + 1, ::2]):
             if w.shape[1] != z - a:
                 w = w[:, :z - a, :]
             rows = wide[:, a:a + w.shape[1]]
