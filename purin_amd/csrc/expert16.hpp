@@ -13,6 +13,11 @@
 //            wavefront reads at once fall on 8 places
 // With 16-byte rows at 16-byte addresses the stages are loaded straight into LDS (buffer loads
 // whose addresses outside the operand read zeros); others pass through registers.
+//
+// 256 x 256 tiles are bound by the matrix units and what the LDS reads and barriers leave of
+// them: 0.95 PFLOP/s, 1.05 for the weights' gradient (32768 rows, 16 experts, 2048 x 4096, bf16;
+// a library's single product of 8192 reaches 1.2), 0.58 through registers at 1613 x 3618.  The
+// tiles for few rows are bound by memory: 4.8 TB/s (768 rows, 32 experts, 4096 x 1536).
 #pragma once
 
 #include "stages.hpp"

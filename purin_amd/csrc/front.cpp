@@ -92,6 +92,7 @@ struct Workspace {
   Workspace(const std::optional<Tensor>& given, int64_t need, const Tensor& like) {
     if (given) {
       if (!given->is_cuda()) refuse("workspace must be a device tensor");
+      same_device(like, *given, "workspace");
       held = *given;
     } else if (bytes(need)) {
       held = at::empty({need}, like.options().dtype(at::kByte).requires_grad(false));

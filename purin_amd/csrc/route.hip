@@ -9,6 +9,12 @@
 // The order is made by counting: every chunk of pairs counts its experts, then every chunk
 // places its pairs behind the earlier experts' and the earlier chunks'.  Ranks inside a
 // wavefront come from ballots on the expert's bits, so the order is the pairs' own.
+//
+// Moving rows is bound by memory.  A token's row is read once for all its slots (dispatch), its
+// gradient once for both of combine's gradients.  32768 tokens of 4 slots, 4096 bf16: dispatch
+// 234 us (5.7 TB/s; part of its writes stay in the 256 MB cache), combine 292 (4.6) and without
+// weights 275 (4.9), combine's gradients 481 (5.0).  With few tokens the launches count: choosing
+// and sorting 1 token of 64 experts takes 5.6 us, dispatch and combine 3 each.
 
 #include <algorithm>
 #include <type_traits>
@@ -80,7 +86,8 @@ __device__ __forceinline__ K group_max(K v) {
 }
 
 // G lanes to a token, V weights to a lane (expert i * G + lane): slots times, the lanes'
-// best by (weight, lowest expert), then the group's.
+// best by (weight, lowest expert), then the group's.  Bound by that chain: 32768 tokens, 4 of 128
+// experts 11 us (13 with the exchanges through LDS), of which reading the weights takes 3.5.
 template <typename T, int G, int V>
 __device__ __forceinline__ void choose(const T* row, int experts, int slots, int lane,
                                        int32_t* ids, T* chosen) {
