@@ -28,11 +28,16 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int64_t kSortChunk = 2048;  // pairs of a workgroup, at least
 constexpr int64_t kSortGroups = 256;  // workgroups, at most
+// Pairs up to which one workgroup has them all, and no launch counts first (a whole route of 500
+// tokens, 6 of 64 experts: 10.1 us for 13.4; 1000 tokens, 8 slots: 15.8 for 13.2).
+constexpr int64_t kSortOne = 4096;
 
 struct SortShape {
   int64_t chunk, groups;
 };
 static SortShape sort_shape(int64_t pairs) {
+  if (pairs <= kSortOne)
+    return {std::max<int64_t>(1, (pairs + kSortThreads - 1) / kSortThreads) * kSortThreads, 1};
   int64_t chunk = std::max<int64_t>(kSortChunk, (pairs + kSortGroups - 1) / kSortGroups);
   chunk = (chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
   return {chunk, std::max<int64_t>(1, (pairs + chunk - 1) / chunk)};
