@@ -56,13 +56,14 @@ __device__ __forceinline__ uint32_t lds_address(const T* lds) {
 }
 // 16 bytes a lane from the buffer to ``to`` + 16 * lane in LDS.  Written out, without an output
 // register: the compiler would have every later LDS read wait for it, also one of the other
-// stage.  The loop waits for its stage itself.  (M0 holds the place; nothing else in these
-// kernels uses it.)
+// stage.  The loop waits for its stage itself.  M0 holds the place; a load into LDS that follows
+// a scalar write of M0 needs one wait state between them, which nothing but the s_nop supplies
+// (hardware does not, and the compiler does not look inside).
 __device__ __forceinline__ void load_to_lds(U4 r, uint32_t at, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane((int)to)), "v"(at), "s"(r)
-               : "memory");
+               : "memory", "m0");
 }
 
 template <int N>
