@@ -213,6 +213,26 @@ Routed route_experts(const Tensor& experts, int64_t count, const std::optional<T
 
 // -- rows ---------------------------------------------------------------------------------
 
+// A routing's order of rows, as the kernels read it.  The tensors are a caller's by now, who may
+// have replaced them.
+struct Order {
+  Tensor place, offsets;
+  Order(const Tensor& p, const Tensor& o) {
+    check(p, 2, "routing.place", "(tokens, slots)");
+    check(o, 1, "routing.offsets", "(experts + 1)");
+    if (p.size(1) < 1) refuse("routing.place must have a slot");
+    if (o.size(0) < 2) refuse("routing.offsets must have an expert");
+    same_device(p, o, "routing.offsets");
+    place = p.contiguous();
+    offsets = o.contiguous();
+  }
+  static void check(const Tensor& t, int64_t dim, const char* name, const char* shape) {
+    if (!t.is_cuda() || t.layout() != at::kStrided || t.scalar_type() != at::kInt || t.dim() != dim)
+      refuse(name, " must be an int32 tensor ", shape, " on the GPU; got ", t.scalar_type(), " ",
+             t.sizes(), " on ", t.device());
+  }
+};
+
 Tensor run_combine(const Tensor& given, const Tensor& place, const Tensor* weights) {
   const Tensor rows = matrix(given);
   const Call call(rows);
@@ -245,8 +265,10 @@ struct DispatchFn : torch::autograd::Function<DispatchFn> {
   }
 };
 
-Tensor dispatch(const Tensor& x, const Tensor& place, const Tensor& offsets) {
+Tensor dispatch(const Tensor& x, const Tensor& place_given, const Tensor& offsets_given) {
   code_of(x, "x");
+  const Order order(place_given, offsets_given);
+  const Tensor &place = order.place, &offsets = order.offsets;
   same_device(place, x, "x");
   if (x.dim() != 2 || x.size(0) != place.size(0))
     refuse("x must have shape (", place.size(0), ", width); got ", x.sizes());
@@ -280,9 +302,11 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
   }
 };
 
-Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place,
-               const Tensor& offsets) {
+Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place_given,
+               const Tensor& offsets_given) {
   code_of(rows, "rows");
+  const Order order(place_given, offsets_given);
+  const Tensor &place = order.place, &offsets = order.offsets;
   same_device(place, rows, "rows");
   if (rows.dim() != 2 || rows.size(0) != place.numel())
     refuse("rows must have shape (", place.numel(), ", width); got ", rows.sizes());

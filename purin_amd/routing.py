@@ -37,7 +37,9 @@ class Routing:
     there, connected to autograd where the weights given to ``route`` are; ``offsets``
     (count + 1) int32, each expert's first row and the rows' number last; ``place``
     (tokens, slots) int32, a slot's row, -1 where it is empty; ``source`` (tokens * slots) int32,
-    the slot (token * slots + slot) of each row, -1 from ``offsets[count]`` on.
+    the slot (token * slots + slot) of each row, -1 from ``offsets[count]`` on.  ``place`` and
+    ``offsets`` are what the calls below read: their types and shapes are checked there, their
+    values are not (rows outside the buffer are passed over).
     """
 
     tokens: int

@@ -1,0 +1,48 @@
+"""The operators around the projection layer on inputs that need care: what is refused, and what
+has to come out right in spite of an unusual form."""
+
+import dataclasses
+
+import numpy as np
+import pytest
+
+from oracle import train as ot
+from tests._gpu import require_gpu, to_np
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_routing_with_other_index_tensors():
+    """``place`` and ``offsets`` of a routing are read as int32 in order: another type, shape or
+    device is refused, another order in memory is read as what it says."""
+    torch = require_gpu()
+    from purin_amd import combine, dispatch, route
+
+    rng = np.random.default_rng(2)
+    w = torch.as_tensor(rng.random((7, 5)) * (rng.random((7, 5)) < 0.6)).cuda()
+    x = torch.as_tensor(rng.standard_normal((7, 6))).cuda()
+    r = route(w, 3)
+    y = torch.as_tensor(rng.standard_normal((21, 6))).cuda()
+    bad = [dict(place=r.place.long()), dict(place=r.place.float()), dict(place=r.place.cpu()),
+           dict(place=r.place.view(-1)), dict(place=r.place[:, :0]), dict(place=None),
+           dict(offsets=r.offsets.long()), dict(offsets=r.offsets.cpu()), dict(offsets=None),
+           dict(offsets=r.offsets[:1]), dict(offsets=r.offsets.view(2, 3))]
+    for change in bad:
+        other = dataclasses.replace(r, **change)
+        for f in (lambda: dispatch(x, other), lambda: combine(y, other),
+                  lambda: combine(y.clone().requires_grad_(), other)):
+            with pytest.raises(ValueError):
+                f()
+                print("not refused:", change, flush=True)
+    # the same values in another order, and one row of places for all tokens
+    turned = dataclasses.replace(r, place=r.place.t().contiguous().t(),
+                                 offsets=torch.stack((r.offsets, r.offsets), 1)[:, 0])
+    assert not turned.place.is_contiguous() and not turned.offsets.is_contiguous()
+    assert torch.equal(dispatch(x, turned), dispatch(x, r))
+    assert torch.equal(combine(y, turned), combine(y, r))
+    one = dataclasses.replace(r, place=r.place[:1].expand(7, 3))
+    place, chosen = np.repeat(to_np(r.place[:1]), 7, 0), to_np(r.weights)
+    want = ot.combine(to_np(y), place, chosen)
+    terms = ot.combine(np.abs(to_np(y)), place, chosen)
+    # three products and sums in 64 bits
+    assert (np.abs(to_np(combine(y, one)) - want) <= 2 * 5 * 2.0 ** -53 * terms).all()
