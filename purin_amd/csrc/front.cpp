@@ -91,7 +91,9 @@ struct Workspace {
   int64_t size = 0;
   Workspace(const std::optional<Tensor>& given, int64_t need, const Tensor& like) {
     if (given) {
-      if (!given->is_cuda()) refuse("workspace must be a device tensor");
+      // a broadcast or strided tensor has fewer bytes in one piece than it has elements
+      if (!given->is_cuda() || given->layout() != at::kStrided || !given->is_contiguous())
+        refuse("workspace must be a contiguous device tensor");
       same_device(like, *given, "workspace");
       held = *given;
     } else if (bytes(need)) {

@@ -28,7 +28,8 @@ def _list(tensors, name):
 
 
 def clip_workspace_bytes(tensors):
-    """Bytes of a caller's workspace for a list of ``tensors`` gradients (256-byte aligned)."""
+    """Bytes of a caller's workspace, a contiguous device tensor at 256 bytes, for a list of
+    ``tensors`` gradients."""
     return int(_lib.load().purin_train_clip_workspace_bytes(tensors))
 
 

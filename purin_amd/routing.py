@@ -70,8 +70,9 @@ def route(weights, slots, *, workspace=None):
 
     ``weights`` (tokens, experts), any floating type, at most 1024 experts.  Zero and negative
     weights choose nothing, so that a token may have fewer experts than slots, or none; ties go
-    to the lowest expert; NaN counts as larger than any number.  ``workspace``: a device tensor
-    of ``route_workspace_bytes(tokens, experts, slots)`` bytes (new memory otherwise).
+    to the lowest expert; NaN counts as larger than any number.  ``workspace``: a contiguous
+    device tensor of ``route_workspace_bytes(tokens, experts, slots)`` bytes (new memory
+    otherwise).
     """
     if slots.__class__ is not int:
         raise ValueError(f"slots must be a positive integer; got {slots!r}")

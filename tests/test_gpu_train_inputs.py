@@ -46,3 +46,24 @@ def test_a_routing_with_other_index_tensors():
     terms = ot.combine(np.abs(to_np(y)), place, chosen)
     # three products and sums in 64 bits
     assert (np.abs(to_np(combine(y, one)) - want) <= 2 * 5 * 2.0 ** -53 * terms).all()
+
+
+def test_a_workspace_is_one_piece_of_memory():
+    """A broadcast or strided workspace has fewer bytes in one piece than its size says."""
+    torch = require_gpu()
+    from purin_amd import clip_gradients, gradient_norm, route, route_experts
+    from purin_amd.gradients import clip_workspace_bytes
+    from purin_amd.routing import route_workspace_bytes
+
+    w = torch.rand((4000, 20), device="cuda")
+    ids = torch.zeros((4000, 3), dtype=torch.int32, device="cuda")
+    g = [torch.rand(50, device="cuda")]
+    need = max(route_workspace_bytes(4000, 20, 3), clip_workspace_bytes(1))
+    whole = torch.empty((need, 2), dtype=torch.uint8, device="cuda")
+    for ws in (whole[:1, :1].expand(need, 1), whole[:, 0], whole.t(), whole.cpu()):
+        for f in (lambda: route(w, 3, workspace=ws), lambda: route_experts(ids, 20, workspace=ws),
+                  lambda: gradient_norm(g, workspace=ws),
+                  lambda: clip_gradients(g, 1.0, workspace=ws)):
+            with pytest.raises(ValueError, match="workspace"):
+                f()
+    route(w, 3, workspace=whole)
