@@ -6,11 +6,13 @@
 // No kernel is here; libpurin_cp.so, which this links to, holds them and knows nothing of torch.
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -35,6 +37,7 @@ struct LibraryError : std::exception {
   int code;
   std::string message;
   explicit LibraryError(int c) : code(c), message(purin_cp_last_error()) {}
+  LibraryError(int c, std::string m) : code(c), message(std::move(m)) {}
   const char* what() const noexcept override { return message.c_str(); }
 };
 
@@ -75,12 +78,28 @@ Tensor matrix(const Tensor& t) {
   return t;
 }
 
+// Forward-mode differentiation passes these operators by: a result without a tangent would read as
+// one whose tangent is zero.
+void without_tangent(const Tensor& t) {
+  if (t.defined() && t._fw_grad(0).defined())
+    throw LibraryError(PURIN_CP_ERR_UNSUPPORTED,
+                       "forward-mode differentiation is not supported: a tensor has a tangent");
+}
+// A trace would hold the allocations of a call and not its kernels.
+void outside_traces() {
+  if (torch::jit::tracer::isTracing() ||
+      c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+    throw LibraryError(PURIN_CP_ERR_UNSUPPORTED, "the operator cannot be traced");
+}
+
 // The device made current, and its current stream, for one entry point.
 struct Call {
   c10::DeviceGuard guard;
   void* stream;
   explicit Call(const Tensor& t)
-      : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+      : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {
+    outside_traces();
+  }
 };
 
 // A call's scratch: the caller's, or new memory, which the allocator gives to nothing else
@@ -163,6 +182,7 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
     return chosen;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    without_tangent(grads[0]);
     const Tensor ids = ctx->get_saved_variables()[0], g = grads[0].contiguous();
     const int64_t count = ctx->saved_data["count"].toInt();
     const Call call(g);
@@ -181,6 +201,7 @@ Routed route(const Tensor& weights, int64_t slots, const std::optional<Tensor>& 
   const int64_t count = weights.size(1);
   if (slots < 1) refuse("slots must be a positive integer; got ", slots);
   if (count < 1 || slots > count) refuse("slots must not exceed the ", count, " experts; got ", slots);
+  without_tangent(weights);
   Index index;
   Tensor chosen = wants_grad(weights) ? RouteFn::apply(weights, slots, workspace, &index)
                                       : run_route(weights, slots, workspace, &index);
@@ -263,6 +284,7 @@ struct DispatchFn : torch::autograd::Function<DispatchFn> {
     return run_dispatch(x, place, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    without_tangent(grads[0]);
     return once({run_combine(grads[0], ctx->get_saved_variables()[0], nullptr), Tensor(), Tensor()});
   }
 };
@@ -274,6 +296,7 @@ Tensor dispatch(const Tensor& x, const Tensor& place_given, const Tensor& offset
   same_device(place, x, "x");
   if (x.dim() != 2 || x.size(0) != place.size(0))
     refuse("x must have shape (", place.size(0), ", width); got ", x.sizes());
+  without_tangent(x);
   return wants_grad(x) ? DispatchFn::apply(x, place, offsets) : run_dispatch(x, place, offsets);
 }
 
@@ -286,6 +309,7 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
+    for (const Tensor& t : {saved[0], saved[1], grads[0]}) without_tangent(t);
     const Tensor rows = matrix(saved[0]), w = saved[1].contiguous(), g = matrix(grads[0]);
     const Tensor &place = saved[2], &offsets = saved[3];
     const Call call(g);
@@ -316,6 +340,8 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place_gi
   same_device(rows, weights, "weights");
   if (weights.sizes() != place.sizes())
     refuse("weights must have shape ", place.sizes(), "; got ", weights.sizes());
+  without_tangent(rows);
+  without_tangent(weights);
   if (wants_grad(rows) || wants_grad(weights)) return CombineFn::apply(rows, weights, place, offsets);
   const Tensor w = weights.contiguous();
   return run_combine(rows, place, &w);
@@ -368,6 +394,7 @@ struct ProductFn : torch::autograd::Function<ProductFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
+    for (const Tensor& t : {saved[0], saved[1], grads[0]}) without_tangent(t);
     const Tensor a = matrix(saved[0]), w = weight_strides(saved[1]), g = matrix(grads[0]);
     const Tensor& offsets = saved[2];
     Tensor g_rows, g_weight;
@@ -396,6 +423,8 @@ Tensor expert_product(const Tensor& rows, const Tensor& weight, const Tensor& of
     refuse("offsets must be a Routing or an int32 tensor of ", weight.size(0) + 1, " entries");
   same_device(rows, weight, "weight");
   same_device(rows, offsets, "offsets");
+  without_tangent(rows);
+  without_tangent(weight);
   const Tensor at = offsets.contiguous();
   return wants_grad(rows) || wants_grad(weight) ? ProductFn::apply(rows, weight, at)
                                                 : run_product(rows, weight_strides(weight), at);
@@ -436,6 +465,7 @@ bool overlaps_itself(const Tensor& t) {
 int32_t gradient_code(const Tensor& t, const char* name, size_t i) {
   const std::string each = std::string(name) + "[" + std::to_string(i) + "]";
   if (t.layout() != at::kStrided) refuse(each, " must be a dense tensor");
+  without_tangent(t);
   return code_of(t, each.c_str());
 }
 

@@ -11,10 +11,11 @@ exactly zero; a softmax gives weights that are all positive.  From either:
 
 Every call runs in the HIP library (``include/purin_train.h``) on the current stream of its
 tensors' device, waits for nothing and keeps nothing; all are differentiable with torch
-autograd, once.  The reference ends at the projection layer and has no counterpart.
+autograd, once and in reverse.  The reference ends at the projection layer and has no counterpart.
 
 Arguments are checked in ``csrc/front.cpp``, which also holds the autograd nodes: a wrong one
-raises ``ValueError``, what the library cannot do ``PurinError``.
+raises ``ValueError``, what the library cannot do ``PurinError`` (forward-mode tangents and
+tracing among it, where a result would miss its derivative or its kernels).
 """
 
 from __future__ import annotations

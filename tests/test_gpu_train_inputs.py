@@ -67,3 +67,67 @@ def test_a_workspace_is_one_piece_of_memory():
             with pytest.raises(ValueError, match="workspace"):
                 f()
     route(w, 3, workspace=whole)
+
+
+def _layer(torch):
+    """Tensors and the calls that have a derivative, each of one of them."""
+    from purin_amd import clip_gradients, combine, dispatch, expert_product, gradient_norm, route
+
+    rng = np.random.default_rng(4)
+    make = lambda *shape: torch.as_tensor(rng.random(shape), dtype=torch.float32).cuda()  # noqa: E731
+    w, x, y, m = make(6, 4), make(6, 8), make(12, 8), make(4, 8, 5)
+    r = route(w, 2)
+    return [(w, lambda t: route(t, 2).weights), (x, lambda t: dispatch(t, r)),
+            (y, lambda t: combine(t, r)), (r.weights, lambda t: combine(y, r, t)),
+            (y, lambda t: expert_product(t, m, r)), (m, lambda t: expert_product(y, t, r)),
+            (x, lambda t: gradient_norm([t])),
+            (x, lambda t: clip_gradients([t], 1.0, out=[torch.empty_like(x)])),
+            (x, lambda t: clip_gradients([x], 1.0, out=[t]))]
+
+
+def test_a_tangent_is_refused_and_not_lost():
+    torch = require_gpu()
+    import torch.autograd.forward_ad as fw
+    from purin_amd._lib import PurinError
+
+    for i, (t, f) in enumerate(_layer(torch)):
+        for grad in (False, True):
+            with fw.dual_level():
+                dual = fw.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+                with pytest.raises(PurinError, match="forward-mode"):
+                    f(dual)
+                    print("not refused:", i, grad, flush=True)
+        out = f(t.clone())  # outside a level as before
+        assert torch.isfinite(out).all()
+    # forward over reverse: a tangent that comes in with the gradient
+    for i, (t, f) in enumerate(_layer(torch)[:6]):
+        x = t.clone().requires_grad_()
+        out = f(x)
+        with fw.dual_level():
+            cot = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, cot)
+                print("not refused in reverse:", i, flush=True)
+
+
+def test_a_trace_is_refused():
+    """A trace would hold the outputs' allocation and not the kernels that fill them."""
+    torch = require_gpu()
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    for i, (t, f) in enumerate(_layer(torch)[:7]):
+        for trace in (lambda: torch.jit.trace(f, (t,)), lambda: make_fx(f)(t)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                trace()
+                print("not refused:", i, flush=True)
+        assert torch.isfinite(f(t)).all()
+
+
+def test_function_transforms_raise():
+    """Tensors of torch.func have no memory of their own: an error, and no wrong result."""
+    torch = require_gpu()
+    for t, f in _layer(torch)[:7]:
+        for call in (lambda: torch.func.jvp(f, (t,), (t,)), lambda: torch.func.grad(
+                lambda v: f(v).sum())(t), lambda: torch.func.vmap(f)(t[None])):
+            with pytest.raises(Exception):
+                call()
