@@ -71,8 +71,13 @@ void same_device(const Tensor& a, const Tensor& b, const char* name) {
   if (a.device() != b.device()) refuse(name, " must be on ", a.device(), "; got ", b.device());
 }
 
+// The numbers themselves in memory, where torch holds their negatives and a mark (the imaginary
+// part of a conjugate).
+Tensor numbers(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // A matrix with adjacent elements in a row and rows that do not overlap.
-Tensor matrix(const Tensor& t) {
+Tensor matrix(const Tensor& given) {
+  const Tensor t = numbers(given);
   if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1)))
     return t.contiguous();
   return t;
@@ -183,7 +188,7 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     without_tangent(grads[0]);
-    const Tensor ids = ctx->get_saved_variables()[0], g = grads[0].contiguous();
+    const Tensor ids = ctx->get_saved_variables()[0], g = numbers(grads[0]).contiguous();
     const int64_t count = ctx->saved_data["count"].toInt();
     const Call call(g);
     Tensor out = at::empty({ids.size(0), count}, g.options().requires_grad(false));
@@ -304,13 +309,13 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights,
                         const Tensor& place, const Tensor& offsets) {
     ctx->save_for_backward({rows, weights, place, offsets});
-    const Tensor w = weights.contiguous();
+    const Tensor w = numbers(weights).contiguous();
     return run_combine(rows, place, &w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     for (const Tensor& t : {saved[0], saved[1], grads[0]}) without_tangent(t);
-    const Tensor rows = matrix(saved[0]), w = saved[1].contiguous(), g = matrix(grads[0]);
+    const Tensor rows = matrix(saved[0]), w = numbers(saved[1]).contiguous(), g = matrix(grads[0]);
     const Tensor &place = saved[2], &offsets = saved[3];
     const Call call(g);
     Tensor g_rows, g_weights;
@@ -343,7 +348,7 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place_gi
   without_tangent(rows);
   without_tangent(weights);
   if (wants_grad(rows) || wants_grad(weights)) return CombineFn::apply(rows, weights, place, offsets);
-  const Tensor w = weights.contiguous();
+  const Tensor w = numbers(weights).contiguous();
   return run_combine(rows, place, &w);
 }
 
@@ -351,7 +356,8 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& place_gi
 
 // A weight with a unit stride along inner or outer and no overlap inside a matrix; a broadcast
 // over the experts stays one.
-Tensor weight_strides(const Tensor& w) {
+Tensor weight_strides(const Tensor& given) {
+  const Tensor w = numbers(given);
   const int64_t inner = w.size(1), outer = w.size(2), si = w.stride(1), so = w.stride(2);
   if ((so == 1 || outer <= 1) && (si >= outer || inner <= 1)) return w;
   if ((si == 1 || inner <= 1) && (so >= inner || outer <= 1)) return w;
@@ -528,7 +534,9 @@ Tensor clip_gradients(const Tensors& gradients, double largest, const std::optio
         refuse("out[", i, "] must have shape ", g.sizes(), " and type ", g.scalar_type(), "; got ",
                o.sizes(), " and ", o.scalar_type());
     }
-    if (o.is_contiguous() && (in_place || g.is_contiguous())) {
+    // in place the marks of g and out are one, and a factor changes no sign
+    const bool straight = in_place || (g.is_contiguous() && !g.is_neg() && !o.is_neg());
+    if (o.is_contiguous() && straight) {
       list.add(g, o, code);
     } else if (overlaps_itself(o)) {
       refuse("out[", i, "] (or the gradient in place) has elements that share memory");
@@ -536,7 +544,7 @@ Tensor clip_gradients(const Tensors& gradients, double largest, const std::optio
       list.add(g, g, code);
     } else {  // any other order goes through a copy in order
       const Tensor c = at::empty(o.sizes(), o.options().requires_grad(false));
-      list.add(g.contiguous(), c, code);
+      list.add(numbers(g).contiguous(), c, code);
       back.emplace_back(o, c);
     }
   }

@@ -131,3 +131,63 @@ def test_function_transforms_raise():
                 lambda v: f(v).sum())(t), lambda: torch.func.vmap(f)(t[None])):
             with pytest.raises(Exception):
                 call()
+
+
+@pytest.mark.parametrize("width", [1, 8])
+@pytest.mark.parametrize("view", ["imag", "whole"])
+def test_lazily_negated_tensors(view, width):
+    """The imaginary part of a conjugate holds its numbers' negatives and a mark; what a call
+    reads and writes are the numbers."""
+    torch = require_gpu()
+    from purin_amd import (clip_gradients, combine, dispatch, expert_product, gradient_norm, route,
+                           route_experts)
+
+    def negated(t):  # t's numbers behind the mark, in memory of their own
+        if view == "whole":
+            return torch._neg_view(-t)
+        return torch.complex(torch.zeros_like(t), -t).conj().imag
+
+    rng = np.random.default_rng(6)
+    make = lambda *s: torch.as_tensor(rng.standard_normal(s), dtype=torch.float32).cuda()  # noqa: E731
+    w, x, y, m = make(9, 4), make(9, width), make(18, width), make(4, width, 5)
+    assert negated(w).is_neg() and torch.equal(negated(w), w)
+    r = route(w, 2)
+    n = route(negated(w), 2)
+    assert torch.equal(n.weights, r.weights) and torch.equal(n.experts, r.experts)
+    assert torch.equal(dispatch(negated(x), r), dispatch(x, r))
+    assert torch.equal(combine(negated(y), r), combine(y, r))
+    assert torch.equal(combine(y, r, negated(r.weights)), combine(y, r))
+    given = route_experts(r.experts, 4, weights=negated(r.weights))
+    assert torch.equal(combine(y, given), combine(y, r))
+    out = expert_product(y, m, r)
+    assert torch.equal(expert_product(negated(y), m, r), out)
+    assert torch.equal(expert_product(y, negated(m), r), out)
+
+    def gradients(f, inputs, cot):
+        inputs = [t.clone().requires_grad_() for t in inputs]
+        return torch.autograd.grad(f(*inputs), inputs, cot)
+
+    for f, inputs, shape in ((lambda a: route(a, 2).weights, (w,), (9, 2)),
+                             (lambda a: dispatch(a, r), (x,), (18, width)),
+                             (lambda a, b: combine(a, r, b), (y, r.weights), (9, width)),
+                             (lambda a, b: expert_product(a, b, r), (y, m), (18, 5))):
+        cot = make(*shape)
+        want, got = gradients(f, inputs, cot), gradients(f, inputs, negated(cot))
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    # saved for the backward pass behind the mark
+    a = torch.complex(torch.zeros_like(y), -y).requires_grad_()
+    (g,) = torch.autograd.grad(expert_product(a.conj().imag, m, r).sum(), a)
+    (want,) = gradients(lambda v: expert_product(v, m, r), (y,), torch.ones_like(out))
+    assert torch.equal(g.imag, -want)
+
+    assert torch.equal(gradient_norm([negated(x)]), gradient_norm([x]))
+    want = [torch.empty_like(x)]
+    clip_gradients([x], 1.0, out=want)
+    for given, into in ((negated(x), torch.empty_like(x)), (x, negated(x)),
+                        (negated(x), negated(x))):
+        clip_gradients([given], 1.0, out=[into])
+        assert torch.equal(into, want[0])
+        assert torch.equal(given, x)
+    here = negated(x)
+    clip_gradients([here], 1.0)
+    assert torch.equal(here, want[0])
