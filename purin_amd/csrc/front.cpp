@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <numeric>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -468,6 +469,93 @@ bool overlaps_itself(const Tensor& t) {
   return false;
 }
 
+// The bytes of a tensor's elements: ``from`` + the sum of steps (bytes) times indexes, ``size``
+// bytes from each such address on, all below ``to``.
+struct Bytes {
+  int64_t from, to, size;
+  std::vector<std::pair<int64_t, int64_t>> steps;
+  explicit Bytes(const Tensor& t) : from((int64_t)t.data_ptr()), size((int64_t)t.element_size()) {
+    to = from + size;
+    for (const auto& [stride, n] : steps_of(t)) {
+      if (!stride) continue;
+      steps.emplace_back(stride * size, n);
+      to += stride * size * (n - 1);
+    }
+  }
+};
+
+// Whether two tensors may have a byte in common: whether some sum of a's steps less b's, each
+// ``c`` times a whole number between ``low`` and ``high``, is the distance of two such elements.
+// From the largest step on, only numbers that the smaller steps can make up for are tried, and
+// none where the distance is no multiple of what the steps left have in common.  Views of one
+// tensor have steps in common, which count as one, and take a few trials; beyond ``left`` trials
+// the answer is yes.
+struct Shared {
+  struct Term {
+    int64_t c, low, high;
+    int64_t least, most, common;  // of the sums of this term and those behind it
+  };
+  std::vector<Term> terms;
+  int64_t left = 1 << 16;
+
+  static int64_t down(int64_t a, int64_t b) { return a / b - (a % b < 0); }  // b > 0
+  bool within(size_t i, int64_t low, int64_t high) {
+    if (i == terms.size()) return low <= 0 && 0 <= high;
+    const Term& t = terms[i];
+    if (down(high, t.common) * t.common < low) return false;
+    if (--left < 0) return true;
+    const bool more = i + 1 < terms.size();
+    const int64_t least = more ? terms[i + 1].least : 0, most = more ? terms[i + 1].most : 0;
+    const int64_t first = std::max(t.low, -down(-(low - most), t.c));
+    const int64_t last = std::min(t.high, down(high - least, t.c));
+    for (int64_t z = first; z <= last; ++z)
+      if (within(i + 1, low - t.c * z, high - t.c * z)) return true;
+    return false;
+  }
+  bool operator()(const Bytes& a, const Bytes& b) {
+    if (a.from >= b.to || b.from >= a.to) return false;
+    for (const auto& [c, n] : a.steps) terms.push_back({c, 0, n - 1, 0, 0, 0});
+    for (const auto& [c, n] : b.steps) {
+      const auto same = [c = c](const Term& t) { return t.c == c; };
+      const auto at = std::find_if(terms.begin(), terms.end(), same);
+      if (at == terms.end()) terms.push_back({c, 1 - n, 0, 0, 0, 0});
+      else at->low -= n - 1;
+    }
+    std::sort(terms.begin(), terms.end(), [](const Term& x, const Term& y) { return x.c > y.c; });
+    int64_t least = 0, most = 0, common = 0;
+    for (size_t i = terms.size(); i-- > 0;) {
+      Term& t = terms[i];
+      t.least = least += t.c * t.low;
+      t.most = most += t.c * t.high;
+      t.common = common = std::gcd(common, t.c);
+    }
+    const int64_t apart = a.from - b.from;
+    return within(0, 1 - a.size - apart, b.size - 1 - apart);
+  }
+};
+
+// One tensor of a list that is read, or written (``out``); ``copied``: by way of a copy, so that
+// the library does not see its place.
+struct Use {
+  size_t tensor;
+  bool out, copied;
+  Bytes bytes;
+};
+// Refuses an output that shares memory with another tensor's output or gradient, where one of the
+// two is copied (the library looks at the others).
+void check_overlap(std::vector<Use> uses) {
+  std::sort(uses.begin(), uses.end(),
+            [](const Use& a, const Use& b) { return a.bytes.from < b.bytes.from; });
+  for (size_t i = 0; i < uses.size(); ++i)
+    for (size_t j = i + 1; j < uses.size() && uses[j].bytes.from < uses[i].bytes.to; ++j) {
+      const Use &a = uses[i], &b = uses[j];
+      if (a.tensor == b.tensor || !(a.out || b.out) || !(a.copied || b.copied)) continue;
+      if (Shared()(a.bytes, b.bytes))
+        throw LibraryError(PURIN_CP_ERR_ARG, "tensor " + std::to_string((a.out ? a : b).tensor) +
+                                                 ": its output overlaps another tensor");
+    }
+}
+
 int32_t gradient_code(const Tensor& t, const char* name, size_t i) {
   const std::string each = std::string(name) + "[" + std::to_string(i) + "]";
   if (t.layout() != at::kStrided) refuse(each, " must be a dense tensor");
@@ -521,6 +609,7 @@ Tensor clip_gradients(const Tensors& gradients, double largest, const std::optio
     refuse("out must hold ", gradients.size(), " tensors; got ", outs.size());
   List list;
   std::vector<std::pair<Tensor, Tensor>> back;
+  std::vector<char> copied(gradients.size(), 0);
   for (size_t i = 0; i < gradients.size(); ++i) {
     if (gradients[i].has_value() != outs[i].has_value())
       refuse("out[", i, "] must be None exactly where the gradient is");
@@ -534,19 +623,28 @@ Tensor clip_gradients(const Tensors& gradients, double largest, const std::optio
         refuse("out[", i, "] must have shape ", g.sizes(), " and type ", g.scalar_type(), "; got ",
                o.sizes(), " and ", o.scalar_type());
     }
-    // in place the marks of g and out are one, and a factor changes no sign
-    const bool straight = in_place || (g.is_contiguous() && !g.is_neg() && !o.is_neg());
-    if (o.is_contiguous() && straight) {
-      list.add(g, o, code);
-    } else if (overlaps_itself(o)) {
+    if (!o.is_contiguous() && overlaps_itself(o))
       refuse("out[", i, "] (or the gradient in place) has elements that share memory");
-    } else if (in_place && dense(g)) {
-      list.add(g, g, code);
+    // in place the marks of g and out are one, and a factor changes no sign
+    if (in_place ? dense(g)
+                 : g.is_contiguous() && o.is_contiguous() && !g.is_neg() && !o.is_neg()) {
+      list.add(g, o, code);
     } else {  // any other order goes through a copy in order
+      copied[i] = 1;
       const Tensor c = at::empty(o.sizes(), o.options().requires_grad(false));
       list.add(numbers(g).contiguous(), c, code);
       back.emplace_back(o, c);
     }
+  }
+  if (!back.empty()) {
+    std::vector<Use> uses;
+    for (size_t i = 0; i < gradients.size(); ++i) {
+      if (!gradients[i] || !gradients[i]->numel()) continue;
+      const bool by_copy = copied[i];
+      uses.push_back({i, true, by_copy, Bytes(*outs[i])});
+      if (!outs[i]->is_same(*gradients[i])) uses.push_back({i, false, by_copy, Bytes(*gradients[i])});
+    }
+    check_overlap(std::move(uses));
   }
   const Tensor norm = list.run(largest, workspace);
   for (auto& [o, c] : back) o.copy_(c);

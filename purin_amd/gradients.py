@@ -46,8 +46,8 @@ def clip_gradients(gradients, largest, out=None, *, workspace=None):
 
     Where the norm is not above ``largest`` nothing is written.  ``out``: tensors of the
     gradients' shapes and types to write instead, in full, the gradients staying as they are
-    (``None`` beside ``None``).  No two tensors may share memory, but a gradient and its own
-    ``out``.  A NaN norm makes all gradients NaN; an infinite one makes finite gradients zero
+    (``None`` beside ``None``).  An output that shares memory with another tensor of the call is
+    refused; a gradient and its own ``out`` may share theirs.  A NaN norm makes all gradients NaN; an infinite one makes finite gradients zero
     and infinite ones NaN: the returned norm tells.
     """
     return _front.clip_gradients(_list(gradients, "gradients"), float(largest),

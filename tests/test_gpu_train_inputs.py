@@ -191,3 +191,60 @@ def test_lazily_negated_tensors(view, width):
     here = negated(x)
     clip_gradients([here], 1.0)
     assert torch.equal(here, want[0])
+
+
+def test_clip_refuses_strided_views_that_share_memory():
+    torch = require_gpu()
+    from purin_amd import clip_gradients
+    from purin_amd._lib import PurinError
+
+    base = torch.rand((6, 10), device="cuda") + 0.5
+    other = torch.rand((6, 5), device="cuda")
+
+    def refused(make):  # make(b): gradients and outputs on b
+        b, o = base.clone(), other.clone()
+        gradients, out = make(b, o)
+        with pytest.raises((PurinError, ValueError)):
+            clip_gradients(gradients, 0.1, out=out)
+            print("not refused", flush=True)
+        assert torch.equal(b, base) and torch.equal(o, other)  # and nothing was written
+
+    refused(lambda b, o: ([b[:, :5], b[:, 3:8]], None))
+    refused(lambda b, o: ([b[::2, ::3], b[2:, 6:]], None))
+    refused(lambda b, o: ([b.t()[1:9], b[3]], None))
+    refused(lambda b, o: ([b[:, 2], b[2]], None))
+    refused(lambda b, o: ([b[:, 2], b.view(-1)[12:13]], None))
+    # an output over another gradient, and over another output
+    refused(lambda b, o: ([o, b[:, :5]], [b[:, 4:9], o.clone()]))
+    refused(lambda b, o: ([o, b], [b[:, 4:9], b.clone()]))
+    refused(lambda b, o: ([o, o.clone()], [b[:, :5], b[:, 4:9]]))
+    refused(lambda b, o: ([o, o.clone()], [b[:, :5], b.view(-1)[7:37].view(6, 5)]))
+    refused(lambda b, o: ([b[:, :5], o], [o.clone(), b[:, 4:9]]))
+
+    def taken(make):  # disjoint views: as if each had memory of its own
+        b = base.clone()
+        gradients, out = make(b)
+        alone = [g.clone() for g in gradients]
+        norm = clip_gradients(alone, 0.1)
+        assert torch.equal(clip_gradients(gradients, 0.1, out=out), norm)
+        for o, a in zip(gradients if out is None else out, alone):
+            assert torch.equal(o, a)
+
+    taken(lambda b: ([b[:, :5], b[:, 5:]], None))
+    taken(lambda b: ([b[:, i] for i in range(10)], None))
+    taken(lambda b: ([b[::2, ::2], b[1::2, 1::2], b[::2, 1::2], b[1::2, ::2]], None))
+    taken(lambda b: ([b[:2].t(), b[2:4].t(), b[4:, 1::2], b[4:, ::2]], None))
+    taken(lambda b: ([b.t()[:5], b[:, 5], b.view(-1)[6:10], b[1:, 6:]], None))
+    taken(lambda b: ([b[:, :5].clone(), b[:, 5:].clone()], [b[:, 5:], b[:, :5]]))
+    # a gradient and its own output in another order
+    square = torch.rand((8, 8), device="cuda")
+    want = square.clone()
+    norm = clip_gradients([want], 0.1)
+    assert torch.equal(clip_gradients([square], 0.1, out=[square.t()]), norm)
+    assert torch.equal(square.t(), want)
+    # a broadcast gradient is read, and two may read the same memory where nothing is written
+    row = base[:1].expand(4, 10)
+    out = [torch.empty(4, 10, device="cuda"), torch.empty(4, 10, device="cuda")]
+    clip_gradients([row, row.clone()], 0.1, out=out)
+    assert torch.equal(out[0], out[1])
+    clip_gradients([base[:, :5], base[:, 3:8]], 0.1, out=[torch.empty_like(other) for _ in "ab"])
