@@ -152,6 +152,12 @@ int purin_train_clip(void* stream, int64_t count, const purin_train_tensor* tens
                      double largest, void* workspace, int64_t workspace_bytes,
                      int32_t norm_dtype, void* norm);
 
+/* The gradient of clip's norm: out = in * g_norm / norm for each tensor, zero
+ * where the norm is.  norm and g_norm are device scalars of norm_dtype; the
+ * list's rules are clip's. */
+int purin_train_norm_vjp(void* stream, int64_t count, const purin_train_tensor* tensors,
+                         int32_t norm_dtype, const void* norm, const void* g_norm);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,7 @@ TRAIN_SYMBOLS = (
     "purin_train_expert_weights_vjp",
     "purin_train_clip_workspace_bytes",
     "purin_train_clip",
+    "purin_train_norm_vjp",
 )
 
 
@@ -269,6 +270,7 @@ def _declare_train(lib):
                                                    vp, vp, i64, vp]
     lib.purin_train_clip_workspace_bytes.argtypes = [i64]
     lib.purin_train_clip.argtypes = [vp, i64, C.POINTER(TrainTensor), dbl, vp, i64, i32, vp]
+    lib.purin_train_norm_vjp.argtypes = [vp, i64, C.POINTER(TrainTensor), i32, vp, vp]
     for name in TRAIN_SYMBOLS:
         getattr(lib, name).restype = i64 if name.endswith("_bytes") else C.c_int
 

@@ -588,16 +588,64 @@ struct List {
   }
 };
 
-Tensor gradient_norm(const Tensors& gradients, const std::optional<Tensor>& workspace) {
-  const at::NoGradGuard no_grad;
+// A gradient whose elements fill one span of memory, in whatever order.
+Tensor span(const Tensor& t) {
+  const Tensor g = numbers(t);
+  return dense(g) ? g : g.contiguous();
+}
+
+Tensor run_norm(at::TensorList gradients, const std::optional<Tensor>& workspace) {
   List list;
-  for (size_t i = 0; i < gradients.size(); ++i) {
-    if (!gradients[i]) continue;
-    const int32_t code = gradient_code(*gradients[i], "gradients", i);
-    const Tensor g = dense(*gradients[i]) ? *gradients[i] : gradients[i]->contiguous();
-    list.add(g, g, code);
+  for (const Tensor& given : gradients) {
+    const Tensor g = span(given);
+    list.add(g, g, code_of(g, "gradient"));
   }
   return list.run(-1.0, workspace);
+}
+
+struct NormFn : torch::autograd::Function<NormFn> {
+  static Tensor forward(AutogradContext* ctx, at::TensorList gradients,
+                        const std::optional<Tensor>& workspace) {
+    const Tensor norm = run_norm(gradients, workspace);
+    variable_list saved = gradients.vec();
+    saved.push_back(norm);
+    ctx->save_for_backward(std::move(saved));
+    return norm;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list saved = ctx->get_saved_variables();
+    for (const Tensor& t : saved) without_tangent(t);
+    without_tangent(grads[0]);
+    const Tensor norm = saved.back(), g_norm = numbers(grads[0]);
+    saved.pop_back();
+    variable_list out(saved.size() + 1), held;  // the workspace has no gradient
+    std::vector<purin_train_tensor> table;
+    for (size_t i = 0; i < saved.size(); ++i) {
+      if (!ctx->needs_input_grad(i)) continue;
+      const Tensor g = span(saved[i]);
+      out[i] = at::empty_strided(g.sizes(), g.strides(), g.options().requires_grad(false));
+      table.push_back({g.data_ptr(), out[i].data_ptr(), g.numel(), code_of(g, "gradient"), 0});
+      held.push_back(g);
+    }
+    const Call call(norm);
+    check(purin_train_norm_vjp(call.stream, (int64_t)table.size(), table.data(),
+                               code_of(norm, "norm"), norm.data_ptr(), g_norm.data_ptr()));
+    return once(std::move(out));
+  }
+};
+
+Tensor gradient_norm(const Tensors& gradients, const std::optional<Tensor>& workspace) {
+  variable_list given;
+  bool graph = false;
+  for (size_t i = 0; i < gradients.size(); ++i) {
+    if (!gradients[i]) continue;
+    gradient_code(*gradients[i], "gradients", i);
+    given.push_back(*gradients[i]);
+    graph = graph || wants_grad(*gradients[i]);
+  }
+  if (graph) return NormFn::apply(at::TensorList(given), workspace);
+  const at::NoGradGuard no_grad;
+  return run_norm(given, workspace);
 }
 
 Tensor clip_gradients(const Tensors& gradients, double largest, const std::optional<Tensors>& out,

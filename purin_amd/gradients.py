@@ -36,7 +36,9 @@ def clip_workspace_bytes(tensors):
 def gradient_norm(gradients, *, workspace=None):
     """The 2-norm of all gradients together: a tensor without dimensions, float64 if any gradient
     is, float32 otherwise.  ``gradients``: a tensor, or a list whose ``None`` are left out; mixed
-    types are fine.  Squares are summed in 64 bits, in an order that the sizes alone decide."""
+    types are fine.  Squares are summed in 64 bits, in an order that the sizes alone decide.
+    Differentiable once (a gradient's is itself over the norm, zero where the norm is), so that a
+    penalty on gradients reaches what they were made from."""
     return _front.gradient_norm(_list(gradients, "gradients"), workspace)
 
 
@@ -47,8 +49,9 @@ def clip_gradients(gradients, largest, out=None, *, workspace=None):
     Where the norm is not above ``largest`` nothing is written.  ``out``: tensors of the
     gradients' shapes and types to write instead, in full, the gradients staying as they are
     (``None`` beside ``None``).  An output that shares memory with another tensor of the call is
-    refused; a gradient and its own ``out`` may share theirs.  A NaN norm makes all gradients NaN; an infinite one makes finite gradients zero
-    and infinite ones NaN: the returned norm tells.
+    refused, except a gradient's own ``out``.  A NaN norm makes all gradients NaN; an infinite one
+    makes finite gradients zero and infinite ones NaN: the returned norm tells.  Autograd does
+    not see the call: neither the norm nor what is written has a graph.
     """
     return _front.clip_gradients(_list(gradients, "gradients"), float(largest),
                                  None if out is None else _list(out, "out"), workspace)

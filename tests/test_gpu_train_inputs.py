@@ -248,3 +248,101 @@ def test_clip_refuses_strided_views_that_share_memory():
     clip_gradients([row, row.clone()], 0.1, out=out)
     assert torch.equal(out[0], out[1])
     clip_gradients([base[:, :5], base[:, 3:8]], 0.1, out=[torch.empty_like(other) for _ in "ab"])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64", "bf16", "f16", "mixed"])
+def test_the_norm_has_a_gradient(dtype):
+    """g / norm times the incoming gradient.  The norm is rounded to its type (u), the factor to
+    the sums' type and the product once more, then to the gradient's type (h)."""
+    torch = require_gpu()
+    from purin_amd import gradient_norm
+
+    types = {"f32": torch.float32, "f64": torch.float64, "bf16": torch.bfloat16,
+             "f16": torch.float16}
+    names = list(types) if dtype == "mixed" else [dtype] * 4
+    rng = np.random.default_rng(8)
+    shapes = [(700, 41), (1,), (33, 5, 7), (0, 3)]
+    g = [torch.as_tensor(rng.standard_normal(s)).to(types[n]).cuda()
+         for s, n in zip(shapes, names)]
+    g[2] = g[2].permute(2, 0, 1)  # dense in another order
+    with torch.no_grad():
+        plain = gradient_norm(g)
+    g = [t.requires_grad_() for t in g] + [None]
+    norm = gradient_norm(g)
+    assert torch.equal(norm.detach(), plain) and norm.requires_grad
+    wide = norm.dtype == torch.float64
+    got = torch.autograd.grad(norm * 3.0, [t for t in g if t is not None])
+    exact = np.sqrt(sum((to_np(t.detach().double()) ** 2).sum() for t in g if t is not None))
+    for t, d in zip(g, got):
+        assert d.shape == t.shape and d.dtype == t.dtype
+        want = 3.0 * to_np(t.detach().double()) / exact
+        u = 2.0 ** -53 if wide else 2.0 ** -24  # norm, and its incoming gradient times 3
+        a = 2.0 ** -53 if t.dtype == torch.float64 else 2.0 ** -24  # factor and product
+        h = {8: 2.0 ** -53, 4: 2.0 ** -24}.get(t.element_size(),
+                                                2.0 ** -8 if t.dtype == torch.bfloat16 else 2.0 ** -11)
+        step = {torch.float16: 2.0 ** -24, torch.float64: 2.0 ** -1022}.get(t.dtype, 2.0 ** -126)
+        bound = np.abs(want) * (2 * u + 4 * 2.0 ** -53 + 2 * a + h) * 1.01 + step
+        assert (np.abs(to_np(d.double()) - want) <= bound).all()
+
+
+def test_the_norms_gradient_at_the_edges():
+    torch = require_gpu()
+    from purin_amd import gradient_norm
+
+    # at zero: zero, not NaN
+    z = torch.zeros(5, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(gradient_norm([z]), z)
+    assert (g == 0).all()
+    # one of a list, a strided one, a broadcast one
+    x = torch.rand((6, 8), device="cuda", dtype=torch.float64, requires_grad=True)
+    y = torch.rand(3, device="cuda", dtype=torch.float64)
+    (g,) = torch.autograd.grad(gradient_norm([y, x[:, ::2], x[:1].expand(4, 8)]), x)
+    want = x.detach() * 0
+    want[:, ::2] += x.detach()[:, ::2]
+    want[0] += 4 * x.detach()[0]
+    total = (y.square().sum() + x.detach()[:, ::2].square().sum()
+             + 4 * x.detach()[0].square().sum()).sqrt()
+    assert float((g - want / total).abs().max()) < 1e-14
+    # by differences
+    a, b = (torch.rand(s, device="cuda", dtype=torch.float64).requires_grad_() for s in (7, 4))
+    assert torch.autograd.gradcheck(lambda a, b: gradient_norm([a, b]), (a, b), eps=1e-6,
+                                    atol=1e-8, rtol=0)
+    # a factor that 32 bits do not hold
+    tiny = torch.full((4,), 2.0 ** -120, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(gradient_norm([tiny]), tiny)
+    assert (g == 0.5).all()
+    # NaN shows
+    n = torch.tensor([1.0, float("nan")], device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(gradient_norm([n]), n)
+    assert torch.isnan(g).all()
+    # a penalty on gradients reaches what they came from
+    p = torch.rand(9, device="cuda", dtype=torch.float64, requires_grad=True)
+    (d,) = torch.autograd.grad(p.pow(3).sum(), p, create_graph=True)
+    (g,) = torch.autograd.grad(gradient_norm([d]), p)
+    d = d.detach()
+    assert float((g - d / d.norm() * 6 * p.detach()).abs().max()) < 1e-13
+    # no gradients of gradients
+    (g,) = torch.autograd.grad(gradient_norm([p]), p, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), p)
+    # no graph where none is wanted
+    with torch.no_grad():
+        assert not gradient_norm([p]).requires_grad
+    assert not gradient_norm([p.detach()]).requires_grad
+
+
+def test_the_norms_gradient_of_a_long_list():
+    """More tensors than one launch takes, and a tensor of many pieces among them."""
+    torch = require_gpu()
+    from purin_amd import gradient_norm
+
+    rng = np.random.default_rng(9)
+    sizes = [int(n) for n in rng.integers(0, 40, 210)]
+    sizes[100] = 200_003
+    g = [torch.as_tensor(rng.standard_normal(n)).cuda().requires_grad_() for n in sizes]
+    norm = gradient_norm(g)
+    got = torch.autograd.grad(norm, g)
+    exact = np.sqrt(sum((to_np(t) ** 2).sum() for t in g))
+    for t, d in zip(g, got):
+        want = to_np(t) / exact
+        assert (np.abs(to_np(d) - want) <= 8 * 2.0 ** -53 * np.abs(want)).all()
