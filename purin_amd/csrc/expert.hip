@@ -319,9 +319,8 @@ static Cut16 cut_product16(int64_t rows, int64_t inner, int64_t outer, int64_t e
   if (rows <= 32 * experts || tiles <= 128) {
     const int64_t across = (outer + 63) / 64;
     const bool tall = rows > 16 * experts && most_tiles(rows, experts, 64) * across >= 256;
-    const int height = tall ? 64 : 32;
-    return {kThin16, height,
-            splits_of(256, most_tiles(rows, experts, height) * across, steps16(inner), 16)};
+    if (tall) return {kThin16, 64, 1};
+    return {kThin16, 32, splits_of(256, most_tiles(rows, experts, 32) * across, steps16(inner), 16)};
   }
   if (tiles >= 16 * 256) return {k256, 256, 1};
   return {tiles <= 256 ? kDeep16 : k128, 128, 1};
@@ -358,7 +357,7 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
   if (cut.shape == kThin16) {
     constexpr int TN = 64;
     const int64_t tm = most_tiles(rows, experts, cut.height), tn = (outer + TN - 1) / TN;
-    auto tall = [&](auto c, auto h) {
+    auto thin = [&](auto c, auto h) {
       using C = decltype(c);
       constexpr int TM = h;
       auto kernel = along ? (direct ? k_product_thin<T, C, TM, TN, true, true>
@@ -369,9 +368,8 @@ static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer,
                       thin_lds<TM, TN>(), st, a, lda, w, we, ldw, rows, inner, outer, (int)experts,
                       tn, offsets, cut.splits > 1 ? (C*)ws : (C*)out, ldo);
     };
-    auto thin = [&](auto c) { return cut.height == 32 ? tall(c, i32) : tall(c, i64); };
-    if (cut.splits == 1) return thin(T{});
-    if (int rc = thin(float{})) return rc;
+    if (cut.splits == 1) return cut.height == 32 ? thin(T{}, i32) : thin(T{}, i64);
+    if (int rc = thin(float{}, i32)) return rc;
     return join(st, (const float*)ws, cut.splits, rows * outer, out);
   }
   auto go = [&](auto bm, auto wn, auto s) {
