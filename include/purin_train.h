@@ -135,7 +135,7 @@ typedef struct {
   int32_t reserved;
 } purin_train_tensor;
 
-/* Workspace bytes of clip for a list of ``tensors`` gradients. */
+/* Workspace bytes of clip for a list of ``tensors`` gradients (negative: invalid). */
 int64_t purin_train_clip_workspace_bytes(int64_t tensors);
 
 /*

@@ -331,9 +331,14 @@ using namespace purin::train;
 extern "C" {
 
 int64_t purin_train_clip_workspace_bytes(int64_t tensors) {
-  if (tensors < 0) return -1;
-  // one sum per workgroup of the first pass: kSums, and one for each launch's rounding up
-  return (kSums + (tensors + kTable - 1) / kTable) * (int64_t)sizeof(double);
+  int64_t need = -1;
+  (void)guarded([&] {
+    if (tensors < 0) return refuse("tensors must not be negative");
+    // one sum per workgroup of the first pass: kSums, and one for each launch's rounding up
+    need = (kSums + (tensors + kTable - 1) / kTable) * (int64_t)sizeof(double);
+    return (int)PURIN_CP_OK;
+  });
+  return need;
 }
 
 int purin_train_clip(void* stream, int64_t count, const purin_train_tensor* tensors,

@@ -30,7 +30,10 @@ def _list(tensors, name):
 def clip_workspace_bytes(tensors):
     """Bytes of a caller's workspace, a contiguous device tensor at 256 bytes, for a list of
     ``tensors`` gradients."""
-    return int(_lib.load().purin_train_clip_workspace_bytes(tensors))
+    n = int(_lib.load().purin_train_clip_workspace_bytes(tensors))
+    if n < 0:
+        _lib.check(_lib.ERR_ARG)
+    return n
 
 
 def gradient_norm(gradients, *, workspace=None):
