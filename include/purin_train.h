@@ -83,14 +83,16 @@ int purin_train_dispatch(void* stream, int32_t dtype, int64_t tokens, int64_t ex
 /* out(t) = sum over slots, in their order, of weight(t, j) rows[place(t, j)];
  * a token without experts gets zero.  weights (tokens, slots) of ``wdtype``, or
  * NULL for ones (then this is dispatch's gradient).  Sums are held in 32 bits
- * (64 for F64) and rounded once. */
+ * (64 for F64 rows) and rounded once; F64 weights beside narrower rows are
+ * rounded to 32 bits first, and beyond that range are infinite. */
 int purin_train_combine(void* stream, int32_t dtype, int32_t wdtype, int64_t tokens,
                         int64_t slots, int64_t width, const void* rows, int64_t ldr,
                         const int32_t* place, const void* weights, void* out);
 
 /* combine's gradients: g_rows[place(t, j)] = weight(t, j) g_out(t), zero from
  * offsets[experts] on; g_weights(t, j) = <g_out(t), rows[place(t, j)]>, zero
- * beside -1.  Either output may be NULL. */
+ * beside -1.  Either output may be NULL.  Sums and weights as combine's: with
+ * rows narrower than F64 an F64 g_weights holds sums of 32 bits. */
 int purin_train_combine_vjp(void* stream, int32_t dtype, int32_t wdtype, int64_t tokens,
                             int64_t experts, int64_t slots, int64_t width, const void* g_out,
                             int64_t ldg, const void* rows, int64_t ldr, const int32_t* offsets,
@@ -144,9 +146,10 @@ int64_t purin_train_clip_workspace_bytes(int64_t tensors);
  * largest >= 0: out = in * largest / norm where norm > largest, out = in
  * elsewhere (written only where out is not in).  A NaN norm makes every output
  * NaN, an infinite one makes finite elements zero and infinite ones NaN.
- * largest < 0: the norm alone.  ``tensors`` is host memory, read before the
- * call returns.  Outputs that overlap each other or another's input are
- * refused.
+ * largest < 0: the norm alone.  Squares of F64 elements leave the 64-bit range
+ * beyond about 1e154 (the norm is infinite) and below 1e-162 (they count as
+ * zero).  ``tensors`` is host memory, read before the call returns.  Outputs
+ * that overlap each other or another's input are refused.
  */
 int purin_train_clip(void* stream, int64_t count, const purin_train_tensor* tensors,
                      double largest, void* workspace, int64_t workspace_bytes,

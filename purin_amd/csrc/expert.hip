@@ -4,10 +4,10 @@
 //   out(p) = a(p) W[e]                     for the rows p of expert e
 //   g_W[e] = sum over those p of a(p)^T g(p)
 //
-// Products of tiles on the matrix units; a tile belongs to one expert.  The first kernels'
-// tiles are found from the offsets on the device, so the host never waits for the counts: the
-// launch holds the most tiles that any split of the rows can need, and what is left over ends
-// at once.
+// Products of tiles on the matrix units; a tile belongs to one expert.  The tiles of out are found
+// from the offsets on the device, so the host never waits for the counts: the launch holds the
+// most tiles that any split of the rows can need, and what is left over ends at once.  The same
+// goes for the cuts below, which count rows that no expert has.
 
 #include <algorithm>
 #include <type_traits>
@@ -77,7 +77,8 @@ __device__ __forceinline__ void zero_tile(T* c, int64_t ldc, int m, int n) {
 
 // Tiles in 1-D order, XCD by XCD (workgroups are dealt to the 8 XCDs in
 // turn, so number i is on XCD i % 8): an XCD's workgroups take neighbouring tiles, kGroup rows
-// of tiles at a time, and find each other's operands in its L2.
+// of tiles at a time, and find each other's operands in its L2.  The tiles shared out are those
+// launched: where many rows have no expert, the last XCDs' share is tiles without work.
 constexpr int kGroup = 4;
 __device__ __forceinline__ void tile_order(int64_t tiles_m, int64_t tiles_n, int64_t& tm,
                                            int64_t& tn) {
@@ -493,7 +494,7 @@ static int check_product(int32_t dtype, int64_t rows, int64_t inner, int64_t out
     return set_error(PURIN_CP_ERR_UNSUPPORTED, "more than 1024 experts");
   if (rows >= (int64_t(1) << 31))
     return set_error(PURIN_CP_ERR_UNSUPPORTED, "rows must stay below 2^31");
-  // a launch's second dimension counts tiles
+  // so that 64 bits hold the sizes' products
   if (inner > (int64_t(1) << 22) || outer > (int64_t(1) << 22))
     return set_error(PURIN_CP_ERR_UNSUPPORTED, "inner and outer must not exceed 2^22");
   return PURIN_CP_OK;

@@ -1,23 +1,26 @@
 // Tiles of the experts' products in 16-bit types on the matrix units: c = sum over k of
 // a(i, k) b(j, k), sums in 32 bits, for a workgroup's BM x BN tile.
 //
-// The operands pass through LDS kDepth16 of the contraction at a time, two stages, the next one
-// loading while the present one is multiplied.  A stage of an operand whose contraction is
-// contiguous in memory is [i][k]; one whose rows are contiguous is [k][i], and is transposed by
-// the LDS reads themselves (ds_read_b64_tr_b16: 16 lanes read a 4 x 16 block and get its
-// columns).  Both are stored in 16-byte pieces whose places are exchanged by an XOR, so that the
-// lanes of one read fall on different banks:
-//   [i][k]   piece k / 8 of row i at (k / 8) ^ (i % 8): 8 rows' reads of one piece cover all banks
+// The operands pass through LDS kDepth16 of the contraction at a time, in a ring of stages (two;
+// four where tiles, or their rows, are few), the next ones loading while the present one is
+// multiplied.  A stage of an operand whose contraction is contiguous in memory is [i][k]; one
+// whose rows are contiguous is [k][i], and is transposed by the LDS reads themselves
+// (ds_read_b64_tr_b16: 16 lanes read a 4 x 16 block and get its columns).  Both are stored in
+// 16-byte pieces whose places are exchanged by an XOR, which spreads the lanes of one read over
+// the banks:
+//   [i][k]   piece k / 8 of row i at (k / 8) ^ (i % 8): 8 rows' reads of one piece fall on 8 places
 //   [k][i]   pair i / 16 of row k at (i / 16) ^ s(k), s(k) = 2 (k % 4) + (k / 8) % 2 (2 ((k / 2) % 2)
 //            in rows of 64, two of which cover the banks): the 8 blocks of 32 bytes that half a
 //            wavefront reads at once fall on 8 places
+// Counted over the large products, conflicts take 40-50 % of the LDS cycles with [i][k] stages and
+// 4 % in the weights' gradient, which has [k][i] ones alone.
 // With 16-byte rows at 16-byte addresses the stages are loaded straight into LDS (buffer loads
 // whose addresses outside the operand read zeros); others pass through registers.
 //
 // 256 x 256 tiles are bound by the matrix units and what the LDS reads and barriers leave of
 // them: 0.95 PFLOP/s, 1.05 for the weights' gradient (32768 rows, 16 experts, 2048 x 4096, bf16;
 // a library's single product of 8192 reaches 1.2), 0.58 through registers at 1613 x 3618.  The
-// tiles for few rows are bound by memory: 4.8 TB/s (768 rows, 32 experts, 4096 x 1536).
+// tiles for few rows are bound by memory: 4.6-4.8 TB/s (768 rows, 32 experts, 4096 x 1536).
 #pragma once
 
 #include "stages.hpp"

@@ -2,9 +2,10 @@
 // a(i, k) b(j, k).
 //
 // The matrix units take one value a lane of these types (16 x 16 x 4), at 64 operations a cycle
-// and SIMD (32 in 64 bits), so that their time covers the LDS reads with room to spare and one
-// stage of 128 bytes along the contraction on its way is enough.  Stages pass
-// through registers, which takes any alignment and length.  A lane reads 16 bytes along the
+// and SIMD (32 in 64 bits), so that their time covers the LDS reads with room to spare.  A stage
+// is 128 bytes along the contraction, and passes through registers, which takes any alignment and
+// length; three are on their way, each in registers of its own, but for the 128 x 128 tiles, whose
+// sums leave room for one.  A lane reads 16 bytes along the
 // contraction at once: step t of a stage multiplies the t-th value of each lane group's 16
 // bytes, an order that both operands share.
 //

@@ -39,7 +39,8 @@ def clip_workspace_bytes(tensors):
 def gradient_norm(gradients, *, workspace=None):
     """The 2-norm of all gradients together: a tensor without dimensions, float64 if any gradient
     is, float32 otherwise.  ``gradients``: a tensor, or a list whose ``None`` are left out; mixed
-    types are fine.  Squares are summed in 64 bits, in an order that the sizes alone decide.
+    types are fine.  Squares are summed in 64 bits, in an order that the sizes alone decide; those
+    of float64 elements leave that range beyond about 1e154 (an infinite norm) and below 1e-162.
     Differentiable once (a gradient's is itself over the norm, zero where the norm is), so that a
     penalty on gradients reaches what they were made from."""
     return _front.gradient_norm(_list(gradients, "gradients"), workspace)

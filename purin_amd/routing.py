@@ -115,7 +115,9 @@ def dispatch(x, routing):
 def combine(rows, routing, weights=None):
     """Each token's sum of its slots' rows times their weights: ``rows`` (tokens * slots, width)
     to (tokens, width); zeros for a token without experts.  ``weights`` (tokens, slots), of any
-    floating type: ``routing.weights`` where they are not given."""
+    floating type: ``routing.weights`` where they are not given.  Sums are held in 32 bits, in 64
+    for float64 rows: beside narrower rows float64 weights are rounded to 32 bits, and their
+    gradient holds sums of 32 bits."""
     _routing(routing)
     weights = routing.weights if weights is None else weights
     if weights is None:
