@@ -6,7 +6,9 @@
  * experts, most of them exactly zero.  These entry points take such weights to
  * the tokens' experts, the tokens' rows to the experts and back, multiply the
  * rows of each expert by its weight matrix, and scale the gradients of a step
- * to a largest norm.  No counterpart in the reference, which ends at the layer.
+ * to a largest norm; hold the experts' weights in 4 bits and a training step's
+ * rows in 8; and run a whole layer of experts for a few tokens.
+ * No counterpart in the reference, which ends at the layer.
  *
  * Conventions are purin_cp.h's: device pointers as void*, sizes as int64_t,
  * hipStream_t as void*, error codes PURIN_CP_*, purin_cp_last_error() for the
@@ -160,6 +162,108 @@ int purin_train_clip(void* stream, int64_t count, const purin_train_tensor* tens
  * list's rules are clip's. */
 int purin_train_norm_vjp(void* stream, int64_t count, const purin_train_tensor* tensors,
                          int32_t norm_dtype, const void* norm, const void* g_norm);
+
+/*
+ * Microscaled numbers: 32 neighbours of a row share a power of two 2^s, held as
+ * the byte s + 127; m is their largest magnitude.
+ *   FP4   s = max(floor(log2 m) - 2, -127); an element is the nearest of 0, .5,
+ *         1, 1.5, 2, 3, 4, 6 and their negatives to x / 2^s (ties to the even
+ *         code, at most 6), its code those numbers' index and the sign above it,
+ *         two to a byte, the earlier one in the lower half.
+ *   INT8  s = max(floor(log2 m), -127); an element is x / 2^s in 64ths, to the
+ *         nearest (ties to even), from -127 to 127, a signed byte.
+ * A neighbour that is infinite or NaN makes the scale 255 and all 32 NaN.
+ * A row's blocks = ceil(length / 32) lie one after another: codes (rows, blocks
+ * * 16) bytes (FP4) or (rows, blocks * 32) (INT8) at 16-byte addresses, scales
+ * (rows, blocks rounded up to a multiple of 4) at 4-byte addresses.  What is
+ * behind the length is zero in both, and has to be.
+ */
+enum purin_train_kind { PURIN_TRAIN_FP4 = 0, PURIN_TRAIN_INT8 = 1 };
+
+/* Packs x (groups, rows, length), element (g, r, l) at x + g * sg + r * sr + l *
+ * sl with sr or sl 1, as groups * rows rows.  F64 is not packed. */
+int purin_train_pack(void* stream, int32_t dtype, int32_t kind, int64_t groups, int64_t rows,
+                     int64_t length, const void* x, int64_t sg, int64_t sr, int64_t sl, void* codes,
+                     void* scales);
+
+/* The values that packed rows stand for, rounded to dtype (exact in the type
+ * that was packed); not F64. */
+int purin_train_unpack(void* stream, int32_t dtype, int32_t kind, int64_t rows, int64_t length,
+                       const void* codes, const void* scales, void* out, int64_t ldo);
+
+enum purin_train_activation { PURIN_TRAIN_RELU = 0, PURIN_TRAIN_SILU = 1, PURIN_TRAIN_GELU = 2 };
+
+/*
+ * out (rows, hidden) = f(u), or with ``gated`` f(first half) * second half of
+ * u's 2 * hidden columns.  f: max(u, 0) | u / (1 + exp(-u)) | u times the share
+ * of a normal distribution below u.  codes and scales, or NULL: u packed to INT8
+ * on the way, as rows of length hidden, with ``gated`` two for each of u's.
+ */
+int purin_train_activate(void* stream, int32_t dtype, int32_t activation, int32_t gated,
+                         int64_t rows, int64_t hidden, const void* u, int64_t ldu, void* out,
+                         void* codes, void* scales);
+
+/* activate's gradient g_u (rows, hidden or 2 * hidden) from g (rows, hidden), at
+ * u or, where codes and scales are given, at what they stand for (u may then be
+ * NULL).  relu has slope 0 at 0. */
+int purin_train_activate_vjp(void* stream, int32_t dtype, int32_t activation, int32_t gated,
+                             int64_t rows, int64_t hidden, const void* u, int64_t ldu,
+                             const void* codes, const void* scales, const void* g, int64_t ldg,
+                             void* g_u);
+
+/* Workspace bytes of expert_product_packed (0 where none is used). */
+int64_t purin_train_expert_product_packed_workspace_bytes(int32_t dtype, int32_t rows_packed,
+                                                          int64_t rows, int64_t inner,
+                                                          int64_t outer, int64_t experts);
+
+/*
+ * expert_product with weights in FP4: codes and scales of experts * outer rows
+ * of length inner.  a: rows (rows, inner) of dtype (BF16 or F16) with a_scales
+ * NULL, or the codes of rows in FP4 with their scales (then lda is not read, and
+ * dtype is that of out: BF16, F16 or F32).  Sums are held in 32 bits and rounded
+ * once; weights are exact in BF16, and in F16 where they are in its range
+ * (infinite above, rounded below).
+ */
+int purin_train_expert_product_packed(void* stream, int32_t dtype, int64_t rows, int64_t inner,
+                                      int64_t outer, int64_t experts, const void* a, int64_t lda,
+                                      const void* a_scales, const void* codes, const void* scales,
+                                      const int32_t* offsets, void* workspace,
+                                      int64_t workspace_bytes, void* out, int64_t ldo);
+
+/* The experts' matrices (experts, inner, outer): of dtype with scales NULL, then
+ * element (e, i, o) sits at values + e * se + i * si + o * so with si or so 1; or
+ * FP4 codes of experts * outer rows of length inner with their scales (strides
+ * are not read). */
+typedef struct {
+  const void* values;
+  const void* scales;
+  int64_t se, si, so;
+} purin_train_matrices;
+
+#define PURIN_TRAIN_LAYER_TOKENS 64
+#define PURIN_TRAIN_LAYER_PAIRS 1024
+
+/* Workspace bytes of expert_layer (negative: invalid, or more than it takes). */
+int64_t purin_train_expert_layer_workspace_bytes(int32_t dtype, int64_t tokens, int64_t experts,
+                                                 int64_t slots, int64_t width, int64_t hidden,
+                                                 int64_t outer);
+
+/*
+ * out (tokens, outer): the sum over a token's chosen experts e of
+ *   weight(t, e) * f(x(t) inner[e]) outer[e]
+ * with f and ``gated`` as in activate (inner has hidden or 2 * hidden columns)
+ * and experts chosen as route does; zeros for a token without experts.  dtype
+ * BF16 or F16.  Between the products numbers keep twice the type's digits; in F16
+ * weight * f beyond the type's range is infinite.  Sums are held in 32 bits.
+ * At most PURIN_TRAIN_LAYER_TOKENS tokens, tokens * slots at most
+ * PURIN_TRAIN_LAYER_PAIRS, ldx below 2^24.
+ */
+int purin_train_expert_layer(void* stream, int32_t dtype, int32_t wdtype, int64_t tokens,
+                             int64_t experts, int64_t slots, int64_t width, int64_t hidden,
+                             int64_t outer_width, int32_t activation, int32_t gated, const void* x,
+                             int64_t ldx, const void* weights, int64_t ldw,
+                             const purin_train_matrices* inner, const purin_train_matrices* outer,
+                             void* workspace, int64_t workspace_bytes, void* out);
 
 #ifdef __cplusplus
 }

@@ -38,6 +38,11 @@ _EXPORTS = {
     "dispatch": ("routing", "dispatch"),
     "combine": ("routing", "combine"),
     "expert_product": ("routing", "expert_product"),
+    "Microscaled": ("microscaled", "Microscaled"),
+    "pack": ("microscaled", "pack"),
+    "unpack": ("microscaled", "unpack"),
+    "activate": ("experts", "activate"),
+    "expert_layer": ("experts", "expert_layer"),
     "gradient_norm": ("gradients", "gradient_norm"),
     "clip_gradients": ("gradients", "clip_gradients"),
 }

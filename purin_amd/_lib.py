@@ -16,6 +16,9 @@ LIB_PATH = os.path.join(HERE, "libpurin_cp.so")
 
 F32, F64 = 0, 1
 BF16, F16 = 2, 3  # purin_train_dtype, which begins with F32 and F64
+FP4, INT8 = 0, 1  # purin_train_kind
+RELU, SILU, GELU = 0, 1, 2  # purin_train_activation
+LAYER_TOKENS, LAYER_PAIRS = 64, 1024  # PURIN_TRAIN_LAYER_TOKENS, PURIN_TRAIN_LAYER_PAIRS
 MAX_EXPERTS = 1024  # PURIN_TRAIN_MAX_EXPERTS
 NOALLOC_SCRATCH_BYTES = 128 << 20  # PURIN_CP_NOALLOC_SCRATCH_BYTES
 OK, ERR_ARG, ERR_HIP, ERR_UNSUPPORTED, ERR_NOMEM = 0, 1, 2, 3, 4
@@ -66,6 +69,14 @@ TRAIN_SYMBOLS = (
     "purin_train_expert_product",
     "purin_train_expert_weights_vjp_workspace_bytes",
     "purin_train_expert_weights_vjp",
+    "purin_train_pack",
+    "purin_train_unpack",
+    "purin_train_activate",
+    "purin_train_activate_vjp",
+    "purin_train_expert_product_packed_workspace_bytes",
+    "purin_train_expert_product_packed",
+    "purin_train_expert_layer_workspace_bytes",
+    "purin_train_expert_layer",
     "purin_train_clip_workspace_bytes",
     "purin_train_clip",
     "purin_train_norm_vjp",
@@ -157,6 +168,18 @@ class TrainTensor(C.Structure):
         ("count", C.c_int64),
         ("dtype", C.c_int32),
         ("reserved", C.c_int32),
+    ]
+
+
+class TrainMatrices(C.Structure):
+    """purin_train_matrices: the experts' matrices, dense or microscaled."""
+
+    _fields_ = [
+        ("values", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("se", C.c_int64),
+        ("si", C.c_int64),
+        ("so", C.c_int64),
     ]
 
 
@@ -268,6 +291,18 @@ def _declare_train(lib):
     lib.purin_train_expert_weights_vjp_workspace_bytes.argtypes = [i32, i64, i64, i64, i64]
     lib.purin_train_expert_weights_vjp.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, vp, i64,
                                                    vp, vp, i64, vp]
+    lib.purin_train_pack.argtypes = [vp, i32, i32, i64, i64, i64, vp, i64, i64, i64, vp, vp]
+    lib.purin_train_unpack.argtypes = [vp, i32, i32, i64, i64, vp, vp, vp, i64]
+    lib.purin_train_activate.argtypes = [vp, i32, i32, i32, i64, i64, vp, i64, vp, vp, vp]
+    lib.purin_train_activate_vjp.argtypes = [vp, i32, i32, i32, i64, i64, vp, i64, vp, vp, vp, i64,
+                                             vp]
+    lib.purin_train_expert_product_packed_workspace_bytes.argtypes = [i32, i32, i64, i64, i64, i64]
+    lib.purin_train_expert_product_packed.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, vp, vp,
+                                                      vp, vp, vp, i64, vp, i64]
+    lib.purin_train_expert_layer_workspace_bytes.argtypes = [i32, i64, i64, i64, i64, i64, i64]
+    lib.purin_train_expert_layer.argtypes = [vp, i32, i32, i64, i64, i64, i64, i64, i64, i32, i32,
+                                             vp, i64, vp, i64, C.POINTER(TrainMatrices),
+                                             C.POINTER(TrainMatrices), vp, i64, vp]
     lib.purin_train_clip_workspace_bytes.argtypes = [i64]
     lib.purin_train_clip.argtypes = [vp, i64, C.POINTER(TrainTensor), dbl, vp, i64, i32, vp]
     lib.purin_train_norm_vjp.argtypes = [vp, i64, C.POINTER(TrainTensor), i32, vp, vp]

@@ -28,7 +28,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(os.path.dirname(HERE), "_build")
 LIB = os.path.join(HERE, "libpurin_cp.so")
 SOURCES = ["plan.hip", "forward.hip", "adjoint.hip", "gmres.hip", "solo.hip", "route.hip",
-           "expert.hip", "clip.hip"]
+           "expert.hip", "clip.hip", "micro.hip", "packed.hip", "layer.hip"]
 RESIDENT_SOURCE = "resident_launch.hip"
 RESIDENT_VARIANTS = [(f64, slr) for f64 in (1, 0) for slr in (1, 2, 3, 4)]
 FRONT = os.path.join(HERE, "_front.so")

@@ -71,7 +71,8 @@ __device__ __forceinline__ void load_to_lds(U4 r, uint32_t at, uint32_t to) {
 
 template <int N>
 __device__ __forceinline__ int pair_swap(int k) {
-  if constexpr (N == 64) return 2 * ((k >> 1) & 1);
+  if constexpr (N == 32) return 0;  // four rows cover the banks, and those are read at once
+  else if constexpr (N == 64) return 2 * ((k >> 1) & 1);
   else return 2 * (k & 3) + ((k >> 3) & 1);
 }
 
@@ -229,6 +230,43 @@ constexpr int tile16_lds() {
   return ring > out ? ring : out;
 }
 
+// The sums of a workgroup's BM x BN tile, of which m x n are there, to c.
+template <typename T, typename C, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void tile_out(const F16x (&acc)[BM / WM / 32][BN / WN / 32],
+                                         unsigned char* lds, int m, int n, C* c, int64_t ldc) {
+  constexpr int THREADS = WM * WN * 64, X = BM / WM / 32, Y = BN / WN / 32;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
+  // b's rows run along the sums' registers: 4 neighbours of c's row to a lane.  The tile passes
+  // through LDS, so that whole rows leave in 16-byte pieces; a row's pieces are exchanged by its
+  // number, so that a wavefront's writes, one column of 32 rows, fall on different banks.
+  constexpr int V = kVec<C>, kPieces = BN / V;
+  C* out = reinterpret_cast<C*>(lds);
+#pragma unroll
+  for (int x = 0; x < X; ++x) {
+    const int i = wi + 32 * x + (lane & 31);
+#pragma unroll
+    for (int y = 0; y < Y; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int j = wj + 32 * y + 2 * r + 4 * (lane >> 5);
+        typedef C V4 __attribute__((ext_vector_type(4)));
+        V4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = (C)acc[x][y][r + q];
+        *reinterpret_cast<V4*>(out + i * BN + (((j / V) ^ (i & (kPieces - 1))) * V + j % V)) = v;
+      }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int at = threadIdx.x; at < BM * kPieces; at += THREADS) {
+    const int i = at / kPieces, j = at % kPieces * V;
+    if (i >= m || j >= n) continue;
+    store_upto(c + i * ldc + j, load16(out + i * BN + ((j / V) ^ (i & (kPieces - 1))) * V),
+               n - j);
+  }
+}
+
 // A workgroup of WM * WN wavefronts; sums are written as C.
 template <typename T, typename C, int BM, int BN, int WM, int WN, bool ALONG_A, bool ALONG_B,
           bool DIRECT, int S>
@@ -260,34 +298,7 @@ __device__ __forceinline__ void tile16(Side<T> a, Side<T> b, int64_t depth, unsi
             for (int y = 0; y < Y; ++y) acc[x][y] = mma32(T{}, fb[y], fa[x], acc[x][y]);
         }
       });
-  // b's rows run along the sums' registers: 4 neighbours of c's row to a lane.  The tile passes
-  // through LDS, so that whole rows leave in 16-byte pieces; a row's pieces are exchanged by its
-  // number, so that a wavefront's writes, one column of 32 rows, fall on different banks.
-  constexpr int V = kVec<C>, kPieces = BN / V;
-  C* out = reinterpret_cast<C*>(lds);
-#pragma unroll
-  for (int x = 0; x < X; ++x) {
-    const int i = wi + 32 * x + (lane & 31);
-#pragma unroll
-    for (int y = 0; y < Y; ++y)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int j = wj + 32 * y + 2 * r + 4 * (lane >> 5);
-        typedef C V4 __attribute__((ext_vector_type(4)));
-        V4 v;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = (C)acc[x][y][r + q];
-        *reinterpret_cast<V4*>(out + i * BN + (((j / V) ^ (i & (kPieces - 1))) * V + j % V)) = v;
-      }
-  }
-  __syncthreads();
-#pragma unroll 4
-  for (int at = threadIdx.x; at < BM * kPieces; at += THREADS) {
-    const int i = at / kPieces, j = at % kPieces * V;
-    if (i >= a.n || j >= b.n) continue;
-    store_upto(c + i * ldc + j, load16(out + i * BN + ((j / V) ^ (i & (kPieces - 1))) * V),
-               b.n - j);
-  }
+  tile_out<T, C, BM, BN, WM, WN>(acc, lds, a.n, b.n, c, ldc);
 }
 
 // Few rows: at most BM, by BN, where reading b is the work.  kThin stages, all but one of them

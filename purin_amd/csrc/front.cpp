@@ -393,30 +393,159 @@ Tensor run_weights_vjp(const Tensor& a, const Tensor& g, const Tensor& offsets, 
   return out;
 }
 
+// -- microscaled numbers --------------------------------------------------------------------
+
+int64_t micro_blocks(int64_t length) { return (length + 31) / 32; }
+int64_t micro_row_bytes(int32_t kind, int64_t length) {
+  return micro_blocks(length) * (kind == PURIN_TRAIN_FP4 ? 16 : 32);
+}
+int64_t micro_scales(int64_t length) { return (micro_blocks(length) + 3) / 4 * 4; }
+
+// Packed rows of a length: codes and scales, as they are in memory.
+struct Packed {
+  Tensor codes, scales;
+  Packed() = default;
+  Packed(std::vector<int64_t> lead, int32_t kind, int64_t length, const Tensor& like) {
+    const auto o = like.options().dtype(at::kByte).requires_grad(false);
+    lead.push_back(micro_row_bytes(kind, length));
+    codes = at::empty(lead, o);
+    lead.back() = micro_scales(length);
+    scales = at::empty(lead, o);
+  }
+};
+
+// A Microscaled's fields, which a caller may have made: ``lead`` is its shape without the axis
+// that the blocks lie along.
+Packed check_packed(const Tensor& codes, const Tensor& scales, int32_t kind,
+                    const std::vector<int64_t>& shape, int64_t axis, const char* name) {
+  const int64_t dims = (int64_t)shape.size();
+  if (dims < 1 || axis < -dims || axis >= dims)
+    refuse(name, " must be a Microscaled with an axis of its shape; got axis ", axis);
+  std::vector<int64_t> lead = shape;
+  const int64_t length = lead[axis < 0 ? axis + dims : axis];
+  lead.erase(lead.begin() + (axis < 0 ? axis + dims : axis));
+  lead.push_back(0);
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& t = i ? scales : codes;
+    const char* part = i ? "scales" : "codes";
+    lead.back() = i ? micro_scales(length) : micro_row_bytes(kind, length);
+    if (!t.is_cuda() || t.layout() != at::kStrided || t.scalar_type() != at::kByte || t.sizes() != at::IntArrayRef(lead))
+      refuse(name, ".", part, " must be a uint8 tensor ", at::IntArrayRef(lead), " on the GPU; got ",
+             t.scalar_type(), " ", t.sizes(), " on ", t.device());
+  }
+  same_device(codes, scales, name);
+  Packed p;
+  p.codes = codes.contiguous();
+  p.scales = scales.contiguous();
+  return p;
+}
+
+// Rows along the last dimension of ``t``, which has at most three.
+Packed run_pack(const Tensor& given, int32_t kind) {
+  Tensor t = numbers(given);
+  const std::vector<int64_t> lead(t.sizes().begin(), t.sizes().end() - 1);
+  while (t.dim() < 3) t = t.unsqueeze(0);
+  if (t.stride(2) != 1 && t.size(2) > 1 && t.stride(1) != 1 && t.size(1) > 1) t = t.contiguous();
+  int64_t groups = t.size(0), rows = t.size(1), sg = t.stride(0), sr = t.stride(1);
+  const int64_t length = t.size(2), sl = length > 1 ? t.stride(2) : 1;
+  if (rows == 1 && sl == 1) std::swap(groups, rows), std::swap(sg, sr);
+  if (rows > 1 && sg == rows * sr) {
+    rows *= groups;
+    groups = 1;
+  }
+  const Call call(t);
+  Packed p(lead, kind, length, t);
+  check(purin_train_pack(call.stream, code_of(t, "tensor"), kind, groups, rows, length, t.data_ptr(),
+                         sg, sr, sl, p.codes.data_ptr(), p.scales.data_ptr()));
+  return p;
+}
+
+// The values of packed rows, (lead..., length) contiguous.
+Tensor run_unpack(const Packed& p, int32_t kind, int64_t length, at::ScalarType dtype) {
+  const Call call(p.codes);
+  std::vector<int64_t> sizes(p.codes.sizes().begin(), p.codes.sizes().end());
+  int64_t rows = 1;
+  for (size_t i = 0; i + 1 < sizes.size(); ++i) rows *= sizes[i];
+  sizes.back() = length;
+  Tensor out = at::empty(sizes, p.codes.options().dtype(dtype));
+  check(purin_train_unpack(call.stream, code_of(out, "dtype"), kind, rows, length,
+                           p.codes.data_ptr(), p.scales.data_ptr(), out.data_ptr(), length));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> pack(const Tensor& t, int32_t kind, int64_t axis) {
+  if (code_of(t, "tensor") == PURIN_TRAIN_F64)
+    refuse("tensor must be float32, bfloat16 or float16 to be packed; got float64");
+  if (t.layout() != at::kStrided) refuse("tensor must be dense");
+  if (t.dim() < 1 || axis < -t.dim() || axis >= t.dim())
+    refuse("axis must be one of the tensor's ", t.dim(), " dimensions; got ", axis);
+  without_tangent(t);
+  if (wants_grad(t))
+    throw LibraryError(PURIN_CP_ERR_UNSUPPORTED, "pack has no gradient: give it a detached tensor");
+  const Tensor moved = t.movedim(axis, -1);
+  if (moved.dim() <= 3) {
+    const Packed p = run_pack(moved, kind);
+    return {p.codes, p.scales};
+  }
+  std::vector<int64_t> lead(moved.sizes().begin(), moved.sizes().end() - 1);
+  const Packed p = run_pack(moved.flatten(0, -3), kind);
+  lead.push_back(p.codes.size(-1));
+  const Tensor codes = p.codes.view(lead);
+  lead.back() = p.scales.size(-1);
+  return {codes, p.scales.view(lead)};
+}
+
+Tensor unpack(const Tensor& codes, const Tensor& scales, int32_t kind,
+              const std::vector<int64_t>& shape, int64_t axis, at::ScalarType dtype) {
+  const Packed p = check_packed(codes, scales, kind, shape, axis, "packed");
+  if (dtype != at::kFloat && dtype != at::kBFloat16 && dtype != at::kHalf)
+    refuse("dtype must be float32, bfloat16 or float16; got ", dtype);
+  const int64_t length = shape[axis < 0 ? axis + (int64_t)shape.size() : axis];
+  return run_unpack(p, kind, length, dtype).movedim(-1, axis);
+}
+
+// -- the products' graph --------------------------------------------------------------------
+
 struct ProductFn : torch::autograd::Function<ProductFn> {
+  // ``saved``: what the weights' gradient reads of rows is kept in 8 bits
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weight,
-                        const Tensor& offsets) {
-    ctx->save_for_backward({rows, weight, offsets});
+                        const Tensor& offsets, bool saved) {
+    Packed kept;
+    if (saved && weight.requires_grad()) kept = run_pack(rows.detach(), PURIN_TRAIN_INT8);
+    ctx->saved_data["saved"] = saved;
+    ctx->save_for_backward({saved ? Tensor() : rows, weight, offsets, kept.codes, kept.scales});
     return run_product(rows, weight_strides(weight), offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     for (const Tensor& t : {saved[0], saved[1], grads[0]}) without_tangent(t);
-    const Tensor a = matrix(saved[0]), w = weight_strides(saved[1]), g = matrix(grads[0]);
+    const Tensor w = weight_strides(saved[1]), g = matrix(grads[0]);
     const Tensor& offsets = saved[2];
     Tensor g_rows, g_weight;
     if (ctx->needs_input_grad(0)) g_rows = run_product(g, w.transpose(1, 2), offsets);
     if (ctx->needs_input_grad(1)) {
+      Packed kept;
+      kept.codes = saved[3];
+      kept.scales = saved[4];
+      const Tensor a = ctx->saved_data["saved"].toBool()
+                           ? run_unpack(kept, PURIN_TRAIN_INT8, w.size(1), w.scalar_type())
+                           : matrix(saved[0]);
       if (w.stride(2) == 1 || w.size(2) <= 1)
         g_weight = run_weights_vjp(a, g, offsets, w.size(0));
       else  // the weight's own order: (a^T g)^T = g^T a
         g_weight = run_weights_vjp(g, a, offsets, w.size(0)).transpose(1, 2);
     }
-    return once({g_rows, g_weight, Tensor()});
+    return once({g_rows, g_weight, Tensor(), Tensor()});
   }
 };
 
-Tensor expert_product(const Tensor& rows, const Tensor& weight, const Tensor& offsets) {
+void check_offsets(const Tensor& rows, const Tensor& offsets, int64_t experts) {
+  if (offsets.scalar_type() != at::kInt || offsets.dim() != 1 || offsets.size(0) != experts + 1)
+    refuse("offsets must be a Routing or an int32 tensor of ", experts + 1, " entries");
+  same_device(rows, offsets, "offsets");
+}
+
+Tensor expert_product(const Tensor& rows, const Tensor& weight, const Tensor& offsets, bool saved) {
   code_of(rows, "rows");
   code_of(weight, "weight");
   if (rows.scalar_type() != weight.scalar_type())
@@ -425,16 +554,248 @@ Tensor expert_product(const Tensor& rows, const Tensor& weight, const Tensor& of
   if (rows.dim() != 2 || weight.dim() != 3 || rows.size(1) != weight.size(1))
     refuse("rows must have shape (rows, inner) and weight (experts, inner, outer); got ",
            rows.sizes(), " and ", weight.sizes());
-  if (offsets.scalar_type() != at::kInt || offsets.dim() != 1 ||
-      offsets.size(0) != weight.size(0) + 1)
-    refuse("offsets must be a Routing or an int32 tensor of ", weight.size(0) + 1, " entries");
   same_device(rows, weight, "weight");
-  same_device(rows, offsets, "offsets");
+  check_offsets(rows, offsets, weight.size(0));
+  if (saved && rows.scalar_type() == at::kDouble) refuse("rows of float64 are not kept in 8 bits");
   without_tangent(rows);
   without_tangent(weight);
   const Tensor at = offsets.contiguous();
-  return wants_grad(rows) || wants_grad(weight) ? ProductFn::apply(rows, weight, at)
+  return wants_grad(rows) || wants_grad(weight) ? ProductFn::apply(rows, weight, at, saved)
                                                 : run_product(rows, weight_strides(weight), at);
+}
+
+// Weights of (experts, inner, outer) in FP4, blocks along inner.
+struct PackedWeight {
+  Packed p;
+  int64_t experts, inner, outer;
+  PackedWeight(const Tensor& codes, const Tensor& scales, int32_t kind,
+               const std::vector<int64_t>& shape, int64_t axis, const char* name) {
+    if (kind != PURIN_TRAIN_FP4 || shape.size() != 3 || (axis != 1 && axis != -2))
+      refuse(name, " must be packed as \"fp4\", of shape (experts, inner, outer) along axis 1; got ",
+             at::IntArrayRef(shape), " along axis ", axis);
+    p = check_packed(codes, scales, kind, shape, axis, name);
+    experts = shape[0];
+    inner = shape[1];
+    outer = shape[2];
+    if (experts < 1) refuse(name, " must have an expert");
+  }
+};
+
+Tensor run_product_packed(const Tensor& rows, const Packed* packed_rows, int32_t code,
+                          const Packed& w, const Tensor& offsets, int64_t inner, int64_t outer,
+                          const at::TensorOptions& options) {
+  const Call call(rows);
+  const int64_t p = rows.size(0), experts = w.codes.size(0);
+  // the library knows packed rows by their scales, which empty ones lack
+  if (packed_rows && (!p || !inner || !outer)) return at::zeros({p, outer}, options);
+  const Workspace ws(std::nullopt,
+                     purin_train_expert_product_packed_workspace_bytes(
+                         code, packed_rows != nullptr, p, inner, outer, experts),
+                     rows);
+  Tensor out = at::empty({p, outer}, options);
+  check(purin_train_expert_product_packed(
+      call.stream, code, p, inner, outer, experts, rows.data_ptr(), packed_rows ? 0 : rows.stride(0),
+      packed_rows ? packed_rows->scales.data_ptr() : nullptr, w.codes.data_ptr(),
+      w.scales.data_ptr(), ints(offsets), ws.at, ws.size, out.data_ptr(), outer));
+  return out;
+}
+
+struct PackedProductFn : torch::autograd::Function<PackedProductFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& codes,
+                        const Tensor& scales, const Tensor& offsets, int64_t outer) {
+    ctx->save_for_backward({codes, scales, offsets});
+    ctx->saved_data["inner"] = rows.size(1);
+    Packed w;
+    w.codes = codes;
+    w.scales = scales;
+    const Tensor a = matrix(rows);
+    return run_product_packed(a, nullptr, code_of(a, "rows"), w, offsets, a.size(1), outer,
+                              a.options().requires_grad(false));
+  }
+  // the weights unpacked, (experts, outer, inner): the contraction runs across their blocks
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    without_tangent(grads[0]);
+    Packed w;
+    w.codes = saved[0];
+    w.scales = saved[1];
+    const Tensor g = matrix(grads[0]);
+    const Tensor full = run_unpack(w, PURIN_TRAIN_FP4, ctx->saved_data["inner"].toInt(), g.scalar_type());
+    return once({run_product(g, full, saved[2]), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor expert_product_packed(const Tensor& rows, const Tensor& codes, const Tensor& scales,
+                             int32_t kind, const std::vector<int64_t>& shape, int64_t axis,
+                             const Tensor& offsets) {
+  const PackedWeight w(codes, scales, kind, shape, axis, "weight");
+  const int32_t code = code_of(rows, "rows");
+  if (rows.dim() != 2 || rows.size(1) != w.inner)
+    refuse("rows must have shape (rows, ", w.inner, "); got ", rows.sizes());
+  if (code == PURIN_TRAIN_F64) refuse("rows must be float32, bfloat16 or float16 beside packed weights");
+  same_device(rows, w.p.codes, "weight");
+  check_offsets(rows, offsets, w.experts);
+  without_tangent(rows);
+  const Tensor at = offsets.contiguous();
+  if (code == PURIN_TRAIN_F32)  // the weights as numbers of 32 bits
+    return expert_product(rows, run_unpack(w.p, kind, w.inner, at::kFloat).transpose(1, 2), at, false);
+  if (wants_grad(rows)) return PackedProductFn::apply(rows, w.p.codes, w.p.scales, at, w.outer);
+  const Tensor a = matrix(rows);
+  return run_product_packed(a, nullptr, code, w.p, at, w.inner, w.outer,
+                            a.options().requires_grad(false));
+}
+
+Tensor expert_product_both(const Tensor& rows_codes, const Tensor& rows_scales, int32_t rows_kind,
+                           const std::vector<int64_t>& rows_shape, int64_t rows_axis,
+                           at::ScalarType dtype, const Tensor& codes, const Tensor& scales,
+                           int32_t kind, const std::vector<int64_t>& shape, int64_t axis,
+                           const Tensor& offsets) {
+  const PackedWeight w(codes, scales, kind, shape, axis, "weight");
+  if (rows_kind != PURIN_TRAIN_FP4 || rows_shape.size() != 2 || (rows_axis != 1 && rows_axis != -1) ||
+      rows_shape[1] != w.inner)
+    refuse("packed rows must be \"fp4\", of shape (rows, ", w.inner, ") along axis 1; got ",
+           at::IntArrayRef(rows_shape), " along axis ", rows_axis);
+  const Packed a = check_packed(rows_codes, rows_scales, rows_kind, rows_shape, rows_axis, "rows");
+  same_device(a.codes, w.p.codes, "weight");
+  check_offsets(a.codes, offsets, w.experts);
+  const int32_t code = dtype == at::kFloat      ? PURIN_TRAIN_F32
+                       : dtype == at::kBFloat16 ? PURIN_TRAIN_BF16
+                       : dtype == at::kHalf     ? PURIN_TRAIN_F16
+                                                : -1;
+  if (code < 0) refuse("packed rows must be of float32, bfloat16 or float16; got ", dtype);
+  return run_product_packed(a.codes, &a, code, w.p, offsets.contiguous(), w.inner, w.outer,
+                            a.codes.options().dtype(dtype));
+}
+
+// -- the activation -------------------------------------------------------------------------
+
+Tensor run_activate(const Tensor& given, int32_t act, bool gated, Packed* kept) {
+  const Tensor u = matrix(given);
+  const int64_t rows = u.size(0), hidden = gated ? u.size(1) / 2 : u.size(1);
+  const Call call(u);
+  Tensor out = at::empty({rows, hidden}, u.options().requires_grad(false));
+  if (kept) *kept = Packed({rows, gated ? 2 : 1}, PURIN_TRAIN_INT8, hidden, u);
+  check(purin_train_activate(call.stream, code_of(u, "rows"), act, gated, rows, hidden, u.data_ptr(),
+                             u.stride(0), out.data_ptr(), kept ? kept->codes.data_ptr() : nullptr,
+                             kept ? kept->scales.data_ptr() : nullptr));
+  return out;
+}
+
+struct ActivateFn : torch::autograd::Function<ActivateFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& u, int64_t act, bool gated, bool saved) {
+    Packed kept;
+    Tensor out = run_activate(u, (int32_t)act, gated, saved ? &kept : nullptr);
+    ctx->save_for_backward({saved ? Tensor() : u, kept.codes, kept.scales});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["gated"] = gated;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    for (const Tensor& t : {saved[0], grads[0]}) without_tangent(t);
+    const bool gated = ctx->saved_data["gated"].toBool(), packed = saved[1].defined();
+    const Tensor g = matrix(grads[0]);
+    const Tensor u = packed ? Tensor() : matrix(saved[0]);
+    const Call call(g);
+    const int64_t rows = g.size(0), hidden = g.size(1);
+    Tensor out = at::empty({rows, gated ? 2 * hidden : hidden}, g.options().requires_grad(false));
+    check(purin_train_activate_vjp(
+        call.stream, code_of(g, "gradient"), (int32_t)ctx->saved_data["act"].toInt(), gated, rows,
+        hidden, packed ? nullptr : u.data_ptr(), packed ? 0 : u.stride(0),
+        packed ? saved[1].data_ptr() : nullptr, packed ? saved[2].data_ptr() : nullptr, g.data_ptr(),
+        g.stride(0), out.data_ptr()));
+    return once({out, Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor activate(const Tensor& rows, int64_t act, bool gated, bool saved) {
+  const int32_t code = code_of(rows, "rows");
+  if (rows.dim() != 2 || (gated && rows.size(1) % 2))
+    refuse("rows must have two dimensions, with a gate an even number of columns; got ", rows.sizes());
+  if (saved && code == PURIN_TRAIN_F64) refuse("rows of float64 are not kept in 8 bits");
+  without_tangent(rows);
+  return wants_grad(rows) ? ActivateFn::apply(rows, act, gated, saved)
+                          : run_activate(rows, (int32_t)act, gated, nullptr);
+}
+
+// -- a whole layer --------------------------------------------------------------------------
+
+// A weight as the library reads it; ``held`` keeps what it points to.
+using MicroFields = std::tuple<Tensor, Tensor, int32_t, std::vector<int64_t>, int64_t>;
+struct LayerWeight {
+  purin_train_matrices m{};
+  Tensor held;
+  Packed packed;
+  int64_t experts, inner, outer;
+  LayerWeight(const std::optional<Tensor>& dense, const std::optional<MicroFields>& fields,
+              const Tensor& x, const char* name) {
+    if (dense) {
+      code_of(*dense, name);
+      if (dense->dim() != 3 || dense->size(0) < 1 || dense->scalar_type() != x.scalar_type())
+        refuse(name, " must have shape (experts, inner, outer) and type ", x.scalar_type(), "; got ",
+               dense->sizes(), " and ", dense->scalar_type());
+      same_device(x, *dense, name);
+      without_tangent(*dense);
+      held = weight_strides(*dense);
+      experts = held.size(0), inner = held.size(1), outer = held.size(2);
+      m = {held.data_ptr(), nullptr, held.stride(0), held.stride(1), held.stride(2)};
+    } else {
+      const auto& [codes, scales, kind, shape, axis] = *fields;
+      const PackedWeight w(codes, scales, kind, shape, axis, name);
+      same_device(x, w.p.codes, name);
+      packed = w.p;
+      experts = w.experts, inner = w.inner, outer = w.outer;
+      m = {packed.codes.data_ptr(), packed.scales.data_ptr(), 0, 0, 0};
+    }
+  }
+};
+
+// None where the kernels do not take the call (types, sizes, a gradient wanted), after its checks.
+std::optional<Tensor> expert_layer(const Tensor& x, const Tensor& weights, int64_t slots,
+                                   const std::optional<Tensor>& inner,
+                                   const std::optional<MicroFields>& inner_packed,
+                                   const std::optional<Tensor>& outer,
+                                   const std::optional<MicroFields>& outer_packed, int32_t act,
+                                   const std::optional<Tensor>& workspace) {
+  const int32_t code = code_of(x, "x"), wcode = code_of(weights, "weights");
+  if (x.dim() != 2 || weights.dim() != 2 || weights.size(0) != x.size(0))
+    refuse("x must have shape (tokens, width) and weights (tokens, experts); got ", x.sizes(), " and ",
+           weights.sizes());
+  same_device(x, weights, "weights");
+  if (code == PURIN_TRAIN_F64 && (inner_packed || outer_packed))
+    refuse("x must be float32, bfloat16 or float16 beside packed weights");
+  const LayerWeight a(inner, inner_packed, x, "inner"), b(outer, outer_packed, x, "outer");
+  const int64_t tokens = x.size(0), experts = weights.size(1), hidden = b.inner;
+  if (a.experts != experts || b.experts != experts)
+    refuse("inner and outer must have the weights' ", experts, " experts; got ", a.experts, " and ",
+           b.experts);
+  if (a.inner != x.size(1)) refuse("inner must have ", x.size(1), " rows to an expert; got ", a.inner);
+  if (a.outer != hidden && a.outer != 2 * hidden)
+    refuse("inner must have ", hidden, " or, with a gate, ", 2 * hidden, " columns; got ", a.outer);
+  if (slots < 1 || slots > experts)
+    refuse("slots must be from 1 to the ", experts, " experts; got ", slots);
+  without_tangent(x);
+  without_tangent(weights);
+  const bool graph = wants_grad(x) || wants_grad(weights) || (inner && wants_grad(*inner)) ||
+                     (outer && wants_grad(*outer));
+  if (graph || (code != PURIN_TRAIN_BF16 && code != PURIN_TRAIN_F16) ||
+      tokens > PURIN_TRAIN_LAYER_TOKENS || tokens * slots > PURIN_TRAIN_LAYER_PAIRS)
+    return std::nullopt;
+  const at::NoGradGuard no_grad;
+  Tensor rows = matrix(x);
+  if (rows.size(0) > 1 && rows.stride(0) >= (1 << 24)) rows = rows.contiguous();
+  const Tensor w = matrix(weights);
+  const Call call(rows);
+  const Workspace ws(workspace,
+                     purin_train_expert_layer_workspace_bytes(code, tokens, experts, slots,
+                                                              a.inner, hidden, b.outer),
+                     rows);
+  Tensor out = at::empty({tokens, b.outer}, rows.options());
+  check(purin_train_expert_layer(call.stream, code, wcode, tokens, experts, slots, a.inner, hidden,
+                                 b.outer, act, a.outer != hidden, rows.data_ptr(), rows.stride(0),
+                                 w.data_ptr(), w.stride(0), &a.m, &b.m, ws.at, ws.size,
+                                 out.data_ptr()));
+  return out;
 }
 
 // -- the global norm ------------------------------------------------------------------------
@@ -718,6 +1079,12 @@ PYBIND11_MODULE(_front, m) {
   m.def("dispatch", &dispatch);
   m.def("combine", &combine);
   m.def("expert_product", &expert_product);
+  m.def("pack", &pack);
+  m.def("unpack", &unpack);
+  m.def("expert_product_packed", &expert_product_packed);
+  m.def("expert_product_both", &expert_product_both);
+  m.def("activate", &activate);
+  m.def("expert_layer", &expert_layer);
   m.def("gradient_norm", &gradient_norm);
   m.def("clip_gradients", &clip_gradients);
 }

@@ -28,6 +28,7 @@ from purin_amd import _lib
 
 _lib.load()
 from purin_amd import _front  # noqa: E402  (linked to the library, which is built with it)
+from purin_amd.microscaled import Microscaled, fields, kept  # noqa: E402
 
 
 @dataclass(eq=False)
@@ -129,19 +130,37 @@ def combine(rows, routing, weights=None):
                          f"{type(rows).__name__} and {type(weights).__name__}") from None
 
 
-def expert_product(rows, weight, offsets):
+def expert_product(rows, weight, offsets, *, saved=None):
     """Every expert's rows times its matrix: ``rows`` (rows, inner) sorted by expert, ``weight``
     (experts, inner, outer) in either order of its last two dimensions in memory, to
     (rows, outer), zeros behind the last expert's rows.
 
     ``offsets``: a ``Routing``, or (experts + 1) int32 on the GPU: each expert's first row and
     the rows' number last, ascending from 0 and at most ``rows``.
+
+    ``weight`` may be packed (``pack(weight, "fp4", axis=1)``), ``rows`` then float32, bfloat16 or
+    float16, or packed too (``pack(rows, "fp4")``), which gives results of the type that they were
+    packed from.  Sums are held in 32 bits.  Packed operands have no gradient; the rows' beside
+    packed weights, and products of float32 rows with them, unpack the weights to the rows' type
+    for the length of the call.
+
+    ``saved="int8"``: what a graph keeps of the rows for the weights' gradient is held in 8 bits
+    (as ``pack(rows, "int8")``), and that gradient is at the rows which those stand for.  Not for
+    float64.
     """
     if isinstance(offsets, Routing):
         offsets = offsets.offsets
+    keep = kept(saved)
     try:
-        return _front.expert_product(rows, weight, offsets)
+        if isinstance(weight, Microscaled):
+            if keep:
+                raise ValueError("packed weights have no gradient that rows are kept for")
+            if isinstance(rows, Microscaled):
+                return _front.expert_product_both(*fields(rows), rows.dtype, *fields(weight),
+                                                  offsets)
+            return _front.expert_product_packed(rows, *fields(weight), offsets)
+        return _front.expert_product(rows, weight, offsets, keep)
     except TypeError:
-        raise ValueError("rows, weight and offsets must be tensors on the GPU; got "
-                         f"{type(rows).__name__}, {type(weight).__name__} and "
+        raise ValueError("rows, weight and offsets must be tensors on the GPU (packed rows go with "
+                         f"packed weights); got {type(rows).__name__}, {type(weight).__name__} and "
                          f"{type(offsets).__name__}") from None
