@@ -182,11 +182,6 @@ static Cut16 cut_weights16(int64_t rows, int64_t inner, int64_t outer, int64_t e
   return {tiles * splits <= 256 ? kDeep16 : k128, 128, splits};
 }
 
-// Whether a weight is read along inner (a length of one has any stride); along outer otherwise.
-static bool along_inner(int64_t inner, int64_t wi, int64_t wo) {
-  return wo != 1 && (wi == 1 || inner <= 1);
-}
-
 template <typename T>
 static int product16(hipStream_t st, int64_t rows, int64_t inner, int64_t outer, int64_t experts,
                      const T* a, int64_t lda, const T* w, int64_t we, int64_t wi, int64_t wo,

@@ -3,14 +3,14 @@
 //   out(t) = sum over t's experts e of  w(t, e) f(x(t) A[e]) B[e]
 //
 // Every weight of an expert that some token has is read once: that is the work, and the tokens'
-// rows are few beside it.  So nothing is sorted: a workgroup has one expert and 64 columns of its
-// matrix, finds the tokens that have the expert and takes their rows as those of its tile.  Two
-// launches and their sum:
-//   up     chooses the tokens' experts (every workgroup for itself), multiplies by A, applies f
-//          and the token's weight.  The results keep twice the type's digits, as the sum of two
-//          numbers of the type, so that they take part in the second product as they are;
-//   down   multiplies them by B, a row of 32-bit sums for each (token, slot);
-//   sum    adds a token's rows in the order of its slots.
+// rows are few beside it.  Four launches:
+//   choose  one workgroup chooses the tokens' experts and sorts the pairs (token, slot) by expert;
+//           the others lay out x as the products read it, where it is not so already;
+//   up      a workgroup has one expert and 64 columns of A: multiplies its tokens' rows, applies f
+//           and the token's weight.  The results keep twice the type's digits, as the sum of two
+//           numbers of the type, so that they take part in the second product as they are;
+//   down    one expert and 64 columns of B: a row of 32-bit sums for each pair;
+//   sum     adds a token's rows in the order of its slots.
 
 #include <algorithm>
 
@@ -31,40 +31,51 @@ struct Matrices {
   int64_t se, ld;
 };
 
-// The two times 32 columns of a workgroup's tile: starts and how many are there.
-struct Columns {
-  int64_t first[2];
-  int n[2];
-};
-
 // ---------------------------------------------------------------------------
 // sums of BM rows and 2 x 32 columns
 // ---------------------------------------------------------------------------
 
-// Microscaled weights.
+// The products' cores.  run(): rows a (piece k of row(i)), ``inner`` long, times expert e's matrix
+// of ``outer`` columns, of which c are the wavefront's, to sums in LDS (part of its contraction).
+// kRing: the LDS that it needs on the way.
 template <typename T, int BM, int NA>
 struct ThinCodes {
-  using Core = ThinPacked<T, BM, NA, BM * NA <= 64 ? 3 : 2>;  // as many as LDS holds
-  static constexpr int kRing = Core::kRing;
-
+  static constexpr int kRing = kLineLds;
+  static constexpr bool kStreams = true;
   template <typename F>
-  static __device__ __forceinline__ void run(const T* const (&a)[NA], F&& offset, int64_t inner,
+  static __device__ __forceinline__ void run(const Rows (&a)[NA], F&& row, int64_t inner,
                                              const Matrices& w, int e, int64_t outer,
-                                             const Columns& c, unsigned char* lds,
-                                             F16x (&acc)[BM / 32][2]) {
+                                             const Columns& c, int part, int parts,
+                                             unsigned char* lds) {
     const Codes b((const uint8_t*)w.values, w.scales, e * outer, inner);
-    Core::run(a, offset, inner, b,
-              [&](int j) {
-                const bool second = j >= 32;
-                const int in = j & 31;
-                return in < (second ? c.n[1] : c.n[0]) ? (int)(second ? c.first[1] : c.first[0]) + in
-                                                       : -1;
-              },
-              0, b.blocks, lds, acc);
+    ThinAcc<BM> acc;
+    int from, to;
+    share_lines(0, c.n[0] > 0 ? b.lines() : 0, part, parts, from, to);
+    StreamCodes<T, BM, NA>::run(a, row, inner, b, c, from, to, lds, acc);
+    __syncthreads();
+    thin_parts<BM>(acc, reinterpret_cast<float*>(lds));
   }
 };
 
-// Dense weights.
+template <typename T, int BM, int NA>
+struct ThinAlong {
+  static constexpr int kRing = kLineLds;
+  static constexpr bool kStreams = true;
+  template <typename F>
+  static __device__ __forceinline__ void run(const Rows (&a)[NA], F&& row, int64_t inner,
+                                             const Matrices& w, int e, int64_t, const Columns& c,
+                                             int part, int parts, unsigned char* lds) {
+    ThinAcc<BM> acc;
+    int from, to;
+    share_lines(0, c.n[0] > 0 ? (int)((inner + 63) / 64) : 0, part, parts, from, to);
+    StreamDense<T, BM, NA>::run(a, row, inner, (const T*)w.values + e * w.se, w.ld, c, from, to, lds, acc);
+    __syncthreads();
+    thin_parts<BM>(acc, reinterpret_cast<float*>(lds));
+  }
+};
+
+// Dense weights through LDS: a contraction that runs across memory (transposed by the reads), or
+// pieces at any address.  Rows are in one piece each (step 16).
 template <typename T, int BM, int NA, bool ALONG, bool DIRECT>
 struct ThinDense {
   static constexpr int X = BM / 32, S = 4, AHEAD = 3;
@@ -73,6 +84,7 @@ struct ThinDense {
   static constexpr int kStage = NA * SA::kBytes + 2 * SB::kElems * 2;
   static constexpr int kLoads = NA * SA::kMine + 2 * SB::kMine;
   static constexpr int kRing = (DIRECT ? S : 2) * kStage;
+  static constexpr bool kStreams = false;  // the wavefronts share a tile's columns, always in four
 
   static __device__ __forceinline__ void multiply(const uint8_t* la, F16x (&acc)[X][2]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -92,9 +104,23 @@ struct ThinDense {
   }
 
   template <typename F>
-  static __device__ __forceinline__ void run(const T* const (&a)[NA], F&& offset, int64_t inner,
+  static __device__ __forceinline__ void run(const Rows (&rows)[NA], F&& row, int64_t inner,
                                              const Matrices& w, int e, int64_t, const Columns& c,
-                                             unsigned char* lds, F16x (&acc)[X][2]) {
+                                             int, int, unsigned char* lds) {
+    F16x acc[X][2];
+#pragma unroll
+    for (int x = 0; x < X; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+    const T* a[NA];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) a[i] = (const T*)rows[i].p;
+    auto offset = [&](int i) {
+      const int r = row(i);
+      return r < 0 ? kOutside : (uint32_t)r * rows[0].pitch;
+    };
     const T* base = (const T*)w.values + e * w.se;
     Side<T> b[2];
 #pragma unroll
@@ -218,6 +244,18 @@ struct ThinDense {
       }
       __syncthreads();
     }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int x = 0; x < X; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          *reinterpret_cast<F4*>(sums + (wave * BM + 32 * x + (lane & 31)) * kThinPitch + 32 * y + 2 * r +
+                                 4 * (lane >> 5)) =
+              F4{acc[x][y][r], acc[x][y][r + 1], acc[x][y][r + 2], acc[x][y][r + 3]};
+    __syncthreads();
   }
 };
 
@@ -225,206 +263,228 @@ struct ThinDense {
 // who has which expert
 // ---------------------------------------------------------------------------
 
+template <typename K>
 struct AnyRow {
   const void* p;
   int32_t dtype;
   int64_t first;
-  __device__ __forceinline__ double operator[](int e) const {
-    return load_weight<double>(p, dtype, first + e);
-  }
+  __device__ __forceinline__ K operator[](int e) const { return load_weight<K>(p, dtype, first + e); }
 };
 
-template <int G, int V>
+template <typename K, int G, int V>
 __device__ __forceinline__ void choose_tokens(const void* weights, int32_t wdtype, int64_t ldw,
                                               int tokens, int experts, int slots, int32_t* ids,
-                                              double* chosen) {
-  for (int t = threadIdx.x / G; t < tokens; t += 256 / G)
-    choose<double, G, V>(AnyRow{weights, wdtype, t * ldw}, experts, slots, (int)threadIdx.x % G,
-                         ids + t * slots, chosen + t * slots);
+                                              K* chosen) {
+  for (int t = threadIdx.x / G; t < tokens; t += 1024 / G)
+    choose<K, G, V>(AnyRow<K>{weights, wdtype, t * ldw}, experts, slots, (int)threadIdx.x % G,
+                    ids + t * slots, chosen + t * slots);
 }
 
-// The expert that is number ``group`` among those with a token, -1 past the last, and its
-// tokens' pairs (token * slots + slot), in order.  Every wavefront finds the expert by itself.
-struct Group {
-  uint32_t used[PURIN_TRAIN_MAX_EXPERTS / 32];
-  int32_t pair_of[kTokens];
-  int32_t list[kTokens];
-  int32_t count;
+// The pairs (token * slots + slot) sorted by expert.  Group number g of ``groups`` has expert[g]
+// and the places start[g] to start[g + 1]; order, its pairs, in order; place, a pair's place or
+// -1; weight, by place.
+struct Plan {
+  int32_t groups;
+  int32_t expert[kPairs], start[kPairs + 1], order[kPairs], place[kPairs];
+  float weight[kPairs];
 };
-__device__ __forceinline__ int find_group(const int32_t* ids, int pairs, int slots, int group,
-                                          Group& g) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  if (tid < PURIN_TRAIN_MAX_EXPERTS / 32) g.used[tid] = 0;
-  if (tid < kTokens) g.pair_of[tid] = -1;
+
+// Made by one workgroup of 1024 threads from the choice in LDS.
+template <typename K>
+__device__ __forceinline__ void make_plan(const int32_t* ids, const K* chosen, int pairs, Plan* plan) {
+  __shared__ int32_t first[PURIN_TRAIN_MAX_EXPERTS];  // a place for each expert, then its group's
+  __shared__ int32_t wave_rows[16], wave_used[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  first[tid] = 0;
   __syncthreads();
-  for (int p = tid; p < pairs; p += 256) {
-    const int32_t e = ids[p];
-    if (e >= 0) atomicOr(&g.used[e >> 5], 1u << (e & 31));
-  }
+  if (tid < pairs && ids[tid] >= 0) atomicAdd(&first[ids[tid]], 1);
   __syncthreads();
-  uint32_t word = lane < PURIN_TRAIN_MAX_EXPERTS / 32 ? g.used[lane] : 0;
-  const int n = __popc(word);
-  int sum = n;
+  const int count = first[tid];
+  int rows = count, used = count > 0;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int up = __shfl_up(sum, d, 64);
-    if (lane >= d) sum += up;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int r = __shfl_up(rows, d, 64), u = __shfl_up(used, d, 64);
+    if (lane >= d) rows += r, used += u;
   }
-  const uint64_t here = __ballot(lane < 32 && group < sum);
-  if (!here) return -1;
-  const int at = __ffsll((unsigned long long)here) - 1;
-  word = (uint32_t)__shfl((int)word, at, 64);
-  for (int skip = group - (__shfl(sum, at, 64) - __popc(word)); skip > 0; --skip) word &= word - 1;
-  const int expert = __builtin_amdgcn_readfirstlane(at * 32 + __ffs(word) - 1);
-  for (int p = tid; p < pairs; p += 256)
-    if (ids[p] == expert) g.pair_of[p / slots] = p;
+  if (lane == 63) wave_rows[wave] = rows, wave_used[wave] = used;
   __syncthreads();
-  if (tid < kTokens) {
-    const int32_t pair = g.pair_of[tid];
-    const uint64_t have = __ballot(pair >= 0);
-    if (pair >= 0) g.list[__popcll(have & ((uint64_t(1) << tid) - 1))] = pair;
-    if (tid == 0) g.count = __popcll(have);
+  int before_rows = 0, before_used = 0, all_rows = 0, all_used = 0;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    if (v < wave) before_rows += wave_rows[v], before_used += wave_used[v];
+    all_rows += wave_rows[v], all_used += wave_used[v];
   }
+  const int start = before_rows + rows - count, group = before_used + used - 1;
+  if (count) plan->expert[group] = tid, plan->start[group] = start;
+  if (tid == 0) plan->groups = all_used, plan->start[all_used] = all_rows;
+  first[tid] = start;
   __syncthreads();
-  return expert;
+  // a pair's place: behind the earlier pairs of its expert
+  if (tid < pairs) {
+    const int e = ids[tid];
+    int place = -1;
+    if (e >= 0) {
+      place = first[e];
+      const int4* four = reinterpret_cast<const int4*>(ids);
+      for (int p = 0; p < tid / 4; ++p) {
+        const int4 v = four[p];
+        place += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
+      }
+      for (int p = tid & ~3; p < tid; ++p) place += ids[p] == e;
+      plan->order[place] = tid;
+      plan->weight[place] = (float)chosen[tid];
+    }
+    plan->place[tid] = place;
+  }
 }
 
-template <typename T, int BM>
-__device__ __forceinline__ void clear(F16x (&acc)[BM / 32][2]) {
-#pragma unroll
-  for (int x = 0; x < BM / 32; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+struct Choose {
+  const void* weights;
+  int64_t ldw;
+  int32_t wdtype, tokens, experts, slots;
+  // x's rows, and where they go as whole pieces (NULL: they stay)
+  const void* x;
+  int64_t ldx, width;
+  void* to;
+};
+
+template <typename T, typename K>
+__global__ __launch_bounds__(1024) void k_layer_choose(Choose p, Plan* __restrict__ plan) {
+  if (blockIdx.x) {
+    const int64_t per = (p.width + 7) / 8, pieces = per * p.tokens;
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < pieces;
+         i += (int64_t)(gridDim.x - 1) * 1024)
+      align_piece((const T*)p.x, p.ldx, p.width, i / per, i % per, (T*)p.to);
+    return;
+  }
+  __shared__ K chosen[kPairs];
+  __shared__ __align__(16) int32_t ids[kPairs];
+  if (p.experts <= 64)
+    choose_tokens<K, 16, 4>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, ids, chosen);
+  else if (p.experts <= 256)
+    choose_tokens<K, 16, 16>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, ids, chosen);
+  else
+    choose_tokens<K, 64, 16>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, ids, chosen);
+  __syncthreads();
+  make_plan(ids, chosen, p.tokens * p.slots, plan);
 }
 
 template <int BM, typename Core>
 constexpr int layer_lds() {
-  constexpr int choice = kPairs * 12;
-  constexpr int most = Core::kRing > kThinSums<BM> ? Core::kRing : kThinSums<BM>;
-  return most > choice ? most : choice;
+  return Core::kRing > kThinSums<BM> ? Core::kRing : kThinSums<BM>;
+}
+// A wavefront's columns of a tile, ``wide`` to each set of ``parts`` wavefronts, and its part.
+// The second 32 of a gated product lie ``hidden`` behind the first.
+struct Share {
+  Columns c;
+  int part;
+};
+__device__ __forceinline__ Share share_columns(int64_t tile, int parts, int wide, int64_t columns,
+                                               bool gated) {
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int64_t col = (tile * (4 / parts) + wave / parts) * wide;
+  Share s;
+  s.part = wave % parts;
+  s.c.first[0] = min(col, columns);
+  s.c.n[0] = (int)max<int64_t>(0, min<int64_t>(32, columns - col));
+  s.c.first[1] = gated ? columns + s.c.first[0] : min(col + 32, columns);
+  s.c.n[1] = gated ? s.c.n[0] : (int)max<int64_t>(0, min<int64_t>(32, columns - col - 32));
+  return s;
+}
+
+// The group and tile of a workgroup, XCD by XCD (number i is on XCD i % 8): neighbouring tiles,
+// which may share lines of memory, run side by side.  The groups shared out are those there are.
+__device__ __forceinline__ bool find_item(int64_t tiles, int groups, int& group, int& tile) {
+  const int64_t n = groups * tiles, per = (n + 7) / 8, in = blockIdx.x >> 3;
+  const int64_t at = (blockIdx.x & 7) * per + in;
+  if (in >= per || at >= n) return false;
+  group = (int)(at / tiles);
+  tile = (int)(at - group * tiles);
+  return true;
 }
 
 struct Up {
-  const void* weights;
-  int64_t ldw;
-  int32_t wdtype, tokens, experts, slots, act, gated;
-  int64_t ldx, width, hidden, pitch, tiles;
+  int32_t slots, act, gated, parts;
+  int64_t width, hidden, tiles;
+  Rows x;
+  uint32_t pitch;  // bytes of a hidden row; they are in order of places
 };
 
-// Workgroup: expert number blockIdx.x / tiles, columns of tile blockIdx.x % tiles.
+// Workgroup: group number blockIdx.x / tiles, columns of tile blockIdx.x % tiles.
 template <typename T, int BM, typename Core>
-__global__ __launch_bounds__(256) void k_layer_up(Up p, const T* __restrict__ x, Matrices w,
-                                                  int32_t* __restrict__ ids_out,
-                                                  T* __restrict__ high, T* __restrict__ low) {
+__global__ __launch_bounds__(256, 2) void k_layer_up(
+    Up p, Matrices w, const Plan* __restrict__ plan, uint8_t* __restrict__ high,
+    uint8_t* __restrict__ low) {
   extern __shared__ __align__(16) unsigned char lds16[];
-  __shared__ Group group;
-  __shared__ float weight_of[kTokens];
-  const int tid = threadIdx.x, pairs = p.tokens * p.slots;
-  double* chosen = reinterpret_cast<double*>(lds16);
-  int32_t* ids = reinterpret_cast<int32_t*>(lds16 + kPairs * 8);
-  if (p.experts <= 64)
-    choose_tokens<16, 4>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, ids, chosen);
-  else if (p.experts <= 256)
-    choose_tokens<16, 16>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, ids, chosen);
-  else
-    choose_tokens<64, 16>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, ids, chosen);
-  __syncthreads();
-  if (blockIdx.x == 0)
-    for (int i = tid; i < pairs; i += 256) ids_out[i] = ids[i];
-  const int at = (int)(blockIdx.x / p.tiles), tile = (int)(blockIdx.x - at * p.tiles);
-  const int e = find_group(ids, pairs, p.slots, at, group);
-  if (e < 0) return;
-  const int count = group.count;
-  if (tid < count) weight_of[tid] = (float)chosen[group.list[tid]];
-  __syncthreads();
-  const int wide = p.gated ? 32 : 64;  // columns of h
-  const int64_t col = (int64_t)tile * wide, outer = p.gated ? 2 * p.hidden : p.hidden;
-  Columns c;
-  c.first[0] = col;
-  c.n[0] = (int)min<int64_t>(32, p.hidden - col);
-  c.first[1] = p.gated ? p.hidden + col : col + 32;
-  c.n[1] = p.gated ? c.n[0] : (int)max<int64_t>(0, min<int64_t>(32, p.hidden - col - 32));
+  const int tid = threadIdx.x;
+  int at, tile;
+  if (!find_item(p.tiles, plan->groups, at, tile)) return;
+  const int e = plan->expert[at], start = plan->start[at], count = plan->start[at + 1] - start;
+  const int parts = Core::kStreams ? p.parts : 4, wide = p.gated ? 32 : 64;
+  const int64_t col = (int64_t)tile * (4 / parts) * wide;
+  const Share own = share_columns(tile, parts, wide, p.hidden, p.gated);
   for (int r0 = 0; r0 < count; r0 += BM) {
-    F16x acc[BM / 32][2];
-    clear<T, BM>(acc);
-    const T* const a[1] = {x};
-    Core::run(a,
-              [&](int r) {
-                return r0 + r < count
-                           ? (uint32_t)(group.list[r0 + r] / p.slots) * (uint32_t)p.ldx * 2u
-                           : kOutside;
-              },
-              p.hidden ? p.width : 0, w, e, outer, c, lds16, acc);
-    float* sums = reinterpret_cast<float*>(lds16);
-    thin_parts<BM>(acc, sums);
-    for (int i = tid; i < min(BM, count - r0) * (wide / 8); i += 256) {
-      const int r = i / (wide / 8), j = i % (wide / 8) * 8;
-      if (col + j >= p.pitch) continue;
+    const Rows a[1] = {p.x};
+    Core::run(a, [&](int r) { return r0 + r < count ? plan->order[start + r0 + r] / p.slots : -1; },
+              p.hidden ? p.width : 0, w, e, p.gated ? 2 * p.hidden : p.hidden, own.c, own.part, parts,
+              lds16);
+    const float* sums = reinterpret_cast<const float*>(lds16);
+    const int rows = min(BM, count - r0);
+    const int per = 4 / parts * (wide / 8);  // pieces of a row
+    for (int i = tid; i < rows * per; i += 256) {
+      const int r = i / per, j = i % per * 8, place = start + r0 + r;
+      if (col + j >= p.hidden) continue;
+      const int at = p.gated ? (j >> 5 << 6) + (j & 31) : j;  // of the sums
+      const float weight = plan->weight[place];
       Pack<T> hi, lo;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        float h = activation<T>(p.act, thin_sum<BM>(sums, r, j + q));
-        if (p.gated) h *= thin_sum<BM>(sums, r, 32 + j + q);
-        h = col + j + q < p.hidden ? h * weight_of[r0 + r] : 0.0f;
+        float h = activation<T>(p.act, thin_sum<BM>(sums, parts, r, at + q));
+        if (p.gated) h *= thin_sum<BM>(sums, parts, r, at + 32 + q);
+        h = col + j + q < p.hidden ? h * weight : 0.0f;
         hi.v[q] = (T)h;
         const float rest = h - (float)hi.v[q];
         lo.v[q] = (T)(fabsf((float)hi.v[q]) < __builtin_inff() ? rest : 0.0f);
       }
-      const int64_t to = group.list[r0 + r] * p.pitch + col + j;
-      store16(high + to, hi);
-      store16(low + to, lo);
+      const int64_t to = (col + j) * 2 + (int64_t)place * p.pitch;
+      store16(reinterpret_cast<T*>(high + to), hi);
+      store16(reinterpret_cast<T*>(low + to), lo);
     }
     __syncthreads();
   }
 }
 
 struct Down {
-  int32_t tokens, slots;
-  int64_t hidden, outer, pitch, tiles;
+  int64_t hidden, outer, tiles;
+  uint32_t pitch;
+  int32_t parts;
 };
 
 template <typename T, int BM, typename Core>
-__global__ __launch_bounds__(256) void k_layer_down(Down p, const T* __restrict__ high,
-                                                    const T* __restrict__ low, Matrices w,
-                                                    const int32_t* __restrict__ ids_in,
-                                                    float* __restrict__ parts) {
+__global__ __launch_bounds__(256, 2) void k_layer_down(
+    Down p, const uint8_t* __restrict__ high, const uint8_t* __restrict__ low, Matrices w,
+    const Plan* __restrict__ plan, float* __restrict__ out) {
   extern __shared__ __align__(16) unsigned char lds16[];
-  __shared__ Group group;
-  const int tid = threadIdx.x, pairs = p.tokens * p.slots;
-  int32_t* ids = reinterpret_cast<int32_t*>(lds16);
-  for (int i = tid; i < pairs; i += 256) ids[i] = ids_in[i];
-  __syncthreads();
-  const int at = (int)(blockIdx.x / p.tiles), tile = (int)(blockIdx.x - at * p.tiles);
-  const int e = find_group(ids, pairs, p.slots, at, group);
-  if (e < 0) return;
-  const int64_t col = (int64_t)tile * 64;
-  Columns c;
-  c.first[0] = col;
-  c.n[0] = (int)min<int64_t>(32, p.outer - col);
-  c.first[1] = col + 32;
-  c.n[1] = (int)max<int64_t>(0, min<int64_t>(32, p.outer - col - 32));
-  const int n = (int)min<int64_t>(64, p.outer - col), count = group.count;
+  const int tid = threadIdx.x;
+  int at, tile;
+  if (!find_item(p.tiles, plan->groups, at, tile)) return;
+  const int e = plan->expert[at], start = plan->start[at], count = plan->start[at + 1] - start;
+  const int parts = Core::kStreams ? p.parts : 4, wide = 64 * (4 / parts);
+  const int64_t col = (int64_t)tile * wide;
+  const Share own = share_columns(tile, parts, 64, p.outer, false);
+  const int n = (int)min<int64_t>(wide, p.outer - col);
   for (int r0 = 0; r0 < count; r0 += BM) {
-    F16x acc[BM / 32][2];
-    clear<T, BM>(acc);
-    const T* const a[2] = {high, low};
-    Core::run(a,
-              [&](int r) {
-                return r0 + r < count ? (uint32_t)group.list[r0 + r] * (uint32_t)p.pitch * 2u
-                                      : kOutside;
-              },
-              p.hidden, w, e, p.outer, c, lds16, acc);
-    float* sums = reinterpret_cast<float*>(lds16);
-    thin_parts<BM>(acc, sums);
-    for (int i = tid; i < min(BM, count - r0) * 16; i += 256) {
-      const int r = i >> 4, j = (i & 15) * 4;
+    const Rows a[2] = {{high, 16u, p.pitch}, {low, 16u, p.pitch}};
+    Core::run(a, [&](int r) { return r0 + r < count ? start + r0 + r : -1; }, p.hidden, w, e, p.outer,
+              own.c, own.part, parts, lds16);
+    const float* sums = reinterpret_cast<const float*>(lds16);
+    for (int i = tid; i < min(BM, count - r0) * (wide / 4); i += 256) {
+      const int r = i / (wide / 4), j = i % (wide / 4) * 4;
       if (j >= n) continue;
       Pack<float> v;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v.v[q] = thin_sum<BM>(sums, r, j + q);
-      store_upto(parts + group.list[r0 + r] * p.outer + col + j, v, n - j);
+      for (int q = 0; q < 4; ++q) v.v[q] = thin_sum<BM>(sums, parts, r, j + q);
+      store_upto(out + (start + r0 + r) * p.outer + col + j, v, n - j);
     }
     __syncthreads();
   }
@@ -433,14 +493,15 @@ __global__ __launch_bounds__(256) void k_layer_down(Down p, const T* __restrict_
 // A token's rows added up in the order of its slots.
 template <typename T>
 __global__ __launch_bounds__(256) void k_layer_sum(const float* __restrict__ parts,
-                                                   const int32_t* __restrict__ ids, int slots,
+                                                   const Plan* __restrict__ plan, int slots,
                                                    int64_t outer, T* __restrict__ out) {
   const int64_t t = blockIdx.y, j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (j >= outer) return;
   float sum[4] = {0, 0, 0, 0};
   for (int s = 0; s < slots; ++s) {
-    if (ids[t * slots + s] < 0) continue;
-    const Pack<float> v = load_upto(parts + (t * slots + s) * outer + j, outer - j);
+    const int64_t place = plan->place[t * slots + s];
+    if (place < 0) continue;
+    const Pack<float> v = load_upto(parts + place * outer + j, outer - j);
 #pragma unroll
     for (int q = 0; q < 4; ++q) sum[q] += v.v[q];
   }
@@ -451,14 +512,14 @@ __global__ __launch_bounds__(256) void k_layer_sum(const float* __restrict__ par
 
 // The workspace's parts, each at 256 bytes.
 struct LayerSpace {
-  int64_t pitch, ids, high, low, parts, x, bytes;
+  int64_t pieces, plan, high, low, parts, x, bytes;
   LayerSpace(int64_t tokens, int64_t slots, int64_t width, int64_t hidden, int64_t outer) {
     const int64_t pairs = tokens * slots;
-    pitch = (hidden + 63) / 64 * 64;
-    ids = 0;
-    high = ids + whole256(pairs * 4);
-    low = high + whole256(pairs * pitch * 2);
-    parts = low + whole256(pairs * pitch * 2);
+    pieces = (hidden + 7) / 8;  // of a hidden row
+    plan = 0;
+    high = plan + whole256(sizeof(Plan));
+    low = high + whole256(pairs * pieces * 16);
+    parts = low + whole256(pairs * pieces * 16);
     x = parts + whole256(pairs * outer * 4);
     bytes = x + aligned_bytes(tokens, width);
   }
@@ -467,81 +528,97 @@ struct LayerSpace {
 // How an expert's matrices are read.
 enum Reading { kCodes, kAlongDirect, kAcrossDirect, kAlong, kAcross };
 static Reading reading(const purin_train_matrices& m, int64_t inner, int64_t outer, int64_t half,
-                       bool rows_ok, int64_t* ld) {
+                       int64_t* ld) {
   if (m.scales) {
     *ld = 0;
     return kCodes;
   }
-  const bool along = m.so != 1 && (m.si == 1 || inner <= 1);
+  const bool along = along_inner(inner, m.si, m.so);
   *ld = along ? m.so : m.si;
-  const bool direct = rows_ok && direct_ok(m.values, *ld, along ? inner : outer) && m.se % 8 == 0 &&
+  const bool direct = direct_ok(m.values, *ld, along ? inner : outer) && m.se % 8 == 0 &&
                       (along || half % 8 == 0);
   return along ? (direct ? kAlongDirect : kAlong) : (direct ? kAcrossDirect : kAcross);
 }
+// Calls f with a tile's rows and the core of a reading.
+template <typename T, int NA, typename F>
+static int by_reading(Reading how, int height, F&& f) {
+  if (how == kCodes)
+    return height == 16 ? f(i16, ThinCodes<T, 16, NA>{}) : f(i32, ThinCodes<T, 32, NA>{});
+  if (how == kAlongDirect)
+    return height == 16 ? f(i16, ThinAlong<T, 16, NA>{}) : f(i32, ThinAlong<T, 32, NA>{});
+  auto rest = [&](auto bm) {
+    constexpr int BM = bm;
+    if (how == kAcrossDirect) return f(bm, ThinDense<T, BM, NA, false, true>{});
+    if (how == kAlong) return f(bm, ThinDense<T, BM, NA, true, false>{});
+    return f(bm, ThinDense<T, BM, NA, false, false>{});
+  };
+  return height <= 32 ? rest(i32) : rest(i64);
+}
+
+struct Shape {
+  int64_t tokens, experts, slots, width, hidden, outer;
+  int32_t act, gated;
+};
 
 template <typename T>
-static int layer(hipStream_t st, const Up& shape, int64_t outer, const T* x,
-                 const purin_train_matrices& inner, const purin_train_matrices& out_matrices,
-                 uint8_t* ws, T* out) {
-  Up up = shape;
-  const LayerSpace at(up.tokens, up.slots, up.width, up.hidden, outer);
-  const int64_t pairs = (int64_t)up.tokens * up.slots, groups = std::min<int64_t>(up.experts, pairs);
-  int32_t* ids = (int32_t*)(ws + at.ids);
-  T *high = (T*)(ws + at.high), *low = (T*)(ws + at.low);
+static int layer(hipStream_t st, const Shape& s, const void* weights, int32_t wdtype, int64_t ldw,
+                 const T* x, int64_t ldx, const purin_train_matrices& inner,
+                 const purin_train_matrices& outer, uint8_t* ws, T* out) {
+  const LayerSpace at(s.tokens, s.slots, s.width, s.hidden, s.outer);
+  const int64_t pairs = s.tokens * s.slots, groups = std::min(s.experts, pairs);
+  Plan* plan = (Plan*)(ws + at.plan);
+  uint8_t *high = ws + at.high, *low = ws + at.low;
   float* parts = (float*)(ws + at.parts);
-  const int64_t columns = up.gated ? 2 * up.hidden : up.hidden;
   Matrices a{inner.values, (const uint8_t*)inner.scales, inner.se, 0};
-  const bool rows_ok = direct_ok(x, up.ldx, up.width);
-  const Reading how = reading(inner, up.width, columns, up.hidden, rows_ok, &a.ld);
-  if (how == kCodes && up.width && !rows_ok) {
-    if (int rc = align_rows<T>(st, x, up.ldx, up.tokens, up.width, (T*)(ws + at.x))) return rc;
-    x = (const T*)(ws + at.x);
-    up.ldx = (up.width + 7) / 8 * 8;
+  Matrices b{outer.values, (const uint8_t*)outer.scales, outer.se, 0};
+  const Reading how_a = reading(inner, s.width, s.gated ? 2 * s.hidden : s.hidden, s.hidden, &a.ld);
+  const Reading how_b = reading(outer, s.hidden, s.outer, 8, &b.ld);
+
+  const uint32_t pitch = (uint32_t)(at.pieces * 16);
+  // streams of 64 columns, and the workgroups' tiles of them
+  const int64_t wide = s.gated ? 32 : 64, streams_a = std::max<int64_t>(1, (s.hidden + wide - 1) / wide);
+  const int64_t streams_b = (s.outer + 63) / 64;
+  const int parts_a = how_a <= kAlongDirect ? stream_parts(groups * streams_a) : 4;
+  const int parts_b = how_b <= kAlongDirect ? stream_parts(groups * streams_b) : 4;
+  auto tiles = [](int64_t streams, int parts) { return (streams * parts + 3) / 4; };
+  Up up{(int32_t)s.slots, s.act, s.gated, parts_a, s.width, s.hidden, tiles(streams_a, parts_a),
+        {x, 16u, (uint32_t)(ldx * 2)}, pitch};
+  Choose choose{weights, ldw, wdtype, (int32_t)s.tokens, (int32_t)s.experts, (int32_t)s.slots, x, ldx,
+                s.width, nullptr};
+  int64_t moves = 0;
+  // rows whose pieces lie anywhere move to 16 bytes, but for the core that takes those too
+  if (s.width && !direct_ok(x, ldx, s.width) && how_a != kAlong && how_a != kAcross) {
+    const int64_t pieces = (s.width + 7) / 8;
+    choose.to = ws + at.x;
+    up.x = {choose.to, 16u, (uint32_t)pieces * 16u};
+    moves = (pieces * s.tokens + 1023) / 1024;
   }
-  up.pitch = at.pitch;
-  up.tiles = std::max<int64_t>(1, (up.hidden + (up.gated ? 31 : 63)) / (up.gated ? 32 : 64));
-  auto launch_up = [&](auto bm, auto core) {
-    constexpr int BM = bm;
-    using Core = decltype(core);
-    return launch16("k_layer_up", k_layer_up<T, BM, Core>, groups * up.tiles, 1, 1, 256,
-                    layer_lds<BM, Core>(), st, up, x, a, ids, high, low);
-  };
-  auto go_up = [&](auto bm) {
-    constexpr int BM = bm;
-    switch (how) {
-      case kCodes: return launch_up(bm, ThinCodes<T, BM, 1>{});
-      case kAlongDirect: return launch_up(bm, ThinDense<T, BM, 1, true, true>{});
-      case kAcrossDirect: return launch_up(bm, ThinDense<T, BM, 1, false, true>{});
-      case kAlong: return launch_up(bm, ThinDense<T, BM, 1, true, false>{});
-      default: return launch_up(bm, ThinDense<T, BM, 1, false, false>{});
-    }
-  };
-  // an expert with more rows than a tile reads its weights again
-  const bool tall = up.tokens > 32 && pairs > 16 * up.experts;
-  if (int rc = tall ? go_up(i64) : go_up(i32)) return rc;
-  Matrices b{out_matrices.values, (const uint8_t*)out_matrices.scales, out_matrices.se, 0};
-  const Reading how_b = reading(out_matrices, up.hidden, outer, 8, true, &b.ld);
-  const Down down{up.tokens, up.slots, up.hidden, outer, at.pitch, (outer + 63) / 64};
-  auto launch_down = [&](auto bm, auto core) {
-    constexpr int BM = bm;
-    using Core = decltype(core);
-    return launch16("k_layer_down", k_layer_down<T, BM, Core>, groups * down.tiles, 1, 1, 256,
-                    layer_lds<BM, Core>(), st, down, (const T*)high, (const T*)low, b,
-                    (const int32_t*)ids, parts);
-  };
-  auto go_down = [&](auto bm) {
-    constexpr int BM = bm;
-    switch (how_b) {
-      case kCodes: return launch_down(bm, ThinCodes<T, BM, 2>{});
-      case kAlongDirect: return launch_down(bm, ThinDense<T, BM, 2, true, true>{});
-      case kAcrossDirect: return launch_down(bm, ThinDense<T, BM, 2, false, true>{});
-      case kAlong: return launch_down(bm, ThinDense<T, BM, 2, true, false>{});
-      default: return launch_down(bm, ThinDense<T, BM, 2, false, false>{});
-    }
-  };
-  if (int rc = tall ? go_down(i64) : go_down(i32)) return rc;
-  k_layer_sum<T><<<dim3((unsigned)((outer + 1023) / 1024), (unsigned)up.tokens), dim3(256), 0, st>>>(
-      parts, ids, up.slots, outer, out);
+  const dim3 grid((unsigned)(1 + moves));
+  if (wdtype == PURIN_TRAIN_F64)
+    k_layer_choose<T, double><<<grid, dim3(1024), 0, st>>>(choose, plan);
+  else
+    k_layer_choose<T, float><<<grid, dim3(1024), 0, st>>>(choose, plan);
+  if (int rc = launched("k_layer_choose")) return rc;
+
+  // rows of a tile; an expert with more reads its weights again
+  const int height = pairs <= 6 * s.experts || s.tokens <= 16 ? 16
+                     : pairs <= 16 * s.experts || s.tokens <= 32 ? 32 : 64;
+  if (int rc = by_reading<T, 1>(how_a, height, [&](auto bm, auto core) {
+        using Core = decltype(core);
+        return launch16("k_layer_up", k_layer_up<T, bm, Core>, (groups * up.tiles + 7) / 8 * 8, 1, 1,
+                        256, layer_lds<bm, Core>(), st, up, a, (const Plan*)plan, high, low);
+      }))
+    return rc;
+  const Down down{s.hidden, s.outer, tiles(streams_b, parts_b), pitch, parts_b};
+  if (int rc = by_reading<T, 2>(how_b, height, [&](auto bm, auto core) {
+        using Core = decltype(core);
+        return launch16("k_layer_down", k_layer_down<T, bm, Core>, (groups * down.tiles + 7) / 8 * 8, 1,
+                        1, 256, layer_lds<bm, Core>(), st, down, (const uint8_t*)high,
+                        (const uint8_t*)low, b, (const Plan*)plan, parts);
+      }))
+    return rc;
+  k_layer_sum<T><<<dim3((unsigned)((s.outer + 1023) / 1024), (unsigned)s.tokens), dim3(256), 0, st>>>(
+      parts, plan, (int)s.slots, s.outer, out);
   return launched("k_layer_sum");
 }
 
@@ -620,14 +697,13 @@ int purin_train_expert_layer(void* stream, int32_t dtype, int32_t wdtype, int64_
                                  purin_train_expert_layer_workspace_bytes(
                                      dtype, tokens, experts, slots, width, hidden, outer_width)))
       return rc;
-    const Up up{weights,     ldw, wdtype, (int32_t)tokens, (int32_t)experts, (int32_t)slots, activation,
-                gated ? 1 : 0, ldx, width,  hidden,          0,                0};
+    const Shape s{tokens, experts, slots, width, hidden, outer_width, activation, gated ? 1 : 0};
     uint8_t* ws = (uint8_t*)workspace;
     return dtype == PURIN_TRAIN_BF16
-               ? layer<bf16>((hipStream_t)stream, up, outer_width, (const bf16*)x, *inner, *outer, ws,
-                             (bf16*)out)
-               : layer<f16>((hipStream_t)stream, up, outer_width, (const f16*)x, *inner, *outer, ws,
-                            (f16*)out);
+               ? layer<bf16>((hipStream_t)stream, s, weights, wdtype, ldw, (const bf16*)x, ldx, *inner,
+                             *outer, ws, (bf16*)out)
+               : layer<f16>((hipStream_t)stream, s, weights, wdtype, ldw, (const f16*)x, ldx, *inner,
+                            *outer, ws, (f16*)out);
   });
 }
 

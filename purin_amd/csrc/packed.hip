@@ -7,8 +7,8 @@
 namespace purin {
 namespace train {
 
-template <typename T, int B, int WN, int S>
-__global__ __launch_bounds__(2 * WN * 64) void k_product_packed(
+template <typename T, int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__(WM* WN * 64) void k_product_packed(
     const T* __restrict__ a, int64_t lda, const uint8_t* __restrict__ codes,
     const uint8_t* __restrict__ scales, int64_t rows, int64_t inner, int64_t outer, int experts,
     int64_t tiles_m, int64_t tiles_n, const int32_t* __restrict__ offsets, T* __restrict__ out,
@@ -18,65 +18,69 @@ __global__ __launch_bounds__(2 * WN * 64) void k_product_packed(
   tile_order(tiles_m, tiles_n, tm, tn);
   int e;
   int64_t from, to;
-  if (!find_tile(offsets, experts, rows, B, tm, e, from, to)) return;
+  if (!find_tile(offsets, experts, rows, BM, tm, e, from, to)) return;
   e = __builtin_amdgcn_readfirstlane(e);
-  const int64_t col = tn * B;
-  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(B, to - from));
-  const int n = (int)min<int64_t>(B, outer - col);
+  const int64_t col = tn * BN;
+  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
+  const int n = (int)min<int64_t>(BN, outer - col);
   T* c = out + from * ldo + col;
   if (e < 0) {
     zero_tile(c, ldo, m, n);
     return;
   }
-  TileHalf<T, B, B, 2, WN, S>::run(a + from * lda, lda, m, inner,
-                                   Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
+  TileHalf<T, BM, BN, WM, WN, S>::run(a + from * lda, lda, m, inner,
+                                      Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
 }
 
-// Split number blockIdx.y of the contraction writes its own ``out``.
-template <typename T, typename C, int BM, int S>
-__global__ __launch_bounds__(256) void k_product_packed_thin(
-    const T* __restrict__ a, int64_t lda, const uint8_t* __restrict__ codes,
-    const uint8_t* __restrict__ scales, int64_t rows, int64_t inner, int64_t outer, int experts,
-    int64_t tiles_n, const int32_t* __restrict__ offsets, C* __restrict__ out, int64_t ldo) {
-  extern __shared__ __align__(16) unsigned char lds16[];
+// Split number blockIdx.y of the contraction writes its own ``out``.  A tile has 64 columns to each
+// set of ``parts`` wavefronts.
+template <typename T, typename C, int BM>
+__global__ __launch_bounds__(256, 2) void k_product_packed_thin(
+    Rows a, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
+    int64_t inner, int64_t outer, int experts, int parts, int64_t tiles_n,
+    const int32_t* __restrict__ offsets, C* __restrict__ out, int64_t ldo) {
+  constexpr int kLds = kThinSums<BM> > kLineLds ? kThinSums<BM> : kLineLds;
+  __shared__ __align__(16) uint8_t lds[kLds];
   const int64_t tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
   int e;
   int64_t from, to;
   if (!find_tile(offsets, experts, rows, BM, tm, e, from, to)) return;
   e = __builtin_amdgcn_readfirstlane(e);
-  const int64_t col = tn * 64;
+  const int wide = 64 * (4 / parts);
+  const int64_t col = tn * wide;
   const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
-  const int n = (int)min<int64_t>(64, outer - col);
+  const int n = (int)min<int64_t>(wide, outer - col);
   C* c = out + (int64_t)blockIdx.y * rows * ldo + from * ldo + col;
   if (e < 0) {
     zero_tile(c, ldo, m, n);
     return;
   }
-  using Thin = ThinPacked<T, BM, 1, S>;
-  F16x acc[BM / 32][2];
-#pragma unroll
-  for (int x = 0; x < BM / 32; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
-  const Codes b(codes, scales, e * outer + col, inner);
-  const int64_t stages = (b.blocks + 7) / 8, per = (stages + gridDim.y - 1) / gridDim.y;
-  const int64_t first = min<int64_t>(b.blocks, blockIdx.y * per * 8);
-  const T* const from_a[1] = {a + from * lda};
-  Thin::run(from_a, [&](int r) { return r < m ? (uint32_t)r * (uint32_t)lda * 2u : kOutside; }, inner,
-            b, [&](int j) { return j < n ? j : -1; }, first, min<int64_t>(b.blocks - first, per * 8),
-            lds16, acc);
-  float* sums = reinterpret_cast<float*>(lds16);
+  ThinAcc<BM> acc;
+  const Codes b(codes, scales, (int64_t)e * outer, inner);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int own = wave / parts * 64;  // the wavefront's columns
+  Columns cols;
+  cols.first[0] = col + own;
+  cols.first[1] = col + own + 32;
+  cols.n[0] = max(min(n - own, 32), 0);
+  cols.n[1] = max(min(n - own - 32, 32), 0);
+  const Rows from_a[1] = {{(const uint8_t*)a.p + from * a.pitch, a.step, a.pitch}};
+  int first, end, at, upto;
+  share_lines(0, cols.n[0] ? b.lines() : 0, (int)blockIdx.y, (int)gridDim.y, first, end);
+  share_lines(first, end, wave % parts, parts, at, upto);
+  StreamCodes<T, BM, 1>::run(from_a, [&](int r) { return r < m ? r : -1; }, inner, b, cols, at, upto,
+                             lds, acc);
+  float* sums = reinterpret_cast<float*>(lds);
+  __syncthreads();
   thin_parts<BM>(acc, sums);
   constexpr int V = kVec<C>;
-  for (int at = threadIdx.x; at < BM * 64 / V; at += 256) {
-    const int i = at / (64 / V), j = at % (64 / V) * V;
-    if (i >= m || j >= n) continue;
+  for (int i = threadIdx.x; i < m * (wide / V); i += 256) {
+    const int r = i / (wide / V), j = i % (wide / V) * V;
+    if (j >= n) continue;
     Pack<C> v;
 #pragma unroll
-    for (int q = 0; q < V; ++q) v.v[q] = (C)thin_sum<BM>(sums, i, j + q);
-    store_upto(c + i * ldo + j, v, n - j);
+    for (int q = 0; q < V; ++q) v.v[q] = (C)thin_sum<BM>(sums, parts, r, j + q);
+    store_upto(c + r * ldo + j, v, n - j);
   }
 }
 
@@ -108,18 +112,18 @@ __global__ __launch_bounds__(2 * WN * 64) void k_product_both(
 enum ShapePacked { kThinPacked, k128Packed, k256Packed };
 struct CutPacked {
   ShapePacked shape;
-  int height, splits;
+  int height, parts, splits;
 };
 static CutPacked cut_packed(bool both, int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
   const int64_t tiles = most_tiles(rows, experts, 128) * ((outer + 127) / 128);
-  if (!both && (rows <= 32 * experts || tiles <= 128)) {
-    const int64_t across = (outer + 63) / 64;
-    const bool tall = rows > 16 * experts && most_tiles(rows, experts, 64) * across >= 256;
-    if (tall) return {kThinPacked, 64, 1};
-    const int64_t stages = (inner + 255) / 256;
-    return {kThinPacked, 32, splits_of(512, most_tiles(rows, experts, 32) * across, stages, 4)};
+  if (!both && (rows <= 48 * experts || tiles <= 64)) {
+    const int height = rows <= 8 * experts ? 16 : 32;
+    const int64_t streams = most_tiles(rows, experts, height) * ((outer + 63) / 64);
+    const int parts = stream_parts(streams);
+    return {kThinPacked, height, parts,
+            splits_of(1024, streams * parts / 4, (inner + 255) / 256, parts)};
   }
-  return {tiles >= 16 * 256 ? k256Packed : k128Packed, tiles >= 16 * 256 ? 256 : 128, 1};
+  return {tiles >= 16 * 256 ? k256Packed : k128Packed, 0, 0, 1};
 }
 
 template <typename T>
@@ -127,38 +131,43 @@ static int product_packed(hipStream_t st, int64_t rows, int64_t inner, int64_t o
                           int64_t experts, const T* a, int64_t lda, const uint8_t* codes,
                           const uint8_t* scales, const int32_t* offsets, uint8_t* ws, T* out,
                           int64_t ldo) {
-  if (inner && !direct_ok(a, lda, inner)) {
-    if (int rc = align_rows<T>(st, a, lda, rows, inner, (T*)ws)) return rc;
-    a = (const T*)ws;
-    lda = (inner + 7) / 8 * 8;
-  }
   CutPacked cut = cut_packed(false, rows, inner, outer, experts);
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
   if (cut.shape == kThinPacked) {
+    Rows from{a, 16u, (uint32_t)lda * 2u};
+    if (inner && !direct_ok(a, lda, inner)) {
+      if (int rc = align_rows<T>(st, a, lda, rows, inner, ws)) return rc;
+      from = {ws, 16u, (uint32_t)((inner + 7) / 8) * 16u};
+    }
     float* parts = (float*)(ws + aligned_bytes(rows, inner));
-    const int64_t tm = most_tiles(rows, experts, cut.height), tn = (outer + 63) / 64;
-    auto thin = [&](auto c, auto h) {
+    const int wide = 64 * (4 / cut.parts);
+    const int64_t tm = most_tiles(rows, experts, cut.height), tn = (outer + wide - 1) / wide;
+    auto thin = [&](auto c) {
       using C = decltype(c);
-      constexpr int BM = h, S = BM == 32 ? 3 : 3;
-      constexpr int ring = ThinPacked<T, BM, 1, S>::kRing;
-      return launch16("k_product_packed_thin", k_product_packed_thin<T, C, BM, S>, tm * tn,
-                      (unsigned)cut.splits, 1, 256, ring > kThinSums<BM> ? ring : kThinSums<BM>, st,
-                      a, lda, codes, scales, rows, inner, outer, (int)experts, tn, offsets,
-                      cut.splits > 1 ? (C*)parts : (C*)out, ldo);
+      return launch16("k_product_packed_thin",
+                      cut.height == 16 ? k_product_packed_thin<T, C, 16> : k_product_packed_thin<T, C, 32>,
+                      tm * tn, (unsigned)cut.splits, 1, 256, 0, st, from, codes, scales, rows, inner,
+                      outer, (int)experts, cut.parts, tn, offsets, cut.splits > 1 ? (C*)parts : (C*)out,
+                      ldo);
     };
-    if (cut.splits == 1) return cut.height == 32 ? thin(T{}, i32) : thin(T{}, i64);
-    if (int rc = thin(float{}, i32)) return rc;
+    if (cut.splits == 1) return thin(T{});
+    if (int rc = thin(float{})) return rc;
     return join(st, parts, cut.splits, rows * outer, out);
+  }
+  if (inner && !direct_ok(a, lda, inner)) {
+    if (int rc = align_rows<T>(st, a, lda, rows, inner, ws)) return rc;
+    a = (const T*)ws;
+    lda = (inner + 7) / 8 * 8;
   }
   auto go = [&](auto bm, auto wn, auto s) {
     constexpr int B = bm, WN = wn, S = s;
     const int64_t tm = most_tiles(rows, experts, B), tn = (outer + B - 1) / B;
-    return launch16("k_product_packed", k_product_packed<T, B, WN, S>, tm * tn, 1, 1, 2 * WN * 64,
+    return launch16("k_product_packed", k_product_packed<T, B, B, 2, WN, S>, tm * tn, 1, 1, 2 * WN * 64,
                     TileHalf<T, B, B, 2, WN, S>::kLds, st, a, lda, codes, scales, rows, inner, outer,
                     (int)experts, tm, tn, offsets, out, ldo);
   };
-  if (cut.shape == k256Packed) return go(i256, i4, integral_constant<int, 3>{});
-  return go(i128, i2, integral_constant<int, 3>{});
+  constexpr integral_constant<int, 3> i3;
+  return cut.shape == k256Packed ? go(i256, i4, i3) : go(i128, i2, i3);
 }
 
 template <typename C>

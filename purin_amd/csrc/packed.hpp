@@ -20,6 +20,7 @@ namespace train {
 
 typedef int I4 __attribute__((ext_vector_type(4)));
 typedef int I8 __attribute__((ext_vector_type(8)));
+typedef float F4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kOutside = 0x80000000u;  // an offset past every buffer: reads zeros
 
@@ -154,6 +155,7 @@ __device__ __forceinline__ void ring(int64_t steps, L&& load, F&& multiply) {
 struct Codes {
   const uint8_t *codes, *scales;
   int blocks, words;
+  __device__ __forceinline__ int lines() const { return (blocks + 7) / 8; }
   __device__ __forceinline__ Codes(const uint8_t* c, const uint8_t* s, int64_t row, int64_t length)
       : blocks(micro_blocks(length)), words(micro_filled(micro_blocks(length)) / 4) {
     codes = c + row * blocks * 16;
@@ -322,116 +324,340 @@ struct TileBoth {
 // few rows
 // ---------------------------------------------------------------------------
 
-// The sums of BM rows and 64 columns over a contraction that the 4 wavefronts share, a quarter
-// of every stage each: acc holds a wavefront's own part.  NA: the rows are the sum of that many
-// arrays.  Rows of 16 bits: ``offset(row)`` bytes from the arrays' starts, or kOutside.
-template <typename T, int BM, int NA, int S>
-struct ThinPacked {
-  static constexpr int THREADS = 256, X = BM / 32, Y = 2;
-  using SA = PieceStage<BM, 32, THREADS>;  // a depth of 256
-  using SB = PieceStage<64, 8, THREADS>;
-  using SC = ScaleStage<64, 2, THREADS>;
-  static constexpr int kStage = NA * SA::kBytes + SB::kBytes + SC::kBytes;
-  static constexpr int kLoads = NA * SA::kMine + SB::kMine + SC::kMine;
-  static constexpr int kRing = S * kStage;
+// The sums of BM rows and 64 columns to a wavefront.  A workgroup's four have parts of one
+// contraction, or of two, or each columns of its own (``parts`` = 4, 2, 1): the fewer parts, the
+// longer the streams, and the more the wavefronts share of the rows.  Every weight is used by one
+// wavefront, once: it loads 128 bytes of 64 columns at a time, whole lines by 8 neighbouring lanes,
+// keeps two such loads on their way in registers, and brings the pieces to the lanes that multiply
+// them by way of 8 KB of LDS of its own.  No wavefront waits for another, and the many in flight
+// hide each other.  (Loads straight to the lanes that multiply them take a cycle a lane: 64 experts,
+// 4096 x 2816 in 4 bits 112 us.)
+// NA: the rows are the sum of that many arrays.
 
-  // from block ``first`` on ``blocks`` of them; ``row(j)``: the row of codes of column j, -1 for none
-  template <typename FA, typename FB>
-  static __device__ __forceinline__ void run(const T* const (&a)[NA], FA&& offset, int64_t inner,
-                                             const Codes& b, FB&& row, int64_t first,
-                                             int64_t blocks, unsigned char* lds,
-                                             F16x (&acc)[X][Y]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    uint32_t off_a[SA::kMine], off_b[SB::kMine], off_c[SC::kMine];
-    SA::offsets(offset, off_a);
-    SB::offsets([&](int j) { const int r = row(j); return r < 0 ? kOutside : (uint32_t)r * (uint32_t)b.blocks * 16u; }, off_b);
-    SC::offsets([&](int j) { const int r = row(j); return r < 0 ? kOutside : (uint32_t)r * (uint32_t)b.words * 4u; }, off_c);
-    const uint8_t *pb = uniform(b.codes + first * 16), *pc = uniform(b.scales);
-    const uint8_t* pa[NA];
+// Rows of 16 bits in pieces of 8: piece k of row r at p + k * step + r * pitch bytes.
+struct Rows {
+  const void* p;
+  uint32_t step, pitch;
+};
+// Two times 32 columns of a tile: starts and how many are there.
+struct Columns {
+  int64_t first[2];
+  int n[2];
+};
+
+using Buffer = __amdgpu_buffer_rsrc_t;
+__device__ __forceinline__ Buffer buffer_of(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7ffffff0, 0x00020000);
+}
+__device__ __forceinline__ I4 load_piece(Buffer b, uint32_t at, uint32_t uniform_at) {
+  return __builtin_bit_cast(I4, __builtin_amdgcn_raw_buffer_load_b128(b, (int)at, (int)uniform_at, 0));
+}
+
+__device__ __forceinline__ F4 mma16(bf16, S8 a, S8 b, F4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, a),
+                                                 __builtin_bit_cast(B8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ F4 mma16(f16, S8 a, S8 b, F4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(H8, a),
+                                                __builtin_bit_cast(H8, b), c, 0, 0, 0);
+}
+
+// A wavefront's sums: rows 16 x + lane % 16, columns 16 y + 4 (lane / 16) + r.
+template <int BM>
+struct ThinAcc {
+  static constexpr int X = BM / 16;
+  F4 v[X][4];
+  __device__ __forceinline__ ThinAcc() {
 #pragma unroll
-    for (int i = 0; i < NA; ++i) pa[i] = reinterpret_cast<const uint8_t*>(uniform(a[i] + first * 32));
-    const int64_t pieces = min((inner + 7) / 8 - first * 4, blocks * 4);
-    const uint32_t base = lds_address(lds);
-    ring<S, kLoads>(
-        (blocks + 7) / 8,
-        [&](int64_t t, int at) {
-          const uint32_t to = base + (uint32_t)(at * kStage);
+    for (int x = 0; x < X; ++x)
 #pragma unroll
-          for (int i = 0; i < NA; ++i)
-            SA::load(pa[i] + t * 512, off_a, pieces - 32 * t, to + (uint32_t)(i * SA::kBytes));
-          SB::load(pb + t * 128, off_b, blocks - 8 * t, to + (uint32_t)(NA * SA::kBytes));
-          SC::load(pc, off_c, (int)(first / 4 + 2 * t), b.words,
-                   to + (uint32_t)(NA * SA::kBytes + SB::kBytes));
-        },
-        [&](int64_t t, int at) {
-          const uint8_t* la = lds + at * kStage;
-          const uint8_t *lb = la + NA * SA::kBytes, *lc = lb + SB::kBytes;
-          I4 codes[Y];
-          float scale[Y];
-#pragma unroll
-          for (int y = 0; y < Y; ++y) {
-            const int j = 32 * y + (lane & 31);
-            codes[y] = SB::piece(lb, j, 2 * wave + half);
-            scale[y] = scale_of(SC::at(lc, j, wave >> 1), 2 * (wave & 1) + half);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            S8 fb[Y];
-#pragma unroll
-            for (int y = 0; y < Y; ++y) fb[y] = numbers_of(T{}, (uint32_t)codes[y][j], scale[y]);
-#pragma unroll
-            for (int i = 0; i < NA; ++i)
-#pragma unroll
-              for (int x = 0; x < X; ++x) {
-                const S8 fa = __builtin_bit_cast(
-                    S8, SA::piece(la + i * SA::kBytes, 32 * x + (lane & 31), 8 * wave + 4 * half + j));
-#pragma unroll
-                for (int y = 0; y < Y; ++y) acc[x][y] = mma32(T{}, fb[y], fa, acc[x][y]);
-              }
-          }
-        });
+      for (int y = 0; y < 4; ++y) v[x][y] = F4{0, 0, 0, 0};
   }
 };
 
-// The wavefronts' parts of BM x 64 sums, in LDS: row i, column j of part w at thin_at(w, i, j).
+// The wavefronts' BM x 64 sums, in LDS.
 constexpr int kThinPitch = 64 + 4;
 template <int BM>
 constexpr int kThinSums = 4 * BM * kThinPitch * 4;
 template <int BM>
-__device__ __forceinline__ void thin_parts(const F16x (&acc)[BM / 32][2], float* sums) {
+__device__ __forceinline__ void thin_parts(const ThinAcc<BM>& acc, float* sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int x = 0; x < BM / 32; ++x)
+  for (int x = 0; x < BM / 16; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        sums[(wave * BM + 32 * x + (lane & 31)) * kThinPitch + 32 * y + 2 * (r & ~3) +
-             4 * (lane >> 5) + (r & 3)] = acc[x][y][r];
+    for (int y = 0; y < 4; ++y)
+      *reinterpret_cast<F4*>(sums + (wave * BM + 16 * x + (lane & 15)) * kThinPitch + 16 * y +
+                             4 * (lane >> 4)) = acc.v[x][y];
   __syncthreads();
 }
-// Their sum, in the wavefronts' order.
+// Row i, column j (64 to each set of ``parts`` wavefronts): the parts' sum, in their order.
 template <int BM>
-__device__ __forceinline__ float thin_sum(const float* sums, int i, int j) {
-  float s = sums[i * kThinPitch + j];
-#pragma unroll
-  for (int w = 1; w < 4; ++w) s += sums[(w * BM + i) * kThinPitch + j];
+__device__ __forceinline__ float thin_sum(const float* sums, int parts, int i, int j) {
+  const float* at = sums + ((j >> 6) * parts * BM + i) * kThinPitch + (j & 63);
+  float s = at[0];
+  for (int w = 1; w < parts; ++w) s += at[w * BM * kThinPitch];
   return s;
 }
+
+// A lane's rows (16 x + lane % 16 of the tile), and the pieces of them that it multiplies in a
+// unit of ``PIECES`` (LANE apart for the lane groups, INSIDE for its own).
+template <int X, int NA, int PIECES, int LANE, int INSIDE>
+struct RowStream {
+  const uint8_t* p[NA];
+  uint32_t step, at[X];
+  int left;  // pieces of the rows from this lane's first on
+
+  // ``row(i)``: the row of tile row i, -1 for none
+  template <typename F>
+  __device__ __forceinline__ RowStream(const Rows (&a)[NA], F&& row, int64_t pieces)
+      : step(a[0].step) {
+    const int lane = threadIdx.x & 63, group = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) p[i] = uniform((const uint8_t*)a[i].p);
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+      const int r = row(16 * x + (lane & 15));
+      at[x] = r < 0 ? kOutside : (uint32_t)r * a[0].pitch + (uint32_t)(group * LANE) * step;
+    }
+    left = (int)pieces - group * LANE;
+  }
+  __device__ __forceinline__ I4 load(int i, int x, int unit, int k) const {
+    const bool in = unit * PIECES + k * INSIDE < left;
+    return load_piece(buffer_of(p[i] + (int64_t)unit * PIECES * step), in ? at[x] : kOutside,
+                      (uint32_t)(k * INSIDE) * step);
+  }
+};
+
+// Parts of a contraction for a number of 64-column streams of it.
+inline int stream_parts(int64_t streams) { return streams >= 4096 ? 1 : streams >= 1536 ? 2 : 4; }
+// A part of the lines ``first`` to ``end``.
+__device__ __forceinline__ void share_lines(int first, int end, int part, int parts, int& from,
+                                            int& to) {
+  const int per = (max(end - first, 0) + parts - 1) / parts;
+  from = min(end, first + part * per);
+  to = min(end, from + per);
+}
+
+// 64 columns' lines of 128 bytes, in two runs of 32 columns, on their way to the wavefront's LDS:
+// [column][piece], the pieces exchanged by the column's number.
+struct LineStream {
+  const uint8_t* p[2];
+  uint32_t at;          // this lane's piece of column lane / 8; eight columns are ``step`` bytes
+  int step, pieces;     // pieces of 16 bytes, in a column
+  int n[2];
+  I4 v[2][8];
+
+  __device__ __forceinline__ LineStream(const uint8_t* first, const uint8_t* second, const Columns& c,
+                                        int pitch, int count)
+      : step(8 * pitch), pieces(count) {
+    const int lane = threadIdx.x & 63;
+    p[0] = uniform(first);
+    p[1] = uniform(second);
+    at = (uint32_t)((lane >> 3) * pitch + (lane & 7) * 16);
+    n[0] = c.n[0];
+    n[1] = c.n[1];
+  }
+  // line number ``line`` of the columns; from ``to`` on none
+  __device__ __forceinline__ void load(int slot, int line, int to) {
+    const int lane = threadIdx.x & 63;
+    // a column past all of them where the line, or the lane's piece of it, is not there
+    const int j = line < to && 8 * line + (lane & 7) < pieces ? lane >> 3 : 64;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[slot][i] = load_piece(buffer_of(p[i >> 2] + (int64_t)line * 128),
+                              j + 8 * (i & 3) < n[i >> 2] ? at : kOutside,
+                              (uint32_t)(step * (i & 3)));
+  }
+  __device__ __forceinline__ void store(int slot, uint8_t* lds) const {
+    const int lane = threadIdx.x & 63;
+    // columns 8 i + lane / 8 have the number lane / 8 in their eight
+    uint8_t* to = lds + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<I4*>(to + i * 1024) = v[slot][i];
+    __builtin_amdgcn_wave_barrier();  // in order within a wavefront; for the compiler
+  }
+  // piece ``k`` of column 16 y + lane % 16
+  static __device__ __forceinline__ I4 piece(const uint8_t* lds, int y, int k) {
+    const int j = (threadIdx.x & 15);
+    return *reinterpret_cast<const I4*>(lds + (16 * y + j) * 128 + ((k ^ (j & 7)) << 4));
+  }
+};
+constexpr int kLineLds = 4 * 8192;  // a workgroup's
+
+// Microscaled weights: a line is eight blocks, four at a time to the lane groups.  Scales are
+// loaded for two lines at once: a load of them takes a line of the cache a column.
+template <typename T, int BM, int NA>
+struct StreamCodes {
+  static constexpr int X = BM / 16;
+
+  // lines ``from`` to ``to``
+  template <typename F>
+  static __device__ __forceinline__ void run(const Rows (&a)[NA], F&& row, int64_t inner,
+                                             const Codes& b, const Columns& c, int from, int to,
+                                             uint8_t* lds, ThinAcc<BM>& acc) {
+    const int lane = threadIdx.x & 63, group = lane >> 4;
+    lds += (threadIdx.x >> 6) * 8192;
+    LineStream lines(b.codes + c.first[0] * b.blocks * 16, b.codes + c.first[1] * b.blocks * 16, c,
+                     b.blocks * 16, b.blocks);
+    // the scales of column 16 y + lane % 16
+    const int words = b.words * 4;
+    const uint8_t* ps[2] = {uniform(b.scales + c.first[0] * words), uniform(b.scales + c.first[1] * words)};
+    uint32_t at_scale[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int j = 16 * (y & 1) + (lane & 15);
+      at_scale[y] = j < c.n[y >> 1] ? (uint32_t)(j * words) : kOutside;
+    }
+    I4 scales_next[4], rows_now[NA][X][4];
+    uint32_t scales[4];  // the lane group's of the four units
+    // the words of two lines, of which the last row's may end the memory: only those that are there
+    auto load_scales = [&](int line) {
+      if (line < to && 2 * line + 4 <= b.words) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          scales_next[y] = load_piece(buffer_of(ps[y >> 1] + line * 8), at_scale[y], 0);
+      } else {
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            scales_next[y][k] =
+                line < to && 2 * line + k < b.words
+                    ? (int)__builtin_amdgcn_raw_buffer_load_b32(buffer_of(ps[y >> 1] + line * 8 + k * 4),
+                                                                (int)at_scale[y], 0, 0)
+                    : 0;
+      }
+    };
+    load_scales(from);
+    lines.load(0, from, to);
+    lines.load(1, from + 1, to);
+    const RowStream<X, NA, 16, 4, 1> rows(a, row, (inner + 7) / 8);
+    auto load_rows = [&](int j, int unit) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int x = 0; x < X; ++x) rows_now[i][x][j] = rows.load(i, x, unit, j);
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_rows(j, 2 * from);
+    for (int t = from; t < to; t += 2) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        scales[y] = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)  // past the end the codes are zero, and the words another column's
+          if (2 * t + u < 2 * to)
+            scales[y] |= (((uint32_t)scales_next[y][u] >> (8 * group)) & 255u) << (8 * u);
+      }
+      load_scales(t + 2);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {  // past the end: zeros
+        lines.store(s, lds);
+        lines.load(s, t + s + 2, to);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          I4 codes[4];
+          float by[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            codes[y] = LineStream::piece(lds, y, 4 * u + group);
+            by[y] = scale_of(scales[y], 2 * s + u);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            S8 fb[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) fb[y] = numbers_of(T{}, (uint32_t)codes[y][j], by[y]);
+#pragma unroll
+            for (int i = 0; i < NA; ++i)
+#pragma unroll
+              for (int x = 0; x < X; ++x) {
+                const S8 fa = __builtin_bit_cast(S8, rows_now[i][x][j]);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) acc.v[x][y] = mma16(T{}, fb[y], fa, acc.v[x][y]);
+              }
+            load_rows(j, 2 * (t + s) + u + 1);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+};
+
+// Dense weights whose contraction is contiguous (``ld`` elements apart, 16-byte pieces at 16-byte
+// addresses): a line is 64 of it.
+template <typename T, int BM, int NA>
+struct StreamDense {
+  static constexpr int X = BM / 16;
+
+  template <typename F>
+  static __device__ __forceinline__ void run(const Rows (&a)[NA], F&& row, int64_t inner,
+                                             const T* w, int64_t ld, const Columns& c, int from, int to,
+                                             uint8_t* lds, ThinAcc<BM>& acc) {
+    const int lane = threadIdx.x & 63, group = lane >> 4;
+    lds += (threadIdx.x >> 6) * 8192;
+    const int pieces = (int)((inner + 7) / 8);
+    LineStream lines((const uint8_t*)(w + c.first[0] * ld), (const uint8_t*)(w + c.first[1] * ld), c,
+                     (int)ld * 2, pieces);
+    lines.load(0, from, to);
+    lines.load(1, from + 1, to);
+    const RowStream<X, NA, 8, 1, 4> rows(a, row, pieces);
+    I4 rows_now[NA][X][2];
+    auto load_rows = [&](int j, int unit) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int x = 0; x < X; ++x) rows_now[i][x][j] = rows.load(i, x, unit, j);
+    };
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load_rows(j, from);
+    for (int t = from; t < to; t += 2) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {  // past the end: zeros
+        lines.store(s, lds);
+        lines.load(s, t + s + 2, to);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          S8 fb[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            fb[y] = __builtin_bit_cast(S8, LineStream::piece(lds, y, 4 * j + group));
+#pragma unroll
+          for (int i = 0; i < NA; ++i)
+#pragma unroll
+            for (int x = 0; x < X; ++x) {
+              const S8 fa = __builtin_bit_cast(S8, rows_now[i][x][j]);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) acc.v[x][y] = mma16(T{}, fb[y], fa, acc.v[x][y]);
+            }
+          load_rows(j, t + s + 1);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+};
 
 // ---------------------------------------------------------------------------
 // rows at any address
 // ---------------------------------------------------------------------------
 
-// Rows whose 16-byte pieces lie anywhere, to ones at 16 bytes, zeros behind their length.
+// Rows at any address to whole pieces of 8 elements, zeros behind their length.
+template <typename T>
+__device__ __forceinline__ void align_piece(const T* a, int64_t lda, int64_t inner, int64_t row,
+                                            int64_t piece, T* out) {
+  store16(out + (row * ((inner + 7) / 8) + piece) * 8,
+          load_upto(a + row * lda + piece * 8, inner - piece * 8));
+}
 template <typename T>
 static __global__ __launch_bounds__(256) void k_align_rows(const T* __restrict__ a, int64_t lda,
-                                                    int64_t inner, Divider by_row, uint32_t pieces,
-                                                    int64_t first, T* __restrict__ out) {
+                                                           int64_t inner, Divider by,
+                                                           uint32_t pieces, int64_t first,
+                                                           T* __restrict__ out) {
   for (uint32_t n = blockIdx.x * 256 + threadIdx.x; n < pieces; n += gridDim.x * 256) {
-    const uint32_t in = by_row.quotient(n);
-    const int64_t row = first + in, l = (int64_t)(n - in * by_row.d) * 8;
-    store16(out + row * by_row.d * 8 + l, load_upto(a + row * lda + l, inner - l));
+    const uint32_t q = by.quotient(n);
+    align_piece(a, lda, inner, first + q, n - q * by.d, out);
   }
 }
 
@@ -442,12 +668,14 @@ static int64_t aligned_bytes(int64_t rows, int64_t inner) {
 }
 
 template <typename T>
-static int align_rows(hipStream_t st, const T* a, int64_t lda, int64_t rows, int64_t inner, T* out) {
+static int align_rows(hipStream_t st, const T* a, int64_t lda, int64_t rows, int64_t inner,
+                      void* out) {
   const int64_t per = (inner + 7) / 8, most = ((int64_t(1) << 30) - 1) / per;
   const Divider by((uint32_t)per);
   for (int64_t first = 0; first < rows; first += most) {
     const uint32_t pieces = (uint32_t)(std::min(most, rows - first) * per);
-    k_align_rows<T><<<grid_of(pieces, 256), dim3(256), 0, st>>>(a, lda, inner, by, pieces, first, out);
+    k_align_rows<T><<<grid_of(pieces, 256), dim3(256), 0, st>>>(a, lda, inner, by, pieces, first,
+                                                                (T*)out);
     if (int rc = launched("k_align_rows")) return rc;
   }
   return PURIN_CP_OK;

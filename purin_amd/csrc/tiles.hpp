@@ -146,6 +146,7 @@ using std::integral_constant;
 constexpr integral_constant<int, 1> i1;
 constexpr integral_constant<int, 2> i2;
 constexpr integral_constant<int, 4> i4;
+constexpr integral_constant<int, 16> i16;
 constexpr integral_constant<int, 32> i32;
 constexpr integral_constant<int, 64> i64;
 constexpr integral_constant<int, 128> i128;
@@ -167,6 +168,11 @@ template <typename T>
 static int join(hipStream_t st, const float* parts, int splits, int64_t count, T* out) {
   k_join<T><<<grid_of(count, 1024), dim3(256), 0, st>>>(parts, splits, count, out);
   return launched("k_join");
+}
+
+// Whether a weight is read along inner (a length of one has any stride); along outer otherwise.
+static bool along_inner(int64_t inner, int64_t wi, int64_t wo) {
+  return wo != 1 && (wi == 1 || inner <= 1);
 }
 
 // 32-bit sums of the parts, where a product is split.
