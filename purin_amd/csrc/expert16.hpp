@@ -8,7 +8,8 @@
 // (ds_read_b64_tr_b16: 16 lanes read a 4 x 16 block and get its columns).  Both are stored in
 // 16-byte pieces whose places are exchanged by an XOR, which spreads the lanes of one read over
 // the banks:
-//   [i][k]   piece k / 8 of row i at (k / 8) ^ (i % 8): 8 rows' reads of one piece fall on 8 places
+//   [i][k]   piece k / 8 of row i at (k / 8) ^ (i / 2 % 8): two rows cover the banks, and a read of
+//            one piece falls on 16 places from any 16 rows that 8 such pairs make up
 //   [k][i]   pair i / 16 of row k at (i / 16) ^ s(k), s(k) = 2 (k % 4) + (k / 8) % 2 (2 ((k / 2) % 2)
 //            in rows of 64, two of which cover the banks): the 8 blocks of 32 bytes that half a
 //            wavefront reads at once fall on 8 places
@@ -86,7 +87,7 @@ struct Layout16 {
     const int at = m * THREADS + (int)threadIdx.x;
     if constexpr (ALONG) {
       row = at >> 3;
-      first = ((at & 7) ^ (row & 7)) * 8;
+      first = ((at & 7) ^ ((row >> 1) & 7)) * 8;
     } else {
       constexpr int per = N / 8;
       row = at / per;
@@ -155,7 +156,8 @@ __device__ __forceinline__ S8 fragment(const T* lds, int i0, int s) {
   const int lane = threadIdx.x & 63;
   if constexpr (ALONG) {
     const int i = i0 + (lane & 31);
-    return *reinterpret_cast<const S8*>(lds + i * kDepth16 + (((2 * s + (lane >> 5)) ^ (lane & 7)) << 3));
+    return *reinterpret_cast<const S8*>(lds + i * kDepth16 +
+                                        (((2 * s + (lane >> 5)) ^ ((lane >> 1) & 7)) << 3));
   } else {
     const int k4 = 8 * (lane >> 5) + ((lane & 15) >> 2);  // the places repeat after 16
     const int k = 16 * s + k4;

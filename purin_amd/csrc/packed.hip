@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256, 2) void k_product_packed_thin(
   }
 }
 
-template <typename C, int B, int WN, int S>
+template <typename C, int B, int WN, bool CHUNKS>
 __global__ __launch_bounds__(2 * WN * 64) void k_product_both(
     const uint8_t* __restrict__ a, const uint8_t* __restrict__ a_scales,
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
@@ -105,8 +105,8 @@ __global__ __launch_bounds__(2 * WN * 64) void k_product_both(
     zero_tile(c, ldo, m, n);
     return;
   }
-  TileBoth<C, B, B, 2, WN, S>::run(Codes(a, a_scales, from, inner), m,
-                                   Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
+  TileBoth<C, B, B, 2, WN, CHUNKS>::run(Codes(a, a_scales, from, inner), m,
+                                        Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
 }
 
 enum ShapePacked { kThinPacked, k128Packed, k256Packed };
@@ -175,17 +175,25 @@ static int product_both(hipStream_t st, int64_t rows, int64_t inner, int64_t out
                         const uint8_t* a, const uint8_t* a_scales, const uint8_t* codes,
                         const uint8_t* scales, const int32_t* offsets, C* out, int64_t ldo) {
   const CutPacked cut = cut_packed(true, rows, inner, outer, experts);
-  auto go = [&](auto bm, auto wn, auto s) {
-    constexpr int B = bm, WN = wn, S = s;
+  auto go = [&](auto bm, auto wn) {
+    constexpr int B = bm, WN = wn;
     const int64_t tm = most_tiles(rows, experts, B), tn = (outer + B - 1) / B;
-    return launch16("k_product_both", k_product_both<C, B, WN, S>, tm * tn, 1, 1, 2 * WN * 64,
-                    TileBoth<C, B, B, 2, WN, S>::kLds, st, a, a_scales, codes, scales, rows, inner,
-                    outer, (int)experts, tm, tn, offsets, out, ldo);
+    auto run = [&](auto chunks) {
+      using Tile = TileBoth<C, B, B, 2, WN, chunks>;
+      return launch16("k_product_both", k_product_both<C, B, WN, chunks>, tm * tn, 1, 1, 2 * WN * 64,
+                      Tile::kLds, st, a, a_scales, codes, scales, rows, inner, outer, (int)experts, tm,
+                      tn, offsets, out, ldo);
+    };
+    // whole pieces of 16 bytes of a row's scales
+    const bool chunks = micro_filled(micro_blocks(inner)) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(scales) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(a_scales) % 16 == 0;
+    return chunks ? run(std::true_type{}) : run(std::false_type{});
   };
   // a tile of 256 x 256 sums in 32 bits does not fit LDS on its way out
   if constexpr (sizeof(C) == 2)
-    if (cut.shape == k256Packed) return go(i256, i4, i2);
-  return go(i128, i2, i2);
+    if (cut.shape == k256Packed) return go(i256, i4);
+  return go(i128, i2);
 }
 
 static int check_packed(int32_t dtype, int32_t both, int64_t rows, int64_t inner, int64_t outer,

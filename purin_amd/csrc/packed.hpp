@@ -12,6 +12,8 @@
 // (v_mfma_scale, 32 x 32 x 64), at four times the rate of 16 bits.
 #pragma once
 
+#include <type_traits>
+
 #include "expert16.hpp"
 #include "micro.hpp"
 
@@ -54,18 +56,18 @@ __device__ __forceinline__ float scale_of(uint32_t word, int block) {
   return scale_operand((word >> (8 * (block & 3))) & 255u);
 }
 
-// A stage of N rows, PIECES pieces of 16 bytes each, in LDS [row][piece] with the pieces of a row
-// exchanged by the row's number, so that a read of one piece from neighbouring rows falls on
-// different banks.
+// A stage of N rows, PIECES pieces of 16 bytes each, in LDS [row][piece].  The pieces of the rows
+// that cover the banks together (256 bytes) are exchanged by those rows' number, so that a read of
+// one piece from any 16 rows of 16 such sets, as the hardware takes them, falls on different banks.
 template <int N, int PIECES, int THREADS>
 struct PieceStage {
   static constexpr int kMine = N * PIECES / THREADS;
   static constexpr int kBytes = N * PIECES * 16;
   static_assert(N * PIECES % THREADS == 0, "whole pieces per thread");
 
+  static_assert(PIECES <= 16, "a row is no longer than the banks");
   static __device__ __forceinline__ int place(int row, int piece) {
-    if constexpr (PIECES >= 8) return row * PIECES + (piece ^ (row & 7));
-    else return row * PIECES + (piece ^ ((row >> 3) & (PIECES - 1)));
+    return row * PIECES + (piece ^ ((row * PIECES / 16) & (PIECES - 1)));
   }
   // byte offsets of this thread's pieces; ``offset(row)``: the row's, kOutside for none
   template <typename F>
@@ -132,8 +134,44 @@ struct ScaleStage {
   }
 };
 
+// The scales of N rows for 32 blocks (four stages of 256) at a time, two pieces of 16 bytes a row, in
+// LDS [piece][row]; two such chunks.  A load of scales takes a line of the cache a row, however
+// little of it is wanted: with a word of four blocks for each half stage the scales brought as much
+// from L2 to L1 as the codes.  Rows have whole pieces (words % 4 == 0).
+template <int N, int THREADS>
+struct ScaleChunks {
+  static constexpr int kBytes = 2 * N * 32;
+  static_assert(N % THREADS == 0 || THREADS % N == 0, "whole rows per load");
+  static constexpr int kMine = N / THREADS > 0 ? N / THREADS : 1;
+
+  template <typename F>
+  static __device__ __forceinline__ void offsets(F&& offset, uint32_t (&off)[kMine]) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) off[m] = offset((m * THREADS + (int)threadIdx.x) % N);
+  }
+  // piece number 2 ``chunk`` + ``piece`` of the rows, of ``pieces``
+  static __device__ __forceinline__ void load(const uint8_t* p, const uint32_t (&off)[kMine], int chunk,
+                                              int piece, int pieces, uint32_t lds) {
+    const U4 r = buffer_at(p);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int at = 2 * chunk + piece;
+    const uint32_t to = lds + (uint32_t)((chunk & 1) * N * 32 + piece * N * 16);
+#pragma unroll
+    for (int m = 0; m < kMine; ++m)
+      if (N >= THREADS || wave * 64 < N)
+        load_to_lds(r, at < pieces && off[m] != kOutside ? off[m] + (uint32_t)at * 16u : kOutside,
+                    to + (uint32_t)(m * THREADS + wave * 64) * 16u);
+  }
+  // the two words of stage ``t``
+  static __device__ __forceinline__ uint2 at(const uint8_t* lds, int row, int64_t t) {
+    return *reinterpret_cast<const uint2*>(lds + (((int)t >> 2) & 1) * N * 32 +
+                                           (((int)t & 3) >> 1) * N * 16 + row * 16 + ((int)t & 1) * 8);
+  }
+};
+
 // ``steps`` stages in a ring of S places of ``bytes``: S - 1 on their way while one is
-// multiplied.  load(number, place) issues exactly LOADS loads a wavefront, also past the end.
+// multiplied.  load(number, place) issues exactly LOADS loads a wavefront, also past the end (more
+// in some stages only make the waits longer).
 template <int S, int LOADS, typename L, typename F>
 __device__ __forceinline__ void ring(int64_t steps, L&& load, F&& multiply) {
 #pragma unroll
@@ -237,18 +275,23 @@ struct TileHalf {
   }
 };
 
-// A workgroup's BM x BN tile from packed rows; sums are written as C.
-template <typename C, int BM, int BN, int WM, int WN, int S>
+// A workgroup's BM x BN tile from packed rows; sums are written as C.  CHUNKS: scales by
+// ScaleChunks, for rows that have whole pieces of them.  Two stages of 256 (of 128 in four places
+// the half lines cost more than the deeper ring gives: 32768 rows, 16 experts, 2048 x 4096 233 us,
+// 248).  256 x 256 tiles: 128 x 256 and 128 x 128 ones, two workgroups a CU, read more from L2 than
+// their overlap gives (320, 290).
+template <typename C, int BM, int BN, int WM, int WN, bool CHUNKS>
 struct TileBoth {
   static constexpr int THREADS = WM * WN * 64, X = BM / WM / 32, Y = BN / WN / 32;
   using SA = PieceStage<BM, 8, THREADS>;  // a depth of 256
   using SB = PieceStage<BN, 8, THREADS>;
-  using CA = ScaleStage<BM, 2, THREADS>;
-  using CB = ScaleStage<BN, 2, THREADS>;
-  static constexpr int kStage = SA::kBytes + SB::kBytes + CA::kBytes + CB::kBytes;
-  static constexpr int kLoads = SA::kMine + SB::kMine + CA::kMine + CB::kMine;
+  using CA = std::conditional_t<CHUNKS, ScaleChunks<BM, THREADS>, ScaleStage<BM, 2, THREADS>>;
+  using CB = std::conditional_t<CHUNKS, ScaleChunks<BN, THREADS>, ScaleStage<BN, 2, THREADS>>;
+  static constexpr int kScales = CA::kBytes + CB::kBytes;
+  static constexpr int kStage = SA::kBytes + SB::kBytes + (CHUNKS ? 0 : kScales);
   static constexpr int kOut = BM * BN * (int)sizeof(C);
-  static constexpr int kLds = S * kStage > kOut ? S * kStage : kOut;
+  static constexpr int kRing = 2 * kStage + (CHUNKS ? kScales : 0);
+  static constexpr int kLds = kRing > kOut ? kRing : kOut;
 
   static __device__ __forceinline__ void run(const Codes& a, int m, const Codes& b, int n,
                                              unsigned char* lds, C* c, int64_t ldc) {
@@ -270,28 +313,51 @@ struct TileBoth {
     const uint8_t *pa = uniform(a.codes), *pb = uniform(b.codes), *sa = uniform(a.scales),
                   *sb = uniform(b.scales);
     const uint32_t base = lds_address(lds);
-    ring<S, kLoads>(
+    auto load_chunk = [&](int chunk, int piece) {
+      if constexpr (CHUNKS) {
+        CA::load(sa, off_ca, chunk, piece, b.words / 4, base + 2 * kStage);
+        CB::load(sb, off_cb, chunk, piece, b.words / 4, base + 2 * kStage + CA::kBytes);
+      }
+    };
+    load_chunk(0, 0);
+    load_chunk(0, 1);
+    ring<2, 0>(
         (b.blocks + 7) / 8,
         [&](int64_t t, int at) {
           const uint32_t to = base + (uint32_t)(at * kStage);
           SA::load(pa + t * 128, off_a, b.blocks - 8 * t, to);
           SB::load(pb + t * 128, off_b, b.blocks - 8 * t, to + SA::kBytes);
-          CA::load(sa, off_ca, (int)(2 * t), b.words, to + SA::kBytes + SB::kBytes);
-          CB::load(sb, off_cb, (int)(2 * t), b.words, to + SA::kBytes + SB::kBytes + CA::kBytes);
+          if constexpr (CHUNKS) {
+            // the next chunk's, whose place the last chunk but one has left
+            if ((t & 3) >= 2) load_chunk((int)(t >> 2) + 1, (int)(t & 1));
+          } else {
+            CA::load(sa, off_ca, (int)(2 * t), b.words, to + SA::kBytes + SB::kBytes);
+            CB::load(sb, off_cb, (int)(2 * t), b.words, to + SA::kBytes + SB::kBytes + CA::kBytes);
+          }
         },
         [&](int64_t t, int at) {
           const uint8_t* la = lds + at * kStage;
-          const uint8_t *lb = la + SA::kBytes, *ca = lb + SB::kBytes, *cb = ca + CA::kBytes;
+          const uint8_t* lb = la + SA::kBytes;
+          const uint8_t* ca = CHUNKS ? lds + 2 * kStage : lb + SB::kBytes;
+          const uint8_t* cb = ca + CA::kBytes;
+          auto words = [&](auto side, const uint8_t* from, int row) {
+            using S = decltype(side);
+            if constexpr (CHUNKS) return S::at(from, row, t);
+            else return uint2{S::at(from, row, 0), S::at(from, row, 1)};
+          };
+          uint2 wa[X], wb[Y];
+#pragma unroll
+          for (int x = 0; x < X; ++x) wa[x] = words(CA{}, ca, wi + 32 * x + (lane & 31));
+#pragma unroll
+          for (int y = 0; y < Y; ++y) wb[y] = words(CB{}, cb, wj + 32 * y + (lane & 31));
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             // the scales of blocks 4 q + half and 4 q + 2 + half in bytes 0 and 2
             int ka[X], kb[Y];
 #pragma unroll
-            for (int x = 0; x < X; ++x)
-              ka[x] = (int)(CA::at(ca, wi + 32 * x + (lane & 31), q) >> (8 * half));
+            for (int x = 0; x < X; ++x) ka[x] = (int)((q ? wa[x].y : wa[x].x) >> (8 * half));
 #pragma unroll
-            for (int y = 0; y < Y; ++y)
-              kb[y] = (int)(CB::at(cb, wj + 32 * y + (lane & 31), q) >> (8 * half));
+            for (int y = 0; y < Y; ++y) kb[y] = (int)((q ? wb[y].y : wb[y].x) >> (8 * half));
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
               I8 fa[X], fb[Y];
