@@ -3,9 +3,10 @@
 //   out(t) = sum over t's experts e of  w(t, e) f(x(t) A[e]) B[e]
 //
 // Every weight of an expert that some token has is read once: that is the work, and the tokens'
-// rows are few beside it.  Four launches:
+// rows are few beside it.  Three launches, or four:
 //   choose  one workgroup chooses the tokens' experts and sorts the pairs (token, slot) by expert;
-//           the others lay out x as the products read it, where it is not so already;
+//           the others lay out x as the products read it, where it is not so already.  With few
+//           pairs the next launch's workgroups do it themselves;
 //   up      a workgroup has one expert and 64 columns of A: multiplies its tokens' rows, applies f
 //           and the token's weight.  The results keep twice the type's digits, as the sum of two
 //           numbers of the type, so that they take part in the second product as they are;
@@ -275,7 +276,7 @@ template <typename K, int G, int V>
 __device__ __forceinline__ void choose_tokens(const void* weights, int32_t wdtype, int64_t ldw,
                                               int tokens, int experts, int slots, int32_t* ids,
                                               K* chosen) {
-  for (int t = threadIdx.x / G; t < tokens; t += 1024 / G)
+  for (int t = threadIdx.x / G; t < tokens; t += blockDim.x / G)
     choose<K, G, V>(AnyRow<K>{weights, wdtype, t * ldw}, experts, slots, (int)threadIdx.x % G,
                     ids + t * slots, chosen + t * slots);
 }
@@ -348,6 +349,66 @@ struct Choose {
   void* to;
 };
 
+// Few pairs: every workgroup of the first product makes the plan for itself, in LDS, which takes
+// less than a launch (one token, 8 of 64 experts: 5.7 us for the launch, 2 here).
+constexpr int kOwnPairs = 128, kOwnTokens = 16, kOwnExperts = 256;
+struct OwnPlan {
+  int32_t groups;
+  int32_t expert[kOwnPairs], start[kOwnPairs + 1], order[kOwnPairs];
+  float weight[kOwnPairs], chosen[kOwnPairs];
+  alignas(16) int32_t ids[kOwnPairs], first[kOwnPairs];  // first: an expert's first pair has it
+};
+__device__ __forceinline__ void make_own_plan(const Choose& p, OwnPlan& own, Plan* plan) {
+  const int tid = threadIdx.x, pairs = p.tokens * p.slots;
+  if (p.experts <= 64)
+    choose_tokens<float, 16, 4>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, own.ids,
+                                own.chosen);
+  else
+    choose_tokens<float, 16, 16>(p.weights, p.wdtype, p.ldw, p.tokens, p.experts, p.slots, own.ids,
+                                 own.chosen);
+  if (tid >= pairs && tid < kOwnPairs) own.ids[tid] = -1;
+  __syncthreads();
+  // four pairs to a read, so that few of their latencies are in a row
+  const int fours = (pairs + 3) / 4;
+  int e = -1, below = 0, before = 0, all = 0;
+  if (tid < kOwnPairs) {
+    e = own.ids[tid];
+#pragma unroll 4
+    for (int q = 0; q < fours; ++q) {
+      const int4 v = reinterpret_cast<const int4*>(own.ids)[q];
+      all += (v.x >= 0) + (v.y >= 0) + (v.z >= 0) + (v.w >= 0);
+      below += (uint32_t(v.x) < uint32_t(e)) + (uint32_t(v.y) < uint32_t(e)) +
+               (uint32_t(v.z) < uint32_t(e)) + (uint32_t(v.w) < uint32_t(e));
+      before += (v.x == e && 4 * q < tid) + (v.y == e && 4 * q + 1 < tid) +
+                (v.z == e && 4 * q + 2 < tid) + (v.w == e && 4 * q + 3 < tid);
+    }
+    own.first[tid] = e >= 0 && before == 0 ? e : -1;
+  }
+  __syncthreads();
+  const bool writes = blockIdx.x == 0;  // for the later launches
+  if (tid < pairs) {
+    int group = 0, groups = 0;
+#pragma unroll 4
+    for (int q = 0; q < fours; ++q) {
+      const int4 v = reinterpret_cast<const int4*>(own.first)[q];
+      groups += (v.x >= 0) + (v.y >= 0) + (v.z >= 0) + (v.w >= 0);
+      group += (uint32_t(v.x) < uint32_t(e)) + (uint32_t(v.y) < uint32_t(e)) +
+               (uint32_t(v.z) < uint32_t(e)) + (uint32_t(v.w) < uint32_t(e));
+    }
+    const bool first = own.first[tid] >= 0;
+    const int place = e >= 0 ? below + before : -1;
+    if (e >= 0) own.order[place] = tid, own.weight[place] = own.chosen[tid];
+    if (first) own.expert[group] = e, own.start[group] = below;
+    if (tid == 0) own.groups = groups, own.start[groups] = all;
+    if (writes) {
+      plan->place[tid] = place;
+      if (first) plan->expert[group] = e, plan->start[group] = below;
+      if (tid == 0) plan->groups = groups, plan->start[groups] = all;
+    }
+  }
+  __syncthreads();
+}
+
 template <typename T, typename K>
 __global__ __launch_bounds__(1024) void k_layer_choose(Choose p, Plan* __restrict__ plan) {
   if (blockIdx.x) {
@@ -407,35 +468,46 @@ struct Up {
   int32_t slots, act, gated, parts;
   int64_t width, hidden, tiles;
   Rows x;
-  uint32_t pitch;  // bytes of a hidden row; they are in order of places
+  uint32_t step, pitch;  // of the hidden rows, by place
 };
 
 // Workgroup: group number blockIdx.x / tiles, columns of tile blockIdx.x % tiles.
-template <typename T, int BM, typename Core>
-__global__ __launch_bounds__(256, 2) void k_layer_up(
-    Up p, Matrices w, const Plan* __restrict__ plan, uint8_t* __restrict__ high,
-    uint8_t* __restrict__ low) {
+template <typename T, int BM, typename Core, bool OWN>
+__global__ __launch_bounds__(256, 2) void k_layer_up(Up p, Choose choose, Matrices w, Plan* plan,
+                                                     uint8_t* __restrict__ high,
+                                                     uint8_t* __restrict__ low) {
   extern __shared__ __align__(16) unsigned char lds16[];
+  __shared__ std::conditional_t<OWN, OwnPlan, int> made;
+  const auto& from = [&]() -> const auto& {
+    if constexpr (OWN) {
+      make_own_plan(choose, made, plan);
+      return made;
+    } else {
+      return *plan;
+    }
+  }();
   const int tid = threadIdx.x;
   int at, tile;
-  if (!find_item(p.tiles, plan->groups, at, tile)) return;
-  const int e = plan->expert[at], start = plan->start[at], count = plan->start[at + 1] - start;
+  if (!find_item(p.tiles, from.groups, at, tile)) return;
+  const int e = __builtin_amdgcn_readfirstlane(from.expert[at]);
+  const int start = __builtin_amdgcn_readfirstlane(from.start[at]);
+  const int count = __builtin_amdgcn_readfirstlane(from.start[at + 1]) - start;
   const int parts = Core::kStreams ? p.parts : 4, wide = p.gated ? 32 : 64;
   const int64_t col = (int64_t)tile * (4 / parts) * wide;
   const Share own = share_columns(tile, parts, wide, p.hidden, p.gated);
   for (int r0 = 0; r0 < count; r0 += BM) {
     const Rows a[1] = {p.x};
-    Core::run(a, [&](int r) { return r0 + r < count ? plan->order[start + r0 + r] / p.slots : -1; },
+    Core::run(a, [&](int r) { return r0 + r < count ? from.order[start + r0 + r] / p.slots : -1; },
               p.hidden ? p.width : 0, w, e, p.gated ? 2 * p.hidden : p.hidden, own.c, own.part, parts,
               lds16);
     const float* sums = reinterpret_cast<const float*>(lds16);
     const int rows = min(BM, count - r0);
     const int per = 4 / parts * (wide / 8);  // pieces of a row
     for (int i = tid; i < rows * per; i += 256) {
-      const int r = i / per, j = i % per * 8, place = start + r0 + r;
+      const int r = i % rows, j = i / rows * 8, place = start + r0 + r;
       if (col + j >= p.hidden) continue;
       const int at = p.gated ? (j >> 5 << 6) + (j & 31) : j;  // of the sums
-      const float weight = plan->weight[place];
+      const float weight = from.weight[place];
       Pack<T> hi, lo;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
@@ -446,7 +518,7 @@ __global__ __launch_bounds__(256, 2) void k_layer_up(
         const float rest = h - (float)hi.v[q];
         lo.v[q] = (T)(fabsf((float)hi.v[q]) < __builtin_inff() ? rest : 0.0f);
       }
-      const int64_t to = (col + j) * 2 + (int64_t)place * p.pitch;
+      const int64_t to = (col + j) / 8 * p.step + (int64_t)place * p.pitch;
       store16(reinterpret_cast<T*>(high + to), hi);
       store16(reinterpret_cast<T*>(low + to), lo);
     }
@@ -456,7 +528,7 @@ __global__ __launch_bounds__(256, 2) void k_layer_up(
 
 struct Down {
   int64_t hidden, outer, tiles;
-  uint32_t pitch;
+  uint32_t step, pitch;
   int32_t parts;
 };
 
@@ -474,7 +546,7 @@ __global__ __launch_bounds__(256, 2) void k_layer_down(
   const Share own = share_columns(tile, parts, 64, p.outer, false);
   const int n = (int)min<int64_t>(wide, p.outer - col);
   for (int r0 = 0; r0 < count; r0 += BM) {
-    const Rows a[2] = {{high, 16u, p.pitch}, {low, 16u, p.pitch}};
+    const Rows a[2] = {{high, p.step, p.pitch}, {low, p.step, p.pitch}};
     Core::run(a, [&](int r) { return r0 + r < count ? start + r0 + r : -1; }, p.hidden, w, e, p.outer,
               own.c, own.part, parts, lds16);
     const float* sums = reinterpret_cast<const float*>(lds16);
@@ -574,7 +646,9 @@ static int layer(hipStream_t st, const Shape& s, const void* weights, int32_t wd
   const Reading how_a = reading(inner, s.width, s.gated ? 2 * s.hidden : s.hidden, s.hidden, &a.ld);
   const Reading how_b = reading(outer, s.hidden, s.outer, 8, &b.ld);
 
-  const uint32_t pitch = (uint32_t)(at.pieces * 16);
+  // hidden rows: side by side where the second product streams, else each in one piece
+  const bool side = how_b <= kAlongDirect;
+  const uint32_t step = side ? (uint32_t)pairs * 16u : 16u, pitch = side ? 16u : (uint32_t)(at.pieces * 16);
   // streams of 64 columns, and the workgroups' tiles of them
   const int64_t wide = s.gated ? 32 : 64, streams_a = std::max<int64_t>(1, (s.hidden + wide - 1) / wide);
   const int64_t streams_b = (s.outer + 63) / 64;
@@ -582,7 +656,7 @@ static int layer(hipStream_t st, const Shape& s, const void* weights, int32_t wd
   const int parts_b = how_b <= kAlongDirect ? stream_parts(groups * streams_b) : 4;
   auto tiles = [](int64_t streams, int parts) { return (streams * parts + 3) / 4; };
   Up up{(int32_t)s.slots, s.act, s.gated, parts_a, s.width, s.hidden, tiles(streams_a, parts_a),
-        {x, 16u, (uint32_t)(ldx * 2)}, pitch};
+        {x, 16u, (uint32_t)(ldx * 2)}, step, pitch};
   Choose choose{weights, ldw, wdtype, (int32_t)s.tokens, (int32_t)s.experts, (int32_t)s.slots, x, ldx,
                 s.width, nullptr};
   int64_t moves = 0;
@@ -593,23 +667,31 @@ static int layer(hipStream_t st, const Shape& s, const void* weights, int32_t wd
     up.x = {choose.to, 16u, (uint32_t)pieces * 16u};
     moves = (pieces * s.tokens + 1023) / 1024;
   }
-  const dim3 grid((unsigned)(1 + moves));
-  if (wdtype == PURIN_TRAIN_F64)
-    k_layer_choose<T, double><<<grid, dim3(1024), 0, st>>>(choose, plan);
-  else
-    k_layer_choose<T, float><<<grid, dim3(1024), 0, st>>>(choose, plan);
-  if (int rc = launched("k_layer_choose")) return rc;
+  const bool own = s.tokens <= kOwnTokens && pairs <= kOwnPairs && s.experts <= kOwnExperts &&
+                   !moves && wdtype != PURIN_TRAIN_F64;
+  if (!own) {
+    const dim3 grid((unsigned)(1 + moves));
+    if (wdtype == PURIN_TRAIN_F64)
+      k_layer_choose<T, double><<<grid, dim3(1024), 0, st>>>(choose, plan);
+    else
+      k_layer_choose<T, float><<<grid, dim3(1024), 0, st>>>(choose, plan);
+    if (int rc = launched("k_layer_choose")) return rc;
+  }
 
   // rows of a tile; an expert with more reads its weights again
   const int height = pairs <= 6 * s.experts || s.tokens <= 16 ? 16
                      : pairs <= 16 * s.experts || s.tokens <= 32 ? 32 : 64;
   if (int rc = by_reading<T, 1>(how_a, height, [&](auto bm, auto core) {
         using Core = decltype(core);
-        return launch16("k_layer_up", k_layer_up<T, bm, Core>, (groups * up.tiles + 7) / 8 * 8, 1, 1,
-                        256, layer_lds<bm, Core>(), st, up, a, (const Plan*)plan, high, low);
+        auto kernel = k_layer_up<T, bm, Core, false>;
+        // as few tokens have tiles of few rows
+        if constexpr (bm == (Core::kStreams ? 16 : 32))
+          if (own) kernel = k_layer_up<T, bm, Core, true>;
+        return launch16("k_layer_up", kernel, (groups * up.tiles + 7) / 8 * 8, 1, 1, 256,
+                        layer_lds<bm, Core>(), st, up, choose, a, plan, high, low);
       }))
     return rc;
-  const Down down{s.hidden, s.outer, tiles(streams_b, parts_b), pitch, parts_b};
+  const Down down{s.hidden, s.outer, tiles(streams_b, parts_b), step, pitch, parts_b};
   if (int rc = by_reading<T, 2>(how_b, height, [&](auto bm, auto core) {
         using Core = decltype(core);
         return launch16("k_layer_down", k_layer_down<T, bm, Core>, (groups * down.tiles + 7) / 8 * 8, 1,

@@ -135,9 +135,10 @@ static int product_packed(hipStream_t st, int64_t rows, int64_t inner, int64_t o
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
   if (cut.shape == kThinPacked) {
     Rows from{a, 16u, (uint32_t)lda * 2u};
-    if (inner && !direct_ok(a, lda, inner)) {
-      if (int rc = align_rows<T>(st, a, lda, rows, inner, ws)) return rc;
-      from = {ws, 16u, (uint32_t)((inner + 7) / 8) * 16u};
+    // many rows to an expert are worth a launch that lays them side by side
+    if (inner && (rows > 4 * experts || !direct_ok(a, lda, inner))) {
+      if (int rc = turn_rows<T>(st, a, lda, rows, inner, ws)) return rc;
+      from = {ws, (uint32_t)rows * 16u, 16u};
     }
     float* parts = (float*)(ws + aligned_bytes(rows, inner));
     const int wide = 64 * (4 / cut.parts);

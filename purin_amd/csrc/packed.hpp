@@ -400,7 +400,9 @@ struct TileBoth {
 // 4096 x 2816 in 4 bits 112 us.)
 // NA: the rows are the sum of that many arrays.
 
-// Rows of 16 bits in pieces of 8: piece k of row r at p + k * step + r * pitch bytes.
+// Rows of 16 bits in pieces of 8: piece k of row r at p + k * step + r * pitch bytes.  A load of
+// one piece of 16 rows takes a cycle a row where each is in one piece (step 16), and one for four
+// where rows lie side by side (pitch 16).
 struct Rows {
   const void* p;
   uint32_t step, pitch;
@@ -727,6 +729,33 @@ static __global__ __launch_bounds__(256) void k_align_rows(const T* __restrict__
   }
 }
 
+// The same side by side: piece k of row r at out + (k * rows + r) * 16 bytes.  A workgroup turns 32
+// rows by 16 pieces, through LDS: small tiles, so that few rows fill the card (768 rows of 4096:
+// 64 by 32 7.7 us).
+template <typename T>
+static __global__ __launch_bounds__(256) void k_turn_rows(const T* __restrict__ a, int64_t lda,
+                                                          int64_t inner, int64_t rows,
+                                                          int64_t tiles, uint8_t* __restrict__ out) {
+  __shared__ __align__(16) uint8_t lds[32 * 16 * 16];
+  const int64_t pieces = (inner + 7) / 8;
+  const int64_t row = blockIdx.x / tiles * 32, piece = blockIdx.x % tiles * 16;
+#pragma unroll
+  for (int i = threadIdx.x; i < 32 * 16; i += 256) {
+    const int r = i >> 4, k = i & 15;
+    if (row + r < rows && piece + k < pieces)
+      *reinterpret_cast<S8*>(lds + (r * 16 + (k ^ (r & 15))) * 16) = __builtin_bit_cast(
+          S8, load_upto(a + (row + r) * lda + (piece + k) * 8, inner - (piece + k) * 8));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = threadIdx.x; i < 32 * 16; i += 256) {
+    const int k = i >> 5, r = i & 31;
+    if (row + r < rows && piece + k < pieces)
+      *reinterpret_cast<S8*>(out + ((piece + k) * rows + row + r) * 16) =
+          *reinterpret_cast<const S8*>(lds + (r * 16 + (k ^ (r & 15))) * 16);
+  }
+}
+
 static int64_t whole256(int64_t n) { return (n + 255) / 256 * 256; }
 // Bytes of rows that are aligned for the loads.
 static int64_t aligned_bytes(int64_t rows, int64_t inner) {
@@ -745,6 +774,15 @@ static int align_rows(hipStream_t st, const T* a, int64_t lda, int64_t rows, int
     if (int rc = launched("k_align_rows")) return rc;
   }
   return PURIN_CP_OK;
+}
+
+template <typename T>
+static int turn_rows(hipStream_t st, const T* a, int64_t lda, int64_t rows, int64_t inner, void* out) {
+  const int64_t tiles = (inner + 127) / 128, groups = (rows + 31) / 32 * tiles;
+  if (groups >= (int64_t(1) << 24))  // fewer than 2^32 threads
+    return set_error(PURIN_CP_ERR_UNSUPPORTED, "too many tiles for a launch");
+  k_turn_rows<T><<<dim3((unsigned)groups), dim3(256), 0, st>>>(a, lda, inner, rows, tiles, (uint8_t*)out);
+  return launched("k_turn_rows");
 }
 
 }  // namespace train
