@@ -129,7 +129,7 @@ struct ThinDense {
       // columns that are not there: the first ones again, whose sums are dropped
       const int from = !DIRECT && c.n[y] <= 0 ? 0 : y;
       b[y] = {base + (ALONG ? c.first[from] * w.ld : c.first[from]), w.ld, c.n[from],
-              c.first[from] > 0};
+              c.first[from] >= kVec<T>};
     }
     uint32_t off_a[SA::kMine], off_b[2][SB::kMine];
     SA::offsets(offset, off_a);
@@ -638,6 +638,7 @@ static int layer(hipStream_t st, const Shape& s, const void* weights, int32_t wd
                  const purin_train_matrices& outer, uint8_t* ws, T* out) {
   const LayerSpace at(s.tokens, s.slots, s.width, s.hidden, s.outer);
   const int64_t pairs = s.tokens * s.slots, groups = std::min(s.experts, pairs);
+  if (s.tokens == 1) ldx = 0;  // one row has any pitch
   Plan* plan = (Plan*)(ws + at.plan);
   uint8_t *high = ws + at.high, *low = ws + at.low;
   float* parts = (float*)(ws + at.parts);

@@ -131,6 +131,7 @@ static int product_packed(hipStream_t st, int64_t rows, int64_t inner, int64_t o
                           int64_t experts, const T* a, int64_t lda, const uint8_t* codes,
                           const uint8_t* scales, const int32_t* offsets, uint8_t* ws, T* out,
                           int64_t ldo) {
+  if (rows == 1) lda = 0;  // one row has any pitch
   CutPacked cut = cut_packed(false, rows, inner, outer, experts);
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
   if (cut.shape == kThinPacked) {
