@@ -327,6 +327,7 @@ __device__ __forceinline__ void make_plan(const int32_t* ids, const K* chosen, i
     if (e >= 0) {
       place = first[e];
       const int4* four = reinterpret_cast<const int4*>(ids);
+#pragma unroll 8
       for (int p = 0; p < tid / 4; ++p) {
         const int4 v = four[p];
         place += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
@@ -679,9 +680,11 @@ static int layer(hipStream_t st, const Shape& s, const void* weights, int32_t wd
     if (int rc = launched("k_layer_choose")) return rc;
   }
 
-  // rows of a tile; an expert with more reads its weights again
-  const int height = pairs <= 6 * s.experts || s.tokens <= 16 ? 16
-                     : pairs <= 16 * s.experts || s.tokens <= 32 ? 32 : 64;
+  // Rows of a tile; an expert with more reads its weights again.  64 tokens, 4096 x 1408 gated, us
+  // with 16 | 32 rows: 6 of 64 experts in codes 163 | 188, dense 407 | 413; 6 of 32 127 | 127, 245 |
+  // 224; 6 of 16 100 | 80, 198 | 133.  32 | 64 through LDS: 6 of 16 155 | 159, 4 of 8 111 | 92.
+  const int height = pairs <= 8 * s.experts || s.tokens <= 16 ? 16
+                     : pairs <= 24 * s.experts || s.tokens <= 32 ? 32 : 64;
   if (int rc = by_reading<T, 1>(how_a, height, [&](auto bm, auto core) {
         using Core = decltype(core);
         auto kernel = k_layer_up<T, bm, Core, false>;

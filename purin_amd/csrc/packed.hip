@@ -109,6 +109,16 @@ __global__ __launch_bounds__(2 * WN * 64) void k_product_both(
                                         Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
 }
 
+// How a product is cut.  us of 32 experts, 4096 x 1536, so many rows to each, bf16:
+//   rows     1     8    16    24    32    48    64    96   192   400
+//   16    27.2  28.0  31.0    51    49    67     -     -     -     -   streams, 16 rows to a tile
+//   32    30.1  32.4  36.1  38.8    43    67    74    92   158   270   32 rows
+//   128   54.8  54.8  57.1  58.9    59    89    91    98   129   225   128 x 128 tiles
+//   256     89    85    85    85    86    88    89   169   182   203   256 x 256
+// Streams are bound by memory (27.2 us: 4.1 TB/s) until an expert's rows take a second tile, which
+// reads its weights again.  16 experts, 2048 x 4096, 128 | 256, rows of 16 bits: 8192 rows 167 | 171,
+// 16384 293 | 285, 32768 591 | 522; packed rows 66 | 67, 115 | 111, 234 | 201: from 16 tiles of
+// 128 x 128 to a CU on, as in 16 bits.  Where CUs are idle a stream's contraction is split.
 enum ShapePacked { kThinPacked, k128Packed, k256Packed };
 struct CutPacked {
   ShapePacked shape;
@@ -116,8 +126,8 @@ struct CutPacked {
 };
 static CutPacked cut_packed(bool both, int64_t rows, int64_t inner, int64_t outer, int64_t experts) {
   const int64_t tiles = most_tiles(rows, experts, 128) * ((outer + 127) / 128);
-  if (!both && (rows <= 48 * experts || tiles <= 64)) {
-    const int height = rows <= 8 * experts ? 16 : 32;
+  if (!both && (rows <= 96 * experts || tiles <= 64)) {
+    const int height = rows <= 12 * experts ? 16 : 32;
     const int64_t streams = most_tiles(rows, experts, height) * ((outer + 63) / 64);
     const int parts = stream_parts(streams);
     return {kThinPacked, height, parts,
@@ -136,8 +146,9 @@ static int product_packed(hipStream_t st, int64_t rows, int64_t inner, int64_t o
   if (ldo != outer) cut.splits = 1;  // the parts are added up as one row
   if (cut.shape == kThinPacked) {
     Rows from{a, 16u, (uint32_t)lda * 2u};
-    // many rows to an expert are worth a launch that lays them side by side
-    if (inner && (rows > 4 * experts || !direct_ok(a, lda, inner))) {
+    // rows that fill their tiles are worth a launch that lays them side by side (32 experts, 4096 x
+    // 1536, 48 rows to each: 67 us, 80 without; 24 to each, unequal: 47.6, 51; 16 to each: 34, 31)
+    if (inner && (rows > 16 * experts || !direct_ok(a, lda, inner))) {
       if (int rc = turn_rows<T>(st, a, lda, rows, inner, ws)) return rc;
       from = {ws, (uint32_t)rows * 16u, 16u};
     }
