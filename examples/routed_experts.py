@@ -6,7 +6,10 @@ The projection leaves most weights exactly zero; the tokens with a weight for an
 and back, and the gradients of the weights go on through the projection's implicit VJP to the
 router.  The gradients' global norm is limited before the step.
 
-    python examples/routed_experts.py [--steps N]
+    python examples/routed_experts.py [--steps N] [--saved int8]
+
+With ``--saved int8`` the rows that the backward pass needs are kept in 8 bits.  After the training
+the layer answers for a few tokens at a time with its experts in 4 bits.
 """
 
 from __future__ import annotations
@@ -20,8 +23,8 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from purin_amd import (ChambollePockConfig, clip_gradients, combine, dispatch,  # noqa: E402
-                       expert_product, prepare_projection, route)
+from purin_amd import (ChambollePockConfig, activate, clip_gradients, combine,  # noqa: E402
+                       dispatch, expert_layer, expert_product, pack, prepare_projection, route)
 from purin_amd.problems import CanonicalRows  # noqa: E402
 
 
@@ -41,12 +44,13 @@ def routing_polytope(tokens, experts, capacity):
 
 
 class RoutedExperts(torch.nn.Module):
-    """Two matrices to an expert; ``group`` tokens share each expert's capacity."""
+    """Two matrices to an expert; ``group`` tokens share each expert's capacity.  ``saved``: how
+    the rows are kept for the backward pass."""
 
     def __init__(self, width, hidden, experts, group, groups, slots, slack=1.25,
-                 dtype=torch.float32):
+                 dtype=torch.float32, saved=None):
         super().__init__()
-        self.experts, self.slots = experts, slots
+        self.experts, self.slots, self.saved = experts, slots, saved
         rows = routing_polytope(group, experts, slack * group / experts)
         self.layer = prepare_projection(
             rows, batch_size=groups, dtype=dtype,
@@ -64,17 +68,27 @@ class RoutedExperts(torch.nn.Module):
 
     def forward(self, x):
         routing = route(self.weights(x), self.slots)
-        rows = dispatch(x, routing)
-        rows = torch.relu(expert_product(rows, self.inner, routing))
-        return combine(expert_product(rows, self.outer, routing), routing)
+        rows = expert_product(dispatch(x, routing), self.inner, routing, saved=self.saved)
+        rows = activate(rows, "relu", gated=False, saved=self.saved)
+        return combine(expert_product(rows, self.outer, routing, saved=self.saved), routing)
+
+    @torch.no_grad()
+    def packed(self):
+        """The experts' matrices in 4 bits, for ``serve``."""
+        return tuple(pack(w, "fp4", axis=1) for w in (self.inner, self.outer))
+
+    @torch.no_grad()
+    def serve(self, x, weights, packed):
+        """The layer for a few tokens with their routing weights."""
+        return expert_layer(x.bfloat16(), weights, self.slots, *packed, "relu")
 
 
 def train(steps=50, seed=0, width=64, hidden=128, experts=8, group=32, groups=64, slots=4,
-          largest=1.0, rate=0.2, log=print):
+          largest=1.0, rate=0.2, log=print, saved=None):
     """Losses and gradient norms of ``steps`` steps on tokens from a mixture: each kind of token
     has a linear map of its own to learn."""
     torch.manual_seed(seed)
-    model = RoutedExperts(width, hidden, experts, group, groups, slots)
+    model = RoutedExperts(width, hidden, experts, group, groups, slots, saved=saved)
     parameters = list(model.parameters())
     centres = torch.randn(experts, width, device="cuda")
     maps = torch.randn(experts, width, width, device="cuda") / width ** 0.5
@@ -99,4 +113,11 @@ def train(steps=50, seed=0, width=64, hidden=128, experts=8, group=32, groups=64
 if __name__ == "__main__":
     arguments = argparse.ArgumentParser()
     arguments.add_argument("--steps", type=int, default=50)
-    train(arguments.parse_args().steps)
+    arguments.add_argument("--saved", choices=["int8"], default=None)
+    arguments = arguments.parse_args()
+    *_, model = train(arguments.steps, saved=arguments.saved)
+    x = torch.randn(model.layer.batch_size * 32, model.router.shape[0], device="cuda")
+    with torch.no_grad():
+        want, weights, packed = model(x)[:8], model.weights(x)[:8], model.packed()
+    off = (model.serve(x[:8], weights, packed) - want).norm() / want.norm()
+    print(f"8 tokens with the experts in 4 bits: {float(off):.3f} from the layer in 32")

@@ -33,7 +33,8 @@ def activate(rows, kind="silu", *, gated=True, saved=None):
     ``kind``: "relu", "silu" (u / (1 + exp(-u))) or "gelu" (u times the share of a normal
     distribution below u).  ``saved="int8"``: what a graph keeps of the rows is held in 8 bits (each
     half as ``pack(half, "int8")``, made on the way), and the gradient is at the rows which those
-    stand for.  Not for float64.
+    stand for: relu's slope is 0 where a positive number is nearer to zero than half a 64th of its
+    block's power of two, about one in eighty of normal ones.  Not for float64.
     """
     code, keep = _activation(kind), kept(saved)
     try:

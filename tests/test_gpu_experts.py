@@ -142,7 +142,7 @@ PRODUCTS = [((1, 0), 1, 1), ((0, 0, 0, 5), 8, 8), ((8, 0), 64, 64), ((1, 0, 2, 1
             ((3, 130, 0, 17, 2), 37, 53), ((128, 256, 64, 0), 64, 128), ((129, 1, 0, 300, 9), 200, 136),
             ((16,) * 12 + (0,), 256, 192), ((5,) * 70 + (3,), 33, 40), ((600, 40, 0), 136, 264),
             ((1,) * 3 + (0,), 2048, 72), ((2, 1, 4, 0), 72, 1408), ((40, 33, 70, 1), 1032, 2048),
-            ((300, 260), 260, 4100)]
+            ((300, 260), 260, 4100), ((2,) * 40 + (0,), 64, 2600), ((1,) * 100 + (0,), 40, 2700)]
 
 
 def _packed_weight(torch, seed, shape, dtype):
@@ -452,7 +452,13 @@ def test_activation_of_far_values():
 # tokens, experts, slots, width, hidden, outer width
 LAYERS = [(1, 1, 1, 1, 1, 1), (1, 8, 3, 64, 32, 64), (3, 5, 5, 37, 19, 53), (1, 70, 6, 264, 72, 136),
           (17, 9, 2, 128, 40, 72), (33, 6, 3, 96, 64, 200), (64, 4, 2, 72, 136, 64),
-          (64, 300, 8, 40, 24, 33), (40, 40, 3, 520, 200, 65), (2, 1024, 9, 33, 8, 16)]
+          (64, 300, 8, 40, 24, 33), (40, 40, 3, 520, 200, 65), (2, 1024, 9, 33, 8, 16),
+          # on both sides of where a launch of its own chooses
+          (16, 256, 8, 64, 32, 64), (16, 257, 8, 64, 32, 64), (17, 20, 3, 64, 32, 64),
+          (13, 40, 10, 64, 40, 72),
+          # the most pairs; more rows to an expert than a tile has; wide ones, which share less
+          (64, 16, 16, 64, 32, 40), (64, 2, 2, 256, 96, 128), (24, 64, 4, 72, 48, 4104),
+          (24, 64, 4, 40, 1560, 24)]
 
 
 def _layer_weights(torch, packed, order, gated, shape, t):
@@ -606,6 +612,87 @@ def test_layer_as_separate_operators(dtype):
         assert torch.equal(got, other)
     with torch.no_grad():
         assert torch.equal(expert_layer(x, w, 3, a, b, "gelu"), want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_layer_of_packed_weights_with_a_gradient(dtype):
+    """Packed weights beside float32 tokens, or tokens that want a gradient: separate operators."""
+    torch = require_gpu()
+    from purin_amd import activate, combine, dispatch, expert_layer, expert_product, pack, route
+
+    t = _types(torch)[dtype]
+    x = _randn(torch, 1, (20, 40), t).requires_grad_()
+    w = _weights(torch, 2, 20, 6, "f32").requires_grad_()
+    a = pack(_randn(torch, 3, (6, 40, 64), t, 0.2), "fp4", axis=1)
+    b = pack(_randn(torch, 4, (6, 32, 40), t, 0.2), "fp4", axis=1)
+    cot = _randn(torch, 5, (20, 40), t)
+    out = expert_layer(x, w, 3, a, b)
+    r = route(w, 3)
+    want = combine(expert_product(activate(expert_product(dispatch(x, r), a, r)), b, r), r)
+    assert torch.equal(out, want)
+    for got, other in zip(torch.autograd.grad(out, (x, w), cot), torch.autograd.grad(want, (x, w), cot)):
+        assert torch.equal(got, other)
+
+
+# ---------------------------------------------------------------------------
+# beyond 32 bits
+# ---------------------------------------------------------------------------
+
+
+def test_packed_weights_beyond_32_bit_offsets():
+    """More than 2^32 bytes of codes, more than 2^33 elements: both ends."""
+    torch = require_gpu()
+    from purin_amd import Microscaled, expert_layer, expert_product, unpack
+
+    experts, inner, outer = 550, 4096, 4096
+    codes = torch.zeros((experts, outer, inner // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.full((experts, outer, inner // 32), 120, dtype=torch.uint8, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for e in (0, experts - 1):
+        codes[e].random_(0, 256, generator=g)
+    assert codes.numel() > 1 << 32
+    m = Microscaled(codes, scales, "fp4", (experts, inner, outer), 1, torch.bfloat16)
+    x = _randn(torch, 2, (8, inner), torch.bfloat16)
+    at = torch.full((experts + 1,), 3, dtype=torch.int32, device="cuda")
+    at[0], at[-1] = 0, 8
+    out = expert_product(x, m, at).double()
+    weights = torch.zeros((2, experts), device="cuda")
+    weights[0, 0] = weights[1, -1] = 1.0
+    back = Microscaled(codes, scales, "fp4", (experts, outer, inner), 1, torch.bfloat16)
+    layer = expert_layer(x[:2], weights, 1, m, back, "relu").double()
+    for e, (i, j), row in ((0, (0, 3), 0), (experts - 1, (3, 8), 1)):
+        one = unpack(Microscaled(codes[e:e + 1], scales[e:e + 1], "fp4", (1, inner, outer), 1,
+                                 torch.bfloat16))[0].double()
+        want, terms = x[i:j].double() @ one, x[i:j].double().abs() @ one.abs()
+        bound = UNIT["bf16"] * want.abs() + 2 * (inner + 2) * SUMS["bf16"] * terms + STEP["bf16"]
+        assert bool(((out[i:j] - want).abs() <= bound).all())
+        h = torch.relu(x[row].double() @ one)
+        reach = 1.13 * (x[row].double().abs() @ one.abs())
+        want, terms = h @ one, (h + reach) @ one.abs()
+        off = 2 * (inner + outer + 4) * SUMS["bf16"] + 2 * UNIT["bf16"] ** 2
+        bound = UNIT["bf16"] * want.abs() + off * terms + STEP["bf16"]
+        assert bool(((layer[row] - want).abs() <= bound).all())
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Packing, unpacking and the activation of more than 2^33 elements."""
+    torch = require_gpu()
+    from purin_amd import activate, pack, unpack
+
+    rows, length = (1 << 21) + 3, 4128
+    one = _randn(torch, 1, (1, length), torch.bfloat16)
+    x = one.expand(rows, length).contiguous()
+    x[-1] *= 3
+    m, small = pack(x, "int8"), pack(one, "int8")
+    last = pack(x[-1:], "int8")
+    for got, first, end in ((m.codes, small.codes, last.codes), (m.scales, small.scales, last.scales)):
+        assert bool((got[:-1] == first).all()) and torch.equal(got[-1:], end)
+    y = unpack(m)
+    assert bool((y[:-1] == unpack(small)).all()) and torch.equal(y[-1:], unpack(last))
+    del y, m
+    out = activate(x, "relu")
+    assert bool((out[:-1] == activate(one, "relu")).all())
+    assert torch.equal(out[-1:], activate(x[-1:].contiguous(), "relu"))
 
 
 # ---------------------------------------------------------------------------
