@@ -242,6 +242,7 @@ typedef struct {
 
 #define PURIN_TRAIN_LAYER_TOKENS 64
 #define PURIN_TRAIN_LAYER_PAIRS 1024
+#define PURIN_TRAIN_LAYER_WIDTH 1048576
 
 /* Workspace bytes of expert_layer (negative: invalid, or more than it takes). */
 int64_t purin_train_expert_layer_workspace_bytes(int32_t dtype, int64_t tokens, int64_t experts,
@@ -254,9 +255,11 @@ int64_t purin_train_expert_layer_workspace_bytes(int32_t dtype, int64_t tokens, 
  * with f and ``gated`` as in activate (inner has hidden or 2 * hidden columns)
  * and experts chosen as route does; zeros for a token without experts.  dtype
  * BF16 or F16.  Between the products numbers keep twice the type's digits; in F16
- * weight * f beyond the type's range is infinite.  Sums are held in 32 bits.
+ * f beyond the type's range is infinite, and exact to 2^-25 at least.  Sums and
+ * weights are held in 32 bits.
  * At most PURIN_TRAIN_LAYER_TOKENS tokens, tokens * slots at most
- * PURIN_TRAIN_LAYER_PAIRS, ldx below 2^24.
+ * PURIN_TRAIN_LAYER_PAIRS, width, 2 * hidden and outer at most
+ * PURIN_TRAIN_LAYER_WIDTH, ldx below 2^24.
  */
 int purin_train_expert_layer(void* stream, int32_t dtype, int32_t wdtype, int64_t tokens,
                              int64_t experts, int64_t slots, int64_t width, int64_t hidden,

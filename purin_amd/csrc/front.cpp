@@ -600,6 +600,15 @@ Tensor run_product_packed(const Tensor& rows, const Packed* packed_rows, int32_t
   return out;
 }
 
+// Rows of 32 bits: beside the weights as numbers of 32 bits, for the length of the call.
+Tensor run_rows_packed(const Tensor& rows, const Packed& w, const Tensor& offsets, int64_t outer) {
+  const Tensor a = matrix(rows);
+  if (a.scalar_type() == at::kFloat)
+    return run_product(a, run_unpack(w, PURIN_TRAIN_FP4, a.size(1), at::kFloat).transpose(1, 2), offsets);
+  return run_product_packed(a, nullptr, code_of(a, "rows"), w, offsets, a.size(1), outer,
+                            a.options().requires_grad(false));
+}
+
 struct PackedProductFn : torch::autograd::Function<PackedProductFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& codes,
                         const Tensor& scales, const Tensor& offsets, int64_t outer) {
@@ -608,9 +617,7 @@ struct PackedProductFn : torch::autograd::Function<PackedProductFn> {
     Packed w;
     w.codes = codes;
     w.scales = scales;
-    const Tensor a = matrix(rows);
-    return run_product_packed(a, nullptr, code_of(a, "rows"), w, offsets, a.size(1), outer,
-                              a.options().requires_grad(false));
+    return run_rows_packed(rows, w, offsets, outer);
   }
   // the weights unpacked, (experts, outer, inner): the contraction runs across their blocks
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -637,12 +644,8 @@ Tensor expert_product_packed(const Tensor& rows, const Tensor& codes, const Tens
   check_offsets(rows, offsets, w.experts);
   without_tangent(rows);
   const Tensor at = offsets.contiguous();
-  if (code == PURIN_TRAIN_F32)  // the weights as numbers of 32 bits
-    return expert_product(rows, run_unpack(w.p, kind, w.inner, at::kFloat).transpose(1, 2), at, false);
-  if (wants_grad(rows)) return PackedProductFn::apply(rows, w.p.codes, w.p.scales, at, w.outer);
-  const Tensor a = matrix(rows);
-  return run_product_packed(a, nullptr, code, w.p, at, w.inner, w.outer,
-                            a.options().requires_grad(false));
+  return wants_grad(rows) ? PackedProductFn::apply(rows, w.p.codes, w.p.scales, at, w.outer)
+                          : run_rows_packed(rows, w.p, at, w.outer);
 }
 
 Tensor expert_product_both(const Tensor& rows_codes, const Tensor& rows_scales, int32_t rows_kind,
@@ -779,7 +782,8 @@ std::optional<Tensor> expert_layer(const Tensor& x, const Tensor& weights, int64
   const bool graph = wants_grad(x) || wants_grad(weights) || (inner && wants_grad(*inner)) ||
                      (outer && wants_grad(*outer));
   if (graph || (code != PURIN_TRAIN_BF16 && code != PURIN_TRAIN_F16) ||
-      tokens > PURIN_TRAIN_LAYER_TOKENS || tokens * slots > PURIN_TRAIN_LAYER_PAIRS)
+      tokens > PURIN_TRAIN_LAYER_TOKENS || tokens * slots > PURIN_TRAIN_LAYER_PAIRS ||
+      std::max({a.inner, 2 * hidden, b.outer}) > PURIN_TRAIN_LAYER_WIDTH)
     return std::nullopt;
   const at::NoGradGuard no_grad;
   Tensor rows = matrix(x);

@@ -7,10 +7,12 @@
 //   choose  one workgroup chooses the tokens' experts and sorts the pairs (token, slot) by expert;
 //           the others lay out x as the products read it, where it is not so already.  With few
 //           pairs the next launch's workgroups do it themselves;
-//   up      a workgroup has one expert and 64 columns of A: multiplies its tokens' rows, applies f
-//           and the token's weight.  The results keep twice the type's digits, as the sum of two
-//           numbers of the type, so that they take part in the second product as they are;
-//   down    one expert and 64 columns of B: a row of 32-bit sums for each pair;
+//   up      a workgroup has one expert and 64 columns of A (to 256, by the number of them):
+//           multiplies its tokens' rows and applies f.  The results keep twice the type's digits,
+//           as the sum of two numbers of the type, so that they take part in the second product as
+//           they are;
+//   down    the same of B: a row of 32-bit sums, times the token's weight, for each pair.  (The
+//           weight before the second product would leave float16's range sooner.);
 //   sum     adds a token's rows in the order of its slots.
 
 #include <algorithm>
@@ -356,7 +358,7 @@ constexpr int kOwnPairs = 128, kOwnTokens = 16, kOwnExperts = 256;
 struct OwnPlan {
   int32_t groups;
   int32_t expert[kOwnPairs], start[kOwnPairs + 1], order[kOwnPairs];
-  float weight[kOwnPairs], chosen[kOwnPairs];
+  float chosen[kOwnPairs];
   alignas(16) int32_t ids[kOwnPairs], first[kOwnPairs];  // first: an expert's first pair has it
 };
 __device__ __forceinline__ void make_own_plan(const Choose& p, OwnPlan& own, Plan* plan) {
@@ -398,11 +400,12 @@ __device__ __forceinline__ void make_own_plan(const Choose& p, OwnPlan& own, Pla
     }
     const bool first = own.first[tid] >= 0;
     const int place = e >= 0 ? below + before : -1;
-    if (e >= 0) own.order[place] = tid, own.weight[place] = own.chosen[tid];
+    if (e >= 0) own.order[place] = tid;
     if (first) own.expert[group] = e, own.start[group] = below;
     if (tid == 0) own.groups = groups, own.start[groups] = all;
     if (writes) {
       plan->place[tid] = place;
+      if (e >= 0) plan->weight[place] = own.chosen[tid];
       if (first) plan->expert[group] = e, plan->start[group] = below;
       if (tid == 0) plan->groups = groups, plan->start[groups] = all;
     }
@@ -508,13 +511,12 @@ __global__ __launch_bounds__(256, 2) void k_layer_up(Up p, Choose choose, Matric
       const int r = i % rows, j = i / rows * 8, place = start + r0 + r;
       if (col + j >= p.hidden) continue;
       const int at = p.gated ? (j >> 5 << 6) + (j & 31) : j;  // of the sums
-      const float weight = from.weight[place];
       Pack<T> hi, lo;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         float h = activation<T>(p.act, thin_sum<BM>(sums, parts, r, at + q));
         if (p.gated) h *= thin_sum<BM>(sums, parts, r, at + 32 + q);
-        h = col + j + q < p.hidden ? h * weight : 0.0f;
+        if (col + j + q >= p.hidden) h = 0.0f;
         hi.v[q] = (T)h;
         const float rest = h - (float)hi.v[q];
         lo.v[q] = (T)(fabsf((float)hi.v[q]) < __builtin_inff() ? rest : 0.0f);
@@ -554,9 +556,10 @@ __global__ __launch_bounds__(256, 2) void k_layer_down(
     for (int i = tid; i < min(BM, count - r0) * (wide / 4); i += 256) {
       const int r = i / (wide / 4), j = i % (wide / 4) * 4;
       if (j >= n) continue;
+      const float weight = plan->weight[start + r0 + r];
       Pack<float> v;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v.v[q] = thin_sum<BM>(sums, parts, r, j + q);
+      for (int q = 0; q < 4; ++q) v.v[q] = thin_sum<BM>(sums, parts, r, j + q) * weight;
       store_upto(out + (start + r0 + r) * p.outer + col + j, v, n - j);
     }
     __syncthreads();
@@ -721,7 +724,7 @@ static int check_layer(int32_t dtype, int64_t tokens, int64_t experts, int64_t s
   if (tokens > kTokens || tokens * slots > kPairs)
     return set_error(PURIN_CP_ERR_UNSUPPORTED,
                      "expert_layer takes at most 64 tokens, and 1024 slots of all of them");
-  if (width > (int64_t(1) << 20) || hidden > (int64_t(1) << 19) || outer > (int64_t(1) << 20))
+  if (std::max({width, hidden, outer}) > PURIN_TRAIN_LAYER_WIDTH || 2 * hidden > PURIN_TRAIN_LAYER_WIDTH)
     return set_error(PURIN_CP_ERR_UNSUPPORTED,
                      "width and outer must not exceed 2^20, hidden 2^19");
   return PURIN_CP_OK;

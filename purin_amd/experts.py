@@ -3,8 +3,8 @@
     out = expert_layer(x, weights, slots, inner, outer)  # from routing weights to the layer's result
 
 is ``route``, ``dispatch``, ``expert_product``, ``activate``, ``expert_product`` and ``combine`` in
-turn, and for a few tokens of bfloat16 or float16 without a graph three kernels that read every
-weight of the chosen experts once.  The HIP library's conventions are those of ``routing``.  The
+turn, and for a few tokens of bfloat16 or float16 without a graph three or four kernels that read
+every weight of the chosen experts once (a few times for experts with many tokens).  The HIP library's conventions are those of ``routing``.  The
 reference has no counterpart.
 """
 
@@ -61,9 +61,10 @@ def expert_layer(x, weights, slots, inner, outer, activation="silu", *, workspac
     ``inner`` (experts, width, hidden), or (experts, width, 2 * hidden) with a gate (``activate``);
     ``outer`` (experts, hidden, outer width): tensors of x's type in either order of the last two
     dimensions, or packed (``pack(weight, "fp4", axis=1)``).  Up to 64 tokens (and 1024 slots of all
-    of them) of bfloat16 or float16 without a graph run in three kernels, which keep the hidden
-    values to twice the type's digits and need the ``workspace`` (new memory otherwise; left alone
-    by other calls).  All others are the separate operators in turn, which round them to the type.
+    of them) of bfloat16 or float16 without a graph run in three or four kernels, which keep the
+    hidden values to twice the type's digits and need the ``workspace`` (new memory otherwise; left
+    alone by other calls).  All others are the separate operators in turn, which round them to the
+    type.
     """
     code = _activation(activation)
     if slots.__class__ is not int:

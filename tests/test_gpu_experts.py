@@ -336,6 +336,21 @@ def test_kept_rows_take_half_the_memory():
     assert held(lambda r: activate(r * 1, "silu", saved="int8"), rows) == 0
 
 
+def test_a_graph_holds_packed_weights_packed():
+    torch = require_gpu()
+    from purin_amd import expert_product, pack
+
+    at = torch.tensor([0, 16], dtype=torch.int32, device="cuda")
+    m = pack(_randn(torch, 1, (1, 1024, 2048), torch.bfloat16), "fp4", axis=1)
+    for t in (torch.float32, torch.bfloat16):
+        rows = _randn(torch, 2, (16, 1024), t).requires_grad_()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = expert_product(rows, m, at)
+        # the result, and what else an allocation rounds up
+        assert torch.cuda.memory_allocated() - before <= out.numel() * out.element_size() + 4096
+
+
 # ---------------------------------------------------------------------------
 # the activation
 # ---------------------------------------------------------------------------
@@ -587,6 +602,39 @@ def test_hidden_values_beyond_the_type():
     b = torch.full((1, 32, 8), 1.0, dtype=torch.float16, device="cuda")
     out = expert_layer(x, torch.ones((1, 1), device="cuda"), 1, a, b, "relu")
     assert bool((out == float("inf")).all())
+
+
+@pytest.mark.parametrize("experts", [1, 300])  # the choice inside the first product, and before it
+def test_weights_far_from_one(experts):
+    """float16: a token's weight neither takes hidden values out of the range nor results' digits."""
+    torch = require_gpu()
+    from purin_amd import expert_layer
+
+    def run(weight, a, b):
+        ones = lambda *size: torch.ones(size, dtype=torch.float16, device="cuda")  # noqa: E731
+        w = torch.zeros((1, experts), device="cuda")
+        w[0, -1] = weight
+        return expert_layer(ones(1, 64), w, 1, a * ones(experts, 64, 32), b * ones(experts, 32, 8), "relu")
+
+    # all sums are of equal powers of two times 125: exact, and rounded once
+    out = run(1000.0, 15.625, 2.0 ** -10)  # hidden 1000, 31.25 without the weight
+    assert bool((out == torch.tensor(31250.0).half().cuda()).all())
+    out = run(2.0 ** -20, 2.0 ** -16, 2.0 ** 15)  # hidden 2^-10, 2^10 without the weight
+    assert bool((out == 2.0 ** -10).all())
+
+
+def test_layer_wider_than_the_kernels():
+    torch = require_gpu()
+    from purin_amd import expert_layer
+
+    for width, hidden, outer in (((1 << 20) + 8, 2, 2), (2, (1 << 19) + 8, 2), (2, 2, (1 << 20) + 8)):
+        # powers of two: sums within 24 bits, exact, from 1 to 1 + 2^-16, 1 when rounded
+        x = torch.full((2, width), 2.0 ** -(width.bit_length() - 1), dtype=torch.bfloat16, device="cuda")
+        a = torch.ones((1, width, hidden), dtype=torch.bfloat16, device="cuda")
+        b = torch.full((1, hidden, outer), 2.0 ** -(hidden.bit_length() - 1), dtype=torch.bfloat16,
+                       device="cuda")
+        out = expert_layer(x, torch.ones((2, 1), device="cuda"), 1, a, b, "relu")
+        assert out.shape == (2, outer) and bool((out == 1).all())
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f64", "bf16"])
