@@ -23,22 +23,37 @@
 namespace purin {
 namespace train {
 
-// 8 neighbours in 32 bits (64 for F64); ``n`` of them are there, zeros behind.
+// 8 neighbours as they are in memory; ``n`` of them are there, zeros behind.  They become numbers
+// behind the branch, so that several loads are on their way before the first is waited for.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, typename Elem<T>::Acc (&v)[8]) {
-  constexpr int V = kVec<T>;
-  if (n >= 8) {
+struct Eight {
+  static constexpr int kWords = 8 * sizeof(T) / 4;
+  typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
+  Words w;
+  __device__ __forceinline__ Eight() = default;
+  __device__ __forceinline__ Eight(const T* p, int n) {
+    constexpr int V = kVec<T>;
+    struct All {
+      Pack<T> v[8 / V];
+    } all;
+    if (n >= 8) {
 #pragma unroll
-    for (int i = 0; i < 8; i += V) {
-      const Pack<T> x = load16(p + i);
+      for (int i = 0; i < 8; i += V) all.v[i / V] = load16(p + i);
+      w = __builtin_bit_cast(Words, all);
+    } else {
 #pragma unroll
-      for (int q = 0; q < V; ++q) v[i + q] = (typename Elem<T>::Acc)x.v[q];
+      for (int i = 0; i < 8; ++i) all.v[i / V].v[i % V] = i < n ? p[i] : (T)0;
+      w = __builtin_bit_cast(Words, all);
+      asm("" : "+v"(w));  // whole words for both: halves would be taken apart, and waited for, above
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? (typename Elem<T>::Acc)p[i] : 0;
   }
-}
+  __device__ __forceinline__ typename Elem<T>::Acc operator[](int i) const {
+    struct All {
+      T v[8];
+    };
+    return (typename Elem<T>::Acc)__builtin_bit_cast(All, w).v[i];
+  }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int n, const typename Elem<T>::Acc (&v)[8]) {
   constexpr int V = kVec<T>;
@@ -82,8 +97,11 @@ __global__ __launch_bounds__(256) void k_pack(Strided<T> x, Divider by_row, uint
       const int at = (int)(n - in * by_row.d), block = at >> 2;
       const int64_t row = first + in, out = g * x.rows + row;
       const int64_t l = (int64_t)at * 8;
+      const Eight<T> raw(x.p + g * x.sg + row * x.sr + l,
+                         (int)max<int64_t>(0, min<int64_t>(8, x.length - l)));
       float v[8];
-      load8(x.p + g * x.sg + row * x.sr + l, (int)max<int64_t>(0, min<int64_t>(8, x.length - l)), v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = raw[i];
       uint32_t most = magnitude(v[0]);
 #pragma unroll
       for (int i = 1; i < 8; ++i) most = max(most, magnitude(v[i]));
@@ -98,23 +116,28 @@ __global__ __launch_bounds__(256) void k_pack(Strided<T> x, Divider by_row, uint
 // has 64 rows and 8 blocks, and its codes pass through LDS, so that a row's leave together.
 constexpr int kAcross = 64;
 template <typename T, int KIND>
-__global__ __launch_bounds__(256) void k_pack_across(Strided<T> x, int64_t tiles_l,
+__global__ __launch_bounds__(256) void k_pack_across(Strided<T> x, int64_t tiles_r,
                                                      uint8_t* __restrict__ codes,
                                                      uint8_t* __restrict__ scales) {
-  constexpr int kRow = 8 * 32 * kMicroBits<KIND> / 8, kPitch = kRow + 16;  // bytes
-  __shared__ __align__(16) uint8_t held[kAcross * kPitch];
+  constexpr int kRow = 8 * 32 * kMicroBits<KIND> / 8, kPieces = kRow / 16;  // bytes, pieces of 16
+  // row 8 a + r at place 8 r + a, its pieces exchanged by a: a wavefront writes 8 places, two blocks
+  // of each, and these fall on different banks
+  __shared__ __align__(16) uint8_t held[kAcross * kRow];
+  auto place = [](int a, int r, int piece) {
+    return ((8 * r + a) * kPieces + (piece ^ (KIND == kFp4 ? a & 6 : 2 * a))) * 16;
+  };
   __shared__ uint8_t held_scales[kAcross][8];
   const int blocks = micro_blocks(x.length), filled = micro_filled(blocks);
   // lanes: 8 times 8 rows, then the 4 quarters of a block, then the blocks
   const int tid = threadIdx.x, r8 = tid & 7, quarter = (tid >> 3) & 3, block = tid >> 5;
-  const int64_t tr = blockIdx.x / tiles_l, tl = blockIdx.x - tr * tiles_l;
+  const int64_t tl = blockIdx.x / tiles_r, tr = blockIdx.x - tl * tiles_r;
   const int64_t row = tr * kAcross, l = (tl * 8 + block) * 32 + quarter * 8;
   const int n = (int)max<int64_t>(0, min<int64_t>(8, x.rows - row - r8 * 8));
   for (int64_t g = blockIdx.y; g < x.groups; g += gridDim.y) {
-    float v[8][8];  // [neighbour][row]
+    Eight<T> v[8];  // [neighbour][row]
     const T* p = x.p + g * x.sg + row + r8 * 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) load8(p + (l + j) * x.sl, l + j < x.length ? n : 0, v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = Eight<T>(p + (l + j) * x.sl, l + j < x.length ? n : 0);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       uint32_t most = magnitude(v[0][r]);
@@ -126,20 +149,19 @@ __global__ __launch_bounds__(256) void k_pack_across(Strided<T> x, int64_t tiles
       float one[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) one[j] = v[j][r];
-      store_codes<KIND>(held + (r8 * 8 + r) * kPitch + (block * 32 + quarter * 8) * kMicroBits<KIND> / 8,
-                        one, s);
+      const int in = (block * 32 + quarter * 8) * kMicroBits<KIND> / 8;
+      store_codes<KIND>(held + place(r8, r, in / 16) + in % 16, one, s);
       if (quarter == 0) held_scales[r8 * 8 + r][block] = (uint8_t)s;
     }
     __syncthreads();
     const int64_t out = g * x.rows + row;
-    constexpr int per = kRow / 16;
     const int64_t whole = (int64_t)blocks * 32 * kMicroBits<KIND> / 8;  // bytes of a row's codes
-    for (int i = tid; i < kAcross * per; i += 256) {
-      const int r = i / per, c = i % per * 16;
-      const int64_t at = tl * kRow + c;
+    for (int i = tid; i < kAcross * kPieces; i += 256) {
+      const int a = i / kPieces % 8, b = i / kPieces / 8, r = 8 * a + b, c = i % kPieces;
+      const int64_t at = tl * kRow + c * 16;
       if (row + r < x.rows && at < whole)
         *reinterpret_cast<uint4*>(codes + (out + r) * whole + at) =
-            *reinterpret_cast<const uint4*>(held + r * kPitch + c);
+            *reinterpret_cast<const uint4*>(held + place(a, b, c));
     }
     for (int i = tid; i < kAcross * 8; i += 256) {
       const int r = i >> 3, b = i & 7;
@@ -188,10 +210,13 @@ __global__ __launch_bounds__(256) void k_activate(int act, const T* __restrict__
     const int64_t row = first + in, l = (int64_t)at * 8;
     const int some = (int)max<int64_t>(0, min<int64_t>(8, hidden - l));
     A g[8], v[8], h[8];
-    load8(u + row * ldu + l, some, g);
-    if constexpr (GATED) load8(u + row * ldu + hidden + l, some, v);
+    const Eight<T> first_half(u + row * ldu + l, some);
+    Eight<T> second;
+    if constexpr (GATED) second = Eight<T>(u + row * ldu + hidden + l, some);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      g[i] = first_half[i];
+      if constexpr (GATED) v[i] = second[i];
       h[i] = activation<T>(act, g[i]);
       if constexpr (GATED) h[i] *= v[i];
     }
@@ -229,16 +254,25 @@ __global__ __launch_bounds__(256) void k_activate_vjp(
     const int64_t row = first + in, l = (int64_t)at * 8;
     const int some = (int)min<int64_t>(8, hidden - l);
     A x[kParts][8], g[8];
-    load8(g_out + row * ldg + l, some, g);
+    const Eight<T> raw_g(g_out + row * ldg + l, some);
+    if constexpr (KEPT) {
 #pragma unroll
-    for (int half = 0; half < kParts; ++half) {
-      if constexpr (KEPT) {
+      for (int half = 0; half < kParts; ++half) {
         const int64_t from = row * kParts + half;
         load_codes<kInt8>(codes + from * blocks * 32 + l, scales[from * filled + (at >> 2)], x[half]);
-      } else {
-        load8(u + row * ldu + half * hidden + l, some, x[half]);
       }
+    } else {
+      Eight<T> raw[kParts];
+#pragma unroll
+      for (int half = 0; half < kParts; ++half)
+        raw[half] = Eight<T>(u + row * ldu + half * hidden + l, some);
+#pragma unroll
+      for (int half = 0; half < kParts; ++half)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[half][i] = raw[half][i];
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = raw_g[i];
     A to[kParts][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -303,11 +337,11 @@ static int pack(hipStream_t st, const Strided<T>& x, uint8_t* codes, uint8_t* sc
                    });
   }
   const int64_t tiles_l = (micro_filled(micro_blocks(x.length)) + 7) / 8;
-  const int64_t tiles = tiles_l * ((x.rows + kAcross - 1) / kAcross);
+  const int64_t tiles_r = (x.rows + kAcross - 1) / kAcross, tiles = tiles_l * tiles_r;
   if (tiles >= (int64_t(1) << 24)) return set_error(PURIN_CP_ERR_UNSUPPORTED, "too many tiles for a launch");
   const unsigned most = (unsigned)std::max<int64_t>(1, (int64_t(1) << 23) / tiles);  // threads below 2^32
   k_pack_across<T, KIND><<<dim3((unsigned)tiles, std::min(gy, most)), dim3(256), 0, st>>>(
-      x, tiles_l, codes, scales);
+      x, tiles_r, codes, scales);
   return launched("k_pack_across");
 }
 
