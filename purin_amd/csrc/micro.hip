@@ -12,7 +12,10 @@
 // that the type itself has there.
 //
 // All are bound by memory: a thread has 8 neighbours, 4 threads a block, whose largest magnitude
-// passes between them without LDS.
+// passes between them without LDS.  Read and written, us and TB/s: 32768 x 2048 bf16 to 4 bits 35
+// (4.8); 4099 x 1111 float32 to 8 bits 7 and back 7.5 (3.2, 3.0); 16 x 4096 x 2048 bf16 to 4 bits
+// across memory 86-90 (3.8-3.9) and back 58 (5.8, the codes in the cache); the gated activation of
+// 49152 x 2816 bf16 with kept rows 94-98, backward 93-97 (5.7-6.0, part of them in the cache).
 
 #include <algorithm>
 #include <type_traits>
@@ -114,6 +117,7 @@ __global__ __launch_bounds__(256) void k_pack(Strided<T> x, Divider by_row, uint
 
 // Rows that are adjacent themselves, 8 to a thread, whose neighbours are sl apart: a workgroup
 // has 64 rows and 8 blocks, and its codes pass through LDS, so that a row's leave together.
+// Neighbouring workgroups have neighbouring rows (the other order: 90 us for 88).
 constexpr int kAcross = 64;
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void k_pack_across(Strided<T> x, int64_t tiles_r,

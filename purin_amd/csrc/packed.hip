@@ -7,8 +7,8 @@
 namespace purin {
 namespace train {
 
-template <typename T, int BM, int BN, int WM, int WN, int S>
-__global__ __launch_bounds__(WM* WN * 64) void k_product_packed(
+template <typename T, int B, int WN>
+__global__ __launch_bounds__(2 * WN * 64) void k_product_packed(
     const T* __restrict__ a, int64_t lda, const uint8_t* __restrict__ codes,
     const uint8_t* __restrict__ scales, int64_t rows, int64_t inner, int64_t outer, int experts,
     int64_t tiles_m, int64_t tiles_n, const int32_t* __restrict__ offsets, T* __restrict__ out,
@@ -18,22 +18,24 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product_packed(
   tile_order(tiles_m, tiles_n, tm, tn);
   int e;
   int64_t from, to;
-  if (!find_tile(offsets, experts, rows, BM, tm, e, from, to)) return;
+  if (!find_tile(offsets, experts, rows, B, tm, e, from, to)) return;
   e = __builtin_amdgcn_readfirstlane(e);
-  const int64_t col = tn * BN;
-  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(BM, to - from));
-  const int n = (int)min<int64_t>(BN, outer - col);
+  const int64_t col = tn * B;
+  const int m = __builtin_amdgcn_readfirstlane((int)min<int64_t>(B, to - from));
+  const int n = (int)min<int64_t>(B, outer - col);
   T* c = out + from * ldo + col;
   if (e < 0) {
     zero_tile(c, ldo, m, n);
     return;
   }
-  TileHalf<T, BM, BN, WM, WN, S>::run(a + from * lda, lda, m, inner,
-                                      Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
+  TileHalf<T, B, WN>::run(a + from * lda, lda, m, inner,
+                          Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
 }
 
 // Split number blockIdx.y of the contraction writes its own ``out``.  A tile has 64 columns to each
-// set of ``parts`` wavefronts.
+// set of ``parts`` wavefronts.  An expert's tiles are dealt to all XCDs, which reads its rows into each
+// L2 (32 experts, 4096 x 1536, 24 rows to each: 165 MB, 115 of them needed): on one XCD they read 120 MB,
+// but the same rows' lines at the same time, and take 44 us for 37.
 template <typename T, typename C, int BM>
 __global__ __launch_bounds__(256, 2) void k_product_packed_thin(
     Rows a, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
@@ -105,8 +107,8 @@ __global__ __launch_bounds__(2 * WN * 64) void k_product_both(
     zero_tile(c, ldo, m, n);
     return;
   }
-  TileBoth<C, B, B, 2, WN, CHUNKS>::run(Codes(a, a_scales, from, inner), m,
-                                        Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
+  TileBoth<C, B, WN, CHUNKS>::run(Codes(a, a_scales, from, inner), m,
+                                  Codes(codes, scales, e * outer + col, inner), n, lds16, c, ldo);
 }
 
 // How a product is cut.  us of 32 experts, 4096 x 1536, so many rows to each, bf16:
@@ -172,15 +174,14 @@ static int product_packed(hipStream_t st, int64_t rows, int64_t inner, int64_t o
     a = (const T*)ws;
     lda = (inner + 7) / 8 * 8;
   }
-  auto go = [&](auto bm, auto wn, auto s) {
-    constexpr int B = bm, WN = wn, S = s;
+  auto go = [&](auto bm, auto wn) {
+    constexpr int B = bm, WN = wn;
     const int64_t tm = most_tiles(rows, experts, B), tn = (outer + B - 1) / B;
-    return launch16("k_product_packed", k_product_packed<T, B, B, 2, WN, S>, tm * tn, 1, 1, 2 * WN * 64,
-                    TileHalf<T, B, B, 2, WN, S>::kLds, st, a, lda, codes, scales, rows, inner, outer,
-                    (int)experts, tm, tn, offsets, out, ldo);
+    return launch16("k_product_packed", k_product_packed<T, B, WN>, tm * tn, 1, 1, 2 * WN * 64,
+                    TileHalf<T, B, WN>::kLds, st, a, lda, codes, scales, rows, inner, outer, (int)experts,
+                    tm, tn, offsets, out, ldo);
   };
-  constexpr integral_constant<int, 3> i3;
-  return cut.shape == k256Packed ? go(i256, i4, i3) : go(i128, i2, i3);
+  return cut.shape == k256Packed ? go(i256, i4) : go(i128, i2);
 }
 
 template <typename C>
@@ -192,7 +193,7 @@ static int product_both(hipStream_t st, int64_t rows, int64_t inner, int64_t out
     constexpr int B = bm, WN = wn;
     const int64_t tm = most_tiles(rows, experts, B), tn = (outer + B - 1) / B;
     auto run = [&](auto chunks) {
-      using Tile = TileBoth<C, B, B, 2, WN, chunks>;
+      using Tile = TileBoth<C, B, WN, chunks>;
       return launch16("k_product_both", k_product_both<C, B, WN, chunks>, tm * tn, 1, 1, 2 * WN * 64,
                       Tile::kLds, st, a, a_scales, codes, scales, rows, inner, outer, (int)experts, tm,
                       tn, offsets, out, ldo);

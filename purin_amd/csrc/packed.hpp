@@ -205,9 +205,13 @@ struct Codes {
 // many rows
 // ---------------------------------------------------------------------------
 
-// A workgroup's BM x BN tile from rows of 16 bits (16-byte pieces at 16-byte addresses).
-template <typename T, int BM, int BN, int WM, int WN, int S>
+// A workgroup's B x B tile from rows of 16 bits (16-byte pieces at 16-byte addresses), in three
+// stages of 64.  Bound by the matrix units as the product of dense weights is, whose time it has with
+// half the bytes read: 32768 rows, 16 experts, 2048 x 4096, 256 x 256 tiles: 522-570 us, 0.96-1.05
+// PFLOP/s; the units are busy 48 % of the time, 58 % of what the CUs are.
+template <typename T, int B, int WN>
 struct TileHalf {
+  static constexpr int BM = B, BN = B, WM = 2, S = 3;
   static constexpr int THREADS = WM * WN * 64, X = BM / WM / 32, Y = BN / WN / 32;
   using SA = PieceStage<BM, 8, THREADS>;  // a depth of 64
   using SB = PieceStage<BN, 2, THREADS>;
@@ -275,13 +279,16 @@ struct TileHalf {
   }
 };
 
-// A workgroup's BM x BN tile from packed rows; sums are written as C.  CHUNKS: scales by
+// A workgroup's B x B tile from packed rows; sums are written as C.  CHUNKS: scales by
 // ScaleChunks, for rows that have whole pieces of them.  Two stages of 256 (of 128 in four places
 // the half lines cost more than the deeper ring gives: 32768 rows, 16 experts, 2048 x 4096 233 us,
 // 248).  256 x 256 tiles: 128 x 256 and 128 x 128 ones, two workgroups a CU, read more from L2 than
-// their overlap gives (320, 290).
-template <typename C, int BM, int BN, int WM, int WN, bool CHUNKS>
+// their overlap gives (320, 290).  201-245 us in all: 75 of them each tile's first stages and its way
+// out (268 MB), in which its CU, with room for one workgroup, multiplies nothing; the contraction
+// itself runs at 3.6 PFLOP/s.
+template <typename C, int B, int WN, bool CHUNKS>
 struct TileBoth {
+  static constexpr int BM = B, BN = B, WM = 2;
   static constexpr int THREADS = WM * WN * 64, X = BM / WM / 32, Y = BN / WN / 32;
   using SA = PieceStage<BM, 8, THREADS>;  // a depth of 256
   using SB = PieceStage<BN, 8, THREADS>;
