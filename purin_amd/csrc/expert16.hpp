@@ -13,8 +13,7 @@
 //   [k][i]   pair i / 16 of row k at (i / 16) ^ s(k), s(k) = 2 (k % 4) + (k / 8) % 2 (2 ((k / 2) % 2)
 //            in rows of 64, two of which cover the banks): the 8 blocks of 32 bytes that half a
 //            wavefront reads at once fall on 8 places
-// Counted over the large products, conflicts take 40-50 % of the LDS cycles with [i][k] stages and
-// 4 % in the weights' gradient, which has [k][i] ones alone.
+// Counted over the large products, conflicts take 2-4 % of the LDS cycles.
 // With 16-byte rows at 16-byte addresses the stages are loaded straight into LDS (buffer loads
 // whose addresses outside the operand read zeros); others pass through registers.
 //

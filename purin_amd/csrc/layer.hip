@@ -779,7 +779,7 @@ int purin_train_expert_layer(void* stream, int32_t dtype, int32_t wdtype, int64_
     if (!known_dtype(wdtype)) return refuse("unknown dtype");
     if (activation < PURIN_TRAIN_RELU || activation > PURIN_TRAIN_GELU)
       return refuse("unknown activation");
-    if (int rc = check_matrices(inner, width, hidden)) return rc;
+    if (int rc = check_matrices(inner, width, gated ? 2 * hidden : hidden)) return rc;
     if (int rc = check_matrices(outer, hidden, outer_width)) return rc;
     if (!tokens || !outer_width) return (int)PURIN_CP_OK;
     if ((width && !x) || !weights || !out) return refuse("NULL array");

@@ -135,6 +135,8 @@ def test_layer_refusals():
     assert layer(a=_lib.TrainMatrices(X, None, 64, 8, 2)) == _lib.ERR_ARG
     assert layer(a=_lib.TrainMatrices(X, None, -1, 8, 1)) == _lib.ERR_ARG
     assert layer(a=_lib.TrainMatrices(None, None, 64, 8, 1)) == _lib.ERR_ARG
+    # two columns with a gate
+    assert layer(a=_lib.TrainMatrices(X, None, 64, 8, 2), hidden=1, gated=1) == _lib.ERR_ARG
     assert layer(b=_lib.TrainMatrices(X + 8, X, 0, 0, 0)) == _lib.ERR_ARG
     assert layer(b=_lib.TrainMatrices(X, X + 1, 0, 0, 0)) == _lib.ERR_ARG
     assert layer(ws_bytes=16) == _lib.ERR_ARG and layer(ws=X + 4) == _lib.ERR_ARG
