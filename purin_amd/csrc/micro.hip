@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256) void k_activate(int act, const T* __restrict__
         const uint32_t s = micro_scale<kInt8>(most);
         const int64_t to = row * (GATED ? 2 : 1) + half;
         if ((at & 3) == 0) scales[to * filled + (at >> 2)] = (uint8_t)s;
-        store_codes<kInt8>(codes + to * blocks * 32 + l, x, s);
+        if ((at >> 2) < blocks) store_codes<kInt8>(codes + to * blocks * 32 + l, x, s);
       }
     }
   }
@@ -437,7 +437,7 @@ int purin_train_activate(void* stream, int32_t dtype, int32_t activation, int32_
       if constexpr (sizeof(T) != 8)
         if (codes)
           return go(gated ? k_activate<T, true, true> : k_activate<T, false, true>,
-                    micro_blocks(hidden) * 4);
+                    micro_filled(micro_blocks(hidden)) * 4);
       return go(gated ? k_activate<T, true, false> : k_activate<T, false, false>, (hidden + 7) / 8);
     });
   });

@@ -415,6 +415,24 @@ def test_activate_and_gradient(rows, hidden, kind, gated, dtype):
             assert (np.abs(_np(g) - want) <= bound).all()
 
 
+@pytest.mark.parametrize("hidden", [1, 32, 33, 70, 128, 161])
+@pytest.mark.parametrize("gated", [True, False])
+def test_kept_codes_are_packs(hidden, gated):
+    """The codes and scales that activate makes on its way, the zeros behind them included."""
+    torch = require_gpu()
+    from purin_amd import _lib, pack
+
+    halves = 2 if gated else 1
+    u = _randn(torch, 1, (5, halves * hidden), torch.bfloat16)
+    want = pack(u.view(5, halves, hidden), "int8")
+    codes, scales = torch.full_like(want.codes, 77), torch.full_like(want.scales, 77)
+    out = torch.empty((5, hidden), dtype=torch.bfloat16, device="cuda")
+    _lib.check(_lib.load().purin_train_activate(
+        torch.cuda.current_stream().cuda_stream, _lib.BF16, _lib.SILU, int(gated), 5, hidden,
+        u.data_ptr(), halves * hidden, out.data_ptr(), codes.data_ptr(), scales.data_ptr()))
+    assert torch.equal(codes, want.codes) and torch.equal(scales, want.scales)
+
+
 @pytest.mark.parametrize("kind", ["relu", "silu", "gelu"])
 @pytest.mark.parametrize("gated", [True, False])
 def test_activation_gradient_by_differences(kind, gated):
