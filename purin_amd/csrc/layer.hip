@@ -358,8 +358,14 @@ struct Choose {
 };
 
 // Few pairs: every workgroup of the first product makes the plan for itself, in LDS, which takes
-// less than a launch (one token, 8 of 64 experts: 5.7 us for the launch, 2 here).
+// less than a launch (one token, 8 of 64 experts: 5.7 us for the launch, 2 here).  A layer's us so |
+// with the launch, gated bf16: 1 token, 2 of 8 experts, 1024 x 512 17 | 21; 8, 4 of 32, 4096 x 1408 135
+// | 143; 16, 8 of 64, 4096 x 1408 346 | 352; 32, 4 of 64, 1024 x 512 57 | 46.  In codes, two workgroups
+// to a CU, the plans of one round after another show: 8, 4 of 32 (32 pairs, 1408 workgroups) 63.6 | 64.6;
+// 16, 4 of 256, 512 x 256 (64, 512) 28.3 | 28.8; 16, 4 of 64, 1024 x 512 (64, 1024) 44 | 40; 16, 8 of 64
+// (128, 1408) 151 | 141.
 constexpr int kOwnPairs = 128, kOwnTokens = 16, kOwnExperts = 256;
+constexpr int64_t kOwnCodes = 48 * 1024;  // pairs times workgroups
 struct OwnPlan {
   int32_t groups;
   int32_t expert[kOwnPairs], start[kOwnPairs + 1], order[kOwnPairs];
@@ -678,7 +684,8 @@ static int layer(hipStream_t st, const Shape& s, const void* weights, int32_t wd
     moves = (pieces * s.tokens + 1023) / 1024;
   }
   const bool own = s.tokens <= kOwnTokens && pairs <= kOwnPairs && s.experts <= kOwnExperts &&
-                   !moves && wdtype != PURIN_TRAIN_F64;
+                   !moves && wdtype != PURIN_TRAIN_F64 &&
+                   (how_a != kCodes || pairs * groups * up.tiles <= kOwnCodes);
   if (!own) {
     const dim3 grid((unsigned)(1 + moves));
     if (wdtype == PURIN_TRAIN_F64)
