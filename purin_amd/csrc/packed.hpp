@@ -480,11 +480,13 @@ template <int X, int NA, int PIECES, int LANE, int INSIDE>
 struct RowStream {
   const uint8_t* p[NA];
   uint32_t step, at[X];
-  int left;  // pieces of the rows from this lane's first on
+  int left;  // pieces from this lane's first on
 
-  // ``row(i)``: the row of tile row i, -1 for none
+  // ``row(i)``: the row of tile row i, -1 for none.  ``pieces``: those of the rows up to the end of
+  // the wavefront's part.  The loops go on to an even number of lines, with weights of zero, and a
+  // row's elements there are the next part's: an infinity among them, times zero, would be NaN.
   template <typename F>
-  __device__ __forceinline__ RowStream(const Rows (&a)[NA], F&& row, int64_t pieces)
+  __device__ __forceinline__ RowStream(const Rows (&a)[NA], F&& row, int pieces)
       : step(a[0].step) {
     const int lane = threadIdx.x & 63, group = lane >> 4;
 #pragma unroll
@@ -494,7 +496,7 @@ struct RowStream {
       const int r = row(16 * x + (lane & 15));
       at[x] = r < 0 ? kOutside : (uint32_t)r * a[0].pitch + (uint32_t)(group * LANE) * step;
     }
-    left = (int)pieces - group * LANE;
+    left = pieces - group * LANE;
   }
   __device__ __forceinline__ I4 load(int i, int x, int unit, int k) const {
     const bool in = unit * PIECES + k * INSIDE < left;
@@ -608,7 +610,7 @@ struct StreamCodes {
     load_scales(from);
     lines.load(0, from, to);
     lines.load(1, from + 1, to);
-    const RowStream<X, NA, 16, 4, 1> rows(a, row, (inner + 7) / 8);
+    const RowStream<X, NA, 16, 4, 1> rows(a, row, min((int)((inner + 7) / 8), 32 * to));
     auto load_rows = [&](int j, int unit) {
 #pragma unroll
       for (int i = 0; i < NA; ++i)
@@ -679,7 +681,7 @@ struct StreamDense {
                      (int)ld * 2, pieces);
     lines.load(0, from, to);
     lines.load(1, from + 1, to);
-    const RowStream<X, NA, 8, 1, 4> rows(a, row, pieces);
+    const RowStream<X, NA, 8, 1, 4> rows(a, row, min(pieces, 8 * to));
     I4 rows_now[NA][X][2];
     auto load_rows = [&](int j, int unit) {
 #pragma unroll
