@@ -45,9 +45,10 @@ struct Matrices {
 
 // The products' cores.  run(): rows a (piece k of row(i)), ``inner`` long, times expert e's matrix
 // of ``outer`` columns, of which c are the wavefront's, to sums in LDS (part of its contraction).
-// kRing: the LDS that it needs on the way.
+// kRing: the LDS that it needs on the way.  First: the same of rows in one array.
 template <typename T, int BM, int NA>
 struct ThinCodes {
+  using First = ThinCodes<T, BM, 1>;
   static constexpr int kRing = kLineLds;
   static constexpr bool kStreams = true;
   template <typename F>
@@ -67,6 +68,7 @@ struct ThinCodes {
 
 template <typename T, int BM, int NA>
 struct ThinAlong {
+  using First = ThinAlong<T, BM, 1>;
   static constexpr int kRing = kLineLds;
   static constexpr bool kStreams = true;
   template <typename F>
@@ -86,6 +88,7 @@ struct ThinAlong {
 // pieces at any address.  Rows are in one piece each (step 16).
 template <typename T, int BM, int NA, bool ALONG, bool DIRECT>
 struct ThinDense {
+  using First = ThinDense<T, BM, 1, ALONG, DIRECT>;
   static constexpr int X = BM / 32, S = 4, AHEAD = 3;
   using SA = PieceStage<BM, 8, 256>;
   using SB = Stage<T, 32, ALONG, 256>;
@@ -561,19 +564,46 @@ __global__ __launch_bounds__(256, 2) void k_layer_down(
   const int n = (int)min<int64_t>(wide, p.outer - col);
   for (int r0 = 0; r0 < count; r0 += BM) {
     const Rows a[2] = {{high, p.step, p.pitch}, {low, p.step, p.pitch}};
-    Core::run(a, [&](int r) { return r0 + r < count ? start + r0 + r : -1; }, p.hidden, w, e, p.outer,
-              own.c, own.part, parts, lds16);
+    auto row = [&](int r) { return r0 + r < count ? start + r0 + r : -1; };
+    Core::run(a, row, p.hidden, w, e, p.outer, own.c, own.part, parts, lds16);
     const float* sums = reinterpret_cast<const float*>(lds16);
-    for (int i = tid; i < min(BM, count - r0) * (wide / 4); i += 256) {
-      const int r = i / (wide / 4), j = i % (wide / 4) * 4;
-      if (j >= n) continue;
-      const float weight = plan->weight[start + r0 + r];
+    auto sums_of = [&](auto&& f) {  // f(number in the expert's rows, column, 4 sums)
+      for (int i = tid; i < min(BM, count - r0) * (wide / 4); i += 256) {
+        const int r = i / (wide / 4), j = i % (wide / 4) * 4;
+        if (j >= n) continue;
+        F4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = thin_sum<BM>(sums, parts, r, j + q);
+        f(start + r0 + r, j, v);
+      }
+    };
+    bool odd = false;
+    sums_of([&](int at, int j, const F4& s) {
+      const float weight = plan->weight[at];
       Pack<float> v;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v.v[q] = thin_sum<BM>(sums, parts, r, j + q) * weight;
-      store_upto(out + (start + r0 + r) * p.outer + col + j, v, n - j);
+      for (int q = 0; q < 4; ++q) {
+        odd |= !(fabsf(s[q]) < __builtin_inff());
+        v.v[q] = s[q] * weight;
+      }
+      store_upto(out + at * p.outer + col + j, v, n - j);
+    });
+    // An infinite weight times a low part that is zero, or of the other sign, makes NaN of an
+    // infinity.  Where there are such sums, once more with the high parts alone: theirs that are
+    // not finite stand.  (Sums of their own for the low parts all the time take more registers than
+    // there are.)
+    if (__syncthreads_or(odd)) {
+      const Rows first[1] = {a[0]};
+      Core::First::run(first, row, p.hidden, w, e, p.outer, own.c, own.part, parts, lds16);
+      sums_of([&](int at, int j, const F4& s) {
+        const float weight = plan->weight[at];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (j + q < n && !(fabsf(s[q]) < __builtin_inff()))
+            out[at * p.outer + col + j + q] = s[q] * weight;
+      });
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 

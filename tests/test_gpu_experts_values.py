@@ -127,3 +127,37 @@ def test_hidden_values_beyond_the_range_in_every_part(hidden, form, tokens):
         want = np.where(np.isinf(want), want, 1.0) @ full  # a zero changes no infinity
     assert np.isinf(want).all()
     _same_kinds(out, want)
+
+
+@pytest.mark.parametrize("form", ["io", "oi", "odd", "packed"])
+@pytest.mark.parametrize("tokens,hidden", [(1, 64), (3, 40), (16, 768), (40, 200), (64, 264)])
+@pytest.mark.parametrize("exact", [True, False])  # whether hidden values are numbers of the type
+@pytest.mark.parametrize("dtype", HALF)
+def test_infinite_weights_of_a_layers_second_product(form, tokens, hidden, exact, dtype):
+    """Columns with an infinite weight: infinite where the hidden values are not zero.  In codes:
+    weights above float16's range, which are infinite beside float16 (codes have no infinity of
+    their own)."""
+    torch = require_gpu()
+    from purin_amd import Microscaled, expert_layer
+
+    print(f"infinite weights {form} {tokens} {hidden} {exact} {dtype}", flush=True)
+    t = _types(torch)[dtype]
+    a = torch.full((1, 64, hidden), 0.25) if exact else 0.01 + _nonzero(
+        torch, 1, (1, 64, hidden), torch.float32, 0.25).abs().cpu()
+    a, _ = _given(torch, a.to(t).cuda(), form)
+    b = _nonzero(torch, 2, (1, hidden, 40), t, 2.0 ** -8)
+    if form == "packed":
+        # a block of 32 is above the range as a whole
+        wide = b.float()
+        wide[0, :32, 3], wide[0, -(hidden % 32 or 32):, 17] = 2.0 ** 17, -(2.0 ** 17)
+        b, full = _given(torch, wide, form)
+        b = Microscaled(b.codes, b.scales, b.kind, b.shape, b.axis, t)
+        if dtype == "f16":
+            full = np.where(np.abs(full) > 65504, np.copysign(np.inf, full), full)
+    else:
+        b[0, 0, 3], b[0, hidden - 1, 17], b[0, hidden // 2, 18] = (float("inf"), -float("inf"),
+                                                                    float("inf"))
+        b, full = _given(torch, b, form)
+    x = torch.ones((tokens, 64), device="cuda").to(t)
+    out = expert_layer(x, torch.ones((tokens, 1), device="cuda"), 1, a, b, "relu")
+    _same_kinds(out, np.broadcast_to(np.ones(hidden) @ full[0], (tokens, 40)))
