@@ -366,7 +366,10 @@ struct Choose {
 // | 143; 16, 8 of 64, 4096 x 1408 346 | 352; 32, 4 of 64, 1024 x 512 57 | 46.  In codes, two workgroups
 // to a CU, the plans of one round after another show: 8, 4 of 32 (32 pairs, 1408 workgroups) 63.6 | 64.6;
 // 16, 4 of 256, 512 x 256 (64, 512) 28.3 | 28.8; 16, 4 of 64, 1024 x 512 (64, 1024) 44 | 40; 16, 8 of 64
-// (128, 1408) 151 | 141.
+// (128, 1408) 151 | 141.  Between, by pairs times workgroups, gated: 8, 4 of 32, 4096 wide 24576 47.0 | 49.4,
+// 32768 64.6 | 65.5, 40960 76.6 | 77.1; 16, 4 of 64, 1024 wide 32768 27.2 | 28.4, 40960 29.7 | 28.6, 49152
+// 31.6 | 28.7, 57344 38.0 | 35.3; 16, 8 of 64, 4096 wide 40960 36.5 | 35.9, 49152 37.1 | 36.8, 57344
+// 37.8 | 37.6.
 constexpr int kOwnPairs = 128, kOwnTokens = 16, kOwnExperts = 256;
 constexpr int64_t kOwnCodes = 48 * 1024;  // pairs times workgroups
 struct OwnPlan {

@@ -15,7 +15,9 @@
 // passes between them without LDS.  Read and written, us and TB/s: 32768 x 2048 bf16 to 4 bits 35
 // (4.8); 4099 x 1111 float32 to 8 bits 7 and back 7.5 (3.2, 3.0); 16 x 4096 x 2048 bf16 to 4 bits
 // across memory 86-90 (3.8-3.9) and back 58 (5.8, the codes in the cache); the gated activation of
-// 49152 x 2816 bf16 with kept rows 94-98, backward 93-97 (5.7-6.0, part of them in the cache).
+// 49152 x 2816 bf16 with kept rows 94-98, backward 93-97 (5.7-6.0, part of them in the cache), without
+// 73-76 and 113-117 (5.5, 6.0).  gelu is bound by its share of a normal distribution, a 32-bit erfcf for
+// 16-bit results too: 4099 x 777 float16 10.5 both ways, silu 7 and 6.
 
 #include <algorithm>
 #include <type_traits>

@@ -505,9 +505,15 @@ struct RowStream {
   }
 };
 
-// Parts of a contraction for a number of 64-column streams of it.  us with 1 | 2 | 4: one token, 8
-// experts (352 and 256 streams) 62 | 49 | 47; 64 tokens, 64 experts in 4 bits (2816 and 4096)
-// 194 | 190 | 206.
+// Parts of a contraction for a number of 64-column streams of it.  us with 1 | 2 | 4: a layer of one
+// token, 8 experts (352 and 256 streams) 62 | 49 | 47; of 64 tokens, 64 experts in 4 bits (2816 and
+// 4096) 194 | 190 | 206.  Products in 4 bits, one row to an expert, 2560 columns, contractions of 4096,
+// then of 1408:
+//   streams      1040              1600              2560              3200              4160              5120
+//   4096   44 | 44 | 42      59 | 55 | 57      83 | 75 | 80    100 | 97 | 103   129 | 122 | 132   138 | 139 | 156
+//   1408   24 | 24 | 26      32 | 30 | 35      37 | 39 | 48      46 | 51 | 61      57 | 65 | 78      61 | 73 | 92
+// Layers of 16 tokens, dense, 4096 long: 4 from 176 streams (63 | 43 | 38) to 1408 (178 | 169 | 153), equal
+// from 2048 on (214 | 211 | 208).  The turns lie between the long contractions' and the short ones'.
 inline int stream_parts(int64_t streams) { return streams >= 4096 ? 1 : streams >= 1536 ? 2 : 4; }
 // A part of the lines ``first`` to ``end``.
 __device__ __forceinline__ void share_lines(int first, int end, int part, int parts, int& from,

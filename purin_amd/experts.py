@@ -4,8 +4,8 @@
 
 is ``route``, ``dispatch``, ``expert_product``, ``activate``, ``expert_product`` and ``combine`` in
 turn, and for a few tokens of bfloat16 or float16 without a graph three or four kernels that read
-every weight of the chosen experts once (a few times for experts with many tokens).  The HIP library's conventions are those of ``routing``.  The
-reference has no counterpart.
+every weight of the chosen experts once (a few times for experts with many tokens).  The HIP
+library's conventions are those of ``routing``.  The reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -64,7 +64,8 @@ def expert_layer(x, weights, slots, inner, outer, activation="silu", *, workspac
     of them) of bfloat16 or float16 without a graph run in three or four kernels, which keep the
     hidden values to twice the type's digits and need the ``workspace`` (new memory otherwise; left
     alone by other calls).  All others are the separate operators in turn, which round them to the
-    type.
+    type; float32 tokens, and a graph's backward pass, unpack a packed matrix of all experts for the
+    length of its product.
     """
     code = _activation(activation)
     if slots.__class__ is not int:
