@@ -21,7 +21,7 @@ ACTIVATIONS = {"relu": _lib.RELU, "silu": _lib.SILU, "gelu": _lib.GELU}
 
 
 def _activation(kind):
-    if kind not in ACTIVATIONS:
+    if not isinstance(kind, str) or kind not in ACTIVATIONS:
         raise ValueError(f'the activation must be "relu", "silu" or "gelu"; got {kind!r}')
     return ACTIVATIONS[kind]
 

@@ -49,13 +49,15 @@ class Microscaled:
 
 
 def kind_code(kind):
-    if kind not in KINDS:
+    if not isinstance(kind, str) or kind not in KINDS:
         raise ValueError(f'kind must be "fp4" or "int8"; got {kind!r}')
     return KINDS[kind]
 
 
 def fields(packed):
     """What the front end takes of a Microscaled."""
+    if not isinstance(packed.shape, (tuple, list)):
+        raise ValueError(f"a Microscaled's shape must be a tuple; got {packed.shape!r}")
     return packed.codes, packed.scales, kind_code(packed.kind), list(packed.shape), packed.axis
 
 
